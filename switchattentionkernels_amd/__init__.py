@@ -16,7 +16,14 @@ from .prefill import (  # noqa: F401
 from .metadata import SwitchAttentionMetadata, build_switch_attention_metadata  # noqa: F401
 from .flops import routed_flops  # noqa: F401
 from .split import merge_attention_partials, shard_attention_metadata  # noqa: F401
-from .decode import switch_gqa_decode_forward  # noqa: F401
+from .cache import (  # noqa: F401
+    SwitchKVCache,
+    build_switch_kv_cache,
+    switch_kv_cache_append,
+    switch_kv_cache_evict,
+    switch_kv_cache_read,
+)
+from .decode import switch_gqa_decode_forward, switch_gqa_decode_quantized_forward  # noqa: F401
 from .backward import (  # noqa: F401
     SwitchGQAPrefillFunction,
     switch_gqa_prefill,
@@ -35,6 +42,12 @@ __all__ = [
     "shard_attention_metadata",
     "merge_attention_partials",
     "switch_gqa_decode_forward",
+    "SwitchKVCache",
+    "build_switch_kv_cache",
+    "switch_kv_cache_append",
+    "switch_kv_cache_read",
+    "switch_gqa_decode_quantized_forward",
+    "switch_kv_cache_evict",
     "switch_gqa_prefill_backward",
     "switch_gqa_prefill",
     "switch_gqa_prefill_varlen",

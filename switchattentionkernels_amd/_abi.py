@@ -46,6 +46,21 @@ SIGNATURES = {
                                           _i32, _i32, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
 }
 
+# The 8-bit KV cache's entry points; must mirror include/swattn_cache.h exactly.
+CACHE_SIGNATURES = {
+    "swattn_cache_append": (ctypes.c_int, [_vp] * 10 + [_i32, _i64, _i64, _i64, _i32, _i32, _i32,
+                                                        _i32, _vp]),
+    "swattn_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64,
+                                         _i64, _i32, _i32, _i32, _i32, _vp]),
+    "swattn_cache_decode_workspace_bytes": (ctypes.c_size_t, [_i32, _i64, _i32, _i32, _i32]),
+    "swattn_cache_decode_fwd": (ctypes.c_int, [_vp] * 10 + [_i32, _i64, _i32, _i32, _i32, _i32,
+                                                            _i32, _i32, ctypes.c_float, _vp,
+                                                            ctypes.c_size_t, _vp]),
+    "swattn_cache_evict_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i64]),
+    "swattn_cache_evict": (ctypes.c_int, [_vp] * 12 + [_i32, _i64, _i64, _i32, _i32, _i32, _i32,
+                                                       _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+}
+
 # Entry points of libswattn.so for this package only (csrc/swattn_internal.h).
 INTERNAL_SIGNATURES = {
     "swattn_compact_wait": (ctypes.c_int, [_vp, _i32, _i64, ctypes.c_float, _vp, _vp, _vp,

@@ -1,5 +1,5 @@
-"""Bindings of ``libswattn.so``: ctypes for the C ABI (``include/swattn.h``) and
-the native extension for the hot calls (``csrc/native.cpp``).
+"""Bindings of ``libswattn.so``: ctypes for the C ABI (``include/swattn.h``,
+``include/swattn_cache.h``) and the native extension for the hot calls (``csrc/native.cpp``).
 
 The library is built in-tree by ``switchattentionkernels_amd.build``.  There
 is no fallback: if the library is missing every call raises, so a GPU run can
@@ -18,7 +18,8 @@ import threading
 import torch  # loads PyTorch's HIP runtime before the library
 from torch.overrides import has_torch_function_unary
 
-from ._abi import INTERNAL_SIGNATURES, PROBE_SIGNATURES, SIGNATURES, bind  # noqa: F401  -- API
+from ._abi import (CACHE_SIGNATURES, INTERNAL_SIGNATURES, PROBE_SIGNATURES,  # noqa: F401  -- API
+                   SIGNATURES, bind)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libswattn.so")
@@ -46,7 +47,7 @@ def lib() -> ctypes.CDLL:
                 raise LibraryNotBuilt(
                     f"{LIB_PATH} is missing: build it with "
                     "`python -m switchattentionkernels_amd.build`")
-            _lib = bind(bind(ctypes.CDLL(LIB_PATH)), INTERNAL_SIGNATURES)
+            _lib = bind(bind(bind(ctypes.CDLL(LIB_PATH)), CACHE_SIGNATURES), INTERNAL_SIGNATURES)
     return _lib
 
 

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "swattn.h"
+#include "swattn_cache.h"
 #include "swattn_internal.h"
 
 namespace {
@@ -203,6 +204,108 @@ std::tuple<Tensor, Tensor> decode_forward(const Tensor& q, const Tensor& k, cons
   return {out, lse};
 }
 
+// The 8-bit KV cache (codes [B, L, Hkv, 128], scales [B, Hkv, blocks]).
+const float* f32(const Tensor& t) { return static_cast<const float*>(t.const_data_ptr()); }
+
+struct CacheShape {
+  int32_t batch, hkv, dim;
+  int64_t len;
+  explicit CacheShape(const Tensor& k)
+      : batch(static_cast<int32_t>(k.size(0))), hkv(static_cast<int32_t>(k.size(2))),
+        dim(static_cast<int32_t>(k.size(3))), len(k.size(1)) {}
+};
+
+// The new lengths.
+Tensor cache_append(const Tensor& new_k, const Tensor& new_v, const optional<Tensor>& cu,
+                    const optional<Tensor>& counts, const Tensor& lens, const Tensor& k, const Tensor& v,
+                    const Tensor& ks, const Tensor& vs, int64_t rows, int64_t block, int64_t code,
+                    int64_t stream) {
+  const CacheShape c(k);
+  const Tensor out = at::empty({k.size(0)}, lens.options());
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_cache_append(new_k.const_data_ptr(), new_v.const_data_ptr(), i32(cu), i32(counts),
+                                 i32(lens), k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(),
+                                 vs.data_ptr<float>(), out.data_ptr<int32_t>(), c.batch, rows,
+                                 new_k.size(1), c.len, c.hkv, c.dim, static_cast<int32_t>(block),
+                                 static_cast<int32_t>(code), as_stream(stream));
+  }
+  check(status, "swattn_cache_append");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> cache_read(const Tensor& k, const Tensor& v, const Tensor& ks,
+                                      const Tensor& vs, const optional<Tensor>& starts, int64_t start,
+                                      const optional<Tensor>& lens, int64_t rows, int64_t block,
+                                      int64_t code, int64_t stream) {
+  const CacheShape c(k);
+  const auto opts = k.options().dtype(at::kBFloat16);
+  const Tensor out_k = at::empty({k.size(0), rows, k.size(2), k.size(3)}, opts);
+  const Tensor out_v = at::empty(out_k.sizes(), opts);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_cache_read(k.const_data_ptr(), v.const_data_ptr(), f32(ks), f32(vs), i32(starts), start,
+                               i32(lens), out_k.data_ptr(), out_v.data_ptr(), c.batch, rows, c.len, c.hkv,
+                               c.dim, static_cast<int32_t>(block), static_cast<int32_t>(code),
+                               as_stream(stream));
+  }
+  check(status, "swattn_cache_read");
+  return {out_k, out_v};
+}
+
+std::tuple<Tensor, Tensor> cache_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks,
+                                        const Tensor& vs, const Tensor& lens, const Tensor& full,
+                                        const optional<Tensor>& weights, int64_t window, int64_t block,
+                                        int64_t code, double scale_log2, int64_t stream,
+                                        const optional<Tensor>& out_made) {
+  const CacheShape c(k);
+  const int32_t hq = static_cast<int32_t>(q.size(2));
+  const Tensor out = like(q, out_made);
+  const Tensor lse = at::empty({q.size(0), 1, q.size(2)}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes =
+      swattn_cache_decode_workspace_bytes(c.batch, c.len, hq, c.hkv, weights.has_value() ? 1 : 0);
+  const Tensor ws = bytes(q, ws_bytes);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_cache_decode_fwd(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), f32(ks), f32(vs),
+                                     i32(lens), static_cast<const uint8_t*>(full.const_data_ptr()),
+                                     out.data_ptr(), lse.data_ptr<float>(),
+                                     weights.has_value() ? weights->data_ptr<float>() : nullptr, c.batch,
+                                     c.len, hq, c.hkv, c.dim, static_cast<int32_t>(window),
+                                     static_cast<int32_t>(block), static_cast<int32_t>(code),
+                                     static_cast<float>(scale_log2), ws.data_ptr(), ws_bytes,
+                                     as_stream(stream));
+  }
+  check(status, "swattn_cache_decode_fwd");
+  return {out, lse};
+}
+
+// The new lengths.
+Tensor cache_evict(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,
+                   const Tensor& weights, const Tensor& lens, const Tensor& out_k, const Tensor& out_v,
+                   const Tensor& out_ks, const Tensor& out_vs, const Tensor& out_weights, int64_t block,
+                   int64_t code, int64_t budget, int64_t recent, int64_t stream) {
+  const CacheShape c(k);
+  const Tensor out = at::empty({k.size(0)}, lens.options());
+  const size_t ws_bytes = swattn_cache_evict_workspace_bytes(c.batch, c.hkv, budget);
+  const Tensor ws = bytes(k, ws_bytes);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_cache_evict(k.const_data_ptr(), v.const_data_ptr(), f32(ks), f32(vs), f32(weights),
+                                i32(lens), out_k.data_ptr(), out_v.data_ptr(), out_ks.data_ptr<float>(),
+                                out_vs.data_ptr<float>(), out_weights.data_ptr<float>(),
+                                out.data_ptr<int32_t>(), c.batch, c.len, out_k.size(1), c.hkv, c.dim,
+                                static_cast<int32_t>(block), static_cast<int32_t>(code), budget, recent,
+                                ws.data_ptr(), ws_bytes, as_stream(stream));
+  }
+  check(status, "swattn_cache_evict");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -212,4 +315,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("metadata", &metadata);
   m.def("prefill_backward", &prefill_backward);
   m.def("decode_forward", &decode_forward);
+  m.def("cache_append", &cache_append);
+  m.def("cache_read", &cache_read);
+  m.def("cache_decode", &cache_decode);
+  m.def("cache_evict", &cache_evict);
 }

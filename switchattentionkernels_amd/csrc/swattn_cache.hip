@@ -1,0 +1,598 @@
+// The 8-bit KV cache for gfx950: appending bf16 rows, reading rows back, and
+// eviction by accumulated attention weight (include/swattn_cache.h).  No
+// counterpart in the reference, which is prefill-only.
+//
+// A cached value is code * scale, one scale s per block of tokens and KV head:
+//   s = the smallest 2^e >= 2^-100 with max |x| <= qmax * 2^e over the block,
+//   code = round(x / s).
+// A power of two makes x / s exact, so that a value is rounded once, costs e4m3
+// nothing (its steps are relative) and int8 at most one bit, half a bit on
+// average.
+//
+// All three are HBM-bound: a row of one head is 256 bytes in bf16 and 128 as
+// codes, for K and for V.  Workgroups of 256 threads take one block of one head:
+// threads 0-127 its K rows, 128-255 its V rows, 16 rows at a time, 8 threads of
+// 16 values per row.
+
+#include <limits.h>
+
+#include <string>
+
+#include "cache_code.h"
+
+namespace swattn {
+namespace {
+
+using namespace code;
+
+constexpr int kD = 128;
+constexpr int kRowsAtOnce = 16;   // rows that a workgroup's half takes at once
+constexpr int kSelectThreads = 1024;
+
+__device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+
+// Largest value over this half of the workgroup (threads 0-127 or 128-255).
+__device__ __forceinline__ uint32_t half_max(uint32_t x) {
+  __shared__ uint32_t s_max[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), off)));
+  if (lane == 0) s_max[wave] = x;
+  __syncthreads();
+  return max(s_max[wave & 2], s_max[(wave & 2) + 1]);
+}
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+struct AppendParams {
+  const uint16_t* src[2];    // new K, V rows
+  const int32_t* cu;         // packed: offsets, else null
+  const int32_t* counts;     // padded: rows per sequence, or null
+  const int32_t* lens;
+  uint8_t* codes[2];
+  float* scales[2];
+  int32_t* lens_out;
+  int64_t rows, total_rows;
+  int cache_len, hkv, nblk, batch, blocks;   // blocks: per sequence, at most
+};
+
+// One workgroup per (sequence, touched block, KV head).
+template <int kCode, int kBlock>
+__global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
+  constexpr int kIt = kBlock / kRowsAtOnce;
+  const int h = blockIdx.x % p.hkv;
+  const int rest = blockIdx.x / p.hkv;
+  const int i = rest % p.blocks, b = rest / p.blocks;
+  const int len = min(max(p.lens[b], 0), p.cache_len);
+  // This sequence's new rows: src rows first .. first + count - 1.
+  int64_t first = b * p.rows, count = p.rows;
+  if (p.cu != nullptr) {
+    first = min(max(static_cast<int64_t>(p.cu[b]), int64_t{0}), p.total_rows);
+    count = min(min(max(static_cast<int64_t>(p.cu[b + 1]), first), p.total_rows) - first, p.rows);
+  } else if (p.counts != nullptr) {
+    count = min(max(static_cast<int64_t>(p.counts[b]), int64_t{0}), p.rows);
+  }
+  const int end = static_cast<int>(min(len + count, static_cast<int64_t>(p.cache_len)));
+  if (i == 0 && h == 0 && threadIdx.x == 0) p.lens_out[b] = end;
+  const int jb = len / kBlock + i;
+  const int r0 = jb * kBlock;          // the block's rows
+  if (end <= len || r0 >= end) return;   // uniform
+  const int half = threadIdx.x >> 7, t = threadIdx.x & 127;
+  const int sub = t >> 3, piece = t & 7;
+  const uint16_t* src = p.src[half];
+  uint4 raw[kIt][2];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int r = r0 + it * kRowsAtOnce + sub;
+    raw[it][0] = raw[it][1] = make_uint4(0, 0, 0, 0);
+    if (r >= len && r < end) {
+      const uint4* row = reinterpret_cast<const uint4*>(src + ((first + (r - len)) * p.hkv + h) * kD + piece * 16);
+      raw[it][0] = row[0];
+      raw[it][1] = row[1];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t w[4] = {raw[it][u].x, raw[it][u].y, raw[it][u].z, raw[it][u].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) amax = max(amax, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
+    }
+  }
+  amax = half_max(amax);
+  float scale = scale_for<kCode>(amax);
+  const bool begun = r0 < len;
+  float* sp = p.scales[half] + (static_cast<int64_t>(b) * p.hkv + h) * p.nblk + jb;
+  uint8_t* codes = p.codes[half] + (static_cast<int64_t>(b) * p.cache_len * p.hkv + h) * kD + piece * 16;
+  const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
+  if (begun) {
+    const float old = *sp;
+    scale = old != old || old > scale ? old : scale;   // NaN stays NaN
+    __syncthreads();   // every thread has read the scale
+    if (old == old && scale != old) {   // grown (or NaN now): round the held rows again
+      const float ratio = old / scale;
+#pragma unroll
+      for (int it = 0; it < kIt; ++it) {
+        const int r = r0 + it * kRowsAtOnce + sub;
+        if (r < len) {
+          uint4* at = reinterpret_cast<uint4*>(codes + r * stride);
+          float x[16];
+          decode16<kCode>(*at, x);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] *= ratio;
+          *at = encode16<kCode>(x);
+        }
+      }
+    }
+  }
+  if (t == 0) *sp = scale;
+  const float inv = 1.0f / scale;   // exact unless the scale is a begun block's own
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int r = r0 + it * kRowsAtOnce + sub;
+    if (r >= len && r < end) {
+      float x[16];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t w[4] = {raw[it][u].x, raw[it][u].y, raw[it][u].z, raw[it][u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[8 * u + 2 * j] = bf(w[j] & 0xffffu);
+          x[8 * u + 2 * j + 1] = bf(w[j] >> 16);
+        }
+      }
+      if (begun) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = x[j] / scale;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] *= inv;
+      }
+      *reinterpret_cast<uint4*>(codes + r * stride) = encode16<kCode>(x);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Read
+// ---------------------------------------------------------------------------
+struct ReadParams {
+  const uint8_t* codes[2];
+  const float* scales[2];
+  const int32_t* starts;   // or null: `start`
+  const int32_t* lens;     // or null: cache_len
+  uint16_t* out[2];
+  int64_t start, rows, pieces;   // pieces: 16 values each, of K
+  int cache_len, hkv, nblk, block_log;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(a))) |
+         static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(b))) << 16;
+}
+
+// One thread per 16 values; blockIdx.y 0: K, 1: V.
+template <int kCode>
+__global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (x >= p.pieces) return;
+  const int which = blockIdx.y;
+  const int piece = static_cast<int>(x & 7);
+  const int64_t rowh = x >> 3;                 // (b * rows + i) * hkv + h
+  const int64_t row = rowh / p.hkv;
+  const int h = static_cast<int>(rowh - row * p.hkv);
+  const int64_t b = row / p.rows, i = row - b * p.rows;
+  const int64_t r = (p.starts != nullptr ? static_cast<int64_t>(p.starts[b]) : p.start) + i;
+  const int end = p.lens != nullptr ? min(p.lens[b], p.cache_len) : p.cache_len;
+  uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (r >= 0 && r < end) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p.codes[which] + ((b * p.cache_len + r) * p.hkv + h) * kD + piece * 16);
+    const float s = p.scales[which][(b * p.hkv + h) * p.nblk + (r >> p.block_log)];
+    float v[16];
+    decode16<kCode>(u, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      o[j] = make_uint4(pack_bf16(v[8 * j] * s, v[8 * j + 1] * s), pack_bf16(v[8 * j + 2] * s, v[8 * j + 3] * s),
+                        pack_bf16(v[8 * j + 4] * s, v[8 * j + 5] * s), pack_bf16(v[8 * j + 6] * s, v[8 * j + 7] * s));
+  }
+  uint4* out = reinterpret_cast<uint4*>(p.out[which] + x * 16);
+  out[0] = o[0];
+  out[1] = o[1];
+}
+
+// ---------------------------------------------------------------------------
+// Evict
+// ---------------------------------------------------------------------------
+struct EvictParams {
+  const uint8_t* codes[2];
+  const float* scales[2];
+  const float* weights;
+  const int32_t* lens;
+  uint8_t* out_codes[2];
+  float* out_scales[2];
+  float* out_weights;
+  int32_t* lens_out;
+  int32_t* kept;   // [pair][budget - recent] rows that were chosen, ascending
+  int cache_len, out_len, hkv, nblk, out_nblk, out_blocks, budget, recent;
+};
+
+// A weight as an unsigned number of the same order: NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t order_key(float w) {
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  if (w != w) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Inclusive prefix sums over the workgroup of x; `total` of all.
+__device__ __forceinline__ uint32_t scan_1024(uint32_t x, uint32_t* s_wave, uint32_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t y = static_cast<uint32_t>(__shfl_up(static_cast<int>(x), off));
+    x += lane >= off ? y : 0u;
+  }
+  __syncthreads();   // s_wave may still be read by the last call
+  if (lane == 63) s_wave[wave] = x;
+  __syncthreads();
+  total = 0;
+  uint32_t before = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectThreads / 64; ++w) {
+    before += w < wave ? s_wave[w] : 0u;
+    total += s_wave[w];
+  }
+  return x + before;
+}
+
+// Which of the older rows stay: one workgroup per (sequence, KV head).  The
+// (budget - recent)-th largest weight by a radix search, 8 bits a pass, then one
+// ordered pass that writes the rows above it and the first of those equal to it.
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(const EvictParams p) {
+  __shared__ uint32_t s_hist[256];
+  __shared__ uint32_t s_wave[kSelectThreads / 64];
+  __shared__ uint32_t s_pick[2];
+  const int64_t pair = blockIdx.x;
+  const int b = static_cast<int>(pair / p.hkv);
+  const int tid = threadIdx.x;
+  const int len = min(max(p.lens[b], 0), p.cache_len);
+  if (pair - static_cast<int64_t>(b) * p.hkv == 0 && tid == 0) p.lens_out[b] = min(len, p.budget);
+  const int want = p.budget - p.recent;
+  if (len <= p.budget || want == 0) return;   // uniform
+  const int n = len - p.recent;               // more than want
+  const float* w = p.weights + pair * p.cache_len;
+  uint32_t prefix = 0, mask = 0, need = want;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) s_hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelectThreads) {
+      const uint32_t k = order_key(w[i]);
+      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+    }
+    __syncthreads();
+    if (tid < 64) {   // wave 0: bins from the top, four per lane
+      uint32_t c[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[j] = s_hist[255 - 4 * tid - j];
+        sum += c[j];
+      }
+      uint32_t incl = sum;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t y = static_cast<uint32_t>(__shfl_up(static_cast<int>(incl), off));
+        incl += tid >= off ? y : 0u;
+      }
+      uint32_t above = incl - sum;
+      if (above < need && need <= incl) {   // one lane: the sums ascend
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (above < need && need <= above + c[j]) {
+            s_pick[0] = 255 - 4 * tid - j;
+            s_pick[1] = need - above;
+          }
+          above += c[j];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= s_pick[0] << shift;
+    mask |= 255u << shift;
+    need = s_pick[1];
+    __syncthreads();
+  }
+  // `need` of the rows whose key equals prefix stay, all above it do.
+  int32_t* kept = p.kept + pair * want;
+  uint32_t above = 0, equal = 0;   // before this tile
+  for (int base = 0; base < n; base += 4 * kSelectThreads) {
+    uint32_t k[4], cnt = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = base + 4 * tid + j;
+      k[j] = i < n ? order_key(w[i]) : 0u;
+      if (i < n) cnt += k[j] > prefix ? 1u : k[j] == prefix ? 0x10000u : 0u;
+    }
+    uint32_t total;
+    const uint32_t incl = scan_1024(cnt, s_wave, total);
+    uint32_t a = above + ((incl - cnt) & 0xffffu), e = equal + ((incl - cnt) >> 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = base + 4 * tid + j;
+      if (i >= n) continue;
+      const bool eq = k[j] == prefix;
+      const uint32_t at = a + min(e, need);
+      if ((k[j] > prefix || (eq && e < need)) && at < static_cast<uint32_t>(want)) kept[at] = i;
+      a += k[j] > prefix ? 1u : 0u;
+      e += eq ? 1u : 0u;
+    }
+    above += total & 0xffffu;
+    equal += total >> 16;
+  }
+}
+
+// The kept rows into the destination: one workgroup per (sequence, destination
+// block, KV head).
+template <int kCode, int kBlock>
+__global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
+  constexpr int kIt = kBlock / kRowsAtOnce;
+  const int h = blockIdx.x % p.hkv;
+  const int rest = blockIdx.x / p.hkv;
+  const int jb = rest % p.out_blocks, b = rest / p.out_blocks;
+  const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
+  const int len = min(max(p.lens[b], 0), p.cache_len);
+  const int want = p.budget - p.recent;
+  const int end = min(len, p.budget);
+  auto source = [&](int d) {
+    int s = d;
+    if (len > p.budget) s = d < want ? p.kept[pair * want + d] : len - p.budget + d;
+    return min(max(s, 0), p.cache_len - 1);
+  };
+  const int r0 = jb * kBlock;
+  if (threadIdx.x < kBlock) {
+    const int d = r0 + static_cast<int>(threadIdx.x);
+    if (d < p.out_len)
+      p.out_weights[pair * p.out_len + d] = d < end ? p.weights[pair * p.cache_len + source(d)] : 0.f;
+  }
+  if (r0 >= end) return;   // uniform
+  const int half = threadIdx.x >> 7, t = threadIdx.x & 127;
+  const int sub = t >> 3, piece = t & 7;
+  const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
+  const uint8_t* codes = p.codes[half] + (static_cast<int64_t>(b) * p.cache_len * p.hkv + h) * kD + piece * 16;
+  const float* scales = p.scales[half] + pair * p.nblk;
+  uint4 raw[kIt];
+  float s[kIt];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int d = r0 + it * kRowsAtOnce + sub;
+    raw[it] = make_uint4(0, 0, 0, 0);
+    s[it] = 0.f;
+    if (d < end) {
+      const int r = source(d);
+      raw[it] = *reinterpret_cast<const uint4*>(codes + r * stride);
+      s[it] = scales[r / kBlock];
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    float x[16];
+    decode16<kCode>(raw[it], x);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = max(amax, abs_bits(x[j] * s[it]));
+  }
+  amax = half_max(amax);
+  const float scale = scale_for<kCode>(amax);
+  if (t == 0) p.out_scales[half][pair * p.out_nblk + jb] = scale;
+  const float inv = 1.0f / scale;
+  uint8_t* out = p.out_codes[half] + (static_cast<int64_t>(b) * p.out_len * p.hkv + h) * kD + piece * 16;
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int d = r0 + it * kRowsAtOnce + sub;
+    if (d < end) {
+      float x[16];
+      decode16<kCode>(raw[it], x);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
+      *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
+    }
+  }
+}
+
+// Argument checks that the entry points share.
+int check_cache(const std::string& n, int32_t batch, int64_t cache_len, int32_t heads_kv, int32_t head_dim,
+                int32_t block, int32_t codes) {
+  if (head_dim != kD) return invalid(n + ": head_dim must be 128");
+  if (batch < 1 || cache_len < 1 || heads_kv < 1) return invalid(n + ": bad shape");
+  if (batch > 65535 || heads_kv > 65535 || cache_len > INT32_MAX - 256)
+    return invalid(n + ": batch, heads_kv or cache_len too large");
+  if (!block_ok(block)) return invalid(n + ": block must be 16, 32, 64 or 128");
+  if (codes != kE4m3 && codes != kInt8) return invalid(n + ": unknown code");
+  return SWATTN_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// fn<code, block>(grid, stream, params)
+template <template <int, int> class Launch, class P>
+void by_code_and_block(int32_t codes, int32_t block, dim3 grid, hipStream_t st, const P& p) {
+  if (codes == kE4m3) {
+    switch (block) {
+      case 16: return Launch<kE4m3, 16>::go(grid, st, p);
+      case 32: return Launch<kE4m3, 32>::go(grid, st, p);
+      case 64: return Launch<kE4m3, 64>::go(grid, st, p);
+      default: return Launch<kE4m3, 128>::go(grid, st, p);
+    }
+  }
+  switch (block) {
+    case 16: return Launch<kInt8, 16>::go(grid, st, p);
+    case 32: return Launch<kInt8, 32>::go(grid, st, p);
+    case 64: return Launch<kInt8, 64>::go(grid, st, p);
+    default: return Launch<kInt8, 128>::go(grid, st, p);
+  }
+}
+template <int kCode, int kBlock>
+struct LaunchAppend {
+  static void go(dim3 grid, hipStream_t st, const AppendParams& p) {
+    hipLaunchKernelGGL((append_kernel<kCode, kBlock>), grid, dim3(256), 0, st, p);
+  }
+};
+template <int kCode, int kBlock>
+struct LaunchGather {
+  static void go(dim3 grid, hipStream_t st, const EvictParams& p) {
+    hipLaunchKernelGGL((gather_kernel<kCode, kBlock>), grid, dim3(256), 0, st, p);
+  }
+};
+
+}  // namespace
+}  // namespace swattn
+
+using namespace swattn;
+
+extern "C" {
+
+int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
+                        const int32_t* counts, const int32_t* cache_lens, void* k, void* v,
+                        float* k_scales, float* v_scales, int32_t* lens_out, int32_t batch,
+                        int64_t rows, int64_t total_rows, int64_t cache_len, int32_t heads_kv,
+                        int32_t head_dim, int32_t block, int32_t codes, void* stream) {
+  const std::string n("swattn_cache_append");
+  const int st = check_cache(n, batch, cache_len, heads_kv, head_dim, block, codes);
+  if (st != SWATTN_OK) return st;
+  if (rows < 0 || rows > INT32_MAX || total_rows < 0 || total_rows > INT32_MAX)
+    return invalid(n + ": bad number of rows");
+  if (cu_seqlens != nullptr && counts != nullptr) return invalid(n + ": counts and cu_seqlens exclude each other");
+  const bool any = rows > 0 && (cu_seqlens == nullptr || total_rows > 0);
+  if (cache_lens == nullptr || lens_out == nullptr || k == nullptr || v == nullptr || k_scales == nullptr ||
+      v_scales == nullptr || (any && (new_k == nullptr || new_v == nullptr)))
+    return invalid(n + ": null pointer");
+  if (cache_lens == lens_out) return invalid(n + ": lens_out may not be cache_lens");
+  if (!aligned16(k) || !aligned16(v) || (any && (!aligned16(new_k) || !aligned16(new_v))))
+    return invalid(n + ": new_k, new_v, k and v must be 16-byte aligned");
+  AppendParams p{};
+  p.src[0] = static_cast<const uint16_t*>(new_k);
+  p.src[1] = static_cast<const uint16_t*>(new_v);
+  p.cu = cu_seqlens;
+  p.counts = counts;
+  p.lens = cache_lens;
+  p.codes[0] = static_cast<uint8_t*>(k);
+  p.codes[1] = static_cast<uint8_t*>(v);
+  p.scales[0] = k_scales;
+  p.scales[1] = v_scales;
+  p.lens_out = lens_out;
+  p.rows = rows;
+  p.total_rows = total_rows;
+  p.cache_len = static_cast<int>(cache_len);
+  p.hkv = heads_kv;
+  p.nblk = static_cast<int>(ceil_div(cache_len, block));
+  p.batch = batch;
+  // `rows` rows from any place of a block on; no more than the cache has.
+  const int64_t most = rows < 1 ? 1 : (rows + block - 2) / block + 1;
+  p.blocks = static_cast<int>(most < p.nblk ? most : p.nblk);
+  const int64_t grid = static_cast<int64_t>(p.blocks) * batch * heads_kv;
+  if (grid > INT32_MAX) return invalid(n + ": grid too large");
+  by_code_and_block<LaunchAppend>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p);
+  return launch_status(n.c_str());
+}
+
+int swattn_cache_read(const void* k, const void* v, const float* k_scales, const float* v_scales,
+                      const int32_t* starts, int64_t start, const int32_t* cache_lens, void* out_k,
+                      void* out_v, int32_t batch, int64_t rows, int64_t cache_len,
+                      int32_t heads_kv, int32_t head_dim, int32_t block, int32_t codes,
+                      void* stream) {
+  const std::string n("swattn_cache_read");
+  const int st = check_cache(n, batch, cache_len, heads_kv, head_dim, block, codes);
+  if (st != SWATTN_OK) return st;
+  if (rows < 0 || rows > INT32_MAX || start < 0 || start > INT32_MAX) return invalid(n + ": bad range of rows");
+  if (rows == 0) return SWATTN_OK;
+  if (k == nullptr || v == nullptr || k_scales == nullptr || v_scales == nullptr || out_k == nullptr ||
+      out_v == nullptr)
+    return invalid(n + ": null pointer");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(out_k) || !aligned16(out_v))
+    return invalid(n + ": k, v, out_k and out_v must be 16-byte aligned");
+  ReadParams p{};
+  p.codes[0] = static_cast<const uint8_t*>(k);
+  p.codes[1] = static_cast<const uint8_t*>(v);
+  p.scales[0] = k_scales;
+  p.scales[1] = v_scales;
+  p.starts = starts;
+  p.lens = cache_lens;
+  p.out[0] = static_cast<uint16_t*>(out_k);
+  p.out[1] = static_cast<uint16_t*>(out_v);
+  p.start = start;
+  p.rows = rows;
+  p.pieces = static_cast<int64_t>(batch) * rows * heads_kv * (kD / 16);
+  p.cache_len = static_cast<int>(cache_len);
+  p.hkv = heads_kv;
+  p.nblk = static_cast<int>(ceil_div(cache_len, block));
+  p.block_log = __builtin_ctz(static_cast<unsigned>(block));
+  const int64_t grid = ceil_div(p.pieces, 256);
+  if (grid > INT32_MAX) return invalid(n + ": grid too large");
+  const dim3 g(static_cast<uint32_t>(grid), 2);
+  if (codes == kE4m3)
+    hipLaunchKernelGGL(read_kernel<kE4m3>, g, dim3(256), 0, as_stream(stream), p);
+  else
+    hipLaunchKernelGGL(read_kernel<kInt8>, g, dim3(256), 0, as_stream(stream), p);
+  return launch_status(n.c_str());
+}
+
+size_t swattn_cache_evict_workspace_bytes(int32_t batch, int32_t heads_kv, int64_t budget) {
+  if (batch < 1 || heads_kv < 1 || budget < 1) return 0;
+  return (static_cast<size_t>(batch) * heads_kv * budget * sizeof(int32_t) + 255) & ~size_t{255};
+}
+
+int swattn_cache_evict(const void* k, const void* v, const float* k_scales, const float* v_scales,
+                       const float* key_weights, const int32_t* cache_lens, void* out_k,
+                       void* out_v, float* out_k_scales, float* out_v_scales, float* out_weights,
+                       int32_t* lens_out, int32_t batch, int64_t cache_len, int64_t out_len,
+                       int32_t heads_kv, int32_t head_dim, int32_t block, int32_t codes,
+                       int64_t budget, int64_t recent, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  const std::string n("swattn_cache_evict");
+  int st = check_cache(n, batch, cache_len, heads_kv, head_dim, block, codes);
+  if (st != SWATTN_OK) return st;
+  st = check_cache(n, batch, out_len, heads_kv, head_dim, block, codes);
+  if (st != SWATTN_OK) return st;
+  if (budget < 1 || budget > out_len) return invalid(n + ": budget must lie in [1, out_len]");
+  if (recent < 0 || recent > budget) return invalid(n + ": recent must lie in [0, budget]");
+  if (k == nullptr || v == nullptr || k_scales == nullptr || v_scales == nullptr || key_weights == nullptr ||
+      cache_lens == nullptr || out_k == nullptr || out_v == nullptr || out_k_scales == nullptr ||
+      out_v_scales == nullptr || out_weights == nullptr || lens_out == nullptr)
+    return invalid(n + ": null pointer");
+  if (k == out_k || v == out_v || k_scales == out_k_scales || v_scales == out_v_scales ||
+      key_weights == out_weights || cache_lens == lens_out)
+    return invalid(n + ": the destination may not be the source");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(out_k) || !aligned16(out_v))
+    return invalid(n + ": k, v, out_k and out_v must be 16-byte aligned");
+  if (workspace == nullptr || workspace_bytes < swattn_cache_evict_workspace_bytes(batch, heads_kv, budget)) {
+    set_error(n + ": workspace smaller than swattn_cache_evict_workspace_bytes()");
+    return SWATTN_EWORKSPACE;
+  }
+  if (!aligned256(workspace)) return invalid(n + ": workspace must be 256-byte aligned");
+  EvictParams p{};
+  p.codes[0] = static_cast<const uint8_t*>(k);
+  p.codes[1] = static_cast<const uint8_t*>(v);
+  p.scales[0] = k_scales;
+  p.scales[1] = v_scales;
+  p.weights = key_weights;
+  p.lens = cache_lens;
+  p.out_codes[0] = static_cast<uint8_t*>(out_k);
+  p.out_codes[1] = static_cast<uint8_t*>(out_v);
+  p.out_scales[0] = out_k_scales;
+  p.out_scales[1] = out_v_scales;
+  p.out_weights = out_weights;
+  p.lens_out = lens_out;
+  p.kept = static_cast<int32_t*>(workspace);
+  p.cache_len = static_cast<int>(cache_len);
+  p.out_len = static_cast<int>(out_len);
+  p.hkv = heads_kv;
+  p.nblk = static_cast<int>(ceil_div(cache_len, block));
+  p.out_nblk = p.out_blocks = static_cast<int>(ceil_div(out_len, block));
+  p.budget = static_cast<int>(budget);
+  p.recent = static_cast<int>(recent);
+  const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_blocks;
+  if (grid > INT32_MAX) return invalid(n + ": grid too large");
+  hipLaunchKernelGGL(select_kernel, dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), 0, as_stream(stream), p);
+  by_code_and_block<LaunchGather>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p);
+  return launch_status(n.c_str());
+}
+
+}  // extern "C"

@@ -5,7 +5,8 @@ of a sequence (F:145-155): with ``n = cache_lens[b]`` the new token sits at
 position ``n - 1`` -- its own K/V already appended -- and attends keys
 ``[0, n)`` when routed full, else the last ``window_size`` of them.  Output
 follows the prefill's conventions: bf16 O and fp32 LSE in the log2
-convention (V:15, V:236-241).
+convention (V:15, V:236-241).  ``switch_gqa_decode_quantized_forward`` does the
+same over an 8-bit cache (``cache.py``).
 """
 
 from __future__ import annotations
@@ -15,6 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
+from .cache import _CODES, SwitchKVCache, check_cache, check_lens, check_weights
 
 LOG2E = 1.4426950408889634
 
@@ -69,6 +71,56 @@ def switch_gqa_decode_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     with _lib.on_device(dev):
         out, lse = _lib.native().decode_forward(q, k_cache, v_cache, lens, full, int(window_size),
                                                 scale, _lib.stream_handle(dev), _lib.like(q))
+    if squeeze:
+        return out[:, 0], lse[:, 0]
+    return out, lse
+
+
+def switch_gqa_decode_quantized_forward(
+        q: torch.Tensor, cache: SwitchKVCache, cache_lens: torch.Tensor, full_mask: torch.Tensor, *,
+        window_size: int = 1024, sm_scale: Optional[float] = None,
+        key_weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Routed decode step over an 8-bit cache: ``switch_gqa_decode_forward`` with
+    ``cache`` (``SwitchKVCache``) in the place of the bf16 caches.
+
+    With ``key_weights`` (fp32 ``[B, Hkv, L]``) each attended key's softmax
+    weight, summed over the query heads of its KV head, is added there in
+    place; other entries keep their value.  A sequence without keys gives O =
+    NaN and LSE = -inf and adds nothing.
+    """
+    squeeze = q.ndim == 3
+    if squeeze:
+        q = q.unsqueeze(1)
+    check_cache(cache)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("Switch Attention decode requires BF16 Q")
+    if not q.is_contiguous():
+        raise ValueError("Q must be contiguous")
+    if q.ndim != 4 or q.shape[1] != 1 or q.shape[3] != 128:
+        raise ValueError("q must be [B,1,Hq,128]")
+    batch, _, heads, dim = (int(x) for x in q.shape)
+    if cache.k.shape[0] != batch:
+        raise ValueError("Q and KV cache batch sizes must match")
+    kv_heads = int(cache.k.shape[2])
+    if heads == 0 or heads % kv_heads or heads // kv_heads > 8:
+        raise ValueError("query heads must be a multiple (at most 8x) of KV heads")
+    if window_size <= 0:
+        raise ValueError("window_size must be positive")
+    dev = cache.k.device
+    if q.device != dev:
+        raise ValueError("Q and KV cache must be on the same device")
+    lens = check_lens(cache_lens, batch, dev, "cache_lens")
+    if full_mask.dtype != torch.bool or full_mask.shape != (batch,) or full_mask.device != dev:
+        raise ValueError("full_mask must be a bool [B] tensor on the device of Q")
+    if key_weights is not None:
+        check_weights(key_weights, cache)
+    scale = ((1.0 / dim) ** 0.5 if sm_scale is None else float(sm_scale)) * LOG2E
+    with _lib.on_device(dev):
+        out, lse = _lib.native().cache_decode(q, cache.k, cache.v, cache.k_scales, cache.v_scales,
+                                              lens, full_mask.contiguous(), key_weights,
+                                              int(window_size), cache.block_size,
+                                              _CODES[cache.k.dtype], scale,
+                                              _lib.stream_handle(dev), _lib.like(q))
     if squeeze:
         return out[:, 0], lse[:, 0]
     return out, lse
