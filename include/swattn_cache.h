@@ -95,6 +95,29 @@ int swattn_cache_decode_fwd(const void* q, const void* k, const void* v, const f
                             void* stream);
 
 /*
+ * The attention weight that each key received from a prefill's queries:
+ *   key_weights[b][h][j] = sum over listed rows r that may see key j and over
+ *                          the query heads of KV head h of 2^(c q_r.k_j - LSE_r)
+ * (0 for a key that no row sees).  q, k, the lists, the metadata bounds, the
+ * shapes, window and scale_log2 are those of swattn_prefill_fwd and lse is its
+ * result.  Each list's key bounds must be non-decreasing along the list, as
+ * for swattn_prefill_bwd.  scale_log2 must be finite.
+ *   key_weights  fp32 [batch, heads_kv, seq_kv]; every entry is written
+ *   workspace    >= swattn_prefill_key_weights_workspace_bytes(), 256-byte aligned
+ */
+size_t swattn_prefill_key_weights_workspace_bytes(int32_t batch, int64_t seq_kv, int32_t heads_q,
+                                                  int32_t heads_kv, int32_t head_dim,
+                                                  int64_t n_full, int64_t n_local);
+int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
+                               const int32_t* full_idx, int64_t n_full, const int32_t* local_idx,
+                               int64_t n_local, const int32_t* full_starts,
+                               const int32_t* local_starts, const int32_t* causal_ends,
+                               float* key_weights, int32_t batch, int64_t seq_q, int64_t seq_kv,
+                               int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                               int32_t window, float scale_log2, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
  * Evict: copy what a budget keeps of each sequence into another cache.  For a
  * sequence of n = cache_lens[b] rows and each KV head on its own: all rows if
  * n <= budget, else the newest `recent` rows and those budget - recent of the

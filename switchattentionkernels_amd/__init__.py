@@ -24,6 +24,7 @@ from .cache import (  # noqa: F401
     switch_kv_cache_read,
 )
 from .decode import switch_gqa_decode_forward, switch_gqa_decode_quantized_forward  # noqa: F401
+from .weights import switch_gqa_prefill_key_weights  # noqa: F401
 from .backward import (  # noqa: F401
     SwitchGQAPrefillFunction,
     switch_gqa_prefill,
@@ -48,6 +49,7 @@ __all__ = [
     "switch_kv_cache_read",
     "switch_gqa_decode_quantized_forward",
     "switch_kv_cache_evict",
+    "switch_gqa_prefill_key_weights",
     "switch_gqa_prefill_backward",
     "switch_gqa_prefill",
     "switch_gqa_prefill_varlen",

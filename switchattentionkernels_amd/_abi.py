@@ -56,6 +56,12 @@ CACHE_SIGNATURES = {
     "swattn_cache_decode_fwd": (ctypes.c_int, [_vp] * 10 + [_i32, _i64, _i32, _i32, _i32, _i32,
                                                             _i32, _i32, ctypes.c_float, _vp,
                                                             ctypes.c_size_t, _vp]),
+    "swattn_prefill_key_weights_workspace_bytes": (ctypes.c_size_t, [_i32, _i64, _i32, _i32, _i32,
+                                                                     _i64, _i64]),
+    "swattn_prefill_key_weights": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp,
+                                                  _vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32,
+                                                  _i32, ctypes.c_float, _vp, ctypes.c_size_t,
+                                                  _vp]),
     "swattn_cache_evict_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i64]),
     "swattn_cache_evict": (ctypes.c_int, [_vp] * 12 + [_i32, _i64, _i64, _i32, _i32, _i32, _i32,
                                                        _i64, _i64, _vp, ctypes.c_size_t, _vp]),

@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libswattn.so")
 ARCH = "gfx950"
 
 SOURCES = ["swattn_index.hip", "swattn_fwd.hip", "swattn_merge.hip", "swattn_decode.hip",
-           "swattn_cache.hip", "swattn_cache_decode.hip",
+           "swattn_cache.hip", "swattn_cache_decode.hip", "swattn_weights.hip",
            "swattn_bwd.hip"]
 # The measurement probe bench.py uses, in a library of its own (not part of the
 # attention library's ABI).

@@ -283,6 +283,29 @@ std::tuple<Tensor, Tensor> cache_decode(const Tensor& q, const Tensor& k, const 
   return {out, lse};
 }
 
+Tensor prefill_key_weights(const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& full,
+                           const Tensor& local, const optional<Tensor>& full_starts,
+                           const optional<Tensor>& local_starts, const optional<Tensor>& causal_ends,
+                           int64_t window, double scale_log2, int64_t stream) {
+  const CacheShape c(k);
+  const int32_t hq = static_cast<int32_t>(q.size(2));
+  const int64_t nf = full.numel(), nl = local.numel();
+  const Tensor out = at::empty({k.size(0), k.size(2), k.size(1)}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes = swattn_prefill_key_weights_workspace_bytes(c.batch, c.len, hq, c.hkv, c.dim, nf, nl);
+  const Tensor ws = bytes(q, ws_bytes > 0 ? ws_bytes : 1);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_prefill_key_weights(q.const_data_ptr(), k.const_data_ptr(), f32(lse), i32(full), nf, i32(local),
+                                        nl, i32(full_starts), i32(local_starts), i32(causal_ends),
+                                        out.data_ptr<float>(), c.batch, q.size(1), c.len, hq, c.hkv, c.dim,
+                                        static_cast<int32_t>(window), static_cast<float>(scale_log2),
+                                        ws.data_ptr(), ws_bytes, as_stream(stream));
+  }
+  check(status, "swattn_prefill_key_weights");
+  return out;
+}
+
 // The new lengths.
 Tensor cache_evict(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,
                    const Tensor& weights, const Tensor& lens, const Tensor& out_k, const Tensor& out_v,
@@ -318,5 +341,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cache_append", &cache_append);
   m.def("cache_read", &cache_read);
   m.def("cache_decode", &cache_decode);
+  m.def("prefill_key_weights", &prefill_key_weights);
   m.def("cache_evict", &cache_evict);
 }

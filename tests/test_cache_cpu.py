@@ -102,6 +102,31 @@ def test_c_abi_refusals():
     assert L.swattn_cache_evict_workspace_bytes(0, 2, 5) == 0
 
 
+def test_c_abi_refusals_of_the_key_weights():
+    L = _lib.lib()
+
+    def call(batch=1, sq=8, skv=8, hq=4, hkv=2, dim=128, window=4, nf=3, nl=5, q=P, k=P, starts=None,
+             ws=P, size=1 << 30, scale=F):
+        return L.swattn_prefill_key_weights(q, k, P, P, nf, P, nl, starts, None, None, P, batch, sq, skv, hq, hkv,
+                                            dim, window, scale, ws, size, None)
+
+    need = L.swattn_prefill_key_weights_workspace_bytes(1, 8, 4, 2, 128, 3, 5)
+    assert need > 0 and L.swattn_prefill_key_weights_workspace_bytes(1, 8, 5, 2, 128, 3, 5) == 0
+    _refused(call(dim=64), "head_dim")
+    _refused(call(skv=0), "bad shape")
+    _refused(call(hq=5), "multiple")
+    _refused(call(window=0), "window")
+    _refused(call(scale=ctypes.c_float(math.nan)), "finite")
+    _refused(call(nf=4), "index counts")
+    _refused(call(nf=-1), "index counts")
+    _refused(call(sq=2 ** 40, nf=2 ** 40), "2^31")
+    _refused(call(starts=P), "metadata")
+    _refused(call(q=None), "null")
+    _refused(call(k=ctypes.c_void_p(264)), "16-byte")
+    _refused(call(size=need - 1), "workspace", -2)
+    _refused(call(ws=ctypes.c_void_p(272)), "256-byte")
+
+
 def _cache(b=2, n=40, h=2, dtype=torch.int8, block=16):
     s = (b, h, -(-n // block))
     return SwitchKVCache(torch.zeros(b, n, h, 128, dtype=dtype), torch.zeros(b, n, h, 128, dtype=dtype),
@@ -273,6 +298,7 @@ def test_oracle_decode_against_a_loop():
 def test_public_names():
     import switchattentionkernels_amd as swa
     for name in ("SwitchKVCache", "build_switch_kv_cache", "switch_kv_cache_append", "switch_kv_cache_read",
-                 "switch_gqa_decode_quantized_forward", "switch_kv_cache_evict"):
+                 "switch_gqa_decode_quantized_forward", "switch_kv_cache_evict",
+                 "switch_gqa_prefill_key_weights"):
         assert name in swa.__all__ and hasattr(swa, name)
     assert cache_module.BLOCK_SIZES == (16, 32, 64, 128) and decode.LOG2E == math.log2(math.e)
