@@ -13,6 +13,18 @@
 // (column) and a key's sum into a register: a multiply-add, an exponential and
 // an addition per pair, and the sum over lanes only once, at the end.
 //
+// Bound by the matrix cores and the vector ALUs together: per 32 rows and 64 keys
+// a wave has 512 cycles of MFMA and about 560 of vector instructions (8 each for
+// the 32 exponentials), which overlap between the two waves of a SIMD and between
+// one product and the sums of the one before.  Where every row sees every key
+// (S8192 Hq32/Hkv8) it runs at 1030 TFLOP/s of its 2 D flops per pair; with the
+// loads and barriers taken out at 1150, the products alone at 1400, a large matrix
+// product's rate.  S16384 Hq32/Hkv8 W1024 p_full 0.25: 450 us, 832 TFLOP/s; what
+// lies between are blocks that a wave's keys see in part (a seventh of the local
+// ones) or not at all, and the workgroups' starts.  One block per barrier, fetched
+// one ahead, took 570 us; two ahead 495; the final sum by lane moves instead of
+// shuffles through LDS 477; no workgroups without work 463.
+//
 // Rows may be cut: the blocks of both lists form one axis (full first), cut at
 // multiples of `chunk` blocks, and a workgroup takes the blocks of one chunk that
 // its keys are seen by, so that workgroups of different keys read the same rows
@@ -40,13 +52,17 @@ constexpr int kWaveKeys = 64;                    // two 32-key MFMA tiles
 constexpr int kKeys = kWaves * kWaveKeys;        // per workgroup
 constexpr int kRows = 32;                        // per block
 constexpr int kBlockBytes = kRows * kRowBytes;   // 8 KiB of Q in LDS
-constexpr int kSlots = 2;
-// Row info, per block: 32 LSEs, 32 first keys, 32 key ends, 32 element offsets in
-// Q (-1: a row that contributes nothing), and the block's {largest first key,
-// smallest end, smallest first key, largest end}.
-constexpr int kInfoBytes = 768;
-constexpr int kInfoLse = 0, kInfoStart = 32, kInfoEnd = 64, kInfoAll = 160;   // words
-constexpr int kInfoOff = 48;                                                  // int64s
+// Row info, per block: 32 LSEs, 32 first keys, 32 key ends, 32 rows of Q (pos * hq
+// + head), and the block's {largest first key, smallest end, smallest first key,
+// largest end}.  A row that contributes nothing has no keys and forces the mask
+// on its block.
+constexpr int kInfoBytes = 576;
+constexpr int kInfoLse = 0, kInfoStart = 32, kInfoEnd = 64, kInfoRow = 96, kInfoAll = 128;   // words
+constexpr int kInfoLanes = (kInfoAll * 4 + 16) / 16;   // 16-byte pieces that are read
+// LDS rings, in pairs of blocks: Q is fetched two pairs ahead, info three.
+constexpr int kQSlots = 3, kInfoSlots = 4;
+constexpr int kPairBytes = 2 * kBlockBytes, kInfoPairBytes = 2 * 1024;
+constexpr int kWaitButFour = kWaitVmcnt0 | 4;   // s_waitcnt vmcnt(4)
 
 struct WeightParams {
   const uint16_t* q;
@@ -60,7 +76,6 @@ struct WeightParams {
   int32_t nrows[2];          // count * group
   int32_t blocks[2];
   char* info;                // [hkv][blocks[0] + blocks[1]] kInfoBytes
-  uint16_t* zero_row;        // 128 zeros: the source of rows that contribute nothing
   int32_t* ranges;           // [2][tiles][2]: the blocks of each list that see a key tile
   float* part;               // [tile][hkv][chunks][256]
   int32_t tiles, chunk, chunks, prep_wgs;
@@ -80,8 +95,6 @@ __device__ __forceinline__ void prep_rows(const WeightParams& p, int wg) {
   const int per_head = (nblk + 7) >> 3;
   const int kvh = wg / per_head;
   const int blk = (wg - kvh * per_head) * 8 + (threadIdx.x >> 5);
-  if (wg == 0 && threadIdx.x < kRowBytes / 16)
-    reinterpret_cast<uint4*>(p.zero_row)[threadIdx.x] = make_uint4(0, 0, 0, 0);
   const int rr = threadIdx.x & 31;
   const bool in = blk < nblk;
   const int b = blk < p.blocks[0] ? 0 : 1;
@@ -114,7 +127,7 @@ __device__ __forceinline__ void prep_rows(const WeightParams& p, int wg) {
   words[kInfoLse + rr] = live ? p.lse[row] : 0.f;
   ints[kInfoStart + rr] = live ? ks : 0;
   ints[kInfoEnd + rr] = live ? ke : 0;
-  reinterpret_cast<int64_t*>(inf)[kInfoOff + rr] = live ? row * kD : -1;
+  ints[kInfoRow + rr] = live ? static_cast<int>(row) : 0;
   if (rr == 0) *reinterpret_cast<int4*>(ints + kInfoAll) = make_int4(max_start, min_end, min_start, max_end);
 }
 
@@ -128,35 +141,48 @@ __global__ __launch_bounds__(kThreads) void weights_prep_kernel(const WeightPara
     block_ranges<kMeta, kKeys, kRows>(p, p.tiles, wg - p.prep_wgs);
 }
 
-// The blocks of chunk s, on the axis of both lists, that see tile t: [a, a_end)
-// of the full list, then [b, b_end) of the local one.
+// The x-th workgroup of key tile t: the chunk it takes and the blocks of that
+// chunk, on the axis of both lists, that see the tile: [a, a_end) of the full
+// list, then [b, b_end) of the local one.  Chunks of the full list come from its
+// end on, which every tile shares.
 struct Share {
-  int a, a_end, b, b_end;
+  int chunk, a, a_end, b, b_end;
 };
-__device__ __forceinline__ Share chunk_share(const WeightParams& p, int t, int s) {
-  const int lo = s * p.chunk, hi = lo + p.chunk;
-  const int32_t* f = p.ranges + 2 * t;
-  const int32_t* l = p.ranges + 2 * (p.tiles + t);
-  Share x;
-  x.a = max(f[0], lo);
-  x.a_end = max(min(f[1], hi), x.a);
-  x.b = max(l[0] + p.blocks[0], lo);
-  x.b_end = max(min(l[1] + p.blocks[0], hi), x.b);
-  return x;
+__device__ __forceinline__ bool chunk_share(const WeightParams& p, int t, int x, Share& sh) {
+  const int2 f = *reinterpret_cast<const int2*>(p.ranges + 2 * t);
+  int2 l = *reinterpret_cast<const int2*>(p.ranges + 2 * (p.tiles + t));
+  l.x += p.blocks[0];
+  l.y += p.blocks[0];
+  const int f_last = f.x < f.y ? (f.y - 1) / p.chunk : -1, f_first = f.x < f.y ? f.x / p.chunk : 0;
+  const int nf = f_last - f_first + 1;
+  if (x < nf) {
+    sh.chunk = f_last - x;
+  } else {
+    if (l.x >= l.y) return false;
+    sh.chunk = max(l.x / p.chunk, f_last + 1) + (x - nf);
+    if (sh.chunk > (l.y - 1) / p.chunk) return false;
+  }
+  const int lo = sh.chunk * p.chunk, hi = lo + p.chunk;
+  sh.a = max(f.x, lo);
+  sh.a_end = max(min(f.y, hi), sh.a);
+  sh.b = max(l.x, lo);
+  sh.b_end = max(min(l.y, hi), sh.b);
+  return true;
 }
 
-// One workgroup per (chunk, key tile, KV head), KV head fastest.
+// One workgroup per (share, key tile, KV head), KV head fastest.
 __global__ __launch_bounds__(kThreads, 2) void weights_kernel(const WeightParams p) {
-  __shared__ __align__(16) char smem[kSlots * kBlockBytes];
+  __shared__ __align__(16) char smem[kQSlots * kPairBytes + kInfoSlots * kInfoPairBytes];
   const int kvh = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
-  const int t = rest % p.tiles, s = rest / p.tiles;
-  const Share sh = chunk_share(p, t, s);
-  const int na = sh.a_end - sh.a, n = na + sh.b_end - sh.b;
-  if (n <= 0) return;   // uniform
+  const int t = rest % p.tiles;
+  Share sh;
+  if (!chunk_share(p, t, rest / p.tiles, sh)) return;   // uniform
+  const int na = sh.a_end - sh.a, n = na + sh.b_end - sh.b;   // at least 1
   auto block_at = [&](int i) { return i < na ? sh.a + i : sh.b + (i - na); };
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto uniform = [](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))); };
+  const int wave = static_cast<int>(uniform(tid >> 6));
   const int r = lane & 31, hh = lane >> 5;
   const int key0 = t * kKeys + wave * kWaveKeys;
   // K operands: key r of each 32-key tile, dims 16 x + 8 hh .. +7.
@@ -168,100 +194,150 @@ __global__ __launch_bounds__(kThreads, 2) void weights_kernel(const WeightParams
 #pragma unroll
     for (int x = 0; x < 8; ++x) kf[u][x] = *reinterpret_cast<const bf16x8*>(row + 16 * x);
   }
-  // Staging: this wave's two 1 KiB loads of a block, four rows each; LDS chunk
-  // position lane % 16 of row rr takes the row's chunk (lane % 16) ^ swz(rr).
-  const int stage_row = 8 * wave + (lane >> 4);
-  const uint32_t lds0 = lds_addr(smem) + wave * 2048;
-  auto offsets = [&](int i, int64_t (&off)[2]) {
-    const int64_t* o = reinterpret_cast<const int64_t*>(block_info(p, kvh, block_at(min(i, n - 1)))) + kInfoOff;
-    off[0] = o[stage_row];
-    off[1] = o[stage_row + 4];
+  // Staging.  Waves 0 and 1 fetch the info of a pair's blocks; every wave 16 of its
+  // 64 rows, four per 1 KiB load: LDS chunk position lane % 16 of row rr takes the
+  // row's chunk (lane % 16) ^ swz(rr).
+  char* const s_info = smem + kQSlots * kPairBytes;
+  auto stage_info = [&](int i) {
+    if (wave < 2 && lane < kInfoLanes)
+      dma16_gather(block_info(p, kvh, block_at(min(2 * i + wave, n - 1))) + 16 * lane,
+                   uniform(lds_addr(s_info) + (i % kInfoSlots) * kInfoPairBytes + wave * 1024));
   };
-  auto stage = [&](int i, const int64_t (&off)[2]) {
+  const int stage_row = 16 * (wave & 1) + (lane >> 4);   // of block wave / 2
+  auto stage_rows = [&](int i) {
+    const int* rows = reinterpret_cast<const int*>(s_info + (i % kInfoSlots) * kInfoPairBytes + (wave >> 1) * 1024) + kInfoRow;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int c = (lane & 15) ^ swz(stage_row + 4 * x);
-      const uint16_t* src = (off[x] >= 0 ? p.q + off[x] : p.zero_row) + 8 * c;
-      dma16_gather(src, lds0 + (i % kSlots) * kBlockBytes + 1024 * x);
+    for (int x = 0; x < 4; ++x) {
+      const int rr = stage_row + 4 * x;
+      const uint16_t* src = p.q + static_cast<int64_t>(rows[rr]) * kD + 8 * ((lane & 15) ^ swz(rr));
+      dma16_gather(src, uniform(lds_addr(smem) + (i % kQSlots) * kPairBytes + wave * 4096 + 1024 * x));
     }
   };
-  struct RowInfo {
-    float lse;
-    int ks, ke;
-    int4 all;
-  };
-  auto row_info = [&](int i) {
-    const int* w = reinterpret_cast<const int*>(block_info(p, kvh, block_at(min(i, n - 1))));
-    RowInfo x;
-    x.lse = __int_as_float(w[kInfoLse + r]);
-    x.ks = w[kInfoStart + r];
-    x.ke = w[kInfoEnd + r];
-    x.all = *reinterpret_cast<const int4*>(w + kInfoAll);
-    return x;
-  };
-  int64_t off[2];
-  offsets(0, off);
-  stage(0, off);
-  offsets(1, off);
-  RowInfo next = row_info(0);
+  stage_info(0);
+  stage_info(1);
+  stage_info(2);
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+  __syncthreads();
+  stage_rows(0);
+  stage_rows(1);
   f32x16 sum[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int x = 0; x < 16; ++x) sum[u][x] = 0.f;
-  for (int i = 0; i < n; ++i) {
-    // This wave's part of block i is there, and after the barrier all of it; the
-    // slot of block i + 1 was last read for block i - 1, before the barrier.
-    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+  auto product = [&](int u, const bf16x8 (&q)[8], f32x16& d) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) d[x] = 0.f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][x], q[x], d, 0, 0, 0);
+  };
+  auto add = [&](int u, float row_lse, const f32x16& d) {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) sum[u][x] += __builtin_amdgcn_exp2f(__builtin_fmaf(d[x], p.c, -row_lse));
+  };
+  // The last product of a pair is summed up beside the next pair's first: d1, of
+  // rows with LSE lse_p (infinite: nothing left to sum).
+  f32x16 d0, d1;
+  float lse_p = INFINITY;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) d1[x] = 0.f;
+  const int pairs = (n + 1) >> 1;
+  for (int i = 0; i < pairs; ++i) {
+    // All but this wave's last four loads (rows of pair i + 1) are there: its rows
+    // of pair i and its info of pair i + 2; after the barrier, everyone's.  Pair
+    // i - 1's rows and info, whose slots are filled next, were last read before it.
+    __builtin_amdgcn_s_waitcnt(kWaitButFour);
     __syncthreads();
-    const RowInfo info = next;
-    if (i + 1 < n) {
-      stage(i + 1, off);
-      offsets(i + 2, off);
-      next = row_info(i + 1);
+    stage_info(i + 3);
+    const char* inf = s_info + (i % kInfoSlots) * kInfoPairBytes;
+    int4 all[2];
+    float lse[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      all[y] = *reinterpret_cast<const int4*>(inf + 1024 * y + 4 * kInfoAll);
+      lse[y] = reinterpret_cast<const float*>(inf + 1024 * y)[kInfoLse + r];
     }
-    const int max_start = __builtin_amdgcn_readfirstlane(info.all.x), min_end = __builtin_amdgcn_readfirstlane(info.all.y);
-    const int min_start = __builtin_amdgcn_readfirstlane(info.all.z), max_end = __builtin_amdgcn_readfirstlane(info.all.w);
-    if (max_end <= key0 || min_start >= key0 + kWaveKeys) continue;   // none of this wave's keys
-    const char* blk = smem + (i % kSlots) * kBlockBytes + r * kRowBytes;
+    bool none[2], whole[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int max_start = __builtin_amdgcn_readfirstlane(all[y].x), min_end = __builtin_amdgcn_readfirstlane(all[y].y);
+      const int min_start = __builtin_amdgcn_readfirstlane(all[y].z), max_end = __builtin_amdgcn_readfirstlane(all[y].w);
+      none[y] = max_end <= key0 || min_start >= key0 + kWaveKeys || 2 * i + y >= n;
+      whole[y] = max_start <= key0 && min_end >= key0 + kWaveKeys && 2 * i + y < n;
+    }
+    const char* slot = smem + (i % kQSlots) * kPairBytes + r * kRowBytes;
+    auto q_at = [&](int y, int x) { return *reinterpret_cast<const bf16x8*>(slot + y * kBlockBytes + 16 * ((2 * x + hh) ^ swz(r))); };
     bf16x8 qf[8];
+    if (whole[0] && whole[1]) {   // every row sees every key
 #pragma unroll
-    for (int x = 0; x < 8; ++x) qf[x] = *reinterpret_cast<const bf16x8*>(blk + 16 * ((2 * x + hh) ^ swz(r)));
-    f32x16 d[2];
+      for (int x = 0; x < 8; ++x) qf[x] = q_at(0, x);
+      stage_rows(i + 2);
+      product(0, qf, d0);
+      add(1, lse_p, d1);
+      product(1, qf, d1);
+      add(0, lse[0], d0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x) d[u][x] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) d[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[u][x], qf[x], d[u], 0, 0, 0);
+      for (int x = 0; x < 8; ++x) qf[x] = q_at(1, x);
+      product(0, qf, d0);
+      add(1, lse[0], d1);
+      product(1, qf, d1);
+      add(0, lse[1], d0);
+      lse_p = lse[1];
+      continue;
     }
-    if (max_start <= key0 && min_end >= key0 + kWaveKeys) {   // every row sees every key
+    stage_rows(i + 2);
+    add(1, lse_p, d1);   // what the last pair left
+    lse_p = INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int y = 0; y < 2; ++y) {
+      if (none[y]) continue;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) sum[u][x] += __builtin_amdgcn_exp2f(__builtin_fmaf(d[u][x], p.c, -info.lse));
-    } else {
+      for (int x = 0; x < 8; ++x) qf[x] = q_at(y, x);
+      if (whole[y]) {
+        product(0, qf, d0);
+        product(1, qf, d1);
+        add(0, lse[y], d0);
+        add(1, lse[y], d1);
+        continue;
+      }
+      const int ks = reinterpret_cast<const int*>(inf + 1024 * y)[kInfoStart + r];
+      const int ke = reinterpret_cast<const int*>(inf + 1024 * y)[kInfoEnd + r];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        product(u, qf, d0);
+        const int first = ks - key0 - 32 * u - 4 * hh;
+        const uint32_t keys = ke - ks;
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const int key = key0 + 32 * u + 8 * (x >> 2) + 4 * hh + (x & 3);
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(d[u][x], p.c, -info.lse));
-          sum[u][x] += key >= info.ks && key < info.ke ? w : 0.f;
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(d0[x], p.c, -lse[y]));
+          sum[u][x] += static_cast<uint32_t>(8 * (x >> 2) + (x & 3) - first) < keys ? w : 0.f;
         }
+      }
     }
+#pragma unroll
+    for (int x = 0; x < 16; ++x) d1[x] = 0.f;
   }
-  // Sums over the 32 row lanes; lane 0 of each half holds its keys'.
-  float* out = p.part + ((static_cast<int64_t>(t) * p.hkv + kvh) * p.chunks + s) * kKeys + wave * kWaveKeys;
+  add(1, lse_p, d1);
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);   // no load into LDS outlives the workgroup
+  // Sums over the 32 row lanes, with lane moves only: neighbours, pairs, the mirror
+  // image within 8 and 16 lanes, and the other 16.
+  float* out = p.part + ((static_cast<int64_t>(t) * p.hkv + kvh) * p.chunks + sh.chunk) * kKeys + wave * kWaveKeys;
+  float mine = 0.f;   // lane r: element r % 16 of tile r / 16
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
+      constexpr int kMoves[4] = {0xB1, 0x4E, 0x141, 0x140};
       float w = sum[u][x];
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) w += __shfl_xor(w, o);
-      if (r == 0) out[32 * u + 8 * (x >> 2) + 4 * hh + (x & 3)] = w;
+      w += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w), kMoves[0], 0xf, 0xf, false));
+      w += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w), kMoves[1], 0xf, 0xf, false));
+      w += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w), kMoves[2], 0xf, 0xf, false));
+      w += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(w), kMoves[3], 0xf, 0xf, false));
+      const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(w), __float_as_uint(w), false, false);
+      w = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+      mine = r == 16 * u + x ? w : mine;
     }
+  out[32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * hh + (r & 3)] = mine;
 }
 
 // The chunks' sums, in their order: one workgroup per (key tile, KV head), a thread
@@ -290,11 +366,13 @@ __global__ __launch_bounds__(kThreads) void weights_reduce_kernel(const WeightPa
 
 struct Layout {
   int64_t tiles, blocks[2], chunk, chunks;
-  size_t off_zero, off_ranges, off_part, bytes;
+  size_t off_ranges, off_part, bytes;
 };
 
 // Chunks: short enough that the workgroups outnumber the chip's slots several
-// times over, long enough that the partial sums stay small.
+// times over, long enough that the partial sums stay small.  (S16384: 64 blocks
+// 450 us, 32 472, 96 467, 128 462, 192 458; S8192 of 5 heads per KV head 230, 228,
+// 229, 261, 247.)
 constexpr int64_t kMinChunk = 8;
 constexpr int64_t kMaxChunk = 64;
 constexpr int64_t kWantWgs = 4096;                // workgroups, if all chunks had blocks
@@ -313,7 +391,6 @@ Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full,
   L.chunks = ceil_div(axis, L.chunk);
   auto al = [](size_t x) { return (x + 255) & ~size_t{255}; };
   size_t o = al(static_cast<size_t>(axis * heads_kv) * kInfoBytes);
-  L.off_zero = o;    o += kRowBytes;
   L.off_ranges = o;  o = al(o + static_cast<size_t>(2 * L.tiles) * 2 * sizeof(int32_t));
   L.off_part = o;    o = al(o + static_cast<size_t>(pairs * L.chunks) * kKeys * sizeof(float));
   L.bytes = o;
@@ -359,6 +436,7 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
     return invalid(n + ": bad index counts");
   const int64_t group = heads_q / heads_kv;
   if ((n_full + n_local) * group > INT32_MAX - 2 * kRows) return invalid(n + ": too many rows");
+  if (total_q * heads_q > INT32_MAX) return invalid(n + ": more than 2^31 - 1 rows of Q");
   const bool meta = full_starts != nullptr || local_starts != nullptr || causal_ends != nullptr;
   if (meta && (full_starts == nullptr || local_starts == nullptr || causal_ends == nullptr))
     return invalid(n + ": metadata needs full_starts, local_starts and causal_ends");
@@ -373,7 +451,15 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
     return SWATTN_EWORKSPACE;
   }
   if (!aligned256(workspace)) return invalid(n + ": workspace must be 256-byte aligned");
-  const int64_t pairs = L.tiles * heads_kv, grid = pairs * L.chunks;
+  // Workgroups per tile: chunks of the full list, and of the local rows that can see
+  // a tile: window - 1 positions more than its keys, for each sequence in it.
+  int64_t local = L.blocks[1];
+  if (!meta) {
+    const int64_t reach = std::min<int64_t>(window, seq_q), parts = kKeys / seq_kv + 2;
+    local = std::min(local, (kKeys + parts * reach) * group / kRows + 2);
+  }
+  const int64_t shares = std::min(L.chunks, ceil_div(L.blocks[0], L.chunk) + ceil_div(local, L.chunk) + 1);
+  const int64_t pairs = L.tiles * heads_kv, grid = pairs * std::max<int64_t>(shares, 1);
   const int64_t prep = ceil_div(L.blocks[0] + L.blocks[1], 8) * heads_kv, ranges = ceil_div(2 * L.tiles, kThreads / 64);
   if (grid > INT32_MAX || prep + ranges > INT32_MAX) return invalid(n + ": grid too large");
   char* ws = static_cast<char*>(workspace);
@@ -394,7 +480,6 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
     p.blocks[b] = static_cast<int32_t>(L.blocks[b]);
   }
   p.info = ws;
-  p.zero_row = reinterpret_cast<uint16_t*>(ws + L.off_zero);
   p.ranges = reinterpret_cast<int32_t*>(ws + L.off_ranges);
   p.part = reinterpret_cast<float*>(ws + L.off_part);
   p.tiles = static_cast<int32_t>(L.tiles);

@@ -120,6 +120,7 @@ def test_c_abi_refusals_of_the_key_weights():
     _refused(call(nf=4), "index counts")
     _refused(call(nf=-1), "index counts")
     _refused(call(sq=2 ** 40, nf=2 ** 40), "2^31")
+    _refused(call(sq=2 ** 29, nf=2, nl=2, size=1 << 60), "rows of Q")
     _refused(call(starts=P), "metadata")
     _refused(call(q=None), "null")
     _refused(call(k=ctypes.c_void_p(264)), "16-byte")
