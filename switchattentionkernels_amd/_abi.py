@@ -73,6 +73,10 @@ INTERNAL_SIGNATURES = {
                                            ctypes.c_size_t, _vp]),
     "swattn_build_metadata_host": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32,
                                                   _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "swattn_prefill_key_weights_checked": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
+                                                          _vp, _vp, _vp, _i32, _i64, _i64, _i32,
+                                                          _i32, _i32, _i32, ctypes.c_float, _vp,
+                                                          ctypes.c_size_t, _vp, _vp, _vp]),
     "swattn_check_bounds": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
 }
 

@@ -48,16 +48,20 @@ const int32_t* i32(const optional<Tensor>& t) { return t.has_value() ? i32(*t) :
 // waits for its counts before it returns, so that a thread has at most one
 // compaction in flight.  After a HIP error a kernel may still be queued that
 // reports there: the buffer is then left to it for good.
-thread_local c10::DataPtr t_words;
-int32_t* host_words() {
-  if (!t_words)
-    t_words = at::getHostAllocator(at::kCUDA)->allocate(SWATTN_COMPACT_HOST_WORDS * sizeof(int32_t));
-  return static_cast<int32_t*>(t_words.get());
-}
-void abandon_host_words() {
-  (void)t_words.release_context();
-  t_words = c10::DataPtr();
-}
+template <int kWords>
+struct HostWords {
+  c10::DataPtr ptr;
+  int32_t* get() {
+    if (!ptr) ptr = at::getHostAllocator(at::kCUDA)->allocate(kWords * sizeof(int32_t));
+    return static_cast<int32_t*>(ptr.get());
+  }
+  void abandon() {
+    (void)ptr.release_context();
+    ptr = c10::DataPtr();
+  }
+};
+thread_local HostWords<SWATTN_COMPACT_HOST_WORDS> t_words;
+thread_local HostWords<SWATTN_KEY_WEIGHTS_HOST_WORDS> t_check_words;
 
 // (full, local) of a byte mask (dtype -1) or of router logits.
 std::tuple<Tensor, Tensor> compact(const Tensor& x, int64_t dtype, double threshold,
@@ -67,7 +71,7 @@ std::tuple<Tensor, Tensor> compact(const Tensor& x, int64_t dtype, double thresh
   const size_t ws_bytes = swattn_compact_workspace_bytes(n);
   Tensor ws;
   if (ws_bytes > 0) ws = bytes(x, ws_bytes);
-  int32_t* host = host_words();
+  int32_t* host = t_words.get();
   int status = 0;
   {
     pybind11::gil_scoped_release release;
@@ -76,7 +80,7 @@ std::tuple<Tensor, Tensor> compact(const Tensor& x, int64_t dtype, double thresh
                                  ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
                                  as_stream(stream));
   }
-  if (status > 0) abandon_host_words();
+  if (status > 0) t_words.abandon();
   check(status, dtype < 0 ? "swattn_compact" : "swattn_compact_logits");
   const int64_t nf = host[0];
   return {out.narrow(0, 0, nf), out.narrow(0, nf, n - nf)};
@@ -283,27 +287,38 @@ std::tuple<Tensor, Tensor> cache_decode(const Tensor& q, const Tensor& k, const 
   return {out, lse};
 }
 
-Tensor prefill_key_weights(const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& full,
+// With `unchecked` lists also their check's bits.
+std::tuple<Tensor, int64_t> prefill_key_weights(const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& full,
                            const Tensor& local, const optional<Tensor>& full_starts,
                            const optional<Tensor>& local_starts, const optional<Tensor>& causal_ends,
-                           int64_t window, double scale_log2, int64_t stream) {
+                           int64_t window, double scale_log2, bool unchecked, int64_t stream) {
   const CacheShape c(k);
   const int32_t hq = static_cast<int32_t>(q.size(2));
   const int64_t nf = full.numel(), nl = local.numel();
+  int32_t* host = unchecked ? t_check_words.get() : nullptr;
+  int32_t flags = 0;
   const Tensor out = at::empty({k.size(0), k.size(2), k.size(1)}, q.options().dtype(at::kFloat));
   const size_t ws_bytes = swattn_prefill_key_weights_workspace_bytes(c.batch, c.len, hq, c.hkv, c.dim, nf, nl);
   const Tensor ws = bytes(q, ws_bytes > 0 ? ws_bytes : 1);
   int status = 0;
   {
     pybind11::gil_scoped_release release;
-    status = swattn_prefill_key_weights(q.const_data_ptr(), k.const_data_ptr(), f32(lse), i32(full), nf, i32(local),
-                                        nl, i32(full_starts), i32(local_starts), i32(causal_ends),
-                                        out.data_ptr<float>(), c.batch, q.size(1), c.len, hq, c.hkv, c.dim,
-                                        static_cast<int32_t>(window), static_cast<float>(scale_log2),
-                                        ws.data_ptr(), ws_bytes, as_stream(stream));
+    const void *qp = q.const_data_ptr(), *kp = k.const_data_ptr();
+    const int32_t w = static_cast<int32_t>(window);
+    const float scale = static_cast<float>(scale_log2);
+    status = unchecked
+                 ? swattn_prefill_key_weights_checked(
+                       qp, kp, f32(lse), i32(full), nf, i32(local), nl, i32(full_starts), i32(local_starts),
+                       i32(causal_ends), out.data_ptr<float>(), c.batch, q.size(1), c.len, hq, c.hkv, c.dim, w,
+                       scale, ws.data_ptr(), ws_bytes, as_stream(stream), host, &flags)
+                 : swattn_prefill_key_weights(
+                       qp, kp, f32(lse), i32(full), nf, i32(local), nl, i32(full_starts), i32(local_starts),
+                       i32(causal_ends), out.data_ptr<float>(), c.batch, q.size(1), c.len, hq, c.hkv, c.dim, w,
+                       scale, ws.data_ptr(), ws_bytes, as_stream(stream));
   }
+  if (status > 0 && unchecked) t_check_words.abandon();
   check(status, "swattn_prefill_key_weights");
-  return out;
+  return {out, flags};
 }
 
 // The new lengths.

@@ -52,6 +52,27 @@ int swattn_check_bounds(const int32_t* full, int64_t n_full, const int32_t* loca
                         const int32_t* causal_ends, int64_t total_q, int32_t* flags,
                         void* stream);
 
+/*
+ * swattn_prefill_key_weights with the check of the lists (swattn_check_indices)
+ * in its first kernel: on return *flags holds the SWATTN_ERR_* bits, while the
+ * sums may still be running.  (With the check and its read-back ahead of the
+ * launches a call took 40 us more.)
+ *   host  SWATTN_KEY_WEIGHTS_HOST_WORDS int32 of pinned host memory, one call at
+ *         a time; after a HIP error (a positive status) not to be used again.
+ * A stream under capture is refused (SWATTN_EINVAL) before anything is launched.
+ */
+#define SWATTN_KEY_WEIGHTS_HOST_WORDS 1024
+int swattn_prefill_key_weights_checked(const void* q, const void* k, const float* lse,
+                                       const int32_t* full_idx, int64_t n_full,
+                                       const int32_t* local_idx, int64_t n_local,
+                                       const int32_t* full_starts, const int32_t* local_starts,
+                                       const int32_t* causal_ends, float* key_weights,
+                                       int32_t batch, int64_t seq_q, int64_t seq_kv,
+                                       int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                       int32_t window, float scale_log2, void* workspace,
+                                       size_t workspace_bytes, void* stream, int32_t* host,
+                                       int32_t* flags);
+
 #ifdef __cplusplus
 }  // extern "C"
 #endif

@@ -35,10 +35,13 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <string>
 
 #include "row_blocks.h"
 #include "swattn_cache.h"
+#include "swattn_internal.h"
 #include "tiles.h"
 
 namespace swattn {
@@ -78,7 +81,8 @@ struct WeightParams {
   char* info;                // [hkv][blocks[0] + blocks[1]] kInfoBytes
   int32_t* ranges;           // [2][tiles][2]: the blocks of each list that see a key tile
   float* part;               // [tile][hkv][chunks][256]
-  int32_t tiles, chunk, chunks, prep_wgs;
+  int32_t* host;             // pinned words that the lists' check reports to, one per workgroup, or null
+  int32_t tiles, chunk, chunks, prep_wgs, check_wgs;
   int32_t seq_q, seq_kv, total_q, total_kv;
   int32_t hq, hkv, group, window;
   float c;                   // sm_scale * log2(e)
@@ -131,11 +135,33 @@ __device__ __forceinline__ void prep_rows(const WeightParams& p, int wg) {
   if (rr == 0) *reinterpret_cast<int4*>(ints + kInfoAll) = make_int4(max_start, min_end, min_start, max_end);
 }
 
-// Row info and block ranges need nothing of each other: one launch.
+// The check of the lists, reported to a host that polls: the word carries the
+// answer itself and orders nothing else.
+constexpr int kReported = 1 << 30;
+__device__ __forceinline__ void check_lists(const WeightParams& p, int wg) {
+  int f = 0;
+  const int64_t n = max(p.count[0], p.count[1]);
+  for (int64_t i = static_cast<int64_t>(wg) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(p.check_wgs) * kThreads)
+    f |= list_flags(p.idx[0], p.count[0], p.idx[1], p.count[1], p.total_q, i);
+  __shared__ int s_flags[kThreads / 64];
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) f |= __shfl_xor(f, off);
+  if ((threadIdx.x & 63) == 0) s_flags[threadIdx.x >> 6] = f;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    __hip_atomic_store(p.host + wg, s_flags[0] | s_flags[1] | s_flags[2] | s_flags[3] | kReported,
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
+// The lists' check, row info and block ranges need nothing of each other: one
+// launch.
 template <bool kMeta>
 __global__ __launch_bounds__(kThreads) void weights_prep_kernel(const WeightParams p) {
-  const int wg = blockIdx.x;
-  if (wg < p.prep_wgs)
+  const int wg = static_cast<int>(blockIdx.x) - p.check_wgs;
+  if (wg < 0)
+    check_lists(p, blockIdx.x);
+  else if (wg < p.prep_wgs)
     prep_rows<kMeta>(p, wg);
   else
     block_ranges<kMeta, kKeys, kRows>(p, p.tiles, wg - p.prep_wgs);
@@ -397,31 +423,24 @@ Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full,
   return L;
 }
 
+// Workgroups that check the lists, each with a word to report to.
+int check_wgs(int64_t slots) {
+  return static_cast<int>(std::min<int64_t>(SWATTN_KEY_WEIGHTS_HOST_WORDS, ceil_div(slots, kThreads)));
+}
+
 }  // namespace
 }  // namespace swattn
 
 using namespace swattn;
 using namespace swattn::tiles;
 
-extern "C" {
-
-size_t swattn_prefill_key_weights_workspace_bytes(int32_t batch, int64_t seq_kv, int32_t heads_q,
-                                                  int32_t heads_kv, int32_t head_dim, int64_t n_full,
-                                                  int64_t n_local) {
-  if (batch < 1 || seq_kv < 1 || seq_kv > INT32_MAX || heads_q < 1 || heads_kv < 1 || heads_q % heads_kv ||
-      head_dim != kD || n_full < 0 || n_local < 0 || n_full > INT32_MAX || n_local > INT32_MAX)
-    return 0;
-  return layout(batch * seq_kv, heads_kv, heads_q / heads_kv, n_full, n_local).bytes;
-}
-
-int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
-                               const int32_t* full_idx, int64_t n_full, const int32_t* local_idx,
-                               int64_t n_local, const int32_t* full_starts,
-                               const int32_t* local_starts, const int32_t* causal_ends,
-                               float* key_weights, int32_t batch, int64_t seq_q, int64_t seq_kv,
-                               int32_t heads_q, int32_t heads_kv, int32_t head_dim,
-                               int32_t window, float scale_log2, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+// The checks and the launches; host: pinned words for the lists' check, or null.
+static int launch_key_weights(
+    const void* q, const void* k, const float* lse, const int32_t* full_idx, int64_t n_full,
+    const int32_t* local_idx, int64_t n_local, const int32_t* full_starts, const int32_t* local_starts,
+    const int32_t* causal_ends, float* key_weights, int32_t batch, int64_t seq_q, int64_t seq_kv,
+    int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t window, float scale_log2, void* workspace,
+    size_t workspace_bytes, void* stream, int32_t* host) {
   const std::string n("swattn_prefill_key_weights");
   if (head_dim != kD) return invalid(n + ": head_dim must be 128");
   if (batch < 1 || seq_q < 0 || seq_kv < 1 || heads_q < 1 || heads_kv < 1) return invalid(n + ": bad shape");
@@ -461,7 +480,7 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
   const int64_t shares = std::min(L.chunks, ceil_div(L.blocks[0], L.chunk) + ceil_div(local, L.chunk) + 1);
   const int64_t pairs = L.tiles * heads_kv, grid = pairs * std::max<int64_t>(shares, 1);
   const int64_t prep = ceil_div(L.blocks[0] + L.blocks[1], 8) * heads_kv, ranges = ceil_div(2 * L.tiles, kThreads / 64);
-  if (grid > INT32_MAX || prep + ranges > INT32_MAX) return invalid(n + ": grid too large");
+  if (grid > INT32_MAX || prep + ranges > INT32_MAX - SWATTN_KEY_WEIGHTS_HOST_WORDS) return invalid(n + ": grid too large");
   char* ws = static_cast<char*>(workspace);
   WeightParams p{};
   p.q = static_cast<const uint16_t*>(q);
@@ -496,7 +515,9 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
   p.window = window;
   p.c = scale_log2;
   const hipStream_t st = as_stream(stream);
-  const dim3 gp(static_cast<uint32_t>(prep + ranges));
+  p.host = host;
+  p.check_wgs = host == nullptr ? 0 : check_wgs(std::max(n_full, n_local));
+  const dim3 gp(static_cast<uint32_t>(p.check_wgs + prep + ranges));
   if (meta)
     hipLaunchKernelGGL(weights_prep_kernel<true>, gp, dim3(kThreads), 0, st, p);
   else
@@ -504,6 +525,74 @@ int swattn_prefill_key_weights(const void* q, const void* k, const float* lse,
   hipLaunchKernelGGL(weights_kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, st, p);
   hipLaunchKernelGGL(weights_reduce_kernel, dim3(static_cast<uint32_t>(pairs)), dim3(kThreads), 0, st, p);
   return launch_status(n.c_str());
+}
+
+extern "C" {
+
+size_t swattn_prefill_key_weights_workspace_bytes(int32_t batch, int64_t seq_kv, int32_t heads_q,
+                                                  int32_t heads_kv, int32_t head_dim, int64_t n_full,
+                                                  int64_t n_local) {
+  if (batch < 1 || seq_kv < 1 || seq_kv > INT32_MAX || heads_q < 1 || heads_kv < 1 || heads_q % heads_kv ||
+      head_dim != kD || n_full < 0 || n_local < 0 || n_full > INT32_MAX || n_local > INT32_MAX)
+    return 0;
+  return layout(batch * seq_kv, heads_kv, heads_q / heads_kv, n_full, n_local).bytes;
+}
+
+int swattn_prefill_key_weights(
+    const void* q, const void* k, const float* lse, const int32_t* full_idx, int64_t n_full,
+    const int32_t* local_idx, int64_t n_local, const int32_t* full_starts, const int32_t* local_starts,
+    const int32_t* causal_ends, float* key_weights, int32_t batch, int64_t seq_q, int64_t seq_kv,
+    int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t window, float scale_log2, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  return launch_key_weights(q, k, lse, full_idx, n_full, local_idx, n_local, full_starts, local_starts, causal_ends,
+                     key_weights, batch, seq_q, seq_kv, heads_q, heads_kv, head_dim, window, scale_log2,
+                     workspace, workspace_bytes, stream, nullptr);
+}
+
+int swattn_prefill_key_weights_checked(
+    const void* q, const void* k, const float* lse, const int32_t* full_idx, int64_t n_full,
+    const int32_t* local_idx, int64_t n_local, const int32_t* full_starts, const int32_t* local_starts,
+    const int32_t* causal_ends, float* key_weights, int32_t batch, int64_t seq_q, int64_t seq_kv,
+    int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t window, float scale_log2, void* workspace,
+    size_t workspace_bytes, void* stream, int32_t* host, int32_t* flags) {
+  const std::string n("swattn_prefill_key_weights");
+  if (host == nullptr || flags == nullptr) return invalid(n + ": null pointer");
+  *flags = 0;
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(as_stream(stream), &capture) == hipSuccess && capture != hipStreamCaptureStatusNone)
+    return invalid(n + ": waits for the check of the index lists and cannot be captured");
+  const int words = n_full < 0 || n_local < 0 ? 0 : check_wgs(std::max(n_full, n_local));
+  for (int i = 0; i < words; ++i) host[i] = 0;
+  const int status = launch_key_weights(q, k, lse, full_idx, n_full, local_idx, n_local, full_starts, local_starts,
+                                 causal_ends, key_weights, batch, seq_q, seq_kv, heads_q, heads_kv, head_dim,
+                                 window, scale_log2, workspace, workspace_bytes, stream, host);
+  if (status != SWATTN_OK) {
+    // After a HIP error a kernel may be queued all the same, and must not report
+    // into the next call's words.
+    if (status > 0) (void)hipStreamSynchronize(as_stream(stream));
+    return status;
+  }
+  // Poll for a while (the stream may hold any amount of earlier work, or have
+  // failed), then wait for the stream.
+  volatile int32_t* word = host;
+  const auto t0 = std::chrono::steady_clock::now();
+  int done = 0;
+  while (done < words) {
+    if (word[done] != 0) {
+      *flags |= word[done++] & ~kReported;
+      continue;
+    }
+    __builtin_ia32_pause();
+    if (std::chrono::steady_clock::now() - t0 > std::chrono::milliseconds(2)) break;
+  }
+  if (done == words) return SWATTN_OK;
+  const hipError_t e = hipStreamSynchronize(as_stream(stream));
+  if (e != hipSuccess) {
+    set_error(n + ": " + hipGetErrorString(e));
+    return static_cast<int>(e);
+  }
+  for (; done < words; ++done) *flags |= word[done] & ~kReported;
+  return SWATTN_OK;
 }
 
 }  // extern "C"

@@ -17,7 +17,8 @@ import torch
 from . import _lib
 from .backward import _check_monotone
 from .metadata import SwitchAttentionMetadata
-from .prefill import LOG2E, _check_lists, _check_metadata, check_qkv
+from .prefill import (ERR_OVERLAP, LOG2E, MSG_DISJOINT, _check_lists, _check_metadata,
+                      _is_untouched_compaction, _note_sync, _prepare_indices, _raise_for, check_qkv)
 
 
 def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor,
@@ -51,14 +52,30 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
         raise ValueError("sm_scale must be finite")
     if metadata is not None:
         _check_metadata(metadata, q_len, kv_len, q.device)
-    full, local = _check_lists(full_query_indices, local_query_indices, batch * q_len, q.device)
-    if metadata is not None:
-        _check_monotone(metadata, full, local)
-    if 0 in k.shape:
-        return torch.zeros(batch, k.shape[2], kv_len, dtype=torch.float32, device=q.device)
+    total_q, dev = batch * q_len, q.device
     fs, ls, ends = (None, None, None) if metadata is None else (
         metadata.full_starts, metadata.local_starts, metadata.causal_ends)
-    with _lib.on_device(q.device):
-        return _lib.native().prefill_key_weights(q, k, lse, full, local, fs, ls, ends,
-                                                 int(window_size), scale * LOG2E,
-                                                 _lib.stream_handle(q.device))
+    full, local, unchecked = full_query_indices, local_query_indices, False
+    if (metadata is None and 0 not in k.shape and full.ndim == 1 and local.ndim == 1
+            and full.numel() + local.numel() == total_q > 0 and full.device == local.device == dev
+            and not _is_untouched_compaction(full, local, total_q)):
+        # The lists' values are checked by the call itself, beside its first kernel.
+        full, local = _prepare_indices(full, device=dev), _prepare_indices(local, device=dev)
+        _note_sync(dev)
+        unchecked = True
+    else:
+        full, local = _check_lists(full, local, total_q, dev)
+        if metadata is not None:
+            _check_monotone(metadata, full, local)
+    if 0 in k.shape:
+        return torch.zeros(batch, k.shape[2], kv_len, dtype=torch.float32, device=dev)
+    with _lib.on_device(dev):
+        out, flags = _lib.native().prefill_key_weights(q, k, lse, full, local, fs, ls, ends,
+                                                       int(window_size), scale * LOG2E, unchecked,
+                                                       _lib.stream_handle(dev))
+    if flags:
+        _raise_for(flags, "full")
+        _raise_for(flags, "local")
+        if flags & ERR_OVERLAP:
+            raise ValueError(MSG_DISJOINT)
+    return out

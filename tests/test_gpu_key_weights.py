@@ -197,3 +197,45 @@ def test_refusals_on_the_device():
     md.causal_ends.copy_(md.causal_ends.flip(0))
     with pytest.raises(ValueError, match="non-decreasing"):
         call(q, k, lse, full, local, metadata=md)
+
+
+def test_lists_of_any_origin_are_checked():
+    """Lists that the compaction did not make: checked by the call, whatever their
+    length, with the errors of the forward and no result."""
+    gen = torch.Generator().manual_seed(7)
+    for s in (30, 3000, 300000):
+        hq = 1 if s > 10000 else 4
+        q, k = torch.randn(1, s, hq, 128, generator=gen).to(torch.bfloat16).to(DEV), None
+        k = q[:, :, :1].contiguous()
+        full, local = build_switch_query_indices((torch.rand(s, generator=gen) < 0.3).to(DEV))
+        _, lse = switch_gqa_prefill_forward(q, k, k, full, local, window_size=50)
+        want = switch_gqa_prefill_key_weights(q, k, lse, full, local, window_size=50)
+        for f, l in ((full.clone(), local.clone()), (full.long(), local.long()), (full[None], local[None])):
+            assert torch.equal(switch_gqa_prefill_key_weights(q, k, lse, f, l, window_size=50), want)
+        for change, words in (((full, -1, s), "outside"), ((full, 0, -1), "outside"), ((local, -1, s + 5), "outside"),
+                              ((full, 1, full[0]), "increasing"), ((local, 2, local[1]), "increasing"),
+                              ((full, 0, local[0]), "disjoint" if local[0] < full[1] else "increasing")):
+            src, at, value = change
+            bad = src.clone()
+            bad[at] = value
+            pair = (bad, local.clone()) if src is full else (full.clone(), bad)
+            with pytest.raises(ValueError, match=words):
+                switch_gqa_prefill_key_weights(q, k, lse, *pair, window_size=50)
+        assert torch.equal(switch_gqa_prefill_key_weights(q, k, lse, full, local, window_size=50), want)
+
+
+def test_unchecked_lists_cannot_be_captured():
+    gen = torch.Generator().manual_seed(8)
+    q, k = (x.to(DEV) for x in _qk(gen, 1, 64, 64, 4, 2))
+    full, local = build_switch_query_indices((torch.rand(64, generator=gen) < 0.5).to(DEV))
+    lse = torch.zeros(1, 64, 4, device=DEV)
+    f, l = full.clone(), local.clone()
+    switch_gqa_prefill_key_weights(q, k, lse, f, l)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            switch_gqa_prefill_key_weights(q, k, lse, f, l)
+        held = switch_gqa_prefill_key_weights(q, k, lse, full, local)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, switch_gqa_prefill_key_weights(q, k, lse, full, local))
