@@ -78,8 +78,20 @@ def build_switch_kv_cache(batch: int, capacity: int, kv_heads: int, *, device,
     return SwitchKVCache(*codes, *scales, block_size)
 
 
+def _parts(cache: SwitchKVCache):
+    return cache.k, cache.v, cache.k_scales, cache.v_scales
+
+
 def check_cache(cache: SwitchKVCache) -> None:
-    """Raise unless ``cache`` is whole: types, shapes, one device."""
+    """Raise unless ``cache`` is whole: types, shapes, one device.  In Python only
+    where one of the conditions fails."""
+    tensors = _parts(cache)
+    if (any(not isinstance(t, torch.Tensor) for t in tensors)
+            or not _lib.native().cache_ok(*tensors, int(cache.block_size))):
+        _validate_cache(cache)
+
+
+def _validate_cache(cache: SwitchKVCache) -> None:
     k, v, ks, vs = cache.k, cache.v, cache.k_scales, cache.v_scales
     if k.dtype not in _CODES or v.dtype != k.dtype:
         raise TypeError("the cache holds float8_e4m3fn or int8 codes, K and V alike")
@@ -101,7 +113,7 @@ def check_cache(cache: SwitchKVCache) -> None:
 
 
 def check_lens(lens: torch.Tensor, batch: int, device, name: str) -> torch.Tensor:
-    if lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or lens.device != device:
+    if lens.dtype != torch.int32 or lens.shape != (batch,) or lens.device != device:
         raise ValueError(f"{name} must be an int32 [B] tensor on the device of the cache")
     return lens.contiguous()
 
@@ -110,28 +122,10 @@ def check_weights(weights: torch.Tensor, cache: SwitchKVCache) -> None:
     b, n, h, _ = cache.k.shape
     if weights.dtype != torch.float32:
         raise TypeError("key_weights must be FP32")
-    if tuple(weights.shape) != (b, h, n) or weights.device != cache.k.device:
+    if weights.shape != (b, h, n) or weights.device != cache.k.device:
         raise ValueError("key_weights must be [B,Hkv,L] on the device of the cache")
     if not weights.is_contiguous():
         raise ValueError("key_weights must be contiguous")
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two contiguous tensors share memory."""
-    pa, pb = a.data_ptr(), b.data_ptr()
-    return (pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
-            and a.device == b.device)
-
-
-def _parts(cache: SwitchKVCache):
-    return cache.k, cache.v, cache.k_scales, cache.v_scales
-
-
-def _check_apart(tensors, message: str) -> None:
-    """No two of a call's outputs, and no output and input, share memory."""
-    for i, a in enumerate(tensors):
-        if any(_overlap(a, b) for b in tensors[:i]):
-            raise ValueError(message)
 
 
 def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tensor,
@@ -151,7 +145,7 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
     own and its new rows', and its rows are rounded again where it grows.
     """
     check_cache(cache)
-    batch, capacity, heads, _ = (int(x) for x in cache.k.shape)
+    batch, capacity, heads, _ = cache.k.shape
     dev = cache.k.device
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise TypeError("Switch Attention caches are filled from BF16 K/V")
@@ -182,8 +176,8 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
         most = rows
     if most > capacity:
         raise ValueError("more rows than the cache holds")
-    _check_apart(_parts(cache) + (k,), "K, V and the cache's tensors must not overlap in memory")
-    _check_apart(_parts(cache) + (v,), "K, V and the cache's tensors must not overlap in memory")
+    if not _lib.native().apart(_parts(cache), (k, v, lens)):
+        raise ValueError("K, V and the cache's tensors must not overlap in memory")
     with _lib.on_device(dev):
         return _lib.native().cache_append(k, v, cu, row_counts, lens, *_parts(cache), most,
                                           cache.block_size, _CODES[cache.k.dtype],
@@ -201,7 +195,7 @@ def switch_kv_cache_read(cache: SwitchKVCache, starts: Union[int, torch.Tensor],
     values are exact in bf16.
     """
     check_cache(cache)
-    dev, batch = cache.k.device, int(cache.k.shape[0])
+    dev, batch = cache.k.device, cache.k.shape[0]
     if rows < 0:
         raise ValueError("rows must not be negative")
     if isinstance(starts, torch.Tensor):
@@ -241,7 +235,7 @@ def switch_kv_cache_evict(cache: SwitchKVCache, cache_lens: torch.Tensor, key_we
     in turn let a captured decode loop go on.
     """
     check_cache(cache)
-    batch, n, heads, _ = (int(x) for x in cache.k.shape)
+    batch, n, heads, _ = cache.k.shape
     dev = cache.k.device
     lens = check_lens(cache_lens, batch, dev, "cache_lens")
     check_weights(key_weights, cache)
@@ -270,10 +264,9 @@ def switch_kv_cache_evict(cache: SwitchKVCache, cache_lens: torch.Tensor, key_we
         if out.k.shape[1] < budget:
             raise ValueError("the destination must hold at least budget rows")
         check_weights(out_weights, out)
-        mine = _parts(out) + (out_weights,)
-        _check_apart(mine, "the destination's tensors must not overlap in memory")
-        if any(_overlap(a, b) for a in mine for b in _parts(cache) + (key_weights, lens)):
-            raise ValueError("the destination must not share memory with the source")
+        if not _lib.native().apart(_parts(out) + (out_weights,), _parts(cache) + (key_weights, lens)):
+            raise ValueError("the destination's tensors must not share memory, with the source or "
+                             "each other")
     with _lib.on_device(dev):
         new_lens = _lib.native().cache_evict(*_parts(cache), key_weights, lens, *_parts(out),
                                              out_weights, cache.block_size, _CODES[cache.k.dtype],

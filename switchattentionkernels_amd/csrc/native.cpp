@@ -219,6 +219,38 @@ struct CacheShape {
         dim(static_cast<int32_t>(k.size(3))), len(k.size(1)) {}
 };
 
+// Whether a cache's tensors meet every precondition (the Python layer finds out
+// which one fails and raises for it).
+bool cache_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t block) {
+  if (!(block == 16 || block == 32 || block == 64 || block == 128)) return false;
+  if (!(k.is_cuda() && k.layout() == at::kStrided && k.dim() == 4 && k.numel() > 0 && k.size(3) == 128 &&
+        (k.scalar_type() == at::kChar || k.scalar_type() == at::kFloat8_e4m3fn)))
+    return false;
+  const int64_t want[3] = {k.size(0), k.size(2), (k.size(1) + block - 1) / block};
+  return v.scalar_type() == k.scalar_type() && v.layout() == at::kStrided && v.sizes() == k.sizes() &&
+         ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.layout() == at::kStrided &&
+         vs.layout() == at::kStrided && ks.sizes() == at::IntArrayRef(want, 3) && vs.sizes() == ks.sizes() &&
+         k.is_contiguous() && v.is_contiguous() && ks.is_contiguous() && vs.is_contiguous() &&
+         v.device() == k.device() && ks.device() == k.device() && vs.device() == k.device();
+}
+
+// Whether contiguous tensors that a call writes share no memory with each other
+// or with those that it reads.
+bool apart(const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
+  const auto overlap = [](const Tensor& a, const Tensor& b) {
+    const char* pa = static_cast<const char*>(a.const_data_ptr());
+    const char* pb = static_cast<const char*>(b.const_data_ptr());
+    return a.device() == b.device() && pa < pb + b.nbytes() && pb < pa + a.nbytes();
+  };
+  for (size_t i = 0; i < written.size(); ++i) {
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(written[i], written[j])) return false;
+    for (const Tensor& t : read)
+      if (overlap(written[i], t)) return false;
+  }
+  return true;
+}
+
 // The new lengths.
 Tensor cache_append(const Tensor& new_k, const Tensor& new_v, const optional<Tensor>& cu,
                     const optional<Tensor>& counts, const Tensor& lens, const Tensor& k, const Tensor& v,
@@ -353,6 +385,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("metadata", &metadata);
   m.def("prefill_backward", &prefill_backward);
   m.def("decode_forward", &decode_forward);
+  m.def("cache_ok", &cache_ok);
+  m.def("apart", &apart);
   m.def("cache_append", &cache_append);
   m.def("cache_read", &cache_read);
   m.def("cache_decode", &cache_decode);

@@ -114,6 +114,9 @@ def switch_gqa_decode_quantized_forward(
         raise ValueError("full_mask must be a bool [B] tensor on the device of Q")
     if key_weights is not None:
         check_weights(key_weights, cache)
+        if not _lib.native().apart((key_weights,), (q, cache.k, cache.v, cache.k_scales,
+                                                    cache.v_scales, lens, full_mask)):
+            raise ValueError("key_weights must not share memory with the other arguments")
     scale = ((1.0 / dim) ** 0.5 if sm_scale is None else float(sm_scale)) * LOG2E
     with _lib.on_device(dev):
         out, lse = _lib.native().cache_decode(q, cache.k, cache.v, cache.k_scales, cache.v_scales,

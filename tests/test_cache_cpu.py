@@ -178,6 +178,12 @@ def test_a_broken_cache_is_refused_everywhere(change, error, words):
             call()
 
 
+def test_arguments_that_are_no_tensors_are_refused():
+    a = np.zeros((2, 40, 2, 128), np.int8)
+    with pytest.raises((TypeError, AttributeError)):
+        switch_kv_cache_read(SwitchKVCache(a, a, a, a, 16), 0, 3)
+
+
 def test_host_caches_are_refused():
     with pytest.raises(ValueError, match="accelerator"):
         switch_kv_cache_read(_cache(), 0, 3)
@@ -259,7 +265,8 @@ def test_decode_and_evict_refusals():
             ((c, lens, w), dict(ok, out=other, out_weights=w[:, :, :9].clone()), ValueError, "Hkv,L"),
             ((c, lens, w), dict(ok, out=c, out_weights=w.clone()), ValueError, "share memory"),
             ((c, lens, w), dict(ok, out=other, out_weights=w), ValueError, "share memory"),
-            ((c, lens, w), dict(ok, out=_swap(other, v=other.k), out_weights=w.clone()), ValueError, "overlap")):
+            ((c, lens, w), dict(ok, out=_swap(other, v=other.k), out_weights=w.clone()), ValueError,
+             "share memory")):
         with pytest.raises(error, match=words):
             switch_kv_cache_evict(*args, **kw)
 

@@ -447,6 +447,18 @@ def test_evict_ties_and_odd_weights(kind):
     _check_evict(cache, lens, w.to(DEV), 700, 0, capacity=700)
 
 
+@pytest.mark.parametrize("n,budget,recent", [(16385, 4000, 1000), (32768, 32767, 3), (32768, 1, 0),
+                                             (50001, 20000, 64), (70000, 300, 299)])
+def test_evict_long_caches(n, budget, recent):
+    """Every way of holding the weights during the search; equal ones among them."""
+    gen = torch.Generator().manual_seed(n)
+    lens = [n, n - 1, budget + 1]
+    cache = _filled(gen, 3, n, 1, INT8, 128, lens)
+    w = torch.exp(2 * torch.randn(3, 1, n, generator=gen))
+    w[1] = torch.round(w[1])
+    _check_evict(cache, lens, w.to(DEV), budget, recent, capacity=budget)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_evict_carries_nan_blocks_and_foreign_scales(dtype):
     gen = torch.Generator().manual_seed(4)
