@@ -73,6 +73,8 @@ INTERNAL_SIGNATURES = {
                                            ctypes.c_size_t, _vp]),
     "swattn_build_metadata_host": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32,
                                                   _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "swattn_cache_append_host": (ctypes.c_int, [_vp] * 9 + [_i32, _i64, _i64, _i64, _i32, _i32,
+                                                            _i32, _i32, _vp]),
     "swattn_prefill_key_weights_checked": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
                                                           _vp, _vp, _vp, _i32, _i64, _i64, _i32,
                                                           _i32, _i32, _i32, ctypes.c_float, _vp,

@@ -37,6 +37,7 @@ from . import _lib
 from .metadata import _as_cu
 
 BLOCK_SIZES = (16, 32, 64, 128)
+HOST_MAX_SEQS = 256   # SWATTN_CACHE_HOST_MAX_SEQS
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}   # SWATTN_CODE_*
 
 
@@ -157,7 +158,7 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
         raise ValueError("K/V must be contiguous")
     lens = check_lens(cache_lens, batch, dev, "cache_lens")
     rows = int(k.shape[1])
-    cu = None
+    cu, host_cu = None, []
     if cu_seqlens is not None:
         if row_counts is not None:
             raise ValueError("row_counts and cu_seqlens exclude each other")
@@ -166,7 +167,10 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
         offsets = _as_cu(cu_seqlens, rows, "cu_seqlens")
         if len(offsets) != batch + 1:
             raise ValueError("cu_seqlens must hold one sequence for each of the cache's")
-        cu = torch.tensor(offsets, dtype=torch.int32, device=dev)
+        if batch <= HOST_MAX_SEQS:
+            host_cu = offsets
+        else:
+            cu = torch.tensor(offsets, dtype=torch.int32, device=dev)
         most = max(b - a for a, b in zip(offsets, offsets[1:]))
     else:
         if k.shape[0] != batch:
@@ -179,7 +183,7 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
     if not _lib.native().apart(_parts(cache), (k, v, lens)):
         raise ValueError("K, V and the cache's tensors must not overlap in memory")
     with _lib.on_device(dev):
-        return _lib.native().cache_append(k, v, cu, row_counts, lens, *_parts(cache), most,
+        return _lib.native().cache_append(k, v, cu, host_cu, row_counts, lens, *_parts(cache), most,
                                           cache.block_size, _CODES[cache.k.dtype],
                                           _lib.stream_handle(dev))
 

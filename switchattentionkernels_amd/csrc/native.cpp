@@ -251,9 +251,9 @@ bool apart(const std::vector<Tensor>& written, const std::vector<Tensor>& read) 
   return true;
 }
 
-// The new lengths.
+// The new lengths.  cu: packed offsets on the device, or host_cu (not empty).
 Tensor cache_append(const Tensor& new_k, const Tensor& new_v, const optional<Tensor>& cu,
-                    const optional<Tensor>& counts, const Tensor& lens, const Tensor& k, const Tensor& v,
+                    const std::vector<int32_t>& host_cu, const optional<Tensor>& counts, const Tensor& lens, const Tensor& k, const Tensor& v,
                     const Tensor& ks, const Tensor& vs, int64_t rows, int64_t block, int64_t code,
                     int64_t stream) {
   const CacheShape c(k);
@@ -261,11 +261,18 @@ Tensor cache_append(const Tensor& new_k, const Tensor& new_v, const optional<Ten
   int status = 0;
   {
     pybind11::gil_scoped_release release;
-    status = swattn_cache_append(new_k.const_data_ptr(), new_v.const_data_ptr(), i32(cu), i32(counts),
-                                 i32(lens), k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(),
-                                 vs.data_ptr<float>(), out.data_ptr<int32_t>(), c.batch, rows,
-                                 new_k.size(1), c.len, c.hkv, c.dim, static_cast<int32_t>(block),
-                                 static_cast<int32_t>(code), as_stream(stream));
+    if (!host_cu.empty())
+      status = swattn_cache_append_host(new_k.const_data_ptr(), new_v.const_data_ptr(), host_cu.data(),
+                                        i32(lens), k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(),
+                                        vs.data_ptr<float>(), out.data_ptr<int32_t>(), c.batch, rows,
+                                        new_k.size(1), c.len, c.hkv, c.dim, static_cast<int32_t>(block),
+                                        static_cast<int32_t>(code), as_stream(stream));
+    else
+      status = swattn_cache_append(new_k.const_data_ptr(), new_v.const_data_ptr(), i32(cu), i32(counts),
+                                   i32(lens), k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(),
+                                   vs.data_ptr<float>(), out.data_ptr<int32_t>(), c.batch, rows,
+                                   new_k.size(1), c.len, c.hkv, c.dim, static_cast<int32_t>(block),
+                                   static_cast<int32_t>(code), as_stream(stream));
   }
   check(status, "swattn_cache_append");
   return out;

@@ -16,9 +16,13 @@
 
 #include <limits.h>
 
+#include <string.h>
+
 #include <string>
+#include <type_traits>
 
 #include "cache_code.h"
+#include "swattn_internal.h"
 
 namespace swattn {
 namespace {
@@ -30,15 +34,31 @@ constexpr int kRowsAtOnce = 16;   // rows that a workgroup's half takes at once
 
 __device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
-// Largest value over this half of the workgroup (threads 0-127 or 128-255).
-__device__ __forceinline__ uint32_t half_max(uint32_t x) {
-  __shared__ uint32_t s_max[4];
+// Largest values over this half of the workgroup (threads 0-127 or 128-255), each of
+// kN on its own: lane moves inside a wave, one exchange between the half's two.
+template <int kN>
+__device__ __forceinline__ void half_max(uint32_t (&x)[kN]) {
+  __shared__ uint32_t s_max[4][kN];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), off)));
-  if (lane == 0) s_max[wave] = x;
+  for (int i = 0; i < kN; ++i) {
+    int v = static_cast<int>(x[i]);   // magnitudes' bits: no sign
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false));    // neighbours
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false));    // pairs
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));   // mirror image of 8
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false));   // and of 16 lanes
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+    const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    x[i] = max(static_cast<uint32_t>(c[0]), static_cast<uint32_t>(c[1]));
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s_max[wave][i] = x[i];
+  }
   __syncthreads();
-  return max(s_max[wave & 2], s_max[(wave & 2) + 1]);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) x[i] = max(s_max[wave & 2][i], s_max[(wave & 2) + 1][i]);
 }
 
 // ---------------------------------------------------------------------------
@@ -46,7 +66,7 @@ __device__ __forceinline__ uint32_t half_max(uint32_t x) {
 // ---------------------------------------------------------------------------
 struct AppendParams {
   const uint16_t* src[2];    // new K, V rows
-  const int32_t* cu;         // packed: offsets, else null
+  const int32_t* cu;         // packed: offsets, else null (or HostOffsets)
   const int32_t* counts;     // padded: rows per sequence, or null
   const int32_t* lens;
   uint8_t* codes[2];
@@ -56,9 +76,15 @@ struct AppendParams {
   int cache_len, hkv, nblk, batch, blocks;   // blocks: per sequence, at most
 };
 
+// Packed offsets as kernel arguments: no copy of them to the device.
+struct HostOffsets {
+  int32_t cu[SWATTN_CACHE_HOST_MAX_SEQS + 1];
+};
+struct NoOffsets {};
+
 // One workgroup per (sequence, touched block, KV head).
-template <int kCode, int kBlock>
-__global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
+template <int kCode, int kBlock, class Offsets>
+__global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const Offsets host) {
   constexpr int kIt = kBlock / kRowsAtOnce;
   const int h = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
@@ -66,9 +92,14 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   const int len = min(max(p.lens[b], 0), p.cache_len);
   // This sequence's new rows: src rows first .. first + count - 1.
   int64_t first = b * p.rows, count = p.rows;
-  if (p.cu != nullptr) {
-    first = min(max(static_cast<int64_t>(p.cu[b]), int64_t{0}), p.total_rows);
-    count = min(min(max(static_cast<int64_t>(p.cu[b + 1]), first), p.total_rows) - first, p.rows);
+  auto packed = [&](const int32_t* cu) {
+    first = min(max(static_cast<int64_t>(cu[b]), int64_t{0}), p.total_rows);
+    count = min(min(max(static_cast<int64_t>(cu[b + 1]), first), p.total_rows) - first, p.rows);
+  };
+  if constexpr (std::is_same<Offsets, HostOffsets>::value) {
+    packed(host.cu);
+  } else if (p.cu != nullptr) {
+    packed(p.cu);
   } else if (p.counts != nullptr) {
     count = min(max(static_cast<int64_t>(p.counts[b]), int64_t{0}), p.rows);
   }
@@ -81,7 +112,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
   const int sub = t >> 3, piece = t & 7;
   const uint16_t* src = p.src[half];
   uint4 raw[kIt][2];
-  uint32_t amax = 0;
+  uint32_t amax[1] = {0};
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
     const int r = r0 + it * kRowsAtOnce + sub;
@@ -95,11 +126,11 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p) {
     for (int u = 0; u < 2; ++u) {
       const uint32_t w[4] = {raw[it][u].x, raw[it][u].y, raw[it][u].z, raw[it][u].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) amax = max(amax, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
+      for (int j = 0; j < 4; ++j) amax[0] = max(amax[0], max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
     }
   }
-  amax = half_max(amax);
-  float scale = scale_for<kCode>(amax);
+  half_max(amax);
+  float scale = scale_for<kCode>(amax[0]);
   const bool begun = r0 < len;
   float* sp = p.scales[half] + (static_cast<int64_t>(b) * p.hkv + h) * p.nblk + jb;
   uint8_t* codes = p.codes[half] + (static_cast<int64_t>(b) * p.cache_len * p.hkv + h) * kD + piece * 16;
@@ -212,7 +243,7 @@ struct EvictParams {
   float* out_weights;
   int32_t* lens_out;
   int32_t* kept;   // [pair][budget - recent] rows that were chosen, ascending
-  int cache_len, out_len, hkv, nblk, out_nblk, out_blocks, budget, recent;
+  int cache_len, out_len, hkv, nblk, out_nblk, out_spans, budget, recent;
 };
 
 // A weight as an unsigned number of the same order: NaN above all, -0 as 0.
@@ -364,14 +395,18 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   });
 }
 
-// The kept rows into the destination: one workgroup per (sequence, destination
-// block, KV head).
+// The kept rows into the destination: one workgroup per (sequence, span of
+// destination rows, KV head); a span is one block, or 64 rows of smaller ones (a
+// 32-row block each: NEWG us for 32 sequences of 1024 to 4096 rows cut to 2047,
+// 8 KV heads, where the spans take OLDG).
+template <int kBlock>
+constexpr int kSpan = kBlock < 64 ? 64 : kBlock;
 template <int kCode, int kBlock>
 __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
-  constexpr int kIt = kBlock / kRowsAtOnce;
+  constexpr int kIt = kSpan<kBlock> / kRowsAtOnce, kBlocks = kSpan<kBlock> / kBlock, kPer = kBlock / kRowsAtOnce;
   const int h = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
-  const int jb = rest % p.out_blocks, b = rest / p.out_blocks;
+  const int js = rest % p.out_spans, b = rest / p.out_spans;
   const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
   const int len = min(max(p.lens[b], 0), p.cache_len);
   const int want = p.budget - p.recent;
@@ -381,8 +416,8 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
     if (len > p.budget) s = d < want ? p.kept[pair * want + d] : len - p.budget + d;
     return min(max(s, 0), p.cache_len - 1);
   };
-  const int r0 = jb * kBlock;
-  if (threadIdx.x < kBlock) {
+  const int r0 = js * kSpan<kBlock>;
+  if (threadIdx.x < kSpan<kBlock>) {
     const int d = r0 + static_cast<int>(threadIdx.x);
     if (d < p.out_len)
       p.out_weights[pair * p.out_len + d] = d < end ? p.weights[pair * p.cache_len + source(d)] : 0.f;
@@ -395,7 +430,6 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
   const float* scales = p.scales[half] + pair * p.nblk;
   uint4 raw[kIt];
   float s[kIt];
-  uint32_t amax = 0;
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
     const int d = r0 + it * kRowsAtOnce + sub;
@@ -407,27 +441,32 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
       s[it] = scales[r / kBlock];
     }
   }
+  uint32_t amax[kBlocks];
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) amax[k] = 0;
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
     float x[16];
     decode16<kCode>(raw[it], x);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax = max(amax, abs_bits(x[j] * s[it]));
+    for (int j = 0; j < 16; ++j) amax[it / kPer] = max(amax[it / kPer], abs_bits(x[j] * s[it]));
   }
-  amax = half_max(amax);
-  const float scale = scale_for<kCode>(amax);
-  if (t == 0) p.out_scales[half][pair * p.out_nblk + jb] = scale;
-  const float inv = 1.0f / scale;
+  half_max(amax);
   uint8_t* out = p.out_codes[half] + (static_cast<int64_t>(b) * p.out_len * p.hkv + h) * kD + piece * 16;
 #pragma unroll
-  for (int it = 0; it < kIt; ++it) {
-    const int d = r0 + it * kRowsAtOnce + sub;
-    if (d < end) {
-      float x[16];
-      decode16<kCode>(raw[it], x);
+  for (int k = 0; k < kBlocks; ++k) {
+    const float scale = scale_for<kCode>(amax[k]), inv = 1.0f / scale;
+    if (t == 0 && r0 + k * kBlock < end) p.out_scales[half][pair * p.out_nblk + js * kBlocks + k] = scale;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
-      *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
+    for (int it = k * kPer; it < (k + 1) * kPer; ++it) {
+      const int d = r0 + it * kRowsAtOnce + sub;
+      if (d < end) {
+        float x[16];
+        decode16<kCode>(raw[it], x);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
+        *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
+      }
     }
   }
 }
@@ -446,28 +485,29 @@ int check_cache(const std::string& n, int32_t batch, int64_t cache_len, int32_t 
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// fn<code, block>(grid, stream, params)
-template <template <int, int> class Launch, class P>
-void by_code_and_block(int32_t codes, int32_t block, dim3 grid, hipStream_t st, const P& p) {
+// Launch<code, block>::go(grid, stream, params...)
+template <template <int, int> class Launch, class... P>
+void by_code_and_block(int32_t codes, int32_t block, dim3 grid, hipStream_t st, const P&... p) {
   if (codes == kE4m3) {
     switch (block) {
-      case 16: return Launch<kE4m3, 16>::go(grid, st, p);
-      case 32: return Launch<kE4m3, 32>::go(grid, st, p);
-      case 64: return Launch<kE4m3, 64>::go(grid, st, p);
-      default: return Launch<kE4m3, 128>::go(grid, st, p);
+      case 16: return Launch<kE4m3, 16>::go(grid, st, p...);
+      case 32: return Launch<kE4m3, 32>::go(grid, st, p...);
+      case 64: return Launch<kE4m3, 64>::go(grid, st, p...);
+      default: return Launch<kE4m3, 128>::go(grid, st, p...);
     }
   }
   switch (block) {
-    case 16: return Launch<kInt8, 16>::go(grid, st, p);
-    case 32: return Launch<kInt8, 32>::go(grid, st, p);
-    case 64: return Launch<kInt8, 64>::go(grid, st, p);
-    default: return Launch<kInt8, 128>::go(grid, st, p);
+    case 16: return Launch<kInt8, 16>::go(grid, st, p...);
+    case 32: return Launch<kInt8, 32>::go(grid, st, p...);
+    case 64: return Launch<kInt8, 64>::go(grid, st, p...);
+    default: return Launch<kInt8, 128>::go(grid, st, p...);
   }
 }
 template <int kCode, int kBlock>
 struct LaunchAppend {
-  static void go(dim3 grid, hipStream_t st, const AppendParams& p) {
-    hipLaunchKernelGGL((append_kernel<kCode, kBlock>), grid, dim3(256), 0, st, p);
+  template <class Offsets>
+  static void go(dim3 grid, hipStream_t st, const AppendParams& p, const Offsets& host) {
+    hipLaunchKernelGGL((append_kernel<kCode, kBlock, Offsets>), grid, dim3(256), 0, st, p, host);
   }
 };
 template <int kCode, int kBlock>
@@ -482,20 +522,20 @@ struct LaunchGather {
 
 using namespace swattn;
 
-extern "C" {
-
-int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
+// The checks and the launch; host: the packed offsets where they are known here, or
+// null.
+static int launch_append(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
                         const int32_t* counts, const int32_t* cache_lens, void* k, void* v,
                         float* k_scales, float* v_scales, int32_t* lens_out, int32_t batch,
                         int64_t rows, int64_t total_rows, int64_t cache_len, int32_t heads_kv,
-                        int32_t head_dim, int32_t block, int32_t codes, void* stream) {
+                        int32_t head_dim, int32_t block, int32_t codes, void* stream, const HostOffsets* host) {
   const std::string n("swattn_cache_append");
   const int st = check_cache(n, batch, cache_len, heads_kv, head_dim, block, codes);
   if (st != SWATTN_OK) return st;
   if (rows < 0 || rows > INT32_MAX || total_rows < 0 || total_rows > INT32_MAX)
     return invalid(n + ": bad number of rows");
   if (cu_seqlens != nullptr && counts != nullptr) return invalid(n + ": counts and cu_seqlens exclude each other");
-  const bool any = rows > 0 && (cu_seqlens == nullptr || total_rows > 0);
+  const bool any = rows > 0 && ((cu_seqlens == nullptr && host == nullptr) || total_rows > 0);
   if (cache_lens == nullptr || lens_out == nullptr || k == nullptr || v == nullptr || k_scales == nullptr ||
       v_scales == nullptr || (any && (new_k == nullptr || new_v == nullptr)))
     return invalid(n + ": null pointer");
@@ -524,8 +564,37 @@ int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_
   p.blocks = static_cast<int>(most < p.nblk ? most : p.nblk);
   const int64_t grid = static_cast<int64_t>(p.blocks) * batch * heads_kv;
   if (grid > INT32_MAX) return invalid(n + ": grid too large");
-  by_code_and_block<LaunchAppend>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p);
+  const dim3 g(static_cast<uint32_t>(grid));
+  if (host != nullptr)
+    by_code_and_block<LaunchAppend>(codes, block, g, as_stream(stream), p, *host);
+  else
+    by_code_and_block<LaunchAppend>(codes, block, g, as_stream(stream), p, NoOffsets{});
   return launch_status(n.c_str());
+}
+
+
+extern "C" {
+
+int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
+                        const int32_t* counts, const int32_t* cache_lens, void* k, void* v,
+                        float* k_scales, float* v_scales, int32_t* lens_out, int32_t batch,
+                        int64_t rows, int64_t total_rows, int64_t cache_len, int32_t heads_kv,
+                        int32_t head_dim, int32_t block, int32_t codes, void* stream) {
+  return launch_append(new_k, new_v, cu_seqlens, counts, cache_lens, k, v, k_scales, v_scales, lens_out, batch,
+                       rows, total_rows, cache_len, heads_kv, head_dim, block, codes, stream, nullptr);
+}
+
+int swattn_cache_append_host(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
+                        const int32_t* cache_lens, void* k, void* v,
+                        float* k_scales, float* v_scales, int32_t* lens_out, int32_t batch,
+                        int64_t rows, int64_t total_rows, int64_t cache_len, int32_t heads_kv,
+                        int32_t head_dim, int32_t block, int32_t codes, void* stream) {
+  if (cu_seqlens == nullptr) return invalid("swattn_cache_append: null pointer");
+  if (batch < 1 || batch > SWATTN_CACHE_HOST_MAX_SEQS) return invalid("swattn_cache_append: too many sequences");
+  HostOffsets host{};
+  memcpy(host.cu, cu_seqlens, (static_cast<size_t>(batch) + 1) * sizeof(int32_t));
+  return launch_append(new_k, new_v, nullptr, nullptr, cache_lens, k, v, k_scales, v_scales, lens_out, batch,
+                       rows, total_rows, cache_len, heads_kv, head_dim, block, codes, stream, &host);
 }
 
 int swattn_cache_read(const void* k, const void* v, const float* k_scales, const float* v_scales,
@@ -620,10 +689,11 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
   p.out_len = static_cast<int>(out_len);
   p.hkv = heads_kv;
   p.nblk = static_cast<int>(ceil_div(cache_len, block));
-  p.out_nblk = p.out_blocks = static_cast<int>(ceil_div(out_len, block));
+  p.out_nblk = static_cast<int>(ceil_div(out_len, block));
+  p.out_spans = static_cast<int>(ceil_div(out_len, block < 64 ? 64 : block));
   p.budget = static_cast<int>(budget);
   p.recent = static_cast<int>(recent);
-  const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_blocks;
+  const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_spans;
   if (grid > INT32_MAX) return invalid(n + ": grid too large");
   const dim3 gs(static_cast<uint32_t>(pairs));
   const hipStream_t hs = as_stream(stream);

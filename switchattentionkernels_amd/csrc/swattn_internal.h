@@ -53,6 +53,18 @@ int swattn_check_bounds(const int32_t* full, int64_t n_full, const int32_t* loca
                         void* stream);
 
 /*
+ * swattn_cache_append of packed rows with the offsets in host memory (read before
+ * the call returns, so that no device copy of them is needed and the call can be
+ * captured), for up to SWATTN_CACHE_HOST_MAX_SEQS sequences.
+ */
+#define SWATTN_CACHE_HOST_MAX_SEQS 256
+int swattn_cache_append_host(const void* new_k, const void* new_v, const int32_t* cu_seqlens,
+                             const int32_t* cache_lens, void* k, void* v, float* k_scales,
+                             float* v_scales, int32_t* lens_out, int32_t batch, int64_t rows,
+                             int64_t total_rows, int64_t cache_len, int32_t heads_kv,
+                             int32_t head_dim, int32_t block, int32_t code, void* stream);
+
+/*
  * swattn_prefill_key_weights with the check of the lists (swattn_check_indices)
  * in its first kernel: on return *flags holds the SWATTN_ERR_* bits, while the
  * sums may still be running.  (With the check and its read-back ahead of the

@@ -116,6 +116,24 @@ def test_append_packed(dtype):
         _check_append(cache, before, part(k), part(v), lens.tolist(), after)
 
 
+def test_append_packed_many_sequences():
+    """More sequences than offsets travel as kernel arguments."""
+    gen = torch.Generator().manual_seed(15)
+    b, n, h, block = 300, 20, 1, 16
+    counts = torch.randint(0, 6, (b,), generator=gen).tolist()
+    lens = torch.randint(0, 18, (b,), generator=gen).tolist()
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    for m in (256, 257, 300):
+        cache = _filled(gen, m, n, h, E4M3, block, lens[:m])
+        k = _rows(gen, 1, cu[m], h, 128)
+        before = _snapshot(cache)
+        after = switch_kv_cache_append(cache, k.to(DEV), (-k).to(DEV), _int32(lens[:m]), cu_seqlens=cu[:m + 1])
+        part = [k[0, x:y].float().numpy() for x, y in zip(cu[:m], cu[1:m + 1])]
+        _check_append(cache, before, part, [-x for x in part], lens[:m], after)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_a_non_finite_value_makes_its_block_nan(dtype, bad):
