@@ -34,31 +34,23 @@ constexpr int kRowsAtOnce = 16;   // rows that a workgroup's half takes at once
 
 __device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
-// Largest values over this half of the workgroup (threads 0-127 or 128-255), each of
-// kN on its own: lane moves inside a wave, one exchange between the half's two.
-template <int kN>
-__device__ __forceinline__ void half_max(uint32_t (&x)[kN]) {
-  __shared__ uint32_t s_max[4][kN];
+// Largest magnitude's bits over this half of the workgroup (threads 0-127 or
+// 128-255): lane moves inside a wave, one exchange between the half's two.
+__device__ __forceinline__ uint32_t half_max(uint32_t x) {
+  __shared__ int s_max[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    int v = static_cast<int>(x[i]);   // magnitudes' bits: no sign
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false));    // neighbours
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false));    // pairs
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));   // mirror image of 8
-    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false));   // and of 16 lanes
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
-    const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    x[i] = max(static_cast<uint32_t>(c[0]), static_cast<uint32_t>(c[1]));
-  }
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) s_max[wave][i] = x[i];
-  }
+  int v = static_cast<int>(x);   // no sign
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false));    // neighbours
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false));    // pairs
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false));   // mirror image of 8
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, false));   // and of 16 lanes
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max(static_cast<int>(c[0]), static_cast<int>(c[1]));
+  if (lane == 0) s_max[wave] = v;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kN; ++i) x[i] = max(s_max[wave & 2][i], s_max[(wave & 2) + 1][i]);
+  return static_cast<uint32_t>(max(s_max[wave & 2], s_max[(wave & 2) + 1]));
 }
 
 // ---------------------------------------------------------------------------
@@ -112,7 +104,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const
   const int sub = t >> 3, piece = t & 7;
   const uint16_t* src = p.src[half];
   uint4 raw[kIt][2];
-  uint32_t amax[1] = {0};
+  uint32_t amax = 0;
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
     const int r = r0 + it * kRowsAtOnce + sub;
@@ -126,11 +118,11 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const
     for (int u = 0; u < 2; ++u) {
       const uint32_t w[4] = {raw[it][u].x, raw[it][u].y, raw[it][u].z, raw[it][u].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) amax[0] = max(amax[0], max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
+      for (int j = 0; j < 4; ++j) amax = max(amax, max((w[j] << 16) & 0x7fffffffu, w[j] & 0x7fff0000u));
     }
   }
-  half_max(amax);
-  float scale = scale_for<kCode>(amax[0]);
+  amax = half_max(amax);
+  float scale = scale_for<kCode>(amax);
   const bool begun = r0 < len;
   float* sp = p.scales[half] + (static_cast<int64_t>(b) * p.hkv + h) * p.nblk + jb;
   uint8_t* codes = p.codes[half] + (static_cast<int64_t>(b) * p.cache_len * p.hkv + h) * kD + piece * 16;
@@ -243,7 +235,7 @@ struct EvictParams {
   float* out_weights;
   int32_t* lens_out;
   int32_t* kept;   // [pair][budget - recent] rows that were chosen, ascending
-  int cache_len, out_len, hkv, nblk, out_nblk, out_spans, budget, recent;
+  int cache_len, out_len, hkv, nblk, out_nblk, budget, recent;
 };
 
 // A weight as an unsigned number of the same order: NaN above all, -0 as 0.
@@ -261,7 +253,8 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // per step, so that ballots count and place them and the waves meet only once.
 // kPer > 0: a thread's kPer weights are read once, into registers; 0: any number,
 // read again in every pass.  Bound by latency: few workgroups for few sequences.
-// 16384 rows, 8 pairs: 26 us with 8-bit digits and four reads, NEWUS so.
+// 16384 rows, 8 pairs: 26 us with 8-bit digits and five reads, 12 so; 4096 rows, 256
+// pairs: 12.7 and 9.9.
 constexpr int kDigits = 2048;
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
@@ -395,18 +388,16 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   });
 }
 
-// The kept rows into the destination: one workgroup per (sequence, span of
-// destination rows, KV head); a span is one block, or 64 rows of smaller ones (a
-// 32-row block each: NEWG us for 32 sequences of 1024 to 4096 rows cut to 2047,
-// 8 KV heads, where the spans take OLDG).
-template <int kBlock>
-constexpr int kSpan = kBlock < 64 ? 64 : kBlock;
+// The kept rows into the destination: one workgroup per (sequence, destination
+// block, KV head).  32 sequences of 1024 to 4096 rows cut to 2047, 8 KV heads,
+// blocks of 32: 59 us, 4.2 TB/s of scattered 128-byte rows (64 rows a workgroup: 64;
+// a block's heads on one XCD: 62).
 template <int kCode, int kBlock>
 __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
-  constexpr int kIt = kSpan<kBlock> / kRowsAtOnce, kBlocks = kSpan<kBlock> / kBlock, kPer = kBlock / kRowsAtOnce;
+  constexpr int kIt = kBlock / kRowsAtOnce;
   const int h = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
-  const int js = rest % p.out_spans, b = rest / p.out_spans;
+  const int jb = rest % p.out_nblk, b = rest / p.out_nblk;
   const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
   const int len = min(max(p.lens[b], 0), p.cache_len);
   const int want = p.budget - p.recent;
@@ -416,8 +407,8 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
     if (len > p.budget) s = d < want ? p.kept[pair * want + d] : len - p.budget + d;
     return min(max(s, 0), p.cache_len - 1);
   };
-  const int r0 = js * kSpan<kBlock>;
-  if (threadIdx.x < kSpan<kBlock>) {
+  const int r0 = jb * kBlock;
+  if (threadIdx.x < kBlock) {
     const int d = r0 + static_cast<int>(threadIdx.x);
     if (d < p.out_len)
       p.out_weights[pair * p.out_len + d] = d < end ? p.weights[pair * p.cache_len + source(d)] : 0.f;
@@ -441,32 +432,27 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
       s[it] = scales[r / kBlock];
     }
   }
-  uint32_t amax[kBlocks];
-#pragma unroll
-  for (int k = 0; k < kBlocks; ++k) amax[k] = 0;
+  uint32_t amax = 0;
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
     float x[16];
     decode16<kCode>(raw[it], x);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax[it / kPer] = max(amax[it / kPer], abs_bits(x[j] * s[it]));
+    for (int j = 0; j < 16; ++j) amax = max(amax, abs_bits(x[j] * s[it]));
   }
-  half_max(amax);
+  amax = half_max(amax);
+  const float scale = scale_for<kCode>(amax), inv = 1.0f / scale;
+  if (t == 0) p.out_scales[half][pair * p.out_nblk + jb] = scale;
   uint8_t* out = p.out_codes[half] + (static_cast<int64_t>(b) * p.out_len * p.hkv + h) * kD + piece * 16;
 #pragma unroll
-  for (int k = 0; k < kBlocks; ++k) {
-    const float scale = scale_for<kCode>(amax[k]), inv = 1.0f / scale;
-    if (t == 0 && r0 + k * kBlock < end) p.out_scales[half][pair * p.out_nblk + js * kBlocks + k] = scale;
+  for (int it = 0; it < kIt; ++it) {
+    const int d = r0 + it * kRowsAtOnce + sub;
+    if (d < end) {
+      float x[16];
+      decode16<kCode>(raw[it], x);
 #pragma unroll
-    for (int it = k * kPer; it < (k + 1) * kPer; ++it) {
-      const int d = r0 + it * kRowsAtOnce + sub;
-      if (d < end) {
-        float x[16];
-        decode16<kCode>(raw[it], x);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
-        *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
-      }
+      for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
+      *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
     }
   }
 }
@@ -690,10 +676,9 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
   p.hkv = heads_kv;
   p.nblk = static_cast<int>(ceil_div(cache_len, block));
   p.out_nblk = static_cast<int>(ceil_div(out_len, block));
-  p.out_spans = static_cast<int>(ceil_div(out_len, block < 64 ? 64 : block));
   p.budget = static_cast<int>(budget);
   p.recent = static_cast<int>(recent);
-  const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_spans;
+  const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_nblk;
   if (grid > INT32_MAX) return invalid(n + ": grid too large");
   const dim3 gs(static_cast<uint32_t>(pairs));
   const hipStream_t hs = as_stream(stream);

@@ -47,8 +47,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;            // waves per workgroup
 constexpr int kMaxG = 8;
 constexpr int kStep = 32;            // keys a wave takes at once
-constexpr int kAhead = 3;            // steps a wave's loads run ahead
-constexpr uint32_t kPairPad = 384;   // a pair's start, in keys
+constexpr int kAhead = 1;            // steps a wave's loads run ahead
+constexpr uint32_t kPairPad = 192;   // a pair's start, in keys
 
 struct CacheDecodeParams : DecodeCommon {
   static constexpr uint32_t kMinShare = 128;     // line positions per workgroup, at least
@@ -102,7 +102,7 @@ struct Step {
 // 32-key steps w, w + 4, ... of a piece, which begin at multiples of 32 of the
 // sequence; rows outside the piece are read as its nearest row and masked.
 template <int kCode, bool kInline, bool kScores>
-__global__ __launch_bounds__(256) void cache_split_kernel(const CacheDecodeParams p) {
+__global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodeParams p) {
   __shared__ float s_m[kWaves][kMaxG], s_l[kWaves][kMaxG];
   __shared__ float s_acc[kWaves][kMaxG][kD];
   __shared__ SeqEntry s_ent[kInline ? kInlineSeqs : 1];
@@ -333,9 +333,10 @@ __global__ __launch_bounds__(256) void cache_split_kernel(const CacheDecodeParam
 }
 
 // Workgroups below batch * hq merge an output row each; the rest add the weights
-// of kWeightKeys keys of one (sequence, KV head) each, from the scores and the
-// pair's LSEs, which they compute from the partials as the merge does.
-constexpr int kWeightKeys = 1024;
+// of kWeightKeys keys of one (sequence, KV head) each, a thread per key, from the
+// scores and the pair's LSEs, which they compute from the partials as the merge
+// does.
+constexpr int kWeightKeys = 256;
 __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheDecodeParams p) {
   const int64_t rows = static_cast<int64_t>(p.batch) * p.hq;
   if (blockIdx.x < rows) {
@@ -358,6 +359,14 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheDecodeParam
   const int nch = static_cast<int>(quotient(off + seq.n - 1, share) - wg0) + 1;
   const int64_t slot0 = static_cast<int64_t>(wg0) + static_cast<int64_t>(seq.rank) * p.hkv + kvh;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G = p.group;
+  const int64_t j = first + threadIdx.x;
+  const bool live = j >= lo && j < lo + static_cast<int64_t>(n);
+  const float* sc = p.scores + (static_cast<int64_t>(b) * p.hq + kvh * G) * p.score_len + j;
+  float score[kMaxG];
+#pragma unroll
+  for (int h = 0; h < kMaxG; ++h) score[h] = live && h < G ? sc[h * p.score_len] : -INFINITY;
+  float* w = p.weights + pair * p.cache_len + j;
+  const float before = live ? *w : 0.f;
   for (int h = wave; h < G; h += 4) {
     float mx = -INFINITY, sum = 0.f;
     float2 ml[kMaxSplitsDev / 64];
@@ -378,20 +387,18 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheDecodeParam
     if (lane == 0) s_lse[h] = mx + log2f(sum);
   }
   __syncthreads();
-  const float* sc = p.scores + (static_cast<int64_t>(b) * p.hq + kvh * G) * p.score_len;
-  float* w = p.weights + pair * p.cache_len;
-  const int64_t end = min(first + kWeightKeys, lo + static_cast<int64_t>(n));
-  for (int64_t j = max(first, static_cast<int64_t>(lo)) + threadIdx.x; j < end; j += 256) {
-    float sum = 0.f;
-    for (int h = 0; h < G; ++h) sum += __builtin_amdgcn_exp2f(sc[h * p.score_len + j] - s_lse[h]);
-    w[j] += sum;
-  }
+  if (!live) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int h = 0; h < kMaxG; ++h)
+    if (h < G) sum += __builtin_amdgcn_exp2f(score[h] - s_lse[h]);
+  *w = before + sum;
 }
 
-// Workgroups that the line is shared out over: two per CU; the workspace holds
-// four per CU plus one per pair partials, as swattn_decode_fwd's.
-constexpr int kSplitTarget = 2;
-constexpr int kSplitRoom = 4;
+// Workgroups that the line is shared out over: three per CU, as many as are
+// resident at once; the workspace holds six per CU plus one per pair partials.
+constexpr int kSplitTarget = 3;
+constexpr int kSplitRoom = 6;
 static_assert(2 * kSplitTarget <= kSplitRoom, "every share has its partial");
 
 int cu_count() {
