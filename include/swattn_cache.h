@@ -65,6 +65,7 @@ int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_
  * Read `rows` rows per sequence as bf16 [batch, rows, heads_kv, 128], from
  * row starts[b] (starts NULL: from row `start` in every sequence).  Rows
  * outside [0, cache_lens[b]) (cache_lens NULL: [0, cache_len)) come out as 0.
+ * rows * heads_kv below 2^28.
  */
 int swattn_cache_read(const void* k, const void* v, const float* k_scales, const float* v_scales,
                       const int32_t* starts, int64_t start, const int32_t* cache_lens, void* out_k,

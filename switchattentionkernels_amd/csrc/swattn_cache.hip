@@ -184,7 +184,8 @@ struct ReadParams {
   const int32_t* starts;   // or null: `start`
   const int32_t* lens;     // or null: cache_len
   uint16_t* out[2];
-  int64_t start, rows, pieces;   // pieces: 16 values each, of K
+  int64_t start;
+  int32_t pieces;          // 16 values each, of one sequence's K
   int cache_len, hkv, nblk, block_log;
 };
 
@@ -193,17 +194,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
          static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(b))) << 16;
 }
 
-// One thread per 16 values; blockIdx.y 0: K, 1: V.
+// One thread per 16 values; blockIdx.y: sequence, blockIdx.z 0: K, 1: V.
 template <int kCode>
 __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
-  const int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (x >= p.pieces) return;
-  const int which = blockIdx.y;
-  const int piece = static_cast<int>(x & 7);
-  const int64_t rowh = x >> 3;                 // (b * rows + i) * hkv + h
-  const int64_t row = rowh / p.hkv;
-  const int h = static_cast<int>(rowh - row * p.hkv);
-  const int64_t b = row / p.rows, i = row - b * p.rows;
+  const uint32_t x = blockIdx.x * 256u + threadIdx.x;
+  if (x >= static_cast<uint32_t>(p.pieces)) return;
+  const int64_t b = blockIdx.y;
+  const int which = blockIdx.z;
+  const int piece = static_cast<int>(x & 7u);
+  const uint32_t rowh = x >> 3, i = rowh / static_cast<uint32_t>(p.hkv);   // i * hkv + h
+  const int h = static_cast<int>(rowh - i * static_cast<uint32_t>(p.hkv));
   const int64_t r = (p.starts != nullptr ? static_cast<int64_t>(p.starts[b]) : p.start) + i;
   const int end = p.lens != nullptr ? min(p.lens[b], p.cache_len) : p.cache_len;
   uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
       o[j] = make_uint4(pack_bf16(v[8 * j] * s, v[8 * j + 1] * s), pack_bf16(v[8 * j + 2] * s, v[8 * j + 3] * s),
                         pack_bf16(v[8 * j + 4] * s, v[8 * j + 5] * s), pack_bf16(v[8 * j + 6] * s, v[8 * j + 7] * s));
   }
-  uint4* out = reinterpret_cast<uint4*>(p.out[which] + x * 16);
+  uint4* out = reinterpret_cast<uint4*>(p.out[which] + (b * p.pieces + x) * 16);
   out[0] = o[0];
   out[1] = o[1];
 }
@@ -608,15 +608,14 @@ int swattn_cache_read(const void* k, const void* v, const float* k_scales, const
   p.out[0] = static_cast<uint16_t*>(out_k);
   p.out[1] = static_cast<uint16_t*>(out_v);
   p.start = start;
-  p.rows = rows;
-  p.pieces = static_cast<int64_t>(batch) * rows * heads_kv * (kD / 16);
+  const int64_t pieces = rows * heads_kv * (kD / 16);
+  if (pieces > INT32_MAX) return invalid(n + ": too many rows at once");
+  p.pieces = static_cast<int32_t>(pieces);
   p.cache_len = static_cast<int>(cache_len);
   p.hkv = heads_kv;
   p.nblk = static_cast<int>(ceil_div(cache_len, block));
   p.block_log = __builtin_ctz(static_cast<unsigned>(block));
-  const int64_t grid = ceil_div(p.pieces, 256);
-  if (grid > INT32_MAX) return invalid(n + ": grid too large");
-  const dim3 g(static_cast<uint32_t>(grid), 2);
+  const dim3 g(static_cast<uint32_t>(ceil_div(pieces, 256)), batch, 2);
   if (codes == kE4m3)
     hipLaunchKernelGGL(read_kernel<kE4m3>, g, dim3(256), 0, as_stream(stream), p);
   else

@@ -398,8 +398,8 @@ struct Layout {
 // Chunks: short enough that the workgroups outnumber the chip's slots several
 // times over, long enough that the partial sums stay small.  (S16384: 64 blocks
 // 450 us, 32 472, 96 467, 128 462, 192 458; S8192 of 5 heads per KV head 230, 228,
-// 229, 261, 247.)
-constexpr int64_t kMinChunk = 8;
+// 229, 261, 247.  S1024, 128 blocks: at least 4 a chunk 16.6 us, 8 19.4, 2 19.0.)
+constexpr int64_t kMinChunk = 4;
 constexpr int64_t kMaxChunk = 64;
 constexpr int64_t kWantWgs = 4096;                // workgroups, if all chunks had blocks
 constexpr int64_t kMaxPartBytes = int64_t{64} << 20;

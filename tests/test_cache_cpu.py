@@ -61,6 +61,7 @@ def test_c_abi_refusals():
 
     _refused(read(rows=-1), "range of rows")
     _refused(read(start=-1), "range of rows")
+    _refused(read(rows=2 ** 27), "too many rows")
     _refused(read(k=None), "null")
     _refused(read(out=ctypes.c_void_p(264)), "16-byte")
     _refused(read(block=8), "block must be")
