@@ -25,6 +25,15 @@
 // * A group has at most 8 heads and the tiles have 16 columns: columns 8-15 repeat
 //   the heads, and take p's rounding error, p - bf16(p), where columns 0-7 take
 //   bf16(p).  Their sum carries 16 bits of p at no further matrix instruction.
+//
+// Measured, Hkv 8, as a large copy's 5.2 TB/s goes: B16 L16384-32768 Hq64 int8 all
+// full 163 us, 4.95 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full 0.25
+// 71 us, of which the merge and its launch are about 8; B1 L4096 Hq32 12 us, bound
+// by dependent latencies (plan, first keys, combine, merge) and, at that length, by
+// the host's calls.  Two workgroups per CU with loads three steps ahead: 12.8 us
+// (B1), 77 (B64); four with one step ahead 13 and 85.  Joining the pieces in the same
+// launch, the last workgroup of a pair waiting for the others' tags, took half
+// as long again (B64 104 us): every release writes an L2 back.
 
 #include <limits.h>
 #include <math.h>
@@ -91,6 +100,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, x);
 }
 
+// Caches that the 256 MB memory-side cache cannot hold are streamed past it: B64 of
+// 8192 rows, 8 KV heads 73.4 -> 70.7 us, B16 of 32768 169 -> 163.  Smaller ones may
+// still be there from the last call: B24 of 2999 29.7 us, streamed 35.6; B8 of 4096
+// 17.5 and 18.9.
+constexpr int64_t kStreamBytes = int64_t{256} << 20;
+template <bool kStream, class Raw, class T>
+__device__ __forceinline__ T load_bytes(const uint8_t* at) {
+  const Raw* p = reinterpret_cast<const Raw*>(at);
+  if constexpr (kStream) return __builtin_bit_cast(T, __builtin_nontemporal_load(p));
+  return __builtin_bit_cast(T, *p);
+}
+
 // One step's data: 32 keys of K and V and the scales of both key tiles.
 struct Step {
   uint4 k[2][2];   // [key tile][64-byte half of the row]
@@ -101,7 +122,7 @@ struct Step {
 // One workgroup per share of the line, as decode_split_kernel.  Wave w takes the
 // 32-key steps w, w + 4, ... of a piece, which begin at multiples of 32 of the
 // sequence; rows outside the piece are read as its nearest row and masked.
-template <int kCode, bool kInline, bool kScores>
+template <int kCode, bool kInline, bool kScores, bool kStream>
 __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodeParams p) {
   __shared__ float s_m[kWaves][kMaxG], s_l[kWaves][kMaxG];
   __shared__ float s_acc[kWaves][kMaxG][kD];
@@ -162,13 +183,13 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
         for (int t = 0; t < 2; ++t) {
           const int row = min(max(kk + 16 * t + c, k0), k1 - 1);
           const uint8_t* at = kb + row * stride;
-          s.k[t][0] = *reinterpret_cast<const uint4*>(at);
-          s.k[t][1] = *reinterpret_cast<const uint4*>(at + 64);
+          s.k[t][0] = load_bytes<kStream, u32x4, uint4>(at);
+          s.k[t][1] = load_bytes<kStream, u32x4, uint4>(at + 64);
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           const int row = min(max(kk + 16 * (t >> 2) + 4 * g + (t & 3), k0), k1 - 1);
-          s.v[t] = *reinterpret_cast<const uint2*>(vb + row * stride);
+          s.v[t] = load_bytes<kStream, uint64_t, uint2>(vb + row * stride);
         }
         // Of a tile without a row of the piece: the scale of the nearest block, not
         // a block that may hold no valid row.
@@ -428,12 +449,21 @@ Layout layout(int64_t batch, int64_t cache_len, int64_t heads_q, int64_t heads_k
   return L;
 }
 
-template <int kCode, bool kScores>
-void launch_split(bool inline_plan, dim3 grid, hipStream_t st, const CacheDecodeParams& p) {
-  if (inline_plan)
-    hipLaunchKernelGGL((cache_split_kernel<kCode, true, kScores>), grid, dim3(256), 0, st, p);
+template <int kCode, bool kInline, bool kScores>
+void launch_split(bool streamed, dim3 grid, hipStream_t st, const CacheDecodeParams& p) {
+  if (streamed)
+    hipLaunchKernelGGL((cache_split_kernel<kCode, kInline, kScores, true>), grid, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((cache_split_kernel<kCode, false, kScores>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((cache_split_kernel<kCode, kInline, kScores, false>), grid, dim3(256), 0, st, p);
+}
+template <int kCode>
+void launch_split(bool inline_plan, bool streamed, dim3 grid, hipStream_t st, const CacheDecodeParams& p) {
+  if (inline_plan)
+    p.scores != nullptr ? launch_split<kCode, true, true>(streamed, grid, st, p)
+                        : launch_split<kCode, true, false>(streamed, grid, st, p);
+  else
+    p.scores != nullptr ? launch_split<kCode, false, true>(streamed, grid, st, p)
+                        : launch_split<kCode, false, false>(streamed, grid, st, p);
 }
 
 }  // namespace
@@ -522,13 +552,11 @@ int swattn_cache_decode_fwd(const void* q, const void* k, const void* v, const f
     hipLaunchKernelGGL(decode_plan_kernel<CacheDecodeParams>, dim3(1), dim3(kPlanThreads), 0, st, p);
   const int64_t most = pairs * ((cache_len + p.pad + CacheDecodeParams::kMinShare - 1) / CacheDecodeParams::kMinShare);
   const dim3 grid(static_cast<uint32_t>(most < 2 * p.target ? most : 2 * p.target));
-  if (codes == kE4m3) {
-    if (p.scores != nullptr) launch_split<kE4m3, true>(inline_plan, grid, st, p);
-    else launch_split<kE4m3, false>(inline_plan, grid, st, p);
-  } else {
-    if (p.scores != nullptr) launch_split<kInt8, true>(inline_plan, grid, st, p);
-    else launch_split<kInt8, false>(inline_plan, grid, st, p);
-  }
+  const bool streamed = rows * 2 * kD >= kStreamBytes;
+  if (codes == kE4m3)
+    launch_split<kE4m3>(inline_plan, streamed, grid, st, p);
+  else
+    launch_split<kInt8>(inline_plan, streamed, grid, st, p);
   hipLaunchKernelGGL(cache_merge_kernel, dim3(static_cast<uint32_t>(merge_grid)), dim3(256), 0, st, p);
   return launch_status(n.c_str());
 }

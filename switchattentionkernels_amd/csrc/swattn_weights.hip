@@ -395,13 +395,16 @@ struct Layout {
   size_t off_ranges, off_part, bytes;
 };
 
-// Chunks: short enough that the workgroups outnumber the chip's slots several
-// times over, long enough that the partial sums stay small.  (S16384: 64 blocks
+// Chunks: on small grids about as many as run at once (two workgroups per CU; half of
+// the chunks see nothing); on large ones short enough that the workgroups outnumber
+// the slots several times over.  (Chunks of 4, 8, 16 and 32 blocks: B2 S980 Hq8/Hkv2,
+// 245 blocks and 16 pairs of key tile and head, 26.7 us, 22.5, -, -; S2048 Hq32/Hkv8,
+// 256 blocks and 64 pairs, 46, -, 35.6, 43.  S16384: 64 blocks
 // 450 us, 32 472, 96 467, 128 462, 192 458; S8192 of 5 heads per KV head 230, 228,
 // 229, 261, 247.  S1024, 128 blocks: at least 4 a chunk 16.6 us, 8 19.4, 2 19.0.)
 constexpr int64_t kMinChunk = 4;
 constexpr int64_t kMaxChunk = 64;
-constexpr int64_t kWantWgs = 4096;                // workgroups, if all chunks had blocks
+constexpr int64_t kWantWgs = 768;
 constexpr int64_t kMaxPartBytes = int64_t{64} << 20;
 
 Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full, int64_t n_local) {
