@@ -83,11 +83,18 @@ def _parts(cache: SwitchKVCache):
     return cache.k, cache.v, cache.k_scales, cache.v_scales
 
 
+def _all_tensors(*args) -> bool:
+    for t in args:
+        if not isinstance(t, torch.Tensor):
+            return False
+    return True
+
+
 def check_cache(cache: SwitchKVCache) -> None:
     """Raise unless ``cache`` is whole: types, shapes, one device.  In Python only
     where one of the conditions fails."""
     tensors = _parts(cache)
-    if (any(not isinstance(t, torch.Tensor) for t in tensors)
+    if (not _all_tensors(*tensors)
             or not _lib.native().cache_ok(*tensors, int(cache.block_size))):
         _validate_cache(cache)
 
@@ -129,22 +136,9 @@ def check_weights(weights: torch.Tensor, cache: SwitchKVCache) -> None:
         raise ValueError("key_weights must be contiguous")
 
 
-def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tensor,
-                           cache_lens: torch.Tensor, *,
-                           row_counts: Optional[torch.Tensor] = None,
-                           cu_seqlens=None) -> torch.Tensor:
-    """Quantise new rows into the cache, behind each sequence's ``cache_lens[b]``
-    valid ones; returns the new lengths, int32 ``[B]`` (``cache_lens`` itself is
-    left as it is).
-
-    ``k``/``v``: bf16 ``[B, T, Hkv, 128]``, of which sequence b appends its first
-    ``row_counts[b]`` (int32 ``[B]`` on the device, clamped to ``[0, T]``; default
-    all).  Or, with ``cu_seqlens`` (int list or tensor of ``B + 1`` offsets),
-    packed ``[1, total, Hkv, 128]`` as for ``switch_gqa_prefill_varlen_forward``.
-    Rows that do not fit the cache any more are dropped, and the new length is
-    the capacity.  A block that already held rows takes the larger scale of its
-    own and its new rows', and its rows are rounded again where it grows.
-    """
+def _append_arguments(cache, k, v, cache_lens, row_counts, cu_seqlens):
+    """(cache_lens, row_counts, offsets on the device, offsets on the host, most
+    rows of a sequence), checked."""
     check_cache(cache)
     batch, capacity, heads, _ = cache.k.shape
     dev = cache.k.device
@@ -182,8 +176,36 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
         raise ValueError("more rows than the cache holds")
     if not _lib.native().apart(_parts(cache), (k, v, lens)):
         raise ValueError("K, V and the cache's tensors must not overlap in memory")
+    return lens, row_counts, cu, host_cu, most
+
+
+def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tensor,
+                           cache_lens: torch.Tensor, *,
+                           row_counts: Optional[torch.Tensor] = None,
+                           cu_seqlens=None) -> torch.Tensor:
+    """Quantise new rows into the cache, behind each sequence's ``cache_lens[b]``
+    valid ones; returns the new lengths, int32 ``[B]`` (``cache_lens`` itself is
+    left as it is).
+
+    ``k``/``v``: bf16 ``[B, T, Hkv, 128]``, of which sequence b appends its first
+    ``row_counts[b]`` (int32 ``[B]`` on the device, clamped to ``[0, T]``; default
+    all).  Or, with ``cu_seqlens`` (int list or tensor of ``B + 1`` offsets),
+    packed ``[1, total, Hkv, 128]`` as for ``switch_gqa_prefill_varlen_forward``.
+    Rows that do not fit the cache any more are dropped, and the new length is
+    the capacity.  A block that already held rows takes the larger scale of its
+    own and its new rows', and its rows are rounded again where it grows.
+    """
+    lens, cu, host_cu = cache_lens, None, []
+    tensors = _parts(cache)
+    if cu_seqlens is None and _all_tensors(*tensors, k, v, lens) and _lib.native().append_ok(
+            *tensors, int(cache.block_size), k, v, lens, row_counts):
+        most = k.shape[1]
+    else:
+        lens, row_counts, cu, host_cu, most = _append_arguments(cache, k, v, cache_lens, row_counts,
+                                                                cu_seqlens)
+    dev = cache.k.device
     with _lib.on_device(dev):
-        return _lib.native().cache_append(k, v, cu, host_cu, row_counts, lens, *_parts(cache), most,
+        return _lib.native().cache_append(k, v, cu, host_cu, row_counts, lens, *tensors, most,
                                           cache.block_size, _CODES[cache.k.dtype],
                                           _lib.stream_handle(dev))
 
@@ -198,20 +220,24 @@ def switch_kv_cache_read(cache: SwitchKVCache, starts: Union[int, torch.Tensor],
     come out as 0.  With the power-of-two scales that this package writes the
     values are exact in bf16.
     """
-    check_cache(cache)
-    dev, batch = cache.k.device, cache.k.shape[0]
-    if rows < 0:
-        raise ValueError("rows must not be negative")
-    if isinstance(starts, torch.Tensor):
-        first, starts = 0, check_lens(starts, batch, dev, "starts")
-    else:
+    first, tensors = 0, _parts(cache)
+    if not isinstance(starts, torch.Tensor):
         first, starts = int(starts), None
-        if not 0 <= first < 2 ** 31:
-            raise ValueError("starts must not be negative")
-    if cache_lens is not None:
-        cache_lens = check_lens(cache_lens, batch, dev, "cache_lens")
+    if rows < 0 or not _all_tensors(*tensors) or not _lib.native().read_ok(
+            *tensors, int(cache.block_size), starts, cache_lens):
+        check_cache(cache)
+        if rows < 0:
+            raise ValueError("rows must not be negative")
+        batch, dev = cache.k.shape[0], cache.k.device
+        if starts is not None:
+            starts = check_lens(starts, batch, dev, "starts")
+        if cache_lens is not None:
+            cache_lens = check_lens(cache_lens, batch, dev, "cache_lens")
+    if not 0 <= first < 2 ** 31:
+        raise ValueError("starts must not be negative")
+    dev = cache.k.device
     with _lib.on_device(dev):
-        return _lib.native().cache_read(*_parts(cache), starts, first, cache_lens, int(rows),
+        return _lib.native().cache_read(*tensors, starts, first, cache_lens, int(rows),
                                         cache.block_size, _CODES[cache.k.dtype],
                                         _lib.stream_handle(dev))
 

@@ -251,6 +251,39 @@ bool apart(const std::vector<Tensor>& written, const std::vector<Tensor>& read) 
   return true;
 }
 
+bool lens_ok(const Tensor& t, const Tensor& k) {
+  return t.scalar_type() == at::kInt && t.layout() == at::kStrided && t.dim() == 1 && t.size(0) == k.size(0) &&
+         t.is_contiguous() && t.device() == k.device();
+}
+
+// Whether a whole call's arguments meet every precondition, in their usual form:
+// where not, the Python layer looks closer and raises, or makes them so.
+bool append_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t block,
+               const Tensor& new_k, const Tensor& new_v, const Tensor& lens, const optional<Tensor>& counts) {
+  return cache_ok(k, v, ks, vs, block) && new_k.scalar_type() == at::kBFloat16 &&
+         new_v.scalar_type() == at::kBFloat16 && new_k.layout() == at::kStrided &&
+         new_v.layout() == at::kStrided && new_k.device() == k.device() && new_v.device() == k.device() &&
+         new_k.dim() == 4 && new_v.sizes() == new_k.sizes() && new_k.size(0) == k.size(0) &&
+         new_k.size(1) <= k.size(1) && new_k.size(2) == k.size(2) && new_k.size(3) == 128 &&
+         new_k.is_contiguous() && new_v.is_contiguous() && lens_ok(lens, k) &&
+         (!counts.has_value() || lens_ok(*counts, k)) && apart({k, v, ks, vs}, {new_k, new_v, lens});
+}
+
+bool read_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t block,
+             const optional<Tensor>& starts, const optional<Tensor>& lens) {
+  return cache_ok(k, v, ks, vs, block) && (!starts.has_value() || lens_ok(*starts, k)) && (!lens.has_value() || lens_ok(*lens, k));
+}
+
+bool decode_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,
+               int64_t block, const Tensor& lens, const Tensor& full) {
+  return cache_ok(k, v, ks, vs, block) && q.scalar_type() == at::kBFloat16 && q.layout() == at::kStrided &&
+         q.dim() == 4 && q.is_contiguous() && q.device() == k.device() && q.size(0) == k.size(0) &&
+         q.size(1) == 1 && q.size(3) == 128 && q.size(2) > 0 && q.size(2) % k.size(2) == 0 &&
+         q.size(2) / k.size(2) <= 8 && lens_ok(lens, k) && full.scalar_type() == at::kBool &&
+         full.layout() == at::kStrided && full.dim() == 1 && full.size(0) == k.size(0) &&
+         full.is_contiguous() && full.device() == k.device();
+}
+
 // The new lengths.  cu: packed offsets on the device, or host_cu (not empty).
 Tensor cache_append(const Tensor& new_k, const Tensor& new_v, const optional<Tensor>& cu,
                     const std::vector<int32_t>& host_cu, const optional<Tensor>& counts, const Tensor& lens, const Tensor& k, const Tensor& v,
@@ -394,6 +427,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_forward", &decode_forward);
   m.def("cache_ok", &cache_ok);
   m.def("apart", &apart);
+  m.def("append_ok", &append_ok);
+  m.def("read_ok", &read_ok);
+  m.def("decode_ok", &decode_ok);
   m.def("cache_append", &cache_append);
   m.def("cache_read", &cache_read);
   m.def("cache_decode", &cache_decode);

@@ -38,6 +38,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include <atomic>
 #include <string>
 
 #include "cache_code.h"
@@ -422,11 +423,14 @@ constexpr int kSplitTarget = 3;
 constexpr int kSplitRoom = 6;
 static_assert(2 * kSplitTarget <= kSplitRoom, "every share has its partial");
 
+// Compute units of the current device, looked up once per device.
 int cu_count() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -25,11 +25,10 @@
 // one ahead, took 570 us; two ahead 495; the final sum by lane moves instead of
 // shuffles through LDS 477; no workgroups without work 463.
 //
-// Rows may be cut: the blocks of both lists form one axis (full first), cut at
-// multiples of `chunk` blocks, and a workgroup takes the blocks of one chunk that
-// its keys are seen by, so that workgroups of different keys read the same rows
-// at the same time.  Each leaves 256 fp32 sums, added in the chunks' order by
-// a last kernel: no atomics.
+// Rows may be cut: each list's blocks at multiples of its chunk, and a workgroup
+// takes the blocks of one chunk that its keys are seen by, so that workgroups of
+// different keys read the same rows at the same time.  Each leaves 256 fp32 sums,
+// added in the chunks' order, the full list's first, by a last kernel: no atomics.
 
 #include <limits.h>
 #include <math.h>
@@ -82,7 +81,8 @@ struct WeightParams {
   int32_t* ranges;           // [2][tiles][2]: the blocks of each list that see a key tile
   float* part;               // [tile][hkv][chunks][256]
   int32_t* host;             // pinned words that the lists' check reports to, one per workgroup, or null
-  int32_t tiles, chunk, chunks, prep_wgs, check_wgs;
+  int32_t chunk[2], chunks[2];   // blocks per chunk and chunks of each list
+  int32_t tiles, prep_wgs, check_wgs;
   int32_t seq_q, seq_kv, total_q, total_kv;
   int32_t hq, hkv, group, window;
   float c;                   // sm_scale * log2(e)
@@ -167,32 +167,27 @@ __global__ __launch_bounds__(kThreads) void weights_prep_kernel(const WeightPara
     block_ranges<kMeta, kKeys, kRows>(p, p.tiles, wg - p.prep_wgs);
 }
 
-// The x-th workgroup of key tile t: the chunk it takes and the blocks of that
-// chunk, on the axis of both lists, that see the tile: [a, a_end) of the full
-// list, then [b, b_end) of the local one.  Chunks of the full list come from its
-// end on, which every tile shares.
+// The x-th workgroup of key tile t: the list and chunk that it takes and the blocks
+// of that chunk that see the tile, [a, a_end) on the axis of both lists.  Chunks of
+// the full list come first, from its end on, which every tile shares.
 struct Share {
-  int chunk, a, a_end, b, b_end;
+  int part, a, a_end;
 };
 __device__ __forceinline__ bool chunk_share(const WeightParams& p, int t, int x, Share& sh) {
   const int2 f = *reinterpret_cast<const int2*>(p.ranges + 2 * t);
-  int2 l = *reinterpret_cast<const int2*>(p.ranges + 2 * (p.tiles + t));
-  l.x += p.blocks[0];
-  l.y += p.blocks[0];
-  const int f_last = f.x < f.y ? (f.y - 1) / p.chunk : -1, f_first = f.x < f.y ? f.x / p.chunk : 0;
+  const int2 l = *reinterpret_cast<const int2*>(p.ranges + 2 * (p.tiles + t));
+  const int f_last = f.x < f.y ? (f.y - 1) / p.chunk[0] : -1, f_first = f.x < f.y ? f.x / p.chunk[0] : 0;
   const int nf = f_last - f_first + 1;
-  if (x < nf) {
-    sh.chunk = f_last - x;
-  } else {
-    if (l.x >= l.y) return false;
-    sh.chunk = max(l.x / p.chunk, f_last + 1) + (x - nf);
-    if (sh.chunk > (l.y - 1) / p.chunk) return false;
-  }
-  const int lo = sh.chunk * p.chunk, hi = lo + p.chunk;
-  sh.a = max(f.x, lo);
-  sh.a_end = max(min(f.y, hi), sh.a);
-  sh.b = max(l.x, lo);
-  sh.b_end = max(min(l.y, hi), sh.b);
+  const int b = x < nf ? 0 : 1;
+  if (b == 1 && l.x >= l.y) return false;
+  const int c = b == 0 ? f_last - x : l.x / p.chunk[1] + (x - nf);
+  const int2 r = b == 0 ? f : l;
+  const int lo = c * p.chunk[b], hi = lo + p.chunk[b];
+  if (lo >= r.y) return false;
+  sh.part = b == 0 ? c : p.chunks[0] + c;
+  const int base = b == 0 ? 0 : p.blocks[0];
+  sh.a = base + max(r.x, lo);
+  sh.a_end = base + min(r.y, hi);
   return true;
 }
 
@@ -204,8 +199,8 @@ __global__ __launch_bounds__(kThreads, 2) void weights_kernel(const WeightParams
   const int t = rest % p.tiles;
   Share sh;
   if (!chunk_share(p, t, rest / p.tiles, sh)) return;   // uniform
-  const int na = sh.a_end - sh.a, n = na + sh.b_end - sh.b;   // at least 1
-  auto block_at = [&](int i) { return i < na ? sh.a + i : sh.b + (i - na); };
+  const int n = sh.a_end - sh.a;   // at least 1
+  auto block_at = [&](int i) { return sh.a + i; };
   const int tid = threadIdx.x, lane = tid & 63;
   auto uniform = [](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x))); };
   const int wave = static_cast<int>(uniform(tid >> 6));
@@ -347,7 +342,7 @@ __global__ __launch_bounds__(kThreads, 2) void weights_kernel(const WeightParams
   __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);   // no load into LDS outlives the workgroup
   // Sums over the 32 row lanes, with lane moves only: neighbours, pairs, the mirror
   // image within 8 and 16 lanes, and the other 16.
-  float* out = p.part + ((static_cast<int64_t>(t) * p.hkv + kvh) * p.chunks + sh.chunk) * kKeys + wave * kWaveKeys;
+  float* out = p.part + ((static_cast<int64_t>(t) * p.hkv + kvh) * (p.chunks[0] + p.chunks[1]) + sh.part) * kKeys + wave * kWaveKeys;
   float mine = 0.f;   // lane r: element r % 16 of tile r / 16
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -371,18 +366,14 @@ __global__ __launch_bounds__(kThreads, 2) void weights_kernel(const WeightParams
 __global__ __launch_bounds__(kThreads) void weights_reduce_kernel(const WeightParams p) {
   const int kvh = blockIdx.x % p.hkv, t = blockIdx.x / p.hkv;
   const int key = t * kKeys + threadIdx.x;
-  const int32_t* f = p.ranges + 2 * t;
-  const int32_t* l = p.ranges + 2 * (p.tiles + t);
-  const float* part = p.part + (static_cast<int64_t>(t) * p.hkv + kvh) * p.chunks * kKeys + threadIdx.x;
+  const float* part = p.part + (static_cast<int64_t>(t) * p.hkv + kvh) * (p.chunks[0] + p.chunks[1]) * kKeys + threadIdx.x;
   float w = 0.f;
-  int from = 0;
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const int lo = (b ? l[0] + p.blocks[0] : f[0]), hi = (b ? l[1] + p.blocks[0] : f[1]);
-    if (lo >= hi) continue;
-    const int end = (hi - 1) / p.chunk + 1;
-    for (int s = max(lo / p.chunk, from); s < end; ++s) w += part[static_cast<int64_t>(s) * kKeys];
-    from = end;   // a chunk that holds blocks of both lists counts once
+    const int2 r = *reinterpret_cast<const int2*>(p.ranges + 2 * (b * p.tiles + t));
+    if (r.x >= r.y) continue;
+    const int end = (r.y - 1) / p.chunk[b] + 1;
+    for (int s = r.x / p.chunk[b]; s < end; ++s) w += part[static_cast<int64_t>(b * p.chunks[0] + s) * kKeys];
   }
   if (key < p.total_kv) {
     const int b = key / p.seq_kv;
@@ -391,19 +382,19 @@ __global__ __launch_bounds__(kThreads) void weights_reduce_kernel(const WeightPa
 }
 
 struct Layout {
-  int64_t tiles, blocks[2], chunk, chunks;
+  int64_t tiles, blocks[2], chunk[2], chunks[2];
   size_t off_ranges, off_part, bytes;
 };
 
 // Chunks: on small grids about as many as run at once (two workgroups per CU; half of
 // the chunks see nothing); on large ones short enough that the workgroups outnumber
-// the slots several times over.  (Chunks of 4, 8, 16 and 32 blocks: B2 S980 Hq8/Hkv2,
-// 245 blocks and 16 pairs of key tile and head, 26.7 us, 22.5, -, -; S2048 Hq32/Hkv8,
-// 256 blocks and 64 pairs, 46, -, 35.6, 43.  S16384: 64 blocks
-// 450 us, 32 472, 96 467, 128 462, 192 458; S8192 of 5 heads per KV head 230, 228,
-// 229, 261, 247.  S1024, 128 blocks: at least 4 a chunk 16.6 us, 8 19.4, 2 19.0.)
+// the slots several times over, the local list's half as long, since they run last.
+// (Chunks of 4, 8, 16 and 32 blocks: B2 S980 Hq8/Hkv2, 245 blocks and 16 pairs of key
+// tile and head, 26.7 us, 22.5, -, -; S2048 Hq32/Hkv8, 256 blocks and 64 pairs, 46, -,
+// 35.6, 43.  S16384: 128 and 64 460 us, 64 and 64 466, 64 and 32 467, 128 and 32 462;
+// S8192 of 5 heads per KV head 230, 236, 225, 222.)
 constexpr int64_t kMinChunk = 4;
-constexpr int64_t kMaxChunk = 64;
+constexpr int64_t kMaxChunk = 128;
 constexpr int64_t kWantWgs = 768;
 constexpr int64_t kMaxPartBytes = int64_t{64} << 20;
 
@@ -414,14 +405,16 @@ Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full,
   L.blocks[1] = ceil_div(n_local * group, kRows);
   const int64_t axis = std::max<int64_t>(1, L.blocks[0] + L.blocks[1]);
   const int64_t pairs = L.tiles * heads_kv;
-  L.chunk = std::min(kMaxChunk, std::max(kMinChunk, ceil_div(axis * pairs, kWantWgs)));
-  const int64_t most = std::max<int64_t>(1, kMaxPartBytes / (pairs * kKeys * 4));   // chunks per pair
-  L.chunk = std::max(L.chunk, ceil_div(axis, most));
-  L.chunks = ceil_div(axis, L.chunk);
+  int64_t chunk = std::min(kMaxChunk, std::max(kMinChunk, ceil_div(axis * pairs, kWantWgs)));
+  const int64_t most = std::max<int64_t>(2, kMaxPartBytes / (pairs * kKeys * 4));   // chunks per pair
+  chunk = std::max(chunk, ceil_div(3 * axis, 2 * most));
+  L.chunk[0] = chunk;
+  L.chunk[1] = chunk >= 64 ? chunk / 2 : chunk;
+  for (int b = 0; b < 2; ++b) L.chunks[b] = ceil_div(L.blocks[b], L.chunk[b]);
   auto al = [](size_t x) { return (x + 255) & ~size_t{255}; };
   size_t o = al(static_cast<size_t>(axis * heads_kv) * kInfoBytes);
   L.off_ranges = o;  o = al(o + static_cast<size_t>(2 * L.tiles) * 2 * sizeof(int32_t));
-  L.off_part = o;    o = al(o + static_cast<size_t>(pairs * L.chunks) * kKeys * sizeof(float));
+  L.off_part = o;    o = al(o + static_cast<size_t>(pairs * (L.chunks[0] + L.chunks[1])) * kKeys * sizeof(float));
   L.bytes = o;
   return L;
 }
@@ -480,7 +473,7 @@ static int launch_key_weights(
     const int64_t reach = std::min<int64_t>(window, seq_q), parts = kKeys / seq_kv + 2;
     local = std::min(local, (kKeys + parts * reach) * group / kRows + 2);
   }
-  const int64_t shares = std::min(L.chunks, ceil_div(L.blocks[0], L.chunk) + ceil_div(local, L.chunk) + 1);
+  const int64_t shares = L.chunks[0] + std::min(L.chunks[1], ceil_div(local, L.chunk[1]) + 1);
   const int64_t pairs = L.tiles * heads_kv, grid = pairs * std::max<int64_t>(shares, 1);
   const int64_t prep = ceil_div(L.blocks[0] + L.blocks[1], 8) * heads_kv, ranges = ceil_div(2 * L.tiles, kThreads / 64);
   if (grid > INT32_MAX || prep + ranges > INT32_MAX - SWATTN_KEY_WEIGHTS_HOST_WORDS) return invalid(n + ": grid too large");
@@ -505,8 +498,10 @@ static int launch_key_weights(
   p.ranges = reinterpret_cast<int32_t*>(ws + L.off_ranges);
   p.part = reinterpret_cast<float*>(ws + L.off_part);
   p.tiles = static_cast<int32_t>(L.tiles);
-  p.chunk = static_cast<int32_t>(std::min<int64_t>(L.chunk, INT32_MAX / 2));
-  p.chunks = static_cast<int32_t>(L.chunks);
+  for (int b = 0; b < 2; ++b) {
+    p.chunk[b] = static_cast<int32_t>(L.chunk[b]);
+    p.chunks[b] = static_cast<int32_t>(L.chunks[b]);
+  }
   p.prep_wgs = static_cast<int32_t>(prep);
   p.seq_q = static_cast<int32_t>(seq_q);
   p.seq_kv = static_cast<int32_t>(seq_kv);

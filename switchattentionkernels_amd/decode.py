@@ -16,7 +16,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .cache import _CODES, SwitchKVCache, check_cache, check_lens, check_weights
+from .cache import (_CODES, SwitchKVCache, _all_tensors, check_cache, check_lens,
+                    check_weights)
 
 LOG2E = 1.4426950408889634
 
@@ -76,6 +77,30 @@ def switch_gqa_decode_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     return out, lse
 
 
+def _check_quantized(q, cache: SwitchKVCache, cache_lens, full_mask):
+    """(cache_lens, full_mask) for the kernels, or raise."""
+    check_cache(cache)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("Switch Attention decode requires BF16 Q")
+    if not q.is_contiguous():
+        raise ValueError("Q must be contiguous")
+    if q.ndim != 4 or q.shape[1] != 1 or q.shape[3] != 128:
+        raise ValueError("q must be [B,1,Hq,128]")
+    batch, _, heads, _ = (int(x) for x in q.shape)
+    if cache.k.shape[0] != batch:
+        raise ValueError("Q and KV cache batch sizes must match")
+    kv_heads = int(cache.k.shape[2])
+    if heads == 0 or heads % kv_heads or heads // kv_heads > 8:
+        raise ValueError("query heads must be a multiple (at most 8x) of KV heads")
+    dev = cache.k.device
+    if q.device != dev:
+        raise ValueError("Q and KV cache must be on the same device")
+    lens = check_lens(cache_lens, batch, dev, "cache_lens")
+    if full_mask.dtype != torch.bool or full_mask.shape != (batch,) or full_mask.device != dev:
+        raise ValueError("full_mask must be a bool [B] tensor on the device of Q")
+    return lens, full_mask.contiguous()
+
+
 def switch_gqa_decode_quantized_forward(
         q: torch.Tensor, cache: SwitchKVCache, cache_lens: torch.Tensor, full_mask: torch.Tensor, *,
         window_size: int = 1024, sm_scale: Optional[float] = None,
@@ -91,36 +116,23 @@ def switch_gqa_decode_quantized_forward(
     squeeze = q.ndim == 3
     if squeeze:
         q = q.unsqueeze(1)
-    check_cache(cache)
-    if q.dtype != torch.bfloat16:
-        raise TypeError("Switch Attention decode requires BF16 Q")
-    if not q.is_contiguous():
-        raise ValueError("Q must be contiguous")
-    if q.ndim != 4 or q.shape[1] != 1 or q.shape[3] != 128:
-        raise ValueError("q must be [B,1,Hq,128]")
-    batch, _, heads, dim = (int(x) for x in q.shape)
-    if cache.k.shape[0] != batch:
-        raise ValueError("Q and KV cache batch sizes must match")
-    kv_heads = int(cache.k.shape[2])
-    if heads == 0 or heads % kv_heads or heads // kv_heads > 8:
-        raise ValueError("query heads must be a multiple (at most 8x) of KV heads")
+    lens, full = cache_lens, full_mask
+    if not _all_tensors(q, cache.k, cache.v, cache.k_scales, cache.v_scales, lens, full) or \
+            not _lib.native().decode_ok(q, cache.k, cache.v, cache.k_scales, cache.v_scales,
+                                        int(cache.block_size), lens, full):
+        lens, full = _check_quantized(q, cache, cache_lens, full_mask)
     if window_size <= 0:
         raise ValueError("window_size must be positive")
-    dev = cache.k.device
-    if q.device != dev:
-        raise ValueError("Q and KV cache must be on the same device")
-    lens = check_lens(cache_lens, batch, dev, "cache_lens")
-    if full_mask.dtype != torch.bool or full_mask.shape != (batch,) or full_mask.device != dev:
-        raise ValueError("full_mask must be a bool [B] tensor on the device of Q")
+    dev = q.device
     if key_weights is not None:
         check_weights(key_weights, cache)
         if not _lib.native().apart((key_weights,), (q, cache.k, cache.v, cache.k_scales,
-                                                    cache.v_scales, lens, full_mask)):
+                                                    cache.v_scales, lens, full)):
             raise ValueError("key_weights must not share memory with the other arguments")
-    scale = ((1.0 / dim) ** 0.5 if sm_scale is None else float(sm_scale)) * LOG2E
+    scale = (128 ** -0.5 if sm_scale is None else float(sm_scale)) * LOG2E
     with _lib.on_device(dev):
         out, lse = _lib.native().cache_decode(q, cache.k, cache.v, cache.k_scales, cache.v_scales,
-                                              lens, full_mask.contiguous(), key_weights,
+                                              lens, full, key_weights,
                                               int(window_size), cache.block_size,
                                               _CODES[cache.k.dtype], scale,
                                               _lib.stream_handle(dev), _lib.like(q))
