@@ -67,7 +67,8 @@ def cache_values(codes: torch.Tensor, scales: torch.Tensor, block: int) -> np.nd
     """[B, L, Hkv, 128] in 64 bits."""
     n = codes.shape[1]
     s = np.repeat(scales.double().cpu().numpy(), block, axis=2)[:, :, :n]
-    return code_values(codes) * s.transpose(0, 2, 1)[..., None]
+    with np.errstate(invalid="ignore"):
+        return code_values(codes) * s.transpose(0, 2, 1)[..., None]
 
 
 def append(codes: torch.Tensor, scales: torch.Tensor, block: int, new, lens):
@@ -99,8 +100,9 @@ def append(codes: torch.Tensor, scales: torch.Tensor, block: int, new, lens):
                 sc[b, h, j] = s
                 with np.errstate(invalid="ignore"):
                     raw[b, lo:hi, h] = round_code(x / np.float32(s), dtype)
-    values = raw.astype(np.float64) * np.repeat(sc.astype(np.float64), block, axis=2)[:, :, :cap] \
-        .transpose(0, 2, 1)[..., None]
+    with np.errstate(invalid="ignore"):
+        values = raw.astype(np.float64) * np.repeat(sc.astype(np.float64), block, axis=2)[:, :, :cap] \
+            .transpose(0, 2, 1)[..., None]
     return values, sc, after
 
 

@@ -354,6 +354,39 @@ def test_decode_nan_blocks_show(dtype):
     assert torch.isnan(w[0, 0]).all() and torch.isnan(w[2]).sum() == 0
 
 
+def test_decode_nan_codes_and_queries_stay_where_they_are():
+    """A NaN code of a cache made elsewhere: a key's in its head's rows, a value's in
+    its dimension; a NaN or infinite query in its own row."""
+    gen = torch.Generator().manual_seed(28)
+    n, h, grp = 300, 2, 4
+    cache = _filled(gen, 2, n, h, E4M3, 32, [300, 300])
+    q = _q(gen, 2, h * grp)
+    full = torch.tensor([True, True], device=DEV)
+    clean, clean_lse = switch_gqa_decode_quantized_forward(q, cache, _int32([300, 300]), full)
+    keep = cache.v[0, 7, 1, 5].clone().view(torch.uint8)
+    cache.v.view(torch.uint8)[0, 7, 1, 5] = 0x7f
+    o, lse = switch_gqa_decode_quantized_forward(q, cache, _int32([300, 300]), full)
+    assert torch.isnan(o[0, 0, grp:, 5]).all() and torch.isnan(o).sum() == grp and torch.equal(lse, clean_lse)
+    cache.v.view(torch.uint8)[0, 7, 1, 5] = keep
+    cache.k.view(torch.uint8)[1, 299, 0, 127] = 0xff
+    o, lse = switch_gqa_decode_quantized_forward(q, cache, _int32([300, 300]), full)
+    assert torch.isnan(o[1, 0, :grp]).all() and torch.isnan(lse).sum() == grp
+    assert torch.equal(o[0], clean[0]) and torch.equal(o[1, 0, grp:], clean[1, 0, grp:])
+    o, lse = switch_gqa_decode_quantized_forward(q, cache, _int32([300, 299]), full)   # behind the end
+    assert not torch.isnan(o).any() and not torch.isnan(lse).any()
+    for bad in (math.nan, math.inf):
+        q2 = q.clone()
+        q2[0, 0, 2, 9] = bad
+        w = torch.zeros(2, h, n, device=DEV)
+        o, lse = switch_gqa_decode_quantized_forward(q2, cache, _int32([300, 299]), full, key_weights=w)
+        others = torch.ones(h * grp, dtype=torch.bool, device=DEV)
+        others[2] = False
+        assert torch.isnan(o[0, 0, 2]).all() and torch.equal(o[0, 0, others], clean[0, 0, others])
+        assert not torch.isnan(o[1]).any() and not torch.isnan(w[0, 1]).any() and not torch.isnan(w[1]).any()
+    values, _ = switch_kv_cache_read(cache, 0, n)
+    assert torch.isnan(values[1, 299, 0, 127]) and torch.isnan(values).sum() == 1
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_decode_score_jumps_and_large_scales(dtype):
     """Running maxima that move many times, far apart, and caches whose values are
