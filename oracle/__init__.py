@@ -16,6 +16,9 @@ Modules
               (V:103-249) and its backward (the derivative of that
               forward; the reference has none, V:14-15), plus a float64
               pure-Python brute force for tiny inputs used to pin both.
+``cache``     the 8-bit KV cache: codes and scales (bit-exact), decode over
+              them and the attention weight that each key received (float64).
+              The reference has no cache.
 
 Pinning (how each function is checked, see ``tests/test_oracle.py``)
 --------------------------------------------------------------------
@@ -50,6 +53,10 @@ Pinning (how each function is checked, see ``tests/test_oracle.py``)
                            by exactly ``-scale * (dO . (out - O)) * P k`` per
                            row (``delta_shift_bound``), and a dropped or
                            doubled Delta breaks that bound.
+* ``cache``                (``tests/test_cache_cpu.py``) e4m3 rounding == torch's
+                           cast at every value, midpoint and neighbour; scales
+                           == the smallest power of two by search; decode and
+                           its weights == a loop over heads and keys.
 
 Parity of the exact bf16 bits produced by the reference's TileLang kernels is
 unpinned (those kernels need TileLang + Hopper, neither exists here); the

@@ -27,8 +27,8 @@
 //   bf16(p).  Their sum carries 16 bits of p at no further matrix instruction.
 //
 // Measured, Hkv 8, as a large copy's 5.2 TB/s goes: B16 L16384-32768 Hq64 int8 all
-// full 163 us, 4.95 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full 0.25
-// 71 us, of which the merge and its launch are about 8; B1 L4096 Hq32 12 us, bound
+// full 159-163 us, 4.95-5.06 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full
+// 0.25 71-73 us, of which the merge and its launch are about 8; B1 L4096 Hq32 12 us, bound
 // by dependent latencies (plan, first keys, combine, merge) and, at that length, by
 // the host's calls.  Two workgroups per CU with loads three steps ahead: 12.8 us
 // (B1), 77 (B64); four with one step ahead 13 and 85.  Joining the pieces in the same
