@@ -264,11 +264,14 @@ def switch_kv_cache_evict(cache: SwitchKVCache, cache_lens: torch.Tensor, key_we
     ``budget`` rows), which must not share memory with the source: two caches
     in turn let a captured decode loop go on.
     """
-    check_cache(cache)
+    lens, tensors = cache_lens, _parts(cache)
+    if not _all_tensors(*tensors, lens, key_weights) or not _lib.native().evict_ok(
+            *tensors, int(cache.block_size), lens, key_weights):
+        check_cache(cache)
+        lens = check_lens(cache_lens, cache.k.shape[0], cache.k.device, "cache_lens")
+        check_weights(key_weights, cache)
     batch, n, heads, _ = cache.k.shape
     dev = cache.k.device
-    lens = check_lens(cache_lens, batch, dev, "cache_lens")
-    check_weights(key_weights, cache)
     budget, recent = int(budget), int(recent)
     if budget < 1:
         raise ValueError("budget must be positive")
@@ -282,23 +285,24 @@ def switch_kv_cache_evict(cache: SwitchKVCache, cache_lens: torch.Tensor, key_we
         rows = n if capacity is None else int(capacity)
         if rows < budget:
             raise ValueError("the destination must hold at least budget rows")
-        out = build_switch_kv_cache(batch, rows, heads, device=dev, dtype=cache.k.dtype,
-                                    block_size=cache.block_size)
-        out_weights = torch.empty(batch, heads, rows, dtype=torch.float32, device=dev)
-    else:
-        check_cache(out)
-        if (out.k.shape[0], out.k.shape[2]) != (batch, heads) or out.k.device != dev:
-            raise ValueError("out must have the cache's batch size, KV heads and device")
-        if out.k.dtype != cache.k.dtype or out.block_size != cache.block_size:
-            raise ValueError("out must have the cache's dtype and block_size")
-        if out.k.shape[1] < budget:
-            raise ValueError("the destination must hold at least budget rows")
-        check_weights(out_weights, out)
-        if not _lib.native().apart(_parts(out) + (out_weights,), _parts(cache) + (key_weights, lens)):
-            raise ValueError("the destination's tensors must not share memory, with the source or "
-                             "each other")
+        with _lib.on_device(dev):
+            *made, out_weights, new_lens = _lib.native().cache_evict_new(
+                *tensors, key_weights, lens, rows, cache.block_size, _CODES[cache.k.dtype], budget,
+                recent, _lib.stream_handle(dev))
+        return SwitchKVCache(*made, cache.block_size), new_lens, out_weights
+    check_cache(out)
+    if (out.k.shape[0], out.k.shape[2]) != (batch, heads) or out.k.device != dev:
+        raise ValueError("out must have the cache's batch size, KV heads and device")
+    if out.k.dtype != cache.k.dtype or out.block_size != cache.block_size:
+        raise ValueError("out must have the cache's dtype and block_size")
+    if out.k.shape[1] < budget:
+        raise ValueError("the destination must hold at least budget rows")
+    check_weights(out_weights, out)
+    if not _lib.native().apart(_parts(out) + (out_weights,), tensors + (key_weights, lens)):
+        raise ValueError("the destination's tensors must not share memory, with the source or "
+                         "each other")
     with _lib.on_device(dev):
-        new_lens = _lib.native().cache_evict(*_parts(cache), key_weights, lens, *_parts(out),
+        new_lens = _lib.native().cache_evict(*tensors, key_weights, lens, *_parts(out),
                                              out_weights, cache.block_size, _CODES[cache.k.dtype],
                                              budget, recent, _lib.stream_handle(dev))
     return out, new_lens, out_weights

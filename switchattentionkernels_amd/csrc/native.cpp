@@ -274,6 +274,14 @@ bool read_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& v
   return cache_ok(k, v, ks, vs, block) && (!starts.has_value() || lens_ok(*starts, k)) && (!lens.has_value() || lens_ok(*lens, k));
 }
 
+bool evict_ok(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t block,
+              const Tensor& lens, const Tensor& weights) {
+  const int64_t want[3] = {k.dim() == 4 ? k.size(0) : 0, k.dim() == 4 ? k.size(2) : 0, k.dim() == 4 ? k.size(1) : 0};
+  return cache_ok(k, v, ks, vs, block) && lens_ok(lens, k) && weights.scalar_type() == at::kFloat &&
+         weights.layout() == at::kStrided && weights.sizes() == at::IntArrayRef(want, 3) &&
+         weights.is_contiguous() && weights.device() == k.device();
+}
+
 bool decode_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,
                int64_t block, const Tensor& lens, const Tensor& full) {
   return cache_ok(k, v, ks, vs, block) && q.scalar_type() == at::kBFloat16 && q.layout() == at::kStrided &&
@@ -416,6 +424,21 @@ Tensor cache_evict(const Tensor& k, const Tensor& v, const Tensor& ks, const Ten
   return out;
 }
 
+// The same into a new cache of `rows` rows: (k, v, k_scales, v_scales, weights, lengths).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_evict_new(
+    const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& weights,
+    const Tensor& lens, int64_t rows, int64_t block, int64_t code, int64_t budget, int64_t recent,
+    int64_t stream) {
+  const Tensor out_k = at::empty({k.size(0), rows, k.size(2), k.size(3)}, k.options());
+  const Tensor out_v = at::empty(out_k.sizes(), k.options());
+  const Tensor out_ks = at::empty({k.size(0), k.size(2), (rows + block - 1) / block}, ks.options());
+  const Tensor out_vs = at::empty(out_ks.sizes(), ks.options());
+  const Tensor out_weights = at::empty({k.size(0), k.size(2), rows}, weights.options());
+  const Tensor out_lens = cache_evict(k, v, ks, vs, weights, lens, out_k, out_v, out_ks, out_vs, out_weights,
+                                      block, code, budget, recent, stream);
+  return {out_k, out_v, out_ks, out_vs, out_weights, out_lens};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -430,9 +453,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("append_ok", &append_ok);
   m.def("read_ok", &read_ok);
   m.def("decode_ok", &decode_ok);
+  m.def("evict_ok", &evict_ok);
   m.def("cache_append", &cache_append);
   m.def("cache_read", &cache_read);
   m.def("cache_decode", &cache_decode);
   m.def("prefill_key_weights", &prefill_key_weights);
   m.def("cache_evict", &cache_evict);
+  m.def("cache_evict_new", &cache_evict_new);
 }
