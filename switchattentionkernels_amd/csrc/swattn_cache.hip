@@ -253,9 +253,24 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // per step, so that ballots count and place them and the waves meet only once.
 // kPer > 0: a thread's kPer weights are read once, into registers; 0: any number,
 // read again in every pass.  Bound by latency: few workgroups for few sequences.
-// 16384 rows, 8 pairs: 26 us with 8-bit digits and five reads, 12 so; 4096 rows, 256
-// pairs: 12.7 and 9.9.
+// 16384 rows, 8 pairs: 26 us with 8-bit digits and five reads, 12 so, 10 since a search
+// ends where a whole bin stays, mostly after two digits; 4096 rows, 256 pairs: 12.7,
+// 9.9 and 9.
 constexpr int kDigits = 2048;
+
+// Inclusive sums over the lanes of a wave: shifts within 16 lanes, then the last
+// lane of each row of 16 to the rows behind it.
+__device__ __forceinline__ uint32_t wave_sums(uint32_t x) {
+  int v = static_cast<int>(x);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return static_cast<uint32_t>(v);
+}
+
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   constexpr int kWaves = kThreads / 64;
@@ -268,6 +283,8 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   const int b = static_cast<int>(pair / p.hkv);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* w = p.weights + pair * p.cache_len;
+#pragma unroll
+  for (int i = 0; i < kBins; ++i) s_hist[tid + kThreads * i] = 0;
   // The weights do not wait for the length: all rows of the cache may be read.
   float ahead[kPer > 0 ? kPer : 1];
   if constexpr (kPer > 0) {
@@ -305,9 +322,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t digits = pass == 2 ? 1023u : 2047u;
-#pragma unroll
-    for (int i = 0; i < kBins; ++i) s_hist[tid + kThreads * i] = 0;
-    __syncthreads();
+    __syncthreads();   // the bins are clear
     each([&](int64_t, uint32_t k) {
       if (pass == 0 || (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & digits], 1u);
     });
@@ -316,15 +331,12 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
     uint32_t c[kBins], sum = 0;
 #pragma unroll
     for (int j = 0; j < kBins; ++j) {
-      c[j] = s_hist[kDigits - 1 - kBins * tid - j];
+      uint32_t& bin = s_hist[kDigits - 1 - kBins * tid - j];
+      c[j] = bin;
+      bin = 0;   // for the next digit
       sum += c[j];
     }
-    uint32_t incl = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t y = static_cast<uint32_t>(__shfl_up(static_cast<int>(incl), off));
-      incl += lane >= off ? y : 0u;
-    }
+    uint32_t incl = wave_sums(sum);
     if (lane == 63) s_wave[wave] = incl;
     __syncthreads();
 #pragma unroll
@@ -345,6 +357,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
     prefix |= s_pick[0] << shift;
     mask |= digits << shift;
     need = s_pick[1];
+    if (need == s_pick[2]) break;   // uniform: all of the bin stay, whatever their other digits
   }
   // All rows above prefix stay, and the first `need` of those equal to it.
   int32_t* kept = p.kept + pair * want;

@@ -510,6 +510,17 @@ def test_evict_long_caches(n, budget, recent):
     _check_evict(cache, lens, w.to(DEV), budget, recent, capacity=budget)
 
 
+@pytest.mark.parametrize("bits", [1, 10, 21, 31])
+def test_evict_weights_that_differ_in_their_last_bits(bits):
+    """The search ends after one, two or all three digits of a weight."""
+    gen = torch.Generator().manual_seed(bits)
+    cache = _filled(gen, 2, 3000, 2, INT8, 64, [3000, 1500])
+    low = torch.randint(0, 2 ** bits, (2, 2, 3000), generator=gen)
+    w = ((0x3f800000 if bits < 23 else 0) + low).clamp_max(0x7f800000).to(torch.int32).view(torch.float32)
+    for budget in (1, 777, 1499):
+        _check_evict(cache, [3000, 1500], w.to(DEV), budget, 0, capacity=1500)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_evict_carries_nan_blocks_and_foreign_scales(dtype):
     gen = torch.Generator().manual_seed(4)
