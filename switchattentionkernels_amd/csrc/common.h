@@ -46,4 +46,52 @@ __device__ __forceinline__ int count_below(uint64_t mask) {
 
 __device__ __forceinline__ uint64_t wave_ballot(bool p) { return __builtin_amdgcn_ballot_w64(p); }
 
+// Inclusive sums over the lanes of a wave: shifts within 16 lanes, then the last
+// lane of each row of 16 to the rows behind it.
+__device__ __forceinline__ uint32_t wave_sums(uint32_t x) {
+  int v = static_cast<int>(x);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return static_cast<uint32_t>(v);
+}
+
+// x of a lane that a move within 16 lanes names (DPP control kMove).
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kTurn4 = 0x124, kTurn8 = 0x128;
+template <int kMove>
+__device__ __forceinline__ float lane_move(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), kMove, 0xf, 0xf, false));
+}
+// op(x, x of lane ^ 32) and of lane ^ 16, for a commutative op.
+template <class Op>
+__device__ __forceinline__ float with_lane32(float x, Op op) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class Op>
+__device__ __forceinline__ float with_lane16(float x, Op op) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// A commutative op over the wave, the same in every lane, as a butterfly over lane
+// distances 32, 16, 8, 4, 2, 1 without LDS round trips (after distance 8, x repeats
+// every 8 lanes: a turn by 4 is distance 4).
+template <class Op>
+__device__ __forceinline__ float wave_all(float x, Op op) {
+  x = with_lane16(with_lane32(x, op), op);
+  x = op(x, lane_move<kTurn8>(x));
+  x = op(x, lane_move<kTurn4>(x));
+  x = op(x, lane_move<kXor2>(x));
+  return op(x, lane_move<kXor1>(x));
+}
+struct Add {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+
 }  // namespace swattn

@@ -104,13 +104,15 @@ __device__ __forceinline__ void scan_keys(Pos keys, uint32_t cnt, Pos& keys_befo
   __shared__ uint32_t s_cnt[kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Pos ik = keys;
-  uint32_t ic = cnt;
+  const uint32_t ic = wave_sums(cnt);
+  if constexpr (sizeof(Pos) == 4) {
+    ik = wave_sums(keys);
+  } else {
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const Pos uk = __shfl_up(ik, off);
-    const uint32_t uc = __shfl_up(ic, off);
-    ik += lane >= off ? uk : Pos{0};
-    ic += lane >= off ? uc : 0u;
+    for (int off = 1; off < 64; off <<= 1) {
+      const Pos uk = __shfl_up(ik, off);
+      ik += lane >= off ? uk : Pos{0};
+    }
   }
   if (lane == 63) {
     s_keys[wave] = ik;
@@ -328,8 +330,7 @@ __device__ __forceinline__ void merge_row(const P& p, int64_t row) {
   // Maximum over the non-empty splits.
   auto holds = [](float sum) { return P::kKeepNan ? sum != 0.f : sum > 0.f; };
   float mx = holds(ml.y) ? ml.x : -INFINITY;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+  mx = wave_all(mx, Max());
   if (lane == 0) s_red[wave] = mx;
   __syncthreads();
   const float M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
@@ -337,8 +338,7 @@ __device__ __forceinline__ void merge_row(const P& p, int64_t row) {
   const float wt = (holds(ml.y) && M != -INFINITY) ? __builtin_amdgcn_exp2f(ml.x - M) : 0.f;
   s_w[tid] = wt;
   float lsum = wt * ml.y;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) lsum += __shfl_xor(lsum, off);
+  lsum = wave_all(lsum, Add());
   if (lane == 0) s_red[4 + wave] = lsum;
   __syncthreads();
   const float L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);

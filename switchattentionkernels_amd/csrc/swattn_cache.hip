@@ -257,20 +257,6 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // ends where a whole bin stays, mostly after two digits; 4096 rows, 256 pairs: 12.7,
 // 9.9 and 9.
 constexpr int kDigits = 2048;
-
-// Inclusive sums over the lanes of a wave: shifts within 16 lanes, then the last
-// lane of each row of 16 to the rows behind it.
-__device__ __forceinline__ uint32_t wave_sums(uint32_t x) {
-  int v = static_cast<int>(x);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return static_cast<uint32_t>(v);
-}
-
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   constexpr int kWaves = kThreads / 64;

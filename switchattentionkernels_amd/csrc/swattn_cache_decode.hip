@@ -28,7 +28,7 @@
 //
 // Measured, Hkv 8, as a large copy's 5.2 TB/s goes: B16 L16384-32768 Hq64 int8 all
 // full 159-163 us, 4.95-5.06 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full
-// 0.25 71-73 us, of which the merge and its launch are about 8; B1 L4096 Hq32 12 us, bound
+// 0.25 70-73 us, of which the merge and its launch are about 8; B1 L4096 Hq32 11.3 us, bound
 // by dependent latencies (plan, first keys, combine, merge) and, at that length, by
 // the host's calls.  Two workgroups per CU with loads three steps ahead: 12.8 us
 // (B1), 77 (B64); four with one step ahead 13 and 85.  Joining the pieces in the same
@@ -298,9 +298,9 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
         }
       }
       // This wave's partial: column c's sum over its four lanes, and O^T with its
-      // error columns.  acc[t][x]: dim 8 (4 g + x) + t of column c.
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
+      // error columns (by shuffles, as in the maxima's move above: lane moves there cost
+      // the loop its register allocation, B16 158 -> 161 us).  acc[t][x]: dim 8 (4 g + x) + t of column c.
+      l = with_lane32(with_lane16(l, Add()), Add());
 #pragma unroll
       for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -399,13 +399,11 @@ __global__ __launch_bounds__(256) void cache_merge_kernel(const CacheDecodeParam
       if (s < nch) ml[i] = *reinterpret_cast<const float2*>(p.part_ml + ((slot0 + s) * G + h) * 2);
       mx = fmaxf(mx, ml[i].x);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    mx = wave_all(mx, Max());
 #pragma unroll
     for (int i = 0; i < kMaxSplitsDev / 64; ++i)
       if (ml[i].y != 0.f) sum += __builtin_amdgcn_exp2f(ml[i].x - mx) * ml[i].y;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = wave_all(sum, Add());
     if (lane == 0) s_lse[h] = mx + log2f(sum);
   }
   __syncthreads();
