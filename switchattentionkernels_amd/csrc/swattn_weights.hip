@@ -386,16 +386,19 @@ struct Layout {
   size_t off_ranges, off_part, bytes;
 };
 
-// Chunks: on small grids about as many as run at once (two workgroups per CU; half of
-// the chunks see nothing); on large ones short enough that the workgroups outnumber
-// the slots several times over, the local list's half as long, since they run last.
-// (Chunks of 4, 8, 16 and 32 blocks: B2 S980 Hq8/Hkv2, 245 blocks and 16 pairs of key
-// tile and head, 26.7 us, 22.5, -, -; S2048 Hq32/Hkv8, 256 blocks and 64 pairs, 46, -,
-// 35.6, 43.  S16384: 128 and 64 460 us, 64 and 64 466, 64 and 32 467, 128 and 32 462;
-// S8192 of 5 heads per KV head 230, 236, 225, 222.)
+// Chunks: on small grids about as many workgroups with work as run at once (two per
+// CU; half of the chunks see nothing), one block longer since a pair's first and last
+// chunks are partial; on large grids short enough that the workgroups outnumber the
+// slots several times over, the local list's half as long, since they run last.
+// Workgroups wanted in all, 768, 1024 and 1024 with the block more: S2048 Hq32/Hkv8
+// 39.4 us, 36.8, 35.9; S3333 Hq24/Hkv3 71.5, -, 62.7; B4 S1024 Hq16/Hkv8 39.0, 36.4,
+// 38.8; B2 S980 Hq8/Hkv2 22.8, 26.8, 22.4; 640 and 1280 are slower nearly everywhere.
+// (S16384, full and local chunks of 128 and 64 460 us, 64 and 64 466, 64 and 32 467,
+// 128 and 32 462; one long line of blocks cut into equal shares, 2 to 8 per CU, 479 to
+// 467, and S1024 19.6 instead of 17.0.)
 constexpr int64_t kMinChunk = 4;
 constexpr int64_t kMaxChunk = 128;
-constexpr int64_t kWantWgs = 768;
+constexpr int64_t kWantWgs = 1024;
 constexpr int64_t kMaxPartBytes = int64_t{64} << 20;
 
 Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full, int64_t n_local) {
@@ -405,7 +408,7 @@ Layout layout(int64_t total_kv, int64_t heads_kv, int64_t group, int64_t n_full,
   L.blocks[1] = ceil_div(n_local * group, kRows);
   const int64_t axis = std::max<int64_t>(1, L.blocks[0] + L.blocks[1]);
   const int64_t pairs = L.tiles * heads_kv;
-  int64_t chunk = std::min(kMaxChunk, std::max(kMinChunk, ceil_div(axis * pairs, kWantWgs)));
+  int64_t chunk = std::min(kMaxChunk, std::max(kMinChunk, ceil_div(axis * pairs, kWantWgs) + 1));
   const int64_t most = std::max<int64_t>(2, kMaxPartBytes / (pairs * kKeys * 4));   // chunks per pair
   chunk = std::max(chunk, ceil_div(3 * axis, 2 * most));
   L.chunk[0] = chunk;
