@@ -557,7 +557,6 @@ static int launch_append(const void* new_k, const void* new_v, const int32_t* cu
   return launch_status(n.c_str());
 }
 
-
 extern "C" {
 
 int swattn_cache_append(const void* new_k, const void* new_v, const int32_t* cu_seqlens,

@@ -469,11 +469,12 @@ static int launch_key_weights(
     return SWATTN_EWORKSPACE;
   }
   if (!aligned256(workspace)) return invalid(n + ": workspace must be 256-byte aligned");
-  // Workgroups per tile: chunks of the full list, and of the local rows that can see
-  // a tile: window - 1 positions more than its keys, for each sequence in it.
+  // Workgroups per tile: chunks of the full list, and of the local rows between the
+  // first and the last that see the tile: for each sequence in it window - 1 positions
+  // more than its keys there, or those behind the sequence's last key, which may see none.
   int64_t local = L.blocks[1];
   if (!meta) {
-    const int64_t reach = std::min<int64_t>(window, seq_q), parts = kKeys / seq_kv + 2;
+    const int64_t reach = std::min(std::max<int64_t>(window, seq_q - seq_kv), seq_q), parts = kKeys / seq_kv + 2;
     local = std::min(local, (kKeys + parts * reach) * group / kRows + 2);
   }
   const int64_t shares = L.chunks[0] + std::min(L.chunks[1], ceil_div(local, L.chunk[1]) + 1);

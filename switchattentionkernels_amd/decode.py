@@ -133,7 +133,7 @@ def switch_gqa_decode_quantized_forward(
     with _lib.on_device(dev):
         out, lse = _lib.native().cache_decode(q, cache.k, cache.v, cache.k_scales, cache.v_scales,
                                               lens, full, key_weights,
-                                              int(window_size), cache.block_size,
+                                              min(int(window_size), 2 ** 31 - 1), cache.block_size,
                                               _CODES[cache.k.dtype], scale,
                                               _lib.stream_handle(dev), _lib.like(q))
     if squeeze:

@@ -71,7 +71,8 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
         return torch.zeros(batch, k.shape[2], kv_len, dtype=torch.float32, device=dev)
     with _lib.on_device(dev):
         out, flags = _lib.native().prefill_key_weights(q, k, lse, full, local, fs, ls, ends,
-                                                       int(window_size), scale * LOG2E, unchecked,
+                                                       min(int(window_size), 2 ** 31 - 1),
+                                                       scale * LOG2E, unchecked,
                                                        _lib.stream_handle(dev))
     if flags:
         _raise_for(flags, "full")

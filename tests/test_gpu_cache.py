@@ -279,7 +279,7 @@ def test_decode_groups(dtype, group):
     w = torch.rand(len(lens), h, n, generator=gen).to(DEV)
     _check_decode(cache, _q(gen, len(lens), group * h), lens, full, 100, w)
     _check_decode(cache, _q(gen, len(lens), group * h), lens, full, 1, w)
-    _check_decode(cache, _q(gen, len(lens), group * h), lens, full, 10 ** 6, None)
+    _check_decode(cache, _q(gen, len(lens), group * h), lens, full, 2 ** 32 + 1, None)
 
 
 @pytest.mark.parametrize("dtype,batch,n,hq,hkv,window,p,weights", [

@@ -92,6 +92,21 @@ def test_other_lengths_of_q_and_kv_and_scales(sq, skv):
         _check(got, q, k, lse.cpu(), start, end, scale)
 
 
+@pytest.mark.parametrize("b,sq,skv", [(2, 3000, 40), (3, 1000, 300), (5, 600, 257)])
+def test_many_rows_behind_the_keys_of_a_batch(b, sq, skv):
+    """Late local rows without a key lie between the sequences' rows that share a tile
+    of keys; fresh workspaces hold NaN."""
+    gen = torch.Generator().manual_seed(sq)
+    q, k = _qk(gen, b, sq, skv, 8, 2)
+    full, local = build_switch_query_indices((torch.rand(b, sq, generator=gen) < 0.1).to(DEV))
+    for w in (7, 100, 2 ** 40):
+        _, lse = switch_gqa_prefill_forward(q.to(DEV), k.to(DEV), k.to(DEV), full, local, window_size=min(w, sq))
+        torch.cuda.synchronize()
+        torch.full((2 ** 26,), math.nan, device=DEV)
+        got = switch_gqa_prefill_key_weights(q.to(DEV), k.to(DEV), lse, full, local, window_size=w)
+        _check(got, q, k, lse.cpu(), *_default_bounds(b, sq, skv, full, local, w))
+
+
 def test_packed_sequences_and_shards():
     gen = torch.Generator().manual_seed(5)
     lens = [1, 300, 0, 77, 512, 40]
