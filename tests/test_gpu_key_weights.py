@@ -254,3 +254,25 @@ def test_unchecked_lists_cannot_be_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, switch_gqa_prefill_key_weights(q, k, lse, full, local))
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_cases(seed):
+    """Random batches, lengths of Q and of K, groups, windows and routes, in memory that
+    held NaN before.  A sum has n <= 5 * 700 * 8 terms, but a lane adds one of a block of
+    32, at most 128 blocks a part, and there are fewer than 900 blocks in 250 parts:
+    (128 + 5 + 250) * 2^-24 stays below 2^-15."""
+    gen = torch.Generator().manual_seed(500 + seed)
+    pick = lambda *v: v[int(torch.randint(0, len(v), (1,), generator=gen))]  # noqa: E731
+    size = lambda hi: int(2 ** (torch.rand(1, generator=gen).item() * math.log2(hi)))  # noqa: E731
+    b, sq, skv, hkv, group = pick(1, 1, 2, 3, 5), size(700), size(700), pick(1, 2, 3), pick(1, 2, 4, 5, 8)
+    skv = pick(skv, sq)
+    w, p = size(2000), pick(0.0, 0.1, 0.25, 0.5, 0.9, 1.0)
+    print(f"seed {seed}: B{b} Sq{sq} Skv{skv} Hq{hkv * group}/{hkv} W{w} p {p}", flush=True)
+    q, k = _qk(gen, b, sq, skv, hkv * group, hkv)
+    full, local = build_switch_query_indices((torch.rand(b, sq, generator=gen) < p).to(DEV))
+    _, lse = switch_gqa_prefill_forward(q.to(DEV), k.to(DEV), k.to(DEV), full, local, window_size=w)
+    torch.cuda.synchronize()
+    torch.full((2 ** 25,), math.nan, device=DEV)
+    got = switch_gqa_prefill_key_weights(q.to(DEV), k.to(DEV), lse, full, local, window_size=w)
+    _check(got, q, k, lse.cpu(), *_default_bounds(b, sq, skv, full, local, w))
