@@ -470,6 +470,8 @@ int check_cache(const std::string& n, int32_t batch, int64_t cache_len, int32_t 
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+constexpr int64_t kMaxGrid = ((int64_t{1} << 32) - 1) / 256;   // a launch has fewer than 2^32 threads
+
 // Launch<code, block>::go(grid, stream, params...)
 template <template <int, int> class Launch, class... P>
 void by_code_and_block(int32_t codes, int32_t block, dim3 grid, hipStream_t st, const P&... p) {
@@ -548,7 +550,7 @@ static int launch_append(const void* new_k, const void* new_v, const int32_t* cu
   const int64_t most = rows < 1 ? 1 : (rows + block - 2) / block + 1;
   p.blocks = static_cast<int>(most < p.nblk ? most : p.nblk);
   const int64_t grid = static_cast<int64_t>(p.blocks) * batch * heads_kv;
-  if (grid > INT32_MAX) return invalid(n + ": grid too large");
+  if (grid > kMaxGrid) return invalid(n + ": grid too large");
   const dim3 g(static_cast<uint32_t>(grid));
   if (host != nullptr)
     by_code_and_block<LaunchAppend>(codes, block, g, as_stream(stream), p, *host);
@@ -676,7 +678,7 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
   p.budget = static_cast<int>(budget);
   p.recent = static_cast<int>(recent);
   const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_nblk;
-  if (grid > INT32_MAX) return invalid(n + ": grid too large");
+  if (grid > kMaxGrid) return invalid(n + ": grid too large");
   const dim3 gs(static_cast<uint32_t>(pairs));
   const hipStream_t hs = as_stream(stream);
   if (cache_len <= 4096)

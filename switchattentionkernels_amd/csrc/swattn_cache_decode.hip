@@ -547,7 +547,7 @@ int swattn_cache_decode_fwd(const void* q, const void* k, const void* v, const f
   const int64_t out_rows = static_cast<int64_t>(batch) * heads_q;
   p.weight_wgs = static_cast<int>((cache_len + kWeightKeys - 1) / kWeightKeys);
   const int64_t merge_grid = out_rows + (key_weights != nullptr ? pairs * p.weight_wgs : 0);
-  if (merge_grid > INT32_MAX) return invalid(n + ": grid too large");
+  if (merge_grid > ((int64_t{1} << 32) - 1) / 256) return invalid(n + ": grid too large");
   const hipStream_t st = as_stream(stream);
   const bool inline_plan = batch <= kInlineSeqs && rows <= INT32_MAX;
   if (!inline_plan)

@@ -480,7 +480,8 @@ static int launch_key_weights(
   const int64_t shares = L.chunks[0] + std::min(L.chunks[1], ceil_div(local, L.chunk[1]) + 1);
   const int64_t pairs = L.tiles * heads_kv, grid = pairs * std::max<int64_t>(shares, 1);
   const int64_t prep = ceil_div(L.blocks[0] + L.blocks[1], 8) * heads_kv, ranges = ceil_div(2 * L.tiles, kThreads / 64);
-  if (grid > INT32_MAX || prep + ranges > INT32_MAX - SWATTN_KEY_WEIGHTS_HOST_WORDS) return invalid(n + ": grid too large");
+  constexpr int64_t kMaxGrid = ((int64_t{1} << 32) - 1) / kThreads;   // a launch has fewer than 2^32 threads
+  if (grid > kMaxGrid || prep + ranges > kMaxGrid - SWATTN_KEY_WEIGHTS_HOST_WORDS) return invalid(n + ": grid too large");
   char* ws = static_cast<char*>(workspace);
   WeightParams p{};
   p.q = static_cast<const uint16_t*>(q);

@@ -542,6 +542,63 @@ def test_evict_into_a_given_cache_and_lengths_out_of_range():
     assert torch.equal(a.k.view(torch.uint8)[:2, :50], out.k.view(torch.uint8)[:2, :50])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_past_31_bits(dtype):
+    """A cache of 2 x 2.2 GB: its last rows against those of a small cache, and keys of
+    zeros before them, whose scores are 0 and whose values add nothing."""
+    gen = torch.Generator().manual_seed(9)
+    n, h, block, hq = 2_150_003, 8, 64, 8
+    at = n - 500
+    base = (at - 100) // block * block        # the small cache holds rows [base, n)
+    big = build_switch_kv_cache(1, n, h, device=DEV, dtype=dtype, block_size=block)
+    small = build_switch_kv_cache(1, n - base, h, device=DEV, dtype=dtype, block_size=block)
+    for c in (big, small):
+        for x in (c.k, c.v):
+            x.view(torch.uint8).zero_()
+        c.k_scales.fill_(2.0 ** -100)
+        c.v_scales.fill_(2.0 ** -100)
+    k, v = _rows(gen, 1, 480, h, 128).to(DEV), _rows(gen, 1, 480, h, 128).to(DEV)
+    lb, ls = (switch_kv_cache_append(c, k, v, _int32([x])) for c, x in ((big, at), (small, at - base)))
+    assert lb.tolist() == [at + 480] and ls.tolist() == [at + 480 - base]
+    rb = switch_kv_cache_read(big, base, n - base, cache_lens=lb)
+    rs = switch_kv_cache_read(small, 0, n - base, cache_lens=ls)
+    assert all(torch.equal(x, y) for x, y in zip(rb, rs)) and rb[0][0, at - base:at - base + 480].any()
+    # A window inside the small cache: both are within the bounds of the same values.
+    q = _q(gen, 1, hq)
+    full = torch.tensor([False], device=DEV)
+    _check_decode(small, q, ls.tolist(), [False], 490, None)
+    ob, eb = switch_gqa_decode_quantized_forward(q, big, lb, full, window_size=490)
+    os_, es = switch_gqa_decode_quantized_forward(q, small, ls, full, window_size=490)
+    assert (ob.float() - os_.float()).abs().max() <= 2 * 2.0 ** -8 * v.float().abs().max()
+    assert (eb - es).abs().max() <= 1e-4
+    # All keys: `at` scores of 0 beside the others'.
+    sums = torch.zeros(1, h, n, device=DEV)
+    ob, eb = switch_gqa_decode_quantized_forward(q, big, lb, ~full, key_weights=sums)
+    kk, vv = (x[0, at - base:at - base + 480].double().cpu() for x in rs)
+    sc = (q[0, 0].double().cpu()[:, None] * kk.transpose(0, 1)).sum(-1) * 128 ** -0.5
+    total = at + sc.exp().sum(-1)
+    assert (eb[0, 0].double().cpu() - total.log2()).abs().max() <= 1e-4
+    want = (sc.exp() / total[:, None])[:, None] @ vv.transpose(0, 1)
+    # P's two bf16 halves keep 16 bits: far below the output's own rounding.
+    assert ((ob[0, 0].double().cpu() - want[:, 0]).abs() <= 2.0 ** -8 * want[:, 0].abs() + 1e-4 * want.abs().max()).all()
+    ws = sums[0].double().cpu()
+    assert (ws[:, at:at + 480] * total[:, None] / sc.exp() - 1).abs().max() <= 1e-4
+    assert (ws[:, :at] * total[:, None] - 1).abs().max() <= 1e-4 and not ws[:, at + 480:].any()
+    # The heaviest rows are the last ones and a few zeros before them.
+    weights = torch.zeros(1, h, n, device=DEV)
+    weights[:, :, 5], weights[:, :, at + 3], weights[:, :, at + 77] = 3.0, 2.0, 1.0
+    kept, lk, wk = switch_kv_cache_evict(big, lb, weights, budget=103, recent=100, capacity=128)
+    gk = switch_kv_cache_read(kept, 0, 103)
+    rows = [0, at + 3 - base, at + 77 - base] + list(range(at + 380 - base, at + 480 - base))
+    assert lk.tolist() == [103] and wk[0, :, :3].tolist() == [[3.0, 2.0, 1.0]] * h and not wk[0, :, 3:].any()
+    for got, was in zip(gk, rs):
+        x = was[0, rows].float()
+        x[0] = 0
+        # Rounded to the scale of the largest value of its block at most once more.
+        step = 2.0 ** -4 * x.abs() + 2.0 ** -9 * x.abs().amax() if dtype == E4M3 else 2.0 ** -6 * x.abs().amax()
+        assert ((got[0].float() - x).abs() <= step).all() and not got[0, 0].any()
+
+
 # ---------------------------------------------------------------------------
 # As a program uses them
 # ---------------------------------------------------------------------------
