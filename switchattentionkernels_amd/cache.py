@@ -188,9 +188,10 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
     left as it is).
 
     ``k``/``v``: bf16 ``[B, T, Hkv, 128]`` with T at most the capacity, of which
-    sequence b appends its first ``row_counts[b]`` (int32 ``[B]`` on the device, clamped to ``[0, T]``; default
-    all).  Or, with ``cu_seqlens`` (int list or tensor of ``B + 1`` offsets),
-    packed ``[1, total, Hkv, 128]`` as for ``switch_gqa_prefill_varlen_forward``.
+    sequence b appends its first ``row_counts[b]`` (int32 ``[B]`` on the device,
+    clamped to ``[0, T]``; default all).  Or, with ``cu_seqlens`` (int list or
+    tensor of ``B + 1`` offsets), packed ``[1, total, Hkv, 128]`` as for
+    ``switch_gqa_prefill_varlen_forward``, each sequence at most the capacity.
     Rows that do not fit the cache any more are dropped, and the new length is
     the capacity.  A block that already held rows takes the larger scale of its
     own and its new rows', and its rows are rounded again where it grows.
