@@ -11,37 +11,6 @@
 namespace swattn {
 namespace {
 
-// Index validation (V:299-302 on both lists, disjointness of V:341-342) of slot i:
-// its full entry (range, order against the previous entry, binary search in the
-// local list) and its local entry (range, order), as SWATTN_ERR_* bits.  The
-// binary search is only meaningful when the local list is sorted; when it is not,
-// ERR_LOCAL_ORDER is raised and the caller reports that first.
-__device__ __forceinline__ int list_flags(const int32_t* __restrict__ full, int64_t nf,
-                                          const int32_t* __restrict__ local, int64_t nl, int64_t seq_len,
-                                          int64_t i) {
-  int f = 0;
-  if (i < nf) {
-    const int32_t x = full[i];
-    if (x < 0 || x >= seq_len) f |= SWATTN_ERR_FULL_RANGE;
-    if (i > 0 && x <= full[i - 1]) f |= SWATTN_ERR_FULL_ORDER;
-    int64_t lo = 0, hi = nl;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (local[mid] < x)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    if (lo < nl && local[lo] == x) f |= SWATTN_ERR_OVERLAP;
-  }
-  if (i < nl) {
-    const int32_t x = local[i];
-    if (x < 0 || x >= seq_len) f |= SWATTN_ERR_LOCAL_RANGE;
-    if (i > 0 && x <= local[i - 1]) f |= SWATTN_ERR_LOCAL_ORDER;
-  }
-  return f;
-}
-
 // A listed position outside [0, total_q) is never dereferenced: the host
 // checks the lists before the launch, and this keeps a list changed after
 // that check from turning into an out-of-bounds access.

@@ -10,7 +10,7 @@
 #include <chrono>
 #include <string>
 
-#include "row_blocks.h"
+#include "common.h"
 #include "swattn_internal.h"
 
 namespace swattn {
@@ -277,8 +277,12 @@ __global__ __launch_bounds__(kCompactThreads) void compact_scatter_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Index validation, one thread per slot (list_flags).  Any failure ORs its bit into
-// *flags, which flags_clear_kernel zeroes first.
+// Index validation (V:299-302 on both lists, disjointness of V:341-342).
+// One thread per slot; a slot checks its full entry (range, order against the
+// previous entry, binary search in the local list) and its local entry (range,
+// order).  Any failure ORs its bit into *flags, which flags_clear_kernel zeroes
+// first.  The binary search is only meaningful when the local list is sorted;
+// when it is not, ERR_LOCAL_ORDER is raised and the caller reports that first.
 // ---------------------------------------------------------------------------
 __global__ void flags_clear_kernel(int32_t* flags) { flags[0] = 0; }
 
@@ -286,7 +290,26 @@ __global__ __launch_bounds__(256) void check_indices_kernel(
     const int32_t* __restrict__ full, int64_t nf, const int32_t* __restrict__ local, int64_t nl,
     int64_t seq_len, int32_t* __restrict__ flags) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  int f = list_flags(full, nf, local, nl, seq_len, i);
+  int f = 0;
+  if (i < nf) {
+    const int32_t x = full[i];
+    if (x < 0 || x >= seq_len) f |= SWATTN_ERR_FULL_RANGE;
+    if (i > 0 && x <= full[i - 1]) f |= SWATTN_ERR_FULL_ORDER;
+    int64_t lo = 0, hi = nl;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (local[mid] < x)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    if (lo < nl && local[lo] == x) f |= SWATTN_ERR_OVERLAP;
+  }
+  if (i < nl) {
+    const int32_t x = local[i];
+    if (x < 0 || x >= seq_len) f |= SWATTN_ERR_LOCAL_RANGE;
+    if (i > 0 && x <= local[i - 1]) f |= SWATTN_ERR_LOCAL_ORDER;
+  }
   // One atomic per wave that saw a failure.
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) f |= __shfl_xor(f, off);

@@ -65,12 +65,13 @@ int swattn_cache_append_host(const void* new_k, const void* new_v, const int32_t
                              int32_t head_dim, int32_t block, int32_t code, void* stream);
 
 /*
- * swattn_prefill_key_weights with the check of the lists (swattn_check_indices)
- * in its first kernel: on return *flags holds the SWATTN_ERR_* bits, while the
+ * swattn_prefill_key_weights with the check of the lists (what swattn_check_indices
+ * finds) in its first kernel: on return *flags holds the SWATTN_ERR_* bits, while the
  * sums may still be running.  (With the check and its read-back ahead of the
  * launches a call took 40 us more.)
  *   host  SWATTN_KEY_WEIGHTS_HOST_WORDS int32 of pinned host memory, one call at
  *         a time; after a HIP error (a positive status) not to be used again.
+ *   n_full + n_local  batch * seq_q: the check relies on it
  * A stream under capture is refused (SWATTN_EINVAL) before anything is launched.
  */
 #define SWATTN_KEY_WEIGHTS_HOST_WORDS 1024

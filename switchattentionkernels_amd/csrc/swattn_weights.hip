@@ -136,14 +136,30 @@ __device__ __forceinline__ void prep_rows(const WeightParams& p, int wg) {
 }
 
 // The check of the lists, reported to a host that polls: the word carries the
-// answer itself and orders nothing else.
+// answer itself and orders nothing else.  As many rows are listed as there are, so that
+// disjoint lists hold every row: entry i of the full list, row x, has x - i rows of the
+// local list before it.  Two loads in place of a search: S1024 18.6 -> 17.9 us.  (In the
+// next launch, where it would delay no kernel: 26.1, the host's answer comes late.)
 constexpr int kReported = 1 << 30;
 __device__ __forceinline__ void check_lists(const WeightParams& p, int wg) {
   int f = 0;
-  const int64_t n = max(p.count[0], p.count[1]);
-  for (int64_t i = static_cast<int64_t>(wg) * kThreads + threadIdx.x; i < n;
-       i += static_cast<int64_t>(p.check_wgs) * kThreads)
-    f |= list_flags(p.idx[0], p.count[0], p.idx[1], p.count[1], p.total_q, i);
+  const int64_t nf = p.count[0], nl = p.count[1];
+  const int32_t *full = p.idx[0], *local = p.idx[1];
+  for (int64_t i = static_cast<int64_t>(wg) * kThreads + threadIdx.x; i < max(nf, nl);
+       i += static_cast<int64_t>(p.check_wgs) * kThreads) {
+    if (i < nf) {
+      const int64_t x = full[i], before = x - i;   // of the local list
+      if (x < 0 || x >= p.total_q) f |= SWATTN_ERR_FULL_RANGE;
+      if (i > 0 && x <= full[i - 1]) f |= SWATTN_ERR_FULL_ORDER;
+      if (before < 0 || before > nl || (before > 0 && local[before - 1] >= x) || (before < nl && local[before] <= x))
+        f |= SWATTN_ERR_OVERLAP;
+    }
+    if (i < nl) {
+      const int32_t x = local[i];
+      if (x < 0 || x >= p.total_q) f |= SWATTN_ERR_LOCAL_RANGE;
+      if (i > 0 && x <= local[i - 1]) f |= SWATTN_ERR_LOCAL_ORDER;
+    }
+  }
   __shared__ int s_flags[kThreads / 64];
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) f |= __shfl_xor(f, off);
@@ -561,6 +577,7 @@ int swattn_prefill_key_weights_checked(
   const std::string n("swattn_prefill_key_weights");
   if (host == nullptr || flags == nullptr) return invalid(n + ": null pointer");
   *flags = 0;
+  if (n_full + n_local != batch * seq_q) return invalid(n + ": the lists must hold batch * seq_q entries");
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(as_stream(stream), &capture) == hipSuccess && capture != hipStreamCaptureStatusNone)
     return invalid(n + ": waits for the check of the index lists and cannot be captured");
