@@ -67,6 +67,16 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// T's bytes at `at`, loaded as Raw; kStream: past the memory-side cache (data that is
+// there all the same is read from it).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool kStream, class Raw, class T>
+__device__ __forceinline__ T load_bytes(const uint8_t* at) {
+  const Raw* p = reinterpret_cast<const Raw*>(at);
+  if constexpr (kStream) return __builtin_bit_cast(T, __builtin_nontemporal_load(p));
+  return __builtin_bit_cast(T, *p);
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // Host: the bytes of a cache's rows stay addressable and its blocks countable.

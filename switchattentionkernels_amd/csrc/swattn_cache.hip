@@ -18,6 +18,7 @@
 
 #include <string.h>
 
+#include <algorithm>
 #include <string>
 #include <type_traits>
 
@@ -31,6 +32,13 @@ using namespace code;
 
 constexpr int kD = 128;
 constexpr int kRowsAtOnce = 16;   // rows that a workgroup's half takes at once
+// Reads and evictions that move this much stream the codes that they read past the
+// 256 MB memory-side cache, which then keeps what they write: moving 192 MB, 48 us kept
+// and 54 streamed (evict), 31.8 and 35.5 (read); 256 MB 69 and 68 (evict); 280 MB 54.6
+// and 48.4 (read); 437 MB 114 and 104 (evict); 512 MB 136 and 126.  Appends do not: new
+// rows are in that cache as a rule, from the kernel that made them (128 MB of them, made
+// and appended: 85 us, streamed 92).  Streamed stores: a third slower.
+constexpr int64_t kStreamBytes = int64_t{224} << 20;
 
 __device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
 
@@ -195,7 +203,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 // One thread per 16 values; blockIdx.y: sequence, blockIdx.z 0: K, 1: V.
-template <int kCode>
+template <int kCode, bool kStream>
 __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
   const uint32_t x = blockIdx.x * 256u + threadIdx.x;
   if (x >= static_cast<uint32_t>(p.pieces)) return;
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadParams p) {
   const int end = p.lens != nullptr ? min(p.lens[b], p.cache_len) : p.cache_len;
   uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   if (r >= 0 && r < end) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p.codes[which] + ((b * p.cache_len + r) * p.hkv + h) * kD + piece * 16);
+    const uint4 u = load_bytes<kStream, u32x4, uint4>(p.codes[which] + ((b * p.cache_len + r) * p.hkv + h) * kD + piece * 16);
     const float s = p.scales[which][(b * p.hkv + h) * p.nblk + (r >> p.block_log)];
     float v[16];
     decode16<kCode>(u, v);
@@ -389,32 +397,42 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
 
 // The kept rows into the destination: one workgroup per (sequence, destination
 // block, KV head).  32 sequences of 1024 to 4096 rows cut to 2047, 8 KV heads,
-// blocks of 32: 59 us, 4.2 TB/s of scattered 128-byte rows (64 rows a workgroup: 64;
-// a block's heads on one XCD: 62).
-template <int kCode, int kBlock>
+// blocks of 32, then read back: 146.5 us for search, copy and read, 144 since the chosen
+// rows' loads do not wait for the length's, 136 streamed; the copy alone moves scattered
+// 128-byte rows at 4.2 TB/s.  (64 rows a workgroup and a block's heads on one XCD were
+// slower: 59 us, 64 and 62 when the copy took that.)
+template <int kCode, int kBlock, bool kStream>
 __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
   constexpr int kIt = kBlock / kRowsAtOnce;
   const int h = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
   const int jb = rest % p.out_nblk, b = rest / p.out_nblk;
   const int64_t pair = static_cast<int64_t>(b) * p.hkv + h;
-  const int len = min(max(p.lens[b], 0), p.cache_len);
   const int want = p.budget - p.recent;
-  const int end = min(len, p.budget);
-  auto source = [&](int d) {
-    int s = d;
-    if (len > p.budget) s = d < want ? p.kept[pair * want + d] : len - p.budget + d;
-    return min(max(s, 0), p.cache_len - 1);
-  };
   const int r0 = jb * kBlock;
-  if (threadIdx.x < kBlock) {
-    const int d = r0 + static_cast<int>(threadIdx.x);
-    if (d < p.out_len)
-      p.out_weights[pair * p.out_len + d] = d < end ? p.weights[pair * p.cache_len + source(d)] : 0.f;
-  }
-  if (r0 >= end) return;   // uniform
   const int half = threadIdx.x >> 7, t = threadIdx.x & 127;
   const int sub = t >> 3, piece = t & 7;
+  // The chosen rows do not wait for the length (which may leave them unused).
+  const int32_t* kept = p.kept + pair * want;
+  int chosen[kIt], own = 0;
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int d = r0 + it * kRowsAtOnce + sub;
+    chosen[it] = d < want ? kept[d] : 0;
+  }
+  const int dw = r0 + static_cast<int>(threadIdx.x);   // threads 0 .. kBlock - 1: a weight's row
+  if (threadIdx.x < kBlock && dw < want) own = kept[dw];
+  const int len = min(max(p.lens[b], 0), p.cache_len);
+  const int end = min(len, p.budget);
+  auto source = [&](int d, int chosen_row) {
+    int s = d;
+    if (len > p.budget) s = d < want ? chosen_row : len - p.budget + d;
+    return min(max(s, 0), p.cache_len - 1);
+  };
+  if (r0 >= end) {   // uniform
+    if (threadIdx.x < kBlock && dw < p.out_len) p.out_weights[pair * p.out_len + dw] = 0.f;
+    return;
+  }
   const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
   const uint8_t* codes = p.codes[half] + (static_cast<int64_t>(b) * p.cache_len * p.hkv + h) * kD + piece * 16;
   const float* scales = p.scales[half] + pair * p.nblk;
@@ -426,11 +444,13 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
     raw[it] = make_uint4(0, 0, 0, 0);
     s[it] = 0.f;
     if (d < end) {
-      const int r = source(d);
-      raw[it] = *reinterpret_cast<const uint4*>(codes + r * stride);
+      const int r = source(d, chosen[it]);
+      raw[it] = load_bytes<kStream, u32x4, uint4>(codes + r * stride);
       s[it] = scales[r / kBlock];
     }
   }
+  float weight = 0.f;
+  if (threadIdx.x < kBlock && dw < end) weight = p.weights[pair * p.cache_len + source(dw, own)];
   uint32_t amax = 0;
 #pragma unroll
   for (int it = 0; it < kIt; ++it) {
@@ -454,6 +474,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
       *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
     }
   }
+  if (threadIdx.x < kBlock && dw < p.out_len) p.out_weights[pair * p.out_len + dw] = weight;
 }
 
 // Argument checks that the entry points share.
@@ -499,8 +520,11 @@ struct LaunchAppend {
 };
 template <int kCode, int kBlock>
 struct LaunchGather {
-  static void go(dim3 grid, hipStream_t st, const EvictParams& p) {
-    hipLaunchKernelGGL((gather_kernel<kCode, kBlock>), grid, dim3(256), 0, st, p);
+  static void go(dim3 grid, hipStream_t st, const EvictParams& p, bool stream) {
+    if (stream)
+      hipLaunchKernelGGL((gather_kernel<kCode, kBlock, true>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((gather_kernel<kCode, kBlock, false>), grid, dim3(256), 0, st, p);
   }
 };
 
@@ -616,10 +640,12 @@ int swattn_cache_read(const void* k, const void* v, const float* k_scales, const
   p.nblk = static_cast<int>(ceil_div(cache_len, block));
   p.block_log = __builtin_ctz(static_cast<unsigned>(block));
   const dim3 g(static_cast<uint32_t>(ceil_div(pieces, 256)), batch, 2);
+  const bool streamed = batch * pieces * 16 * 6 >= kStreamBytes;   // K and V, codes and bf16
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, as_stream(stream), p); };
   if (codes == kE4m3)
-    hipLaunchKernelGGL(read_kernel<kE4m3>, g, dim3(256), 0, as_stream(stream), p);
+    streamed ? launch(read_kernel<kE4m3, true>) : launch(read_kernel<kE4m3, false>);
   else
-    hipLaunchKernelGGL(read_kernel<kInt8>, g, dim3(256), 0, as_stream(stream), p);
+    streamed ? launch(read_kernel<kInt8, true>) : launch(read_kernel<kInt8, false>);
   return launch_status(n.c_str());
 }
 
@@ -689,7 +715,9 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
     hipLaunchKernelGGL((select_kernel<1024, 32>), gs, dim3(1024), 0, hs, p);
   else
     hipLaunchKernelGGL((select_kernel<1024, 0>), gs, dim3(1024), 0, hs, p);
-  by_code_and_block<LaunchGather>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p);
+  // K and V, read and written.
+  const bool streamed = pairs * std::min(budget, cache_len) * 4 * kD >= kStreamBytes;
+  by_code_and_block<LaunchGather>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p, streamed);
   return launch_status(n.c_str());
 }
 

@@ -52,7 +52,6 @@ using namespace code;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;            // waves per workgroup
 constexpr int kMaxG = 8;
@@ -106,12 +105,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // still be there from the last call: B24 of 2999 29.7 us, streamed 35.6; B8 of 4096
 // 17.5 and 18.9.
 constexpr int64_t kStreamBytes = int64_t{256} << 20;
-template <bool kStream, class Raw, class T>
-__device__ __forceinline__ T load_bytes(const uint8_t* at) {
-  const Raw* p = reinterpret_cast<const Raw*>(at);
-  if constexpr (kStream) return __builtin_bit_cast(T, __builtin_nontemporal_load(p));
-  return __builtin_bit_cast(T, *p);
-}
 
 // One step's data: 32 keys of K and V and the scales of both key tiles.
 struct Step {

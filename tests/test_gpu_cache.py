@@ -543,6 +543,34 @@ def test_evict_into_a_given_cache_and_lengths_out_of_range():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_large_calls_equal_their_parts(dtype):
+    """Reads and evictions of 250 to 400 MB against the same in parts of less than 100."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    b, n, h, block = 4, 16000, 8, 32
+    codes = [torch.randint(0, 0x7f, (b, n, h, 128), generator=gen, device=DEV, dtype=torch.uint8) for _ in range(2)]
+    scales = [torch.rand(b, h, n // block, generator=gen, device=DEV) + 0.5 for _ in range(2)]
+    cache = SwitchKVCache(*(x.view(dtype) for x in codes), *scales, block)
+    lens = _int32([16000, 15990, 15001, 300])
+    whole = switch_kv_cache_read(cache, 0, n, cache_lens=lens)
+    for a in range(0, n, 4000):
+        for x, y in zip(whole, switch_kv_cache_read(cache, a, 4000, cache_lens=lens)):
+            assert torch.equal(x[:, a:a + 4000], y)
+    weights = torch.rand(b, h, n, generator=gen, device=DEV)
+    kept, after, w = switch_kv_cache_evict(cache, lens, weights, budget=15000, recent=100, capacity=15010)
+    for i in range(b):
+        one = SwitchKVCache(*(x[i:i + 1] for x in (cache.k, cache.v, cache.k_scales, cache.v_scales)), block)
+        k1, a1, w1 = switch_kv_cache_evict(one, lens[i:i + 1], weights[i:i + 1], budget=15000, recent=100,
+                                           capacity=15010)
+        m = int(a1[0])
+        assert m == min(int(lens[i]), 15000) == int(after[i]) and torch.equal(w[i], w1[0])
+        for x, y in ((kept.k, k1.k), (kept.v, k1.v)):
+            assert torch.equal(x.view(torch.uint8)[i, :m], y.view(torch.uint8)[0, :m])
+        nb = -(-m // block)
+        assert torch.equal(kept.k_scales[i, :, :nb], k1.k_scales[0, :, :nb])
+        assert torch.equal(kept.v_scales[i, :, :nb], k1.v_scales[0, :, :nb])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_offsets_past_31_bits(dtype):
     """A cache of 2 x 2.2 GB: its last rows against those of a small cache, and keys of
     zeros before them, whose scores are 0 and whose values add nothing."""
