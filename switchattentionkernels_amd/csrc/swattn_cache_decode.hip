@@ -22,13 +22,16 @@
 //   tile n takes dim 8 c + n of each, so that S^T's accumulator layout (column
 //   lane % 16, keys 4 g .. +3) is P's operand layout, and V is transposed
 //   inside a lane.
-// * A group has at most 8 heads and the tiles have 16 columns: columns 8-15 repeat
-//   the heads, and take p's rounding error, p - bf16(p), where columns 0-7 take
-//   bf16(p).  Their sum carries 16 bits of p at no further matrix instruction.
+// * p vs enters the product with V as three bf16 numbers, its value, what that leaves
+//   and what both leave: 24 bits, as in fp32.  A group has at most 8 heads and the
+//   tiles have 16 columns: columns 8-15 repeat the heads and take the second where
+//   columns 0-7 take the first; the third needs a product of its own.  Without it (17
+//   bits) 206 of 131072 outputs of 32768 keys were rounded to the wrong side, 29 with
+//   it and 122 by fp32 sums; it costs 0.3 us of 157.4 there, 1.5 of 72.4 at B64.
 //
 // Measured, Hkv 8, as a large copy's 5.2 TB/s goes: B16 L16384-32768 Hq64 int8 all
-// full 159-163 us, 4.95-5.06 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full
-// 0.25 70-73 us, of which the merge and its launch are about 8; B1 L4096 Hq32 11.3 us, bound
+// full 158 us, 5.1 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full
+// 0.25 74 us, of which the merge and its launch are about 8; B1 L4096 Hq32 11.3 us, bound
 // by dependent latencies (plan, first keys, combine, merge) and, at that length, by
 // the host's calls.  Two workgroups per CU with loads three steps ahead: 12.8 us
 // (B1), 77 (B64); four with one step ahead 13 and 85.  Joining the pieces in the same
@@ -256,22 +259,28 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
 #pragma unroll
             for (int t = 0; t < 8; ++t) acc[t] *= a;
           }
-          u32x4 pk;
+          u32x4 pk, pk2;
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            float pv[4];
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float pr = live[t][x] ? __builtin_amdgcn_exp2f(s[t][x] - m) : 0.f;
-              l += pr;
-              const float y = pr * vs[t];
-              const float rest = y - static_cast<float>(static_cast<__bf16>(y));
-              pv[x] = error_col ? rest : y;
+            for (int x = 0; x < 4; x += 2) {
+              float y[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float pr = live[t][x + i] ? __builtin_amdgcn_exp2f(s[t][x + i] - m) : 0.f;
+                l += pr;
+                y[i] = pr * vs[t];
+              }
+              const uint32_t high = pack2(y[0], y[1]);   // the differences are exact
+              y[0] -= __uint_as_float(high << 16);
+              y[1] -= __uint_as_float(high & 0xffff0000u);
+              const uint32_t mid = pack2(y[0], y[1]);
+              y[0] -= __uint_as_float(mid << 16);
+              y[1] -= __uint_as_float(mid & 0xffff0000u);
+              pk[2 * t + x / 2] = error_col ? mid : high;
+              pk2[2 * t + x / 2] = error_col ? 0u : pack2(y[0], y[1]);
             }
-            pk[2 * t] = pack2(pv[0], pv[1]);
-            pk[2 * t + 1] = pack2(pv[2], pv[3]);
-          }
-          const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
+          const bf16x8 pb = __builtin_bit_cast(bf16x8, pk), pb2 = __builtin_bit_cast(bf16x8, pk2);
           // V^T operands of dims 2 d, 2 d + 1 of this lane's eight: pairs of keys.
 #pragma unroll
           for (int d2 = 0; d2 < 4; ++d2) {
@@ -286,6 +295,8 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
             }
             acc[2 * d2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), pb, acc[2 * d2], 0, 0, 0);
             acc[2 * d2 + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), pb, acc[2 * d2 + 1], 0, 0, 0);
+            acc[2 * d2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), pb2, acc[2 * d2], 0, 0, 0);
+            acc[2 * d2 + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), pb2, acc[2 * d2 + 1], 0, 0, 0);
           }
           load(i + kWaves * kAhead, d);   // refill the slot; past the end: clamped, never used
         }
