@@ -19,7 +19,10 @@
  * Scales that these entry points write are powers of two: for a block's
  * largest magnitude a, the smallest 2^e >= 2^-100 with a <= qmax * 2^e (qmax
  * 448 for e4m3, 127 for int8), so that scaling is exact and a value is rounded
- * once, to the nearest code, ties to even.  A block that takes a NaN or an
+ * once, to the nearest code, ties to even.  Where that code would stand for
+ * more than the largest bf16 number (from 248 * 2^120 on for e4m3, 63.5 *
+ * 2^122 for int8) the next smaller one is taken: finite values read as finite
+ * ones.  A block that takes a NaN or an
  * infinity gets scale NaN: its rows read as NaN until all of them are gone.
  * Caches with other (positive, finite) scales, made elsewhere, may be read,
  * attended, appended to and evicted from.

@@ -14,6 +14,7 @@ import torch
 
 QMAX = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
 MIN_EXP = -100
+BF16_MAX = 255 * 2.0 ** 120
 
 
 def _e4m3_table() -> np.ndarray:
@@ -52,6 +53,16 @@ def round_code(x: np.ndarray, dtype) -> np.ndarray:
     pick = np.where(d_hi < d_lo, hi, np.where(d_lo < d_hi, lo, np.where(hi % 2 == 0, hi, lo)))
     pick = np.where(_TABLE[hi] == a, hi, pick)
     return np.where(nan, math.nan, np.copysign(_TABLE[pick], x))
+
+
+def keep_finite(x: np.ndarray, scale: float, dtype) -> np.ndarray:
+    """Codes' values of a block with this scale; for those whose product lies above
+    bf16's largest number the largest whose product does not."""
+    known = np.arange(128.0) if dtype == torch.int8 else _TABLE
+    if math.isnan(scale) or known[-1] * float(scale) <= BF16_MAX:
+        return x
+    top = known[known * float(scale) <= BF16_MAX].max()
+    return np.clip(x, -top, top)
 
 
 def code_values(codes: torch.Tensor) -> np.ndarray:
@@ -96,10 +107,11 @@ def append(codes: torch.Tensor, scales: torch.Tensor, block: int, new, lens):
                     s = math.nan if math.isnan(old) or math.isnan(s) else max(old, s)
                     if not math.isnan(old) and s != old:
                         ratio = np.float32(old) / np.float32(s)
-                        raw[b, j * block:lo, h] = round_code(raw[b, j * block:lo, h] * ratio, dtype)
+                        raw[b, j * block:lo, h] = keep_finite(
+                            round_code(raw[b, j * block:lo, h] * ratio, dtype), s, dtype)
                 sc[b, h, j] = s
                 with np.errstate(invalid="ignore"):
-                    raw[b, lo:hi, h] = round_code(x / np.float32(s), dtype)
+                    raw[b, lo:hi, h] = keep_finite(round_code(x / np.float32(s), dtype), s, dtype)
     with np.errstate(invalid="ignore"):
         values = raw.astype(np.float64) * np.repeat(sc.astype(np.float64), block, axis=2)[:, :, :cap] \
             .transpose(0, 2, 1)[..., None]
@@ -195,5 +207,6 @@ def evict(k: np.ndarray, v: np.ndarray, weights: np.ndarray, lens, budget: int, 
                     s = scale_for(float(a.max()) if np.isfinite(a).all() else math.inf, dtype)
                     sc[i, h, j // block] = s
                     with np.errstate(invalid="ignore"):
-                        out[i, j:j + len(part), h] = round_code(part / np.float32(s), dtype) * s
+                        out[i, j:j + len(part), h] = keep_finite(
+                            round_code(part / np.float32(s), dtype), s, dtype) * s
     return kept, after, ok, ov, sk, sv, ow

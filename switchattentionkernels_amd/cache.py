@@ -20,7 +20,8 @@ Lengths are the caller's, as for ``switch_gqa_decode_forward``: int32 ``[B]`` on
 the device.  Scales written here are powers of two: for a block's largest
 magnitude ``a`` the smallest ``2^e >= 2^-100`` with ``a <= qmax * 2^e`` (qmax 448
 for e4m3, 127 for int8).  Scaling is then exact and every value is rounded once,
-to the nearest code.  A block that takes a NaN or an infinity reads as NaN.
+to the nearest code that stands for a finite bf16 number.  A block that takes a NaN or an
+infinity reads as NaN.
 
 All device work runs in ``libswattn.so`` (``include/swattn_cache.h``) on torch's
 current stream.

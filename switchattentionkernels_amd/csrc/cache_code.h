@@ -67,6 +67,20 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// Scaled values of a block with this scale, cut to the largest code whose value bf16
+// still holds.  Only the largest numbers need it: above 240 * 2^120 (e4m3) and 63 * 2^122
+// (int8) the nearest code would stand for 2^128.
+template <int kCode>
+__device__ __forceinline__ void keep_finite(float scale, float (&x)[16]) {
+  constexpr float kMax = 0x1.fep127f, kQmax = kCode == kE4m3 ? 448.f : 127.f;
+  if (scale > kMax / kQmax) {
+    float top = kMax / scale;   // to the code below it
+    top = kCode == kE4m3 ? __uint_as_float(__float_as_uint(top) & 0xfff00000u) : __builtin_truncf(top);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = x[j] > top ? top : x[j] < -top ? -top : x[j];   // NaN stays NaN
+  }
+}
+
 // T's bytes at `at`, loaded as Raw; kStream: past the memory-side cache (data that is
 // there all the same is read from it).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -150,6 +150,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const
           decode16<kCode>(*at, x);
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j] *= ratio;
+          keep_finite<kCode>(scale, x);
           *at = encode16<kCode>(x);
         }
       }
@@ -178,6 +179,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] *= inv;
       }
+      keep_finite<kCode>(scale, x);
       *reinterpret_cast<uint4*>(codes + r * stride) = encode16<kCode>(x);
     }
   }
@@ -471,6 +473,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {
       decode16<kCode>(raw[it], x);
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[j] = x[j] * s[it] * inv;
+      keep_finite<kCode>(scale, x);
       *reinterpret_cast<uint4*>(out + d * stride) = encode16<kCode>(x);
     }
   }
