@@ -131,3 +131,10 @@ def on_device(device):
     if idx is None or idx == torch.cuda.current_device():
         return _no_switch
     return torch.cuda.device(idx)
+
+
+def refuse_capture(device, why: str) -> None:
+    """Raise, with nothing enqueued, if torch's current stream is under capture."""
+    with on_device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"the call {why} and cannot be captured")

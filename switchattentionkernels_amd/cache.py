@@ -159,12 +159,15 @@ def _append_arguments(cache, k, v, cache_lens, row_counts, cu_seqlens):
             raise ValueError("row_counts and cu_seqlens exclude each other")
         if k.shape[0] != 1:
             raise ValueError("packed K/V must have batch size 1")
+        if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
+            _lib.refuse_capture(dev, "reads cu_seqlens back from the device")
         offsets = _as_cu(cu_seqlens, rows, "cu_seqlens")
         if len(offsets) != batch + 1:
             raise ValueError("cu_seqlens must hold one sequence for each of the cache's")
         if batch <= HOST_MAX_SEQS:
             host_cu = offsets
         else:
+            _lib.refuse_capture(dev, f"copies cu_seqlens of more than {HOST_MAX_SEQS} sequences to the device")
             cu = torch.tensor(offsets, dtype=torch.int32, device=dev)
         most = max(b - a for a, b in zip(offsets, offsets[1:]))
     else:
@@ -192,7 +195,10 @@ def switch_kv_cache_append(cache: SwitchKVCache, k: torch.Tensor, v: torch.Tenso
     sequence b appends its first ``row_counts[b]`` (int32 ``[B]`` on the device,
     clamped to ``[0, T]``; default all).  Or, with ``cu_seqlens`` (int list or
     tensor of ``B + 1`` offsets), packed ``[1, total, Hkv, 128]`` as for
-    ``switch_gqa_prefill_varlen_forward``, each sequence at most the capacity.
+    ``switch_gqa_prefill_varlen_forward``, each sequence at most the capacity.  The host
+    needs these offsets: a device tensor is read back, which waits for the stream; a captured
+    call keeps the offsets it was captured with (of up to 256 sequences, from a list or a host
+    tensor; others are refused under capture).
     Rows that do not fit the cache any more are dropped, and the new length is
     the capacity.  A block that already held rows takes the larger scale of its
     own and its new rows', and its rows are rounded again where it grows.
