@@ -20,6 +20,8 @@ from .metadata import SwitchAttentionMetadata
 from .prefill import (ERR_OVERLAP, LOG2E, MSG_DISJOINT, _check_lists, _check_metadata,
                       _is_untouched_compaction, _note_sync, _prepare_indices, _raise_for, check_qkv)
 
+WAITS_FOR_LISTS = "waits for the check of the index lists"
+
 
 def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor,
                                    full_query_indices: torch.Tensor,
@@ -60,6 +62,7 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
             and full.numel() + local.numel() == total_q > 0 and full.device == local.device == dev
             and not _is_untouched_compaction(full, local, total_q)):
         # The lists' values are checked by the call itself, beside its first kernel.
+        _lib.refuse_capture(dev, WAITS_FOR_LISTS)
         full, local = _prepare_indices(full, device=dev), _prepare_indices(local, device=dev)
         _note_sync(dev)
         unchecked = True
