@@ -30,8 +30,8 @@ from .prefill import (LOG2E, MSG_META, _check_lists, _check_metadata, check_qkv,
 
 
 def _check_monotone(metadata: SwitchAttentionMetadata, full: torch.Tensor,
-                    local: torch.Tensor) -> None:
-    """The backward finds the rows that see a key block by binary search, so
+                    local: torch.Tensor, what: str = "the backward pass") -> None:
+    """``what`` finds the rows that see a key block by binary search, so
     each list's key bounds must be non-decreasing along the list (true for
     every single causal sequence and for packed sequences in order).  A
     start past its row's end is an empty range and counts as the end, as in
@@ -47,7 +47,7 @@ def _check_monotone(metadata: SwitchAttentionMetadata, full: torch.Tensor,
     _lib.check(st, "swattn_check_bounds")
     if flags.item():
         raise ValueError(MSG_META + ": key bounds must be non-decreasing along each index list "
-                         "for the backward pass")
+                         f"for {what}")
 
 
 def switch_gqa_prefill_backward(

@@ -44,6 +44,49 @@ class SwitchAttentionMetadata:
     causal_ends: torch.Tensor
 
 
+class _Built:
+    """Identity of one ``build_switch_attention_metadata`` result.  Copies of its tensors
+    start version counters of their own: they get None in its place."""
+
+    __slots__ = ()
+
+    def __deepcopy__(self, memo):
+        return None
+
+    def __reduce__(self):
+        return type(None), ()
+
+
+_BOUNDS = ("full_starts", "local_starts", "causal_ends")
+
+
+def _tag_built(md: SwitchAttentionMetadata) -> SwitchAttentionMetadata:
+    """Mark the bounds of fresh metadata: inside a sequence starts (cut to the row's end)
+    and ends do not decrease, and a sequence's are at most the next one's.  Inference
+    tensors have no version counter and stay unmarked."""
+    if not md.full_starts.is_inference():
+        token = _Built()
+        for name in _BOUNDS:
+            t = getattr(md, name)
+            t._swattn_built = (token, name, t._version)
+    return md
+
+
+def _is_untouched(md: SwitchAttentionMetadata) -> bool:
+    """Whether the bounds are those of one build and, by torch's version counters, as it
+    left them."""
+    first = None
+    for name in _BOUNDS:
+        t = getattr(md, name)
+        tag = getattr(t, "_swattn_built", None)
+        if tag is None or tag[0] is None or tag[1] != name or t.is_inference() or t._version != tag[2]:
+            return False
+        first = first or tag[0]
+        if tag[0] is not first:
+            return False
+    return True
+
+
 def _as_cu(cu, total: int, name: str) -> list:
     vals = [int(x) for x in (cu.tolist() if isinstance(cu, torch.Tensor) else cu)]
     if len(vals) < 2 or vals[0] != 0:
@@ -82,8 +125,8 @@ def build_switch_attention_metadata(q_len: int, kv_len: int, *, device, window_s
     with _lib.on_device(dev):
         stream = _lib.stream_handle(dev)
         if nseq <= HOST_MAX_SEQS and max(q_len, kv_len) < 2 ** 31:
-            return SwitchAttentionMetadata(*_lib.native().metadata(cq, ck, q_len, kv_len,
-                                                                   window_size, dev, stream))
+            return _tag_built(SwitchAttentionMetadata(*_lib.native().metadata(
+                cq, ck, q_len, kv_len, window_size, dev, stream)))
         md = SwitchAttentionMetadata(*(torch.empty(n, dtype=torch.int32, device=dev) for n in
                                        (q_len, kv_len, q_len, kv_len, q_len, q_len, q_len)))
         cq_t = torch.tensor(cq, dtype=torch.int32, device=dev)
@@ -94,4 +137,4 @@ def build_switch_attention_metadata(q_len: int, kv_len: int, *, device, window_s
                                          md.kv_segment_ids, md.full_starts, md.local_starts,
                                          md.causal_ends)), stream)
     _lib.check(st, "swattn_build_metadata")
-    return md
+    return _tag_built(md)

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .backward import _check_monotone
-from .metadata import SwitchAttentionMetadata
+from .metadata import SwitchAttentionMetadata, _is_untouched
 from .prefill import (ERR_OVERLAP, LOG2E, MSG_DISJOINT, _check_lists, _check_metadata,
                       _is_untouched_compaction, _note_sync, _prepare_indices, _raise_for, check_qkv)
 
@@ -35,7 +35,9 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
 
     The arguments are those of ``switch_gqa_prefill_forward`` (or, with packed
     sequences, their metadata) without V, and ``lse`` is its result.  Like the
-    backward, it needs each list's key bounds non-decreasing along the list.
+    backward, it needs each list's key bounds non-decreasing along the list: true for metadata
+    of ``build_switch_attention_metadata`` that was not modified since, checked for any other.
+    Lists and bounds that need a check make the call wait for it, and a capture refuse it.
     """
     check_qkv(q, k, k)
     if window_size <= 0:
@@ -67,9 +69,12 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
         _note_sync(dev)
         unchecked = True
     else:
+        if not _is_untouched_compaction(full, local, total_q):
+            _lib.refuse_capture(dev, WAITS_FOR_LISTS)
         full, local = _check_lists(full, local, total_q, dev)
-        if metadata is not None:
-            _check_monotone(metadata, full, local)
+        if metadata is not None and not _is_untouched(metadata):
+            _lib.refuse_capture(dev, "waits for the check of the metadata's bounds")
+            _check_monotone(metadata, full, local, "the sums of attention weights")
     if 0 in k.shape:
         return torch.zeros(batch, k.shape[2], kv_len, dtype=torch.float32, device=dev)
     with _lib.on_device(dev):
