@@ -259,6 +259,8 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
 #pragma unroll
             for (int t = 0; t < 8; ++t) acc[t] *= a;
           }
+          // Only scores of -inf so far (products past fp32's range): they weigh nothing.
+          const float from = m == -INFINITY ? 0.f : m;
           u32x4 pk, pk2;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(256, 3) void cache_split_kernel(const CacheDecodePa
               float y[2];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const float pr = live[t][x + i] ? __builtin_amdgcn_exp2f(s[t][x + i] - m) : 0.f;
+                const float pr = live[t][x + i] ? __builtin_amdgcn_exp2f(s[t][x + i] - from) : 0.f;
                 l += pr;
                 y[i] = pr * vs[t];
               }
