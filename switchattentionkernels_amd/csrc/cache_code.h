@@ -93,7 +93,7 @@ __device__ __forceinline__ T load_bytes(const uint8_t* at) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Host: the bytes of a cache's rows stay addressable and its blocks countable.
+// Host: the blocks that there are kernels for.
 inline bool block_ok(int32_t block) { return block == 16 || block == 32 || block == 64 || block == 128; }
 
 }  // namespace code

@@ -73,7 +73,7 @@ struct AppendParams {
   float* scales[2];
   int32_t* lens_out;
   int64_t rows, total_rows;
-  int cache_len, hkv, nblk, batch, blocks;   // blocks: per sequence, at most
+  int cache_len, hkv, nblk, blocks;   // blocks: per sequence, at most
 };
 
 // Packed offsets as kernel arguments: no copy of them to the device.
@@ -106,8 +106,9 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendParams p, const
   const int end = static_cast<int>(min(len + count, static_cast<int64_t>(p.cache_len)));
   if (i == 0 && h == 0 && threadIdx.x == 0) p.lens_out[b] = end;
   const int jb = len / kBlock + i;
+  // uniform; blocks are counted, for the rows of those behind the cache may pass 2^31
+  if (end <= len || jb > (end - 1) / kBlock) return;
   const int r0 = jb * kBlock;          // the block's rows
-  if (end <= len || r0 >= end) return;   // uniform
   const int half = threadIdx.x >> 7, t = threadIdx.x & 127;
   const int sub = t >> 3, piece = t & 7;
   const uint16_t* src = p.src[half];
@@ -572,7 +573,6 @@ static int launch_append(const void* new_k, const void* new_v, const int32_t* cu
   p.cache_len = static_cast<int>(cache_len);
   p.hkv = heads_kv;
   p.nblk = static_cast<int>(ceil_div(cache_len, block));
-  p.batch = batch;
   // `rows` rows from any place of a block on; no more than the cache has.
   const int64_t most = rows < 1 ? 1 : (rows + block - 2) / block + 1;
   p.blocks = static_cast<int>(most < p.nblk ? most : p.nblk);
