@@ -38,7 +38,8 @@ extern "C" {
 #endif
 
 #define SWATTN_CODE_E4M3 0   /* OCP fp8: sign, 4 exponent and 3 mantissa bits, no infinities */
-#define SWATTN_CODE_INT8 1   /* two's complement; -128 is read but never written */
+#define SWATTN_CODE_INT8 1   /* two's complement; -128 is read, and written only where a begun
+                              * block that holds it takes a slightly larger scale */
 
 /*
  * Append new rows to the sequences of a cache.

@@ -106,3 +106,16 @@ def test_a_decode_over_the_largest_keys_is_finite():
     q = torch.full((1, 1, 2, 128), 2.0 ** -120, dtype=torch.bfloat16, device=DEV)
     out, lse = switch_gqa_decode_quantized_forward(q, cache, lens, torch.tensor([True], device=DEV))
     assert (out == -TOP[INT8]).all() and torch.isfinite(lse).all() and math.isfinite(float(lse.max()))
+
+
+def test_a_held_minus_128_keeps_the_nearest_code():
+    """A block made elsewhere that holds -128 takes the scale of new rows, 2^e: -128 stays
+    only where the old scale is less than 1/256 below it."""
+    for own, code in ((1.0 - 2.0 ** -10, -128), (127.75 / 128, -128), (127.25 / 128, -127), (0.6, -77)):
+        cache = build_switch_kv_cache(1, 32, 1, device=DEV, dtype=INT8, block_size=32)
+        _append(cache, torch.zeros(1, 2, 1, 128, dtype=torch.bfloat16), 0)
+        cache.k[0, :2] = -128
+        cache.k_scales.fill_(own)
+        x = torch.full((1, 1, 1, 128), 100.0, dtype=torch.bfloat16)
+        _append(cache, x, 2)
+        assert float(cache.k_scales[0, 0, 0]) == 1.0 and (cache.k[0, :2] == code).all() and (cache.k[0, 2] == 100).all()
