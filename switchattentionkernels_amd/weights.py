@@ -38,6 +38,9 @@ def switch_gqa_prefill_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.
     backward, it needs each list's key bounds non-decreasing along the list: true for metadata
     of ``build_switch_attention_metadata`` that was not modified since, checked for any other.
     Lists and bounds that need a check make the call wait for it, and a capture refuse it.
+
+    Rows that are padding add to the keys before them like any other; a row whose ``lse`` is
+    set to +inf adds nothing (its Q must be finite).
     """
     check_qkv(q, k, k)
     if window_size <= 0:
