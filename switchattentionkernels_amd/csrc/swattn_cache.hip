@@ -264,9 +264,9 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // per step, so that ballots count and place them and the waves meet only once.
 // kPer > 0: a thread's kPer weights are read once, into registers; 0: any number,
 // read again in every pass.  Bound by latency: few workgroups for few sequences.
-// 16384 rows, 8 pairs: 26 us with 8-bit digits and five reads, 12 so, 10 since a search
-// ends where a whole bin stays, mostly after two digits; 4096 rows, 256 pairs: 12.7,
-// 9.9 and 9.
+// 16384 rows, 8 pairs: 26 us with 8-bit digits and five reads, 12 so, 9.7 since a search
+// ends where a whole bin stays, mostly after two digits.  Rows behind a sequence's end (key
+// 0) stay out of the bins: all in one bin they took 17.5 us for 5000 rows where 7.0 do.
 constexpr int kDigits = 2048;
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
     const uint32_t digits = pass == 2 ? 1023u : 2047u;
     __syncthreads();   // the bins are clear
     each([&](int64_t, uint32_t k) {
-      if (pass == 0 || (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & digits], 1u);
+      if (pass == 0 ? k != 0u : (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & digits], 1u);
     });
     __syncthreads();
     // Bins from the top, kBins per thread; the one that holds the need-th key.
@@ -710,6 +710,9 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
   if (grid > kMaxGrid) return invalid(n + ": grid too large");
   const dim3 gs(static_cast<uint32_t>(pairs));
   const hipStream_t hs = as_stream(stream);
+  // The fewest weights per thread that hold a cache, its registers and steps with them:
+  // 4096 rows 5.1 us, 4097 7.2 and 5000 7.0; 8192 7.8, 16384 9.7, 16385 11.0; 32768 14.7, and
+  // 32769, read again in every pass, 40 (8 pairs; 256 of 4096 rows 5.7).
   if (cache_len <= 4096)
     hipLaunchKernelGGL((select_kernel<1024, 4>), gs, dim3(1024), 0, hs, p);
   else if (cache_len <= 16384)
