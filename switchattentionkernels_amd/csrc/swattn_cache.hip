@@ -268,6 +268,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // ends where a whole bin stays, mostly after two digits.  Rows behind a sequence's end (key
 // 0) stay out of the bins: all in one bin they took 17.5 us for 5000 rows where 7.0 do.
 constexpr int kDigits = 2048;
+constexpr int kSelectThreads = 1024;
 template <int kThreads, int kPer>
 __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
   constexpr int kWaves = kThreads / 64;
@@ -707,20 +708,20 @@ int swattn_cache_evict(const void* k, const void* v, const float* k_scales, cons
   p.budget = static_cast<int>(budget);
   p.recent = static_cast<int>(recent);
   const int64_t pairs = static_cast<int64_t>(batch) * heads_kv, grid = pairs * p.out_nblk;
-  if (grid > kMaxGrid) return invalid(n + ": grid too large");
+  if (grid > kMaxGrid || pairs > kMaxGrid / (kSelectThreads / 256)) return invalid(n + ": grid too large");
   const dim3 gs(static_cast<uint32_t>(pairs));
   const hipStream_t hs = as_stream(stream);
   // The fewest weights per thread that hold a cache, its registers and steps with them:
   // 4096 rows 5.1 us, 4097 7.2 and 5000 7.0; 8192 7.8, 16384 9.7, 16385 11.0; 32768 14.7, and
   // 32769, read again in every pass, 40 (8 pairs; 256 of 4096 rows 5.7).
   if (cache_len <= 4096)
-    hipLaunchKernelGGL((select_kernel<1024, 4>), gs, dim3(1024), 0, hs, p);
+    hipLaunchKernelGGL((select_kernel<kSelectThreads, 4>), gs, dim3(kSelectThreads), 0, hs, p);
   else if (cache_len <= 16384)
-    hipLaunchKernelGGL((select_kernel<1024, 16>), gs, dim3(1024), 0, hs, p);
+    hipLaunchKernelGGL((select_kernel<kSelectThreads, 16>), gs, dim3(kSelectThreads), 0, hs, p);
   else if (cache_len <= 32768)
-    hipLaunchKernelGGL((select_kernel<1024, 32>), gs, dim3(1024), 0, hs, p);
+    hipLaunchKernelGGL((select_kernel<kSelectThreads, 32>), gs, dim3(kSelectThreads), 0, hs, p);
   else
-    hipLaunchKernelGGL((select_kernel<1024, 0>), gs, dim3(1024), 0, hs, p);
+    hipLaunchKernelGGL((select_kernel<kSelectThreads, 0>), gs, dim3(kSelectThreads), 0, hs, p);
   // K and V, read and written.
   const bool streamed = pairs * std::min(budget, cache_len) * 4 * kD >= kStreamBytes;
   by_code_and_block<LaunchGather>(codes, block, dim3(static_cast<uint32_t>(grid)), as_stream(stream), p, streamed);
