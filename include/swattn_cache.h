@@ -106,8 +106,8 @@ int swattn_cache_decode_fwd(const void* q, const void* k, const void* v, const f
  * (0 for a key that no row sees).  q, k, the lists, the metadata bounds, the
  * shapes, window and scale_log2 are those of swattn_prefill_fwd and lse is its
  * result.  Each list's key bounds must be non-decreasing along the list, as
- * for swattn_prefill_bwd.  A row with LSE +inf and finite scores adds nothing.  scale_log2 must be finite, and batch * seq_q *
- * heads_q below 2^31.
+ * for swattn_prefill_bwd.  A row with LSE +inf and finite scores adds nothing.
+ * scale_log2 must be finite, and batch * seq_q * heads_q below 2^31.
  *   key_weights  fp32 [batch, heads_kv, seq_kv]; every entry is written
  *   workspace    >= swattn_prefill_key_weights_workspace_bytes(), 256-byte aligned
  */

@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const EvictParams p) {
 // block, KV head).  32 sequences of 1024 to 4096 rows cut to 2047, 8 KV heads,
 // blocks of 32, then read back: 146.5 us for search, copy and read, 144 since the chosen
 // rows' loads do not wait for the length's, 136 streamed; the copy alone moves scattered
-// 128-byte rows at 4.2 TB/s.  (64 rows a workgroup and a block's heads on one XCD were
+// 128-byte rows at 3.8 (traced) to 4.2 TB/s.  (64 rows a workgroup and a block's heads on one XCD were
 // slower: 59 us, 64 and 62 when the copy took that.)
 template <int kCode, int kBlock, bool kStream>
 __global__ __launch_bounds__(256) void gather_kernel(const EvictParams p) {

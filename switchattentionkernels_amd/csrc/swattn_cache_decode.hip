@@ -31,7 +31,7 @@
 //
 // Measured, Hkv 8, as a large copy's 5.2 TB/s goes: B16 L16384-32768 Hq64 int8 all
 // full 158 us, 5.1 TB/s of codes and scales; B64 L4096-8192 Hq32 e4m3 p_full
-// 0.25 74 us, of which the merge and its launch are about 8; B1 L4096 Hq32 11.3 us, bound
+// 0.25 72-74 us, of which the merge and its launch are about 8; B1 L4096 Hq32 11.3 us, bound
 // by dependent latencies (plan, first keys, combine, merge) and, at that length, by
 // the host's calls.  Two workgroups per CU with loads three steps ahead: 12.8 us
 // (B1), 77 (B64); four with one step ahead 13 and 85.  Joining the pieces in the same
