@@ -24,6 +24,13 @@ from .cache import (  # noqa: F401
     switch_kv_cache_read,
 )
 from .decode import switch_gqa_decode_forward, switch_gqa_decode_quantized_forward  # noqa: F401
+from .rotary import (  # noqa: F401
+    SwitchQKRotaryFunction,
+    switch_qk_rotary,
+    switch_qk_rotary_append,
+    switch_qk_rotary_backward,
+    switch_qk_rotary_forward,
+)
 from .weights import switch_gqa_prefill_key_weights  # noqa: F401
 from .backward import (  # noqa: F401
     SwitchGQAPrefillFunction,
@@ -54,4 +61,9 @@ __all__ = [
     "switch_gqa_prefill",
     "switch_gqa_prefill_varlen",
     "SwitchGQAPrefillFunction",
+    "switch_qk_rotary_forward",
+    "switch_qk_rotary_backward",
+    "switch_qk_rotary",
+    "switch_qk_rotary_append",
+    "SwitchQKRotaryFunction",
 ]

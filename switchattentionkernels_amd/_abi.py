@@ -67,6 +67,20 @@ CACHE_SIGNATURES = {
                                                        _i64, _i64, _vp, ctypes.c_size_t, _vp]),
 }
 
+# Norm and rotation of queries and keys; must mirror include/swattn_rotary.h exactly.
+_f32 = ctypes.c_float
+_i64p = ctypes.POINTER(_i64)
+_HOW = [_vp, _vp, _i32, _i32p, _i32, _i32, _vp, _vp, _i32, _f32]   # positions .. eps
+ROTARY_SIGNATURES = {
+    "swattn_rotary_fwd": (ctypes.c_int, [_vp, _i64p, _vp, _i64p] + _HOW + [_vp, _vp, _i32, _i64, _i32,
+                                                                           _i32, _i32, _vp]),
+    "swattn_rotary_append": (ctypes.c_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p] + _HOW + [_vp] * 6 + [
+        _i32, _i64, _i64, _i32, _i32, _i32, _vp]),
+    "swattn_rotary_bwd_workspace_bytes": (ctypes.c_size_t, [_i32, _i64, _i32, _i32]),
+    "swattn_rotary_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i64p, _vp, _i64p] + _HOW + [_vp] * 4 + [
+        _i32, _i64, _i32, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+}
+
 # Entry points of libswattn.so for this package only (csrc/swattn_internal.h).
 INTERNAL_SIGNATURES = {
     "swattn_compact_wait": (ctypes.c_int, [_vp, _i32, _i64, ctypes.c_float, _vp, _vp, _vp,

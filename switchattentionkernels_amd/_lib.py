@@ -1,5 +1,5 @@
 """Bindings of ``libswattn.so``: ctypes for the C ABI (``include/swattn.h``,
-``include/swattn_cache.h``) and the native extension for the hot calls (``csrc/native.cpp``).
+``include/swattn_cache.h``, ``include/swattn_rotary.h``) and the native extension for the hot calls (``csrc/native.cpp``).
 
 The library is built in-tree by ``switchattentionkernels_amd.build``.  There
 is no fallback: if the library is missing every call raises, so a GPU run can
@@ -19,7 +19,7 @@ import torch  # loads PyTorch's HIP runtime before the library
 from torch.overrides import has_torch_function_unary
 
 from ._abi import (CACHE_SIGNATURES, INTERNAL_SIGNATURES, PROBE_SIGNATURES,  # noqa: F401  -- API
-                   SIGNATURES, bind)
+                   ROTARY_SIGNATURES, SIGNATURES, bind)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libswattn.so")
@@ -47,7 +47,10 @@ def lib() -> ctypes.CDLL:
                 raise LibraryNotBuilt(
                     f"{LIB_PATH} is missing: build it with "
                     "`python -m switchattentionkernels_amd.build`")
-            _lib = bind(bind(bind(ctypes.CDLL(LIB_PATH)), CACHE_SIGNATURES), INTERNAL_SIGNATURES)
+            handle = bind(ctypes.CDLL(LIB_PATH))
+            for signatures in (CACHE_SIGNATURES, ROTARY_SIGNATURES, INTERNAL_SIGNATURES):
+                bind(handle, signatures)
+            _lib = handle
     return _lib
 
 
@@ -105,6 +108,13 @@ def like(t):
     """``torch.empty_like(t)`` where a tensor subclass or a function mode may have
     a say in it, else None: the native layer allocates the output itself."""
     return torch.empty_like(t) if has_torch_function_unary(t) else None
+
+
+def like_contiguous(t):
+    """The same for outputs that are contiguous whatever ``t``'s strides are."""
+    if has_torch_function_unary(t):
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return None
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

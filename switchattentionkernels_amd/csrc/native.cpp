@@ -11,13 +11,16 @@
 #include <ATen/core/CachingHostAllocator.h>
 #include <torch/extension.h>
 
+#include <limits>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "swattn.h"
 #include "swattn_cache.h"
 #include "swattn_internal.h"
+#include "swattn_rotary.h"
 
 namespace {
 
@@ -439,6 +442,181 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_evict_new(
   return {out_k, out_v, out_ks, out_vs, out_weights, out_lens};
 }
 
+// Norm and rotation of queries and keys.
+
+// A row tensor [B, S, H, 128] with free strides (steps of 16 bytes) but for the head rows.
+bool rows_ok(const Tensor& t, at::Device device) {
+  if (!(t.scalar_type() == at::kBFloat16 && t.is_cuda() && t.device() == device && t.layout() == at::kStrided &&
+        t.dim() == 4 && t.size(0) > 0 && t.size(2) > 0 && t.size(3) == 128))
+    return false;
+  if (t.numel() == 0) return true;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && t.stride(i) % 8 != 0) return false;
+  return t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+}
+
+struct RowStrides {
+  int64_t s[3];
+  explicit RowStrides(const Tensor& t) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  }
+};
+
+bool vector_ok(const Tensor& t, at::Device device) {
+  return t.layout() == at::kStrided && t.dim() == 1 && t.is_contiguous() && t.device() == device;
+}
+
+bool rotary_ok(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+               const std::vector<int32_t>& sections, const optional<Tensor>& q_weight,
+               const optional<Tensor>& k_weight, double eps) {
+  const at::Device dev = q.device();
+  if (!rows_ok(q, dev) || !rows_ok(k, dev) || q.size(0) != k.size(0) || q.size(1) != k.size(1)) return false;
+  if (!((inv_freq.scalar_type() == at::kFloat || inv_freq.scalar_type() == at::kDouble) && vector_ok(inv_freq, dev) &&
+        inv_freq.numel() % 8 == 0 && inv_freq.numel() >= 8 && inv_freq.numel() <= 64))
+    return false;
+  int64_t sum = 0;
+  for (const int32_t n : sections) {
+    if (n < 1) return false;
+    sum += n;
+  }
+  if (sections.empty() || sections.size() > SWATTN_ROTARY_MAX_AXES || sum != inv_freq.numel()) return false;
+  const int64_t want[3] = {static_cast<int64_t>(sections.size()), q.size(0), q.size(1)};
+  if (!(positions.scalar_type() == at::kInt && positions.layout() == at::kStrided &&
+        positions.sizes() == at::IntArrayRef(want, 3) && positions.is_contiguous() && positions.device() == dev))
+    return false;
+  for (const optional<Tensor>* w : {&q_weight, &k_weight})
+    if (w->has_value() && !(((*w)->scalar_type() == at::kFloat || (*w)->scalar_type() == at::kBFloat16) &&
+                            vector_ok(**w, dev) && (*w)->numel() == 128))
+      return false;
+  if (q_weight.has_value() && k_weight.has_value() && q_weight->scalar_type() != k_weight->scalar_type()) return false;
+  return eps >= 0.0 && eps < std::numeric_limits<double>::infinity();
+}
+
+bool rotary_append_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc,
+                      const Tensor& lens, const optional<Tensor>& counts) {
+  const auto cache = [&](const Tensor& c) {
+    return c.scalar_type() == at::kBFloat16 && c.layout() == at::kStrided && c.device() == q.device() && c.dim() == 4 &&
+           c.size(0) == k.size(0) && c.size(1) > 0 && c.size(2) == k.size(2) && c.size(3) == 128 && c.is_contiguous() &&
+           reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0;
+  };
+  return rows_ok(v, q.device()) && v.sizes() == k.sizes() && cache(kc) && cache(vc) && kc.sizes() == vc.sizes() &&
+         lens_ok(lens, q) && (!counts.has_value() || lens_ok(*counts, q));
+}
+
+// apart() for tensors of any strides, by the span from their first to their last element.
+bool rotary_apart(const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
+  const auto span = [](const Tensor& t) {
+    const char* first = static_cast<const char*>(t.const_data_ptr());
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      if (t.size(i) == 0) return std::make_pair(first, first);
+      last += (t.size(i) - 1) * t.stride(i);
+    }
+    return std::make_pair(first, first + (last + 1) * static_cast<int64_t>(t.element_size()));
+  };
+  const auto overlap = [&](const Tensor& a, const Tensor& b) {
+    const auto x = span(a), y = span(b);
+    return a.device() == b.device() && x.first < y.second && y.first < x.second;
+  };
+  for (size_t i = 0; i < written.size(); ++i) {
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(written[i], written[j])) return false;
+    for (const Tensor& t : read)
+      if (overlap(written[i], t)) return false;
+  }
+  return true;
+}
+
+const void* weight_ptr(const optional<Tensor>& w) { return w.has_value() ? w->const_data_ptr() : nullptr; }
+int32_t weight_bf16(const optional<Tensor>& q, const optional<Tensor>& k) {
+  return (q.has_value() && q->scalar_type() == at::kBFloat16) || (k.has_value() && k->scalar_type() == at::kBFloat16);
+}
+
+std::tuple<Tensor, Tensor> rotary_forward(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                          const Tensor& inv_freq, const std::vector<int32_t>& sections,
+                                          bool interleaved, const optional<Tensor>& q_weight,
+                                          const optional<Tensor>& k_weight, double eps, int64_t stream,
+                                          const optional<Tensor>& q_made, const optional<Tensor>& k_made) {
+  const Tensor q_out = like(q, q_made), k_out = like(k, k_made);
+  if (q.size(1) == 0) return {q_out, k_out};
+  const RowStrides qs(q), ks(k);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_rotary_fwd(q.const_data_ptr(), qs.s, k.const_data_ptr(), ks.s, i32(positions), inv_freq.const_data_ptr(),
+                               inv_freq.scalar_type() == at::kDouble, sections.data(), static_cast<int32_t>(sections.size()),
+                               interleaved, weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
+                               static_cast<float>(eps), q_out.data_ptr(), k_out.data_ptr(), static_cast<int32_t>(q.size(0)),
+                               q.size(1), static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128,
+                               as_stream(stream));
+  }
+  check(status, "swattn_rotary_fwd");
+  return {q_out, k_out};
+}
+
+std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>> rotary_backward(
+    const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k, const Tensor& positions,
+    const Tensor& inv_freq, const std::vector<int32_t>& sections, bool interleaved, const optional<Tensor>& q_weight,
+    const optional<Tensor>& k_weight, double eps, bool weight_grads, int64_t stream) {
+  const Tensor dq = at::empty(grad_q.sizes(), grad_q.options()), dk = at::empty(grad_k.sizes(), grad_k.options());
+  optional<Tensor> dwq, dwk;
+  const bool none = q.size(1) == 0;
+  if (weight_grads && q_weight.has_value())
+    dwq = none ? at::zeros(q_weight->sizes(), q_weight->options()) : at::empty(q_weight->sizes(), q_weight->options());
+  if (weight_grads && k_weight.has_value())
+    dwk = none ? at::zeros(k_weight->sizes(), k_weight->options()) : at::empty(k_weight->sizes(), k_weight->options());
+  if (none) return {dq, dk, dwq, dwk};
+  const int32_t batch = static_cast<int32_t>(q.size(0)), hq = static_cast<int32_t>(q.size(2));
+  const int32_t hkv = static_cast<int32_t>(k.size(2));
+  const bool sums = dwq.has_value() || dwk.has_value();
+  const size_t ws_bytes = sums ? swattn_rotary_bwd_workspace_bytes(batch, q.size(1), hq, hkv) : 0;
+  Tensor ws;
+  if (sums) ws = bytes(q, ws_bytes);
+  const RowStrides qs(q), ks(k);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_rotary_bwd(grad_q.const_data_ptr(), grad_k.const_data_ptr(), q.const_data_ptr(), qs.s,
+                               k.const_data_ptr(), ks.s, i32(positions), inv_freq.const_data_ptr(),
+                               inv_freq.scalar_type() == at::kDouble, sections.data(), static_cast<int32_t>(sections.size()),
+                               interleaved, weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
+                               static_cast<float>(eps), dq.data_ptr(), dk.data_ptr(),
+                               dwq.has_value() ? dwq->data_ptr() : nullptr, dwk.has_value() ? dwk->data_ptr() : nullptr,
+                               batch, q.size(1), hq, hkv, 128, sums ? ws.data_ptr() : nullptr, ws_bytes, as_stream(stream));
+  }
+  check(status, "swattn_rotary_bwd");
+  return {dq, dk, dwq, dwk};
+}
+
+// (rotated q, the new lengths).
+std::tuple<Tensor, Tensor> rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc,
+                                         const Tensor& vc, const Tensor& lens, const optional<Tensor>& counts,
+                                         const Tensor& positions, const Tensor& inv_freq,
+                                         const std::vector<int32_t>& sections, bool interleaved,
+                                         const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
+                                         int64_t stream, const optional<Tensor>& q_made) {
+  const Tensor q_out = like(q, q_made), lens_out = at::empty({q.size(0)}, lens.options());
+  const RowStrides qs(q), ks(k), vs(v);
+  const bool none = q.size(1) == 0;   // only the lengths are written
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_rotary_append(none ? kc.const_data_ptr() : q.const_data_ptr(), qs.s,
+                                  none ? kc.const_data_ptr() : k.const_data_ptr(), ks.s,
+                                  none ? kc.const_data_ptr() : v.const_data_ptr(), vs.s,
+                                  none ? i32(lens) : i32(positions), inv_freq.const_data_ptr(),
+                                  inv_freq.scalar_type() == at::kDouble, sections.data(),
+                                  static_cast<int32_t>(sections.size()), interleaved, weight_ptr(q_weight),
+                                  weight_ptr(k_weight), weight_bf16(q_weight, k_weight), static_cast<float>(eps),
+                                  none ? kc.data_ptr() : q_out.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(lens),
+                                  i32(counts), lens_out.data_ptr<int32_t>(), static_cast<int32_t>(q.size(0)), q.size(1),
+                                  kc.size(1), static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128,
+                                  as_stream(stream));
+  }
+  check(status, "swattn_rotary_append");
+  return {q_out, lens_out};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -460,4 +638,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefill_key_weights", &prefill_key_weights);
   m.def("cache_evict", &cache_evict);
   m.def("cache_evict_new", &cache_evict_new);
+  m.def("rotary_ok", &rotary_ok);
+  m.def("rotary_append_ok", &rotary_append_ok);
+  m.def("rotary_apart", &rotary_apart);
+  m.def("rotary_forward", &rotary_forward);
+  m.def("rotary_backward", &rotary_backward);
+  m.def("rotary_append", &rotary_append);
 }
