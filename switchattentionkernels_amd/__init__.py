@@ -23,7 +23,11 @@ from .cache import (  # noqa: F401
     switch_kv_cache_evict,
     switch_kv_cache_read,
 )
-from .decode import switch_gqa_decode_forward, switch_gqa_decode_quantized_forward  # noqa: F401
+from .decode import (  # noqa: F401
+    switch_gqa_decode_forward,
+    switch_gqa_decode_quantized_forward,
+    switch_gqa_decode_shared_forward,
+)
 from .rotary import (  # noqa: F401
     SwitchQKRotaryFunction,
     switch_qk_rotary,
@@ -66,4 +70,5 @@ __all__ = [
     "switch_qk_rotary",
     "switch_qk_rotary_append",
     "SwitchQKRotaryFunction",
+    "switch_gqa_decode_shared_forward",
 ]

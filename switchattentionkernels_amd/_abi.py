@@ -81,6 +81,13 @@ ROTARY_SIGNATURES = {
         _i32, _i64, _i32, _i32, _i32, _vp, ctypes.c_size_t, _vp]),
 }
 
+# Decode behind shared prefixes; must mirror include/swattn_shared.h exactly.
+SHARED_SIGNATURES = {
+    "swattn_shared_decode_workspace_bytes": (ctypes.c_size_t, [_i32, _i64, _i32, _i64, _i32, _i32]),
+    "swattn_shared_decode_fwd": (ctypes.c_int, [_vp] * 11 + [_i32, _i64, _i32, _i64, _i32, _i32, _i32, _i32,
+                                                             _f32, _vp, ctypes.c_size_t, _vp]),
+}
+
 # Entry points of libswattn.so for this package only (csrc/swattn_internal.h).
 INTERNAL_SIGNATURES = {
     "swattn_compact_wait": (ctypes.c_int, [_vp, _i32, _i64, ctypes.c_float, _vp, _vp, _vp,

@@ -1,5 +1,6 @@
 """Bindings of ``libswattn.so``: ctypes for the C ABI (``include/swattn.h``,
-``include/swattn_cache.h``, ``include/swattn_rotary.h``) and the native extension for the hot calls (``csrc/native.cpp``).
+``include/swattn_cache.h``, ``include/swattn_rotary.h``,
+``include/swattn_shared.h``) and the native extension for the hot calls (``csrc/native.cpp``).
 
 The library is built in-tree by ``switchattentionkernels_amd.build``.  There
 is no fallback: if the library is missing every call raises, so a GPU run can
@@ -19,7 +20,7 @@ import torch  # loads PyTorch's HIP runtime before the library
 from torch.overrides import has_torch_function_unary
 
 from ._abi import (CACHE_SIGNATURES, INTERNAL_SIGNATURES, PROBE_SIGNATURES,  # noqa: F401  -- API
-                   ROTARY_SIGNATURES, SIGNATURES, bind)
+                   ROTARY_SIGNATURES, SHARED_SIGNATURES, SIGNATURES, bind)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libswattn.so")
@@ -48,7 +49,8 @@ def lib() -> ctypes.CDLL:
                     f"{LIB_PATH} is missing: build it with "
                     "`python -m switchattentionkernels_amd.build`")
             handle = bind(ctypes.CDLL(LIB_PATH))
-            for signatures in (CACHE_SIGNATURES, ROTARY_SIGNATURES, INTERNAL_SIGNATURES):
+            for signatures in (CACHE_SIGNATURES, ROTARY_SIGNATURES, SHARED_SIGNATURES,
+                               INTERNAL_SIGNATURES):
                 bind(handle, signatures)
             _lib = handle
     return _lib

@@ -23,7 +23,7 @@ ARCH = "gfx950"
 
 SOURCES = ["swattn_index.hip", "swattn_fwd.hip", "swattn_merge.hip", "swattn_decode.hip",
            "swattn_cache.hip", "swattn_cache_decode.hip", "swattn_weights.hip",
-           "swattn_rotary.hip", "swattn_bwd.hip"]
+           "swattn_rotary.hip", "swattn_shared.hip", "swattn_bwd.hip"]
 # The measurement probe bench.py uses, in a library of its own (not part of the
 # attention library's ABI).
 PROBE_SOURCES = ["probe/mfma_probe.hip"]

@@ -21,6 +21,7 @@
 #include "swattn_cache.h"
 #include "swattn_internal.h"
 #include "swattn_rotary.h"
+#include "swattn_shared.h"
 
 namespace {
 
@@ -617,6 +618,46 @@ std::tuple<Tensor, Tensor> rotary_append(const Tensor& q, const Tensor& k, const
   return {q_out, lens_out};
 }
 
+// Decode behind shared prefixes.
+bool shared_ok(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& prefix_lens, const Tensor& prefix_ids,
+               const Tensor& k, const Tensor& v, const Tensor& lens, const Tensor& full) {
+  const at::Device dev = q.device();
+  for (const Tensor* t : {&q, &kp, &vp, &k, &v})
+    if (!(t->scalar_type() == at::kBFloat16 && t->is_cuda() && t->device() == dev && t->layout() == at::kStrided &&
+          t->dim() == 4 && t->is_contiguous() && t->numel() > 0 && t->size(3) == 128 &&
+          reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0))
+      return false;
+  return q.size(1) == 1 && kp.sizes() == vp.sizes() && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+         kp.size(2) == k.size(2) && q.size(2) % k.size(2) == 0 && q.size(2) / k.size(2) <= 8 &&
+         q.size(0) <= SWATTN_SHARED_MAX_SEQS && kp.size(0) <= SWATTN_SHARED_MAX_PREFIXES && lens_ok(prefix_lens, kp) &&
+         lens_ok(prefix_ids, q) && lens_ok(lens, q) && full.scalar_type() == at::kBool && full.layout() == at::kStrided &&
+         full.dim() == 1 && full.size(0) == q.size(0) && full.is_contiguous() && full.device() == dev;
+}
+
+std::tuple<Tensor, Tensor> shared_decode(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& prefix_lens,
+                                         const Tensor& prefix_ids, const Tensor& k, const Tensor& v, const Tensor& lens,
+                                         const Tensor& full, int64_t window, double scale_log2, int64_t stream,
+                                         const optional<Tensor>& out_made) {
+  const int32_t batch = static_cast<int32_t>(q.size(0)), hq = static_cast<int32_t>(q.size(2));
+  const int32_t hkv = static_cast<int32_t>(k.size(2)), prefixes = static_cast<int32_t>(kp.size(0));
+  const Tensor out = like(q, out_made);
+  const Tensor lse = at::empty({q.size(0), 1, q.size(2)}, q.options().dtype(at::kFloat));
+  const size_t ws_bytes = swattn_shared_decode_workspace_bytes(batch, k.size(1), prefixes, kp.size(1), hq, hkv);
+  const Tensor ws = bytes(q, ws_bytes > 0 ? ws_bytes : 1);
+  int status = 0;
+  {
+    pybind11::gil_scoped_release release;
+    status = swattn_shared_decode_fwd(q.const_data_ptr(), kp.const_data_ptr(), vp.const_data_ptr(), i32(prefix_lens),
+                                      i32(prefix_ids), k.const_data_ptr(), v.const_data_ptr(), i32(lens),
+                                      static_cast<const uint8_t*>(full.const_data_ptr()), out.data_ptr(),
+                                      lse.data_ptr<float>(), batch, k.size(1), prefixes, kp.size(1), hq, hkv, 128,
+                                      static_cast<int32_t>(window), static_cast<float>(scale_log2), ws.data_ptr(),
+                                      ws_bytes, as_stream(stream));
+  }
+  check(status, "swattn_shared_decode_fwd");
+  return {out, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -644,4 +685,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary_forward", &rotary_forward);
   m.def("rotary_backward", &rotary_backward);
   m.def("rotary_append", &rotary_append);
+  m.def("shared_ok", &shared_ok);
+  m.def("shared_decode", &shared_decode);
 }

@@ -1,0 +1,682 @@
+// Routed GQA decode of sequences that continue shared prefixes, for gfx950
+// (include/swattn_shared.h): the rule of swattn_decode.hip over a prefix's rows and then
+// the sequence's own.  No counterpart in the reference.
+//
+//   s_j = c q.k_j,  p_j = 2^(s_j - m),  O = sum p_j v_j / sum p_j,  LSE = m + log2 sum p_j
+//
+// One launch takes both kinds of keys, a second merges their fp32 partials:
+// * own rows: the line of routed (sequence, KV head) pairs that the decode over whole
+//   caches shares out over workgroups (decode_line.h, decode_pieces.h).  HBM-bound.
+// * prefixes: the query rows of all sequences that attend a prefix form tiles of up to
+//   128 rows per KV head, full and local routes apart; a tile's keys are cut into pieces,
+//   one per workgroup.  K and V are read once per tile, 64 keys at a time, into LDS
+//   (global -> LDS DMA, double-buffered) and both products run on the matrix cores, a
+//   wave per 32 rows: S^T = K Q^T, and O^T = V^T P^T with V transposed by the LDS
+//   reads.  S^T's accumulator layout is P^T's operand layout.  P enters its product as two
+//   bf16 numbers, its value and what that leaves (17 bits; the prefill rounds P to one).
+// The first workgroups take prefix pieces, the others shares of the line; how many of
+// each is settled on the device by every workgroup for itself, from the lengths.
+//
+// Local rows attend the last rows of their prefix only, each from its own start on.
+// Masked weights are 0 there, and V elements that are not finite, which 0 would turn
+// into NaN, are taken out of a masked tile's product and added key by key to the rows
+// that attend them.
+
+#include <limits.h>
+#include <math.h>
+
+#include <string>
+
+#include "decode_pieces.h"
+#include "swattn_shared.h"
+#include "tiles.h"
+
+namespace swattn {
+namespace {
+
+using tiles::bf16x8;
+using tiles::f32x16;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTileRows = 128;       // query rows of a prefix tile, at most
+constexpr int kTileKeys = tiles::kBN;
+constexpr int kMaxGroups = 2 * SWATTN_SHARED_MAX_PREFIXES;   // (prefix, route)
+constexpr uint32_t kMinPiece = 128;  // keys of a prefix piece, at least
+// What a key of a prefix tile costs, in 16ths of a key of the line.
+constexpr uint32_t kTileCost = 10;
+
+struct SharedParams : RowParams {
+  static constexpr uint32_t kMinShare = 128;
+  static constexpr uint32_t kLongShare = UINT32_MAX;
+  static constexpr uint32_t kAlignSlack = 80;
+  static constexpr bool kKeepNan = true;
+  const uint16_t* prefix_k;
+  const uint16_t* prefix_v;
+  const int32_t* prefix_lens;
+  const int32_t* prefix_ids;
+  float* tile_o;      // [piece][tile_rows][128] partials of prefix pieces
+  float* tile_ml;     // [piece][tile_rows][2]
+  int4* place;        // per sequence {first piece of KV head 0, pieces, first row, -}
+  int prefixes, prefix_len;
+  int tile_seqs;      // sequences of a tile, at most
+  int tile_rows;      // rows that a partial has room for
+  uint32_t least;     // workgroups that take the line, at least
+};
+
+// What a workgroup that takes a prefix piece has to know.
+struct Piece {
+  int group, tile, kvh, part;   // group = 2 * prefix + (local)
+  int parts, length;            // pieces of a tile, keys of a piece
+  int first, end;               // keys that the group's rows attend
+  int seqs;                     // of the group
+  int base;                     // the group's first piece
+};
+
+struct Routes {   // of a thread's sequences
+  int group[kInlinePer], start[kInlinePer];   // group -1: attends no prefix row
+  int lo[kInlinePer], n[kInlinePer];          // own rows
+};
+
+__device__ __forceinline__ int prefix_rows(const SharedParams& p, int prefix) {
+  return min(max(p.prefix_lens[prefix], 0), p.prefix_len);
+}
+
+__device__ __forceinline__ void routes_of(const SharedParams& p, int per, Routes& r) {
+#pragma unroll
+  for (int j = 0; j < kInlinePer; ++j) {
+    const int b = static_cast<int>(threadIdx.x) * per + j;
+    r.group[j] = -1;
+    r.start[j] = r.lo[j] = r.n[j] = 0;
+    if (j >= per || b >= p.batch) continue;
+    key_range(p, b, r.lo[j], r.n[j]);
+    const int id = p.prefix_ids[b];
+    if (id < 0 || id >= p.prefixes) continue;
+    const int rows = prefix_rows(p, id), len = r.lo[j] + r.n[j];
+    const bool full = p.full[b] != 0;
+    r.start[j] = full ? 0 : max(rows - max(p.window - len, 0), 0);
+    if (r.start[j] < rows) r.group[j] = 2 * id + (full ? 0 : 1);
+  }
+}
+
+// The workgroup's part: a prefix piece (true), or a share of the line (false; st.take 0
+// past its end).  s_counts: LDS words for the groups' sequences, and the local groups'
+// first keys.
+__device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes& r, int per, int* s_counts, int* s_first,
+                                            SeqEntry* s_ent, Piece& piece, SplitStart& st, uint32_t& wg) {
+  __shared__ Piece s_piece;
+  __shared__ SplitStart s_start;
+  const int tid = threadIdx.x;
+  const int groups = 2 * p.prefixes, gper = (groups + 255) >> 8;
+  for (int g = tid; g < groups; g += 256) {
+    s_counts[g] = 0;
+    s_first[g] = g & 1 ? INT_MAX : 0;
+  }
+  __syncthreads();
+  uint32_t keys = 0, cnt = 0;
+#pragma unroll
+  for (int j = 0; j < kInlinePer; ++j) {
+    keys += r.n[j];
+    cnt += r.n[j] > 0 ? 1 : 0;
+    if (r.group[j] >= 0) {
+      atomicAdd(&s_counts[r.group[j]], 1);
+      if (r.group[j] & 1) atomicMin(&s_first[r.group[j]], r.start[j]);
+    }
+  }
+  uint32_t before, rank, all_keys, all_cnt;
+  scan_keys<4, 0, uint32_t>(keys, cnt, before, rank, all_keys, all_cnt);   // (its barrier orders the atomics too)
+  const uint32_t line = (all_keys + all_cnt * p.pad) * p.hkv;
+  // Positions of all prefix tiles; this thread's groups: tid * gper and on.
+  auto tiles_of = [&](int g) { return static_cast<uint32_t>((s_counts[g] + p.tile_seqs - 1) / p.tile_seqs); };
+  auto keys_of = [&](int g) { return static_cast<uint32_t>(prefix_rows(p, g >> 1) - s_first[g]); };
+  uint32_t positions = 0, tile_cnt = 0, unused0, unused1, all_positions, all_tiles;
+  for (int i = 0; i < gper; ++i) {
+    const int g = tid * gper + i;
+    if (g < groups && s_counts[g] > 0) {
+      positions += tiles_of(g) * keys_of(g);
+      tile_cnt += tiles_of(g);
+    }
+  }
+  scan_keys<4, 1, uint32_t>(positions, tile_cnt, unused0, unused1, all_positions, all_tiles);
+  // Equal shares of the whole cost, and the keys of a piece at that; a tile is spread
+  // over at most 255 pieces.
+  const uint64_t cost = line + (static_cast<uint64_t>(all_positions) * p.hkv * kTileCost + 15u) / 16u;
+  const uint32_t share = static_cast<uint32_t>((cost + p.target - 1) / p.target);
+  const uint32_t by_len = (static_cast<uint32_t>(p.prefix_len) + 254u) / 255u;
+  const uint32_t length = (max(max((share * 16u + kTileCost - 1u) / kTileCost, by_len), kMinPiece) + kTileKeys - 1u) & ~(kTileKeys - 1u);
+  auto length_of = [&](uint32_t n) {   // equal pieces, whole tiles of keys
+    const uint32_t parts = (n + length - 1u) / length;
+    return ((n + parts - 1u) / parts + kTileKeys - 1u) & ~(kTileKeys - 1u);
+  };
+  uint32_t pieces = 0, base, all_pieces;
+  for (int i = 0; i < gper; ++i) {
+    const int g = tid * gper + i;
+    if (g < groups && s_counts[g] > 0) {
+      const uint32_t n = keys_of(g), l = length_of(n);
+      pieces += tiles_of(g) * p.hkv * ((n + l - 1u) / l);
+    }
+  }
+  scan_keys<4, 2, uint32_t>(pieces, 0, base, unused0, all_pieces, unused1);
+  const uint32_t block = blockIdx.x;
+  if (block < all_pieces) {   // uniform
+    for (int i = 0; i < gper; ++i) {
+      const int g = tid * gper + i;
+      if (g >= groups || s_counts[g] == 0) continue;
+      const uint32_t n = keys_of(g), l = length_of(n), parts = (n + l - 1u) / l, here = tiles_of(g) * p.hkv * parts;
+      if (block >= base && block - base < here) {
+        const uint32_t at = block - base, pair = at / parts, tile = pair / p.hkv;
+        s_piece = Piece{g, static_cast<int>(tile), static_cast<int>(pair - tile * p.hkv), static_cast<int>(at - pair * parts),
+                        static_cast<int>(parts), static_cast<int>(l), s_first[g], s_first[g] + static_cast<int>(n),
+                        s_counts[g], static_cast<int>(base)};
+      }
+      base += here;
+    }
+    __syncthreads();
+    piece = s_piece;
+    return true;
+  }
+  // The line, as plan_inline lays it out for the workgroups that the pieces leave.
+  wg = block - all_pieces;
+  SharedParams q = p;
+  q.target = max(p.target > all_pieces ? p.target - all_pieces : 0u, p.least);
+  Line<uint32_t> L = plan_line<uint32_t>(q, all_keys * p.hkv, all_cnt * p.hkv);
+  before += rank * p.pad;
+  if (L.aligned) {
+    uint32_t len = 0, none;
+#pragma unroll
+    for (int j = 0; j < kInlinePer; ++j) len += L.length(r.n[j], 0);
+    scan_keys<4, 3, uint32_t>(len, 0, before, none, L.total, none);
+    L.total *= p.hkv;
+  }
+  const uint64_t pos64 = static_cast<uint64_t>(wg) * L.share;
+  const uint32_t pos = static_cast<uint32_t>(min(pos64, static_cast<uint64_t>(L.total)));
+#pragma unroll
+  for (int j = 0; j < kInlinePer; ++j) {
+    const int b = tid * per + j;
+    const uint32_t off = before * p.hkv, len = L.length(r.n[j], p.pad);
+    if (wg == 0 && j < per && b < p.batch) {
+      p.plan[1 + b] = plan_entry(off, r.n[j], rank, len);
+      if (r.group[j] < 0) p.place[b] = make_int4(0, 0, 0, 0);
+    }
+    if (r.n[j] > 0) {
+      s_ent[rank] = SeqEntry{b, r.lo[j], r.n[j], len};
+      if (pos >= off && pos - off < len * p.hkv) split_start(s_start, rank, pos - off, len);
+      ++rank;
+    }
+    before += len;
+  }
+  if (wg == 0 && tid == 0) p.plan[0] = make_uint4(L.share, L.total, 0u, 0u);
+  st.take = 0;
+  if (pos >= L.total) return false;   // uniform
+  __syncthreads();
+  st = s_start;
+  st.take = min(L.total - pos, L.share);
+  return false;
+}
+
+// 64 keys of K and V as LDS tiles [64][128], 16-byte chunks swizzled by tiles::swz: wave w
+// copies rows 16 w .. 16 w + 15 of both, four rows per instruction; rows behind `last` are
+// read as that one.
+constexpr int kSlotBytes = 2 * tiles::kTileBytes;
+__device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, int64_t stride, int key, int last,
+                                          uint32_t lds, int wave, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = min(key + 16 * wave + 4 * i + (lane >> 4), last);
+    const int chunk = (lane & 15) ^ (((lane >> 4) << 2) | i);
+    const int64_t at = row * stride + 8 * chunk;
+    const uint32_t to = lds + 1024u * static_cast<uint32_t>(4 * wave + i);
+    tiles::dma16_gather(kb + at, to);
+    tiles::dma16_gather(vb + at, to + tiles::kTileBytes);
+  }
+}
+
+__device__ __forceinline__ bool odd_pair(uint32_t x) {   // whether one of two bf16 numbers is not finite
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// A wave's 32 rows: lane (r, h) = (lane % 32, lane / 32) has row r, keys 8 j + 4 h + i of
+// each 32 and dims 32 d + 8 j + 4 h + i.
+struct RowState {
+  float m, l;        // maximum (the same in both lanes of a row); this lane's share of the sum
+  f32x16 acc[4];
+};
+
+template <bool kMasked>
+__device__ __forceinline__ void tile_step(const char* kt, const bf16x8 (&q)[8], float c, int key, int start, int end,
+                                          RowState& w, int lane) {
+  const char* vt = kt + tiles::kTileBytes;
+  const int r = lane & 31, h = lane >> 5;
+  f32x16 s[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[f][i] = 0.f;
+    const char* row = kt + (32 * f + r) * tiles::kRowBytes;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + 16 * ((2 * d + h) ^ tiles::swz(r)));
+      s[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[d], s[f], 0, 0, 0);
+    }
+  }
+  auto live = [&](int f, int i) {
+    const int at = key + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
+    return !kMasked || (at >= start && at < end);
+  };
+  float top = -INFINITY;
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (kMasked && !live(f, i)) s[f][i] = -INFINITY;
+      top = fmaxf(top, s[f][i]);
+    }
+  top *= c;
+  if (__builtin_amdgcn_ballot_w64(top - w.m > 8.0f)) {   // rare: move the maxima, rescale
+    top = tiles::xor32_max(top);
+    const float mn = top - w.m > 8.0f ? top : w.m;
+    const float a = mn == w.m ? 1.0f : __builtin_amdgcn_exp2f(w.m - mn);
+    w.m = mn;
+    w.l *= a;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) w.acc[d] *= a;
+  }
+  const float from = w.m == -INFINITY ? 0.f : w.m;   // only scores of -inf so far: they weigh nothing
+  bool odd = false;
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float y[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int x = 8 * t + 2 * e + i;
+          y[i] = !live(f, x) ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][x], c, -from));
+          w.l += y[i];
+          s[f][x] = y[i];
+        }
+        hi[e] = tiles::pack_bf16x2(y[0], y[1]);
+        lo[e] = tiles::pack_bf16x2(y[0] - __uint_as_float(hi[e] << 16), y[1] - __uint_as_float(hi[e] & 0xffff0000u));
+      }
+      // V^T operands: dim 32 d + lane % 32 of keys 4 h .. +3 and 8 + 4 h .. +3 of the 16.
+      const int g = lane >> 4, i16 = lane & 15;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        uint32_t v[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = 32 * f + 16 * t + 8 * x + 4 * h + (i16 >> 2);
+          const int chunk = (4 * d + 2 * (g & 1) + ((i16 & 3) >> 1)) ^ tiles::swz(at);
+          const char* from_lds = vt + at * tiles::kRowBytes + 16 * chunk + 8 * (i16 & 1);
+          const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(uintptr_t)tiles::lds_addr(from_lds));
+          const uint2 two = __builtin_bit_cast(uint2, four);
+          v[2 * x] = two.x;
+          v[2 * x + 1] = two.y;
+        }
+        if constexpr (kMasked) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            odd = odd || odd_pair(v[x]);
+            if ((v[x] & 0x7f80u) == 0x7f80u) v[x] &= 0xffff0000u;
+            if ((v[x] & 0x7f800000u) == 0x7f800000u) v[x] &= 0xffffu;
+          }
+        }
+        const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
+        w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, hi), w.acc[d], 0, 0, 0);
+        w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, lo), w.acc[d], 0, 0, 0);
+      }
+    }
+  }
+  if constexpr (kMasked) {
+    if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+    // Values that are not finite, key by key: what they add to the rows that attend them.
+    for (int at = 0; at < kTileKeys; ++at) {
+      const char* row = vt + at * tiles::kRowBytes;
+      const uint32_t mine = *reinterpret_cast<const uint32_t*>(row + 16 * ((lane >> 2) ^ tiles::swz(at)) + 4 * (lane & 3));
+      if (__builtin_amdgcn_ballot_w64(odd_pair(mine)) == 0) continue;
+      float pr = 0.f;   // the weight, in the lane whose keys it is among
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (at >> 5 == f && ((at >> 3) & 3) == i >> 2 && (at & 3) == (i & 3)) pr = s[f][i];
+      const float other = __shfl_xor(pr, 32);
+      if (((at >> 2) & 1) != h) pr = other;
+      if (key + at < start || key + at >= end) continue;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
+          const uint32_t bits = *reinterpret_cast<const uint16_t*>(row + 16 * ((dim >> 3) ^ tiles::swz(at)) + 2 * (dim & 7));
+          if ((bits & 0x7f80u) == 0x7f80u) w.acc[d][i] += pr * bf(bits);
+        }
+    }
+  }
+}
+
+// One workgroup: piece `part` of a tile's keys, for KV head kvh.
+__device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes& routes, int per, const Piece& x,
+                                             int2* s_rows, char* ring) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // The tile's sequences, in order.
+  uint32_t cnt = 0, rank, unused0, unused1, unused2;
+#pragma unroll
+  for (int j = 0; j < kInlinePer; ++j) cnt += routes.group[j] == x.group ? 1 : 0;
+  scan_keys<4, 4, uint32_t>(0, cnt, unused0, rank, unused1, unused2);
+  const int first_seq = x.tile * p.tile_seqs, seqs = min(x.seqs - first_seq, p.tile_seqs);
+#pragma unroll
+  for (int j = 0; j < kInlinePer; ++j) {
+    if (routes.group[j] != x.group) continue;
+    const int at = static_cast<int>(rank++) - first_seq, b = tid * per + j;
+    if (at < 0 || at >= seqs) continue;
+    s_rows[at] = make_int2(b, routes.start[j]);
+    if (x.kvh == 0 && x.part == 0)
+      p.place[b] = make_int4(x.base + x.tile * p.hkv * x.parts, x.parts, at * p.group, 0);
+  }
+  const int k0 = x.first + x.part * x.length, k1 = min(k0 + x.length, x.end);
+  const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
+  const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
+  const int64_t base = (static_cast<int64_t>(x.group >> 1) * p.prefix_len * p.hkv + x.kvh) * kD;
+  const uint16_t *kb = p.prefix_k + base, *vb = p.prefix_v + base;
+  const uint32_t lds = tiles::lds_addr(ring);
+  __syncthreads();   // the rows; the ring was the plan's
+  copy_tile(kb, vb, stride, k0, x.end - 1, lds, wave, lane);
+  // This lane's row.
+  const int rows = seqs * p.group, row = 32 * wave + (lane & 31), h = lane >> 5;
+  const bool mine = row < rows, busy = 32 * wave < rows;   // busy: uniform
+  const int seq = min(row, rows - 1) / p.group;
+  const int2 entry = s_rows[seq];
+  const int64_t at = static_cast<int64_t>(entry.x) * p.hq + x.kvh * p.group + (min(row, rows - 1) - seq * p.group);
+  bf16x8 q[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    u32x4 u = *reinterpret_cast<const u32x4*>(p.q + at * kD + 16 * d + 8 * h);
+    if (p.c < 0.f) u ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};   // so that a score's scale is positive
+    if (!mine) u = u32x4{0, 0, 0, 0};
+    q[d] = __builtin_bit_cast(bf16x8, u);
+  }
+  const float c = fabsf(p.c);
+  const int start = entry.y, latest = __builtin_amdgcn_readfirstlane(tiles::wave_max(start));
+  RowState w;
+  // Once, and with all tiles as masked ones if a sum is not finite then: an infinite value
+  // times the second part of a weight may have made NaN of what is infinite.
+  for (int careful = 0; careful < 2; ++careful) {
+    w.m = -INFINITY;
+    w.l = 0.f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w.acc[d][i] = 0.f;
+    for (int j = 0; j < steps; ++j) {
+      const int key = k0 + kTileKeys * j;
+      // Tile j has arrived, and every wave is done with the one before.
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (j + 1 < steps)
+        copy_tile(kb, vb, stride, key + kTileKeys, x.end - 1, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
+      if (!busy) continue;
+      const char* kt = ring + (j & 1) * kSlotBytes;
+      if (careful || key < latest || key + kTileKeys > k1)
+        tile_step<true>(kt, q, c, key, start, k1, w, lane);
+      else
+        tile_step<false>(kt, q, c, key, start, k1, w, lane);
+    }
+    if (careful) break;
+    float sum = 0.f;   // not finite if one of them is not
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(w.acc[d][i], 0.f, sum);
+    if (!__syncthreads_or(mine && sum != 0.f)) break;
+    copy_tile(kb, vb, stride, k0, x.end - 1, lds, wave, lane);
+  }
+  if (!mine) return;
+  w.l = w.l + __shfl_xor(w.l, 32);
+  const int64_t to = static_cast<int64_t>(blockIdx.x) * p.tile_rows + row;
+  if (h == 0) *reinterpret_cast<float2*>(p.tile_ml + 2 * to) = make_float2(w.m, w.l);
+  float* o = p.tile_o + to * kD + 4 * h;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<float4*>(o + 32 * d + 8 * j) =
+          make_float4(w.acc[d][4 * j], w.acc[d][4 * j + 1], w.acc[d][4 * j + 2], w.acc[d][4 * j + 3]);
+}
+
+// The plan's words, a line share's entries and partials, or a ring of two tiles of K and V.
+constexpr int kEntOffset = 2 * kMaxGroups * static_cast<int>(sizeof(int));
+constexpr int kPieceOffset = kEntOffset + kInlineSeqs * static_cast<int>(sizeof(SeqEntry));
+constexpr int kLdsBytes = 2 * kSlotBytes;
+static_assert(kPieceOffset + sizeof(PieceLds<kMaxG>) <= kLdsBytes, "a share's words fit the ring");
+
+template <int G>
+__global__ __launch_bounds__(256, 2) void shared_split_kernel(const SharedParams p) {
+  __shared__ __align__(1024) char s_mem[kLdsBytes];
+  __shared__ int2 s_rows[kTileRows];
+  const int per = (p.batch + 255) >> 8;
+  Routes routes;
+  routes_of(p, per, routes);
+  Piece piece;
+  SplitStart st;
+  uint32_t wg = 0;
+  int* counts = reinterpret_cast<int*>(s_mem);
+  SeqEntry* ent = reinterpret_cast<SeqEntry*>(s_mem + kEntOffset);
+  if (plan_shared(p, routes, per, counts, counts + kMaxGroups, ent, piece, st, wg))
+    prefix_piece(p, routes, per, piece, s_rows, s_mem);
+  else if (st.take > 0)
+    decode_pieces<G, true>(p, wg, st, ent, *reinterpret_cast<PieceLds<G>*>(s_mem + kPieceOffset));
+}
+
+// One workgroup of 256 threads per output row: merge_row over the row's shares of the line
+// and its prefix pieces, up to 256 of each.
+__global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p) {
+  __shared__ float s_w[2 * kMaxSplitsDev];
+  __shared__ float s_red[8];
+  __shared__ float4 s_part[8][kD / 4];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
+  const int kvh = hq / p.group, h = hq - kvh * p.group;
+  const SeqPlace seq = seq_place(p.plan[1 + b]);
+  const uint32_t share = p.plan[0].x;
+  const int4 place = p.place[b];
+  const uint64_t off = seq.off + static_cast<uint64_t>(kvh) * seq.len;
+  const uint32_t wg0 = quotient(off, share);
+  const int own = seq.n > 0 ? static_cast<int>(quotient(off + seq.n - 1, share) - wg0) + 1 : 0;   // at most 256
+  const int pieces = place.y, all = own + pieces;
+  const int64_t slot0 = static_cast<int64_t>(wg0) + static_cast<int64_t>(seq.rank) * p.hkv + kvh;
+  const int64_t row0 = (static_cast<int64_t>(place.x) + static_cast<int64_t>(kvh) * pieces) * p.tile_rows + place.z + h;
+  const int g = tid >> 5, q = tid & 31;
+  auto part = [&](int c) -> const float4* {
+    const float* at = c < own ? p.part_o + ((slot0 + c) * p.group + h) * kD
+                              : p.tile_o + (row0 + static_cast<int64_t>(c - own) * p.tile_rows) * kD;
+    return reinterpret_cast<const float4*>(at) + q;
+  };
+  float2 ml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+  if (tid < own) ml[0] = *reinterpret_cast<const float2*>(p.part_ml + ((slot0 + tid) * p.group + h) * 2);
+  if (tid < pieces) ml[1] = *reinterpret_cast<const float2*>(p.tile_ml + (row0 + static_cast<int64_t>(tid) * p.tile_rows) * 2);
+  float4 ahead[kMergeAhead];
+#pragma unroll
+  for (int i = 0; i < kMergeAhead; ++i) {
+    ahead[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g + 8 * i < all) ahead[i] = *part(g + 8 * i);
+  }
+  float mx = wave_all(fmaxf(ml[0].x, ml[1].x), Max());
+  if (lane == 0) s_red[wave] = mx;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  // Weights 2^(m - M); where no maximum is finite the sums are 0 or NaN, and stay.
+  float wt[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) wt[i] = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[i].x - M);
+  if (tid < own) s_w[tid] = wt[0];
+  if (tid < pieces) s_w[own + tid] = wt[1];
+  const float lsum = wave_all(wt[0] * ml[0].y + wt[1] * ml[1].y, Add());
+  if (lane == 0) s_red[4 + wave] = lsum;
+  __syncthreads();
+  const float L = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int c, const float4& x) {
+    const float w = s_w[c];
+    a.x += w * x.x;
+    a.y += w * x.y;
+    a.z += w * x.z;
+    a.w += w * x.w;
+  };
+#pragma unroll
+  for (int i = 0; i < kMergeAhead; ++i)
+    if (g + 8 * i < all) add(g + 8 * i, ahead[i]);
+#pragma unroll 4
+  for (int c = g + 8 * kMergeAhead; c < all; c += 8) add(c, *part(c));
+  s_part[g][q] = a;
+  __syncthreads();
+  if (tid < kD) {
+    const float* sums = reinterpret_cast<const float*>(s_part) + tid;
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc += sums[i * kD];
+    p.out[row * kD + tid] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(acc / L));   // no key: 0 / 0
+    if (tid == 0) p.lse[row] = M == -INFINITY && L == L ? -INFINITY : M + log2f(L);
+  }
+}
+
+constexpr int kTarget = 2;         // workgroups per CU
+constexpr int kLineLeast = 8;      // of the target, the part that the line gets at least
+
+int shared_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+    return 256;
+  return n;
+}
+
+struct SharedLayout {
+  int64_t slots, pieces, tile_seqs, tile_rows, target, least;
+  int64_t off_ml, off_plan, off_place, off_tile_o, off_tile_ml, bytes;
+};
+
+// Bounds on what the device plans: tiles are at most one per sequence, and one begun
+// per group and one per tile_seqs sequences; pieces the target's shares and one more
+// for each (tile, KV head).
+bool shared_layout(int64_t batch, int64_t cache_len, int64_t prefixes, int64_t prefix_len, int64_t hq, int64_t hkv,
+                   SharedLayout& L) {
+  if (batch < 1 || batch > SWATTN_SHARED_MAX_SEQS || prefixes < 1 || prefixes > SWATTN_SHARED_MAX_PREFIXES) return false;
+  if (cache_len < 1 || prefix_len < 1 || cache_len > INT32_MAX || prefix_len > INT32_MAX) return false;
+  if (hq < 1 || hkv < 1 || hkv > 65535 || hq % hkv != 0 || hq / hkv > kMaxG) return false;
+  const int64_t group = hq / hkv;
+  L.tile_seqs = kTileRows / group;
+  const int64_t by_group = 2 * prefixes + batch / L.tile_seqs, tiles = by_group < batch ? by_group : batch;
+  // The line takes kPairPad positions per pair beside its keys; pieces are whole key tiles.
+  if (batch * hkv * (cache_len + kPairPad) > INT32_MAX || tiles * hkv * (prefix_len + kTileKeys) > INT32_MAX) return false;
+  L.tile_rows = (batch < L.tile_seqs ? batch : L.tile_seqs) * group;
+  L.target = int64_t{kTarget} * shared_cus();
+  L.least = (L.target + kLineLeast - 1) / kLineLeast;
+  L.slots = L.target + L.least + batch * hkv;
+  L.pieces = L.target + tiles * hkv;
+  auto al = [](int64_t x) { return (x + 255) & ~int64_t{255}; };
+  int64_t o = al(L.slots * group * kD * 4);
+  L.off_ml = o;       o = al(o + L.slots * group * 2 * 4);
+  L.off_plan = o;     o = al(o + (1 + batch) * 16);
+  L.off_place = o;    o = al(o + batch * 16);
+  L.off_tile_o = o;   o = al(o + L.pieces * L.tile_rows * kD * 4);
+  L.off_tile_ml = o;  o = al(o + L.pieces * L.tile_rows * 2 * 4);
+  L.bytes = o;
+  return true;
+}
+
+}  // namespace
+}  // namespace swattn
+
+using namespace swattn;
+
+extern "C" {
+
+size_t swattn_shared_decode_workspace_bytes(int32_t batch, int64_t cache_len, int32_t prefixes, int64_t prefix_len,
+                                            int32_t heads_q, int32_t heads_kv) {
+  SharedLayout L;
+  return shared_layout(batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, L) ? static_cast<size_t>(L.bytes) : 0;
+}
+
+int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_prefix, const int32_t* prefix_lens,
+                             const int32_t* prefix_ids, const void* k_cache, const void* v_cache,
+                             const int32_t* cache_lens, const uint8_t* full, void* out, float* lse, int32_t batch,
+                             int64_t cache_len, int32_t prefixes, int64_t prefix_len, int32_t heads_q,
+                             int32_t heads_kv, int32_t head_dim, int32_t window, float scale_log2, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  const char* name = "swattn_shared_decode_fwd";
+  const std::string n(name);
+  if (head_dim != kD) return invalid(n + ": head_dim must be 128");
+  if (batch < 1 || cache_len < 1 || prefixes < 1 || prefix_len < 1 || heads_q < 1 || heads_kv < 1)
+    return invalid(n + ": bad shape");
+  if (heads_q % heads_kv) return invalid(n + ": heads_q must be a multiple of heads_kv");
+  if (heads_q / heads_kv > kMaxG) return invalid(n + ": heads_q / heads_kv must be at most 8");
+  if (window <= 0) return invalid(n + ": window must be positive");
+  SharedLayout L;
+  if (!shared_layout(batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, L))
+    return invalid(n + ": batch, prefixes, heads_kv or the lengths too large");
+  if (q == nullptr || k_prefix == nullptr || v_prefix == nullptr || prefix_lens == nullptr || prefix_ids == nullptr ||
+      k_cache == nullptr || v_cache == nullptr || cache_lens == nullptr || full == nullptr || out == nullptr || lse == nullptr)
+    return invalid(n + ": null pointer");
+  if (!aligned16(q) || !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return invalid(n + ": q, the prefixes, the caches and out must be 16-byte aligned");
+  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(L.bytes)) {
+    set_error(n + ": workspace smaller than swattn_shared_decode_workspace_bytes()");
+    return SWATTN_EWORKSPACE;
+  }
+  if (!aligned256(workspace)) return invalid(n + ": workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  SharedParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k_cache);
+  p.v = static_cast<const uint16_t*>(v_cache);
+  p.c = scale_log2;
+  p.lens = cache_lens;
+  p.full = full;
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + L.off_ml);
+  p.plan = reinterpret_cast<uint4*>(ws + L.off_plan);
+  p.out = static_cast<uint16_t*>(out);
+  p.lse = lse;
+  p.cache_len = static_cast<int>(cache_len);
+  p.batch = batch;
+  p.hq = heads_q;
+  p.hkv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.window = window;
+  p.target = static_cast<uint32_t>(L.target);
+  p.pad = kPairPad;
+  p.prefix_k = static_cast<const uint16_t*>(k_prefix);
+  p.prefix_v = static_cast<const uint16_t*>(v_prefix);
+  p.prefix_lens = prefix_lens;
+  p.prefix_ids = prefix_ids;
+  p.tile_o = reinterpret_cast<float*>(ws + L.off_tile_o);
+  p.tile_ml = reinterpret_cast<float*>(ws + L.off_tile_ml);
+  p.place = reinterpret_cast<int4*>(ws + L.off_place);
+  p.prefixes = prefixes;
+  p.prefix_len = static_cast<int>(prefix_len);
+  p.tile_seqs = static_cast<int>(L.tile_seqs);
+  p.tile_rows = static_cast<int>(L.tile_rows);
+  p.least = static_cast<uint32_t>(L.least);
+  const hipStream_t st = as_stream(stream);
+  const dim3 grid(static_cast<uint32_t>(L.pieces + L.least));
+  switch (p.group) {
+    case 1: hipLaunchKernelGGL(shared_split_kernel<1>, grid, dim3(256), 0, st, p); break;
+    case 2: hipLaunchKernelGGL(shared_split_kernel<2>, grid, dim3(256), 0, st, p); break;
+    case 3: hipLaunchKernelGGL(shared_split_kernel<3>, grid, dim3(256), 0, st, p); break;
+    case 4: hipLaunchKernelGGL(shared_split_kernel<4>, grid, dim3(256), 0, st, p); break;
+    case 5: hipLaunchKernelGGL(shared_split_kernel<5>, grid, dim3(256), 0, st, p); break;
+    case 6: hipLaunchKernelGGL(shared_split_kernel<6>, grid, dim3(256), 0, st, p); break;
+    case 7: hipLaunchKernelGGL(shared_split_kernel<7>, grid, dim3(256), 0, st, p); break;
+    default: hipLaunchKernelGGL(shared_split_kernel<8>, grid, dim3(256), 0, st, p); break;
+  }
+  hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(batch * heads_q)), dim3(256), 0, st, p);
+  return launch_status(name);
+}
+
+}  // extern "C"

@@ -6,7 +6,8 @@ position ``n - 1`` -- its own K/V already appended -- and attends keys
 ``[0, n)`` when routed full, else the last ``window_size`` of them.  Output
 follows the prefill's conventions: bf16 O and fp32 LSE in the log2
 convention (V:15, V:236-241).  ``switch_gqa_decode_quantized_forward`` does the
-same over an 8-bit cache (``cache.py``).
+same over an 8-bit cache (``cache.py``), ``switch_gqa_decode_shared_forward`` for
+sequences that continue shared prefixes.
 """
 
 from __future__ import annotations
@@ -136,6 +137,90 @@ def switch_gqa_decode_quantized_forward(
                                               min(int(window_size), 2 ** 31 - 1), cache.block_size,
                                               _CODES[cache.k.dtype], scale,
                                               _lib.stream_handle(dev), _lib.like(q))
+    if squeeze:
+        return out[:, 0], lse[:, 0]
+    return out, lse
+
+
+SHARED_MAX_SEQS = 1024       # SWATTN_SHARED_MAX_SEQS
+SHARED_MAX_PREFIXES = 1024   # SWATTN_SHARED_MAX_PREFIXES
+
+
+def _check_shared(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens,
+                  full_mask):
+    """(prefix_lens, prefix_ids, cache_lens, full_mask) for the kernels, or raise."""
+    rows = (q, k_prefix, v_prefix, k_cache, v_cache)
+    if not _all_tensors(*rows) or any(t.dtype != torch.bfloat16 for t in rows):
+        raise TypeError("Switch Attention decode requires BF16 Q, prefixes and KV cache")
+    dev = q.device
+    if not q.is_cuda or any(t.device != dev for t in rows):
+        raise ValueError("Q, prefixes and KV cache must be on one supported accelerator device")
+    if any(not t.is_contiguous() or t.data_ptr() % 16 for t in rows):
+        raise ValueError("Q, prefixes and KV cache must be contiguous and 16-byte aligned")
+    if q.ndim != 4 or q.shape[1] != 1 or k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("q must be [B,1,Hq,128] and the caches [B,L,Hkv,128] of one shape")
+    if k_prefix.ndim != 4 or k_prefix.shape != v_prefix.shape:
+        raise ValueError("the prefixes must be [P,Lp,Hkv,128] of one shape")
+    if any(t.shape[3] != 128 for t in rows):
+        raise ValueError("the decode kernel is specialized for head_dim=128")
+    batch, heads, kv_heads = int(q.shape[0]), int(q.shape[2]), int(k_cache.shape[2])
+    if k_cache.shape[0] != batch:
+        raise ValueError("Q and KV cache batch sizes must match")
+    if kv_heads == 0 or heads == 0 or heads % kv_heads or heads // kv_heads > 8:
+        raise ValueError("query heads must be a multiple (at most 8x) of KV heads")
+    if k_prefix.shape[2] != kv_heads:
+        raise ValueError("the prefixes must have the cache's KV heads")
+    if any(t.numel() == 0 for t in rows):
+        raise ValueError("the batch, the prefixes and the KV cache must hold at least one position")
+    if batch > SHARED_MAX_SEQS or k_prefix.shape[0] > SHARED_MAX_PREFIXES:
+        raise ValueError("at most 1024 sequences and 1024 prefixes")
+    lens = check_lens(cache_lens, batch, dev, "cache_lens")
+    ids = check_lens(prefix_ids, batch, dev, "prefix_ids")
+    if (prefix_lens.dtype != torch.int32 or prefix_lens.shape != (k_prefix.shape[0],)
+            or prefix_lens.device != dev):
+        raise ValueError("prefix_lens must be an int32 [P] tensor on the device of Q")
+    if full_mask.dtype != torch.bool or full_mask.shape != (batch,) or full_mask.device != dev:
+        raise ValueError("full_mask must be a bool [B] tensor on the device of Q")
+    return prefix_lens.contiguous(), ids, lens, full_mask.contiguous()
+
+
+def switch_gqa_decode_shared_forward(
+        q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, prefix_lens: torch.Tensor,
+        prefix_ids: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+        cache_lens: torch.Tensor, full_mask: torch.Tensor, *, window_size: int = 1024,
+        sm_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Routed decode step of sequences that continue shared prefixes:
+    ``switch_gqa_decode_forward`` where the rows of a system prompt or a document are kept
+    once, and read once for all sequences that attend them.
+
+    ``q``: bf16 ``[B, 1, Hq, 128]`` (or ``[B, Hq, 128]``); ``k_prefix`` / ``v_prefix``: bf16
+    ``[P, Lp, Hkv, 128]``, of which prefix i holds the first ``prefix_lens[i]`` rows (int32
+    ``[P]``, clamped to ``[0, Lp]``); ``prefix_ids``: int32 ``[B]``, the prefix that each
+    sequence continues (outside ``[0, P)``: none); ``k_cache`` / ``v_cache``: bf16 ``[B, L,
+    Hkv, 128]``, each sequence's own rows behind its prefix, ``cache_lens[b]`` of them, the
+    new token's among them (int32 ``[B]``, clamped to ``[0, L]``); ``full_mask``: bool
+    ``[B]``.  With ``n`` rows of prefix and cache together a sequence attends all of them
+    when routed full, else the last ``window_size``.  Up to 1024 sequences and 1024 prefixes.
+
+    Returns ``(O [B, 1, Hq, 128] bf16, LSE [B, 1, Hq] fp32)``; a sequence without any row
+    gives O = NaN and LSE = -inf.
+    """
+    squeeze = isinstance(q, torch.Tensor) and q.ndim == 3
+    if squeeze:
+        q = q.unsqueeze(1)
+    if not _all_tensors(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens,
+                        full_mask) or not _lib.native().shared_ok(
+            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask):
+        prefix_lens, prefix_ids, cache_lens, full_mask = _check_shared(
+            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask)
+    if window_size <= 0:
+        raise ValueError("window_size must be positive")
+    scale = (128 ** -0.5 if sm_scale is None else float(sm_scale)) * LOG2E
+    dev = q.device
+    with _lib.on_device(dev):
+        out, lse = _lib.native().shared_decode(
+            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask,
+            min(int(window_size), 2 ** 31 - 1), scale, _lib.stream_handle(dev), _lib.like(q))
     if squeeze:
         return out[:, 0], lse[:, 0]
     return out, lse
