@@ -6,7 +6,9 @@
 //
 // One launch takes both kinds of keys, a second merges their fp32 partials:
 // * own rows: the line of routed (sequence, KV head) pairs that the decode over whole
-//   caches shares out over workgroups (decode_line.h, decode_pieces.h).  HBM-bound.
+//   caches shares out over workgroups (decode_line.h).  HBM-bound, with the products on
+//   the matrix cores as in swattn_cache_decode.hip, so that the vector ALUs are free for
+//   the prefixes.
 // * prefixes: the query rows of all sequences that attend a prefix form tiles of up to
 //   128 rows per KV head, full and local routes apart; a tile's keys are cut into pieces,
 //   one per workgroup.  K and V are read once per tile, 64 keys at a time, into LDS
@@ -27,7 +29,7 @@
 
 #include <string>
 
-#include "decode_pieces.h"
+#include "decode_line.h"
 #include "swattn_shared.h"
 #include "tiles.h"
 
@@ -46,11 +48,19 @@ constexpr uint32_t kMinPiece = 128;  // keys of a prefix piece, at least
 // What a key of a prefix tile costs, in 16ths of a key of the line.
 constexpr uint32_t kTileCost = 10;
 
-struct SharedParams : RowParams {
+constexpr int kOwnWaves = 4;         // waves per workgroup
+constexpr int kMaxG = 8;
+constexpr int kOwnStep = 32;         // keys that a wave takes at once of a sequence's own
+constexpr uint32_t kPairPad = 192;   // a pair's start, in keys
+
+struct SharedParams : DecodeCommon {
   static constexpr uint32_t kMinShare = 128;
   static constexpr uint32_t kLongShare = UINT32_MAX;
   static constexpr uint32_t kAlignSlack = 80;
   static constexpr bool kKeepNan = true;
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
   const uint16_t* prefix_k;
   const uint16_t* prefix_v;
   const int32_t* prefix_lens;
@@ -62,7 +72,13 @@ struct SharedParams : RowParams {
   int tile_seqs;      // sequences of a tile, at most
   int tile_rows;      // rows that a partial has room for
   uint32_t least;     // workgroups that take the line, at least
+  float c;            // sm_scale * log2(e)
 };
+
+__device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+__device__ __forceinline__ int uniform(uint32_t x) {
+  return static_cast<int>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
 
 // What a workgroup that takes a prefix piece has to know.
 struct Piece {
@@ -220,11 +236,11 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes&
 constexpr int kSlotBytes = 2 * tiles::kTileBytes;
 __device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, int64_t stride, int key, int last,
                                           uint32_t lds, int wave, int lane) {
+  const int first = key + 16 * wave + (lane >> 4);
+  const int chunk = (lane & 15) ^ ((lane >> 4) << 2);   // of row 4 i + lane / 16: ^ i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = min(key + 16 * wave + 4 * i + (lane >> 4), last);
-    const int chunk = (lane & 15) ^ (((lane >> 4) << 2) | i);
-    const int64_t at = row * stride + 8 * chunk;
+    const int64_t at = min(first + 4 * i, last) * stride + 8 * (chunk ^ i);
     const uint32_t to = lds + 1024u * static_cast<uint32_t>(4 * wave + i);
     tiles::dma16_gather(kb + at, to);
     tiles::dma16_gather(vb + at, to + tiles::kTileBytes);
@@ -242,20 +258,34 @@ struct RowState {
   f32x16 acc[4];
 };
 
+// Where a lane's operands lie in a tile of K and one of V, from LDS address 0: a chunk's
+// number enters by XOR, the rest of a row's place is added.
+struct LaneLds {
+  uint32_t k;   // key r of K, dims 8 h .. +7; ^ 32 d: those of dims 16 d, + 8192 f: key 32 f + r
+  uint32_t v;   // V^T operand: ^ (64 d + 32 x): dims 32 d, + 256 (32 f + 16 t + 8 x): keys of group t, half x
+};
+__device__ __forceinline__ LaneLds lane_lds(uint32_t ring, int lane) {
+  const int r = lane & 31, h = lane >> 5, half = (lane >> 4) & 1, i = lane & 15;
+  return LaneLds{ring + tiles::kRowBytes * r + 16 * (h ^ tiles::swz(r)),
+                 ring + tiles::kTileBytes + tiles::kRowBytes * (4 * h + (i >> 2)) +
+                     16 * ((2 * half + ((i & 3) >> 1)) ^ (((i >> 2) << 2) | h)) + 8 * (i & 1)};
+}
+typedef __attribute__((address_space(3))) const bf16x8* LdsChunk;
+typedef __attribute__((address_space(3))) s16x4* LdsFour;
+
 template <bool kMasked>
-__device__ __forceinline__ void tile_step(const char* kt, const bf16x8 (&q)[8], float c, int key, int start, int end,
-                                          RowState& w, int lane) {
+__device__ __forceinline__ void tile_step(const char* kt, uint32_t slot, const LaneLds& at_lds, const bf16x8 (&q)[8], float c,
+                                          int key, int start, int end, RowState& w, int lane) {
   const char* vt = kt + tiles::kTileBytes;
-  const int r = lane & 31, h = lane >> 5;
+  const int h = lane >> 5;
   f32x16 s[2];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[f][i] = 0.f;
-    const char* row = kt + (32 * f + r) * tiles::kRowBytes;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
-      const bf16x8 a = *reinterpret_cast<const bf16x8*>(row + 16 * ((2 * d + h) ^ tiles::swz(r)));
+      const bf16x8 a = *(LdsChunk)(uintptr_t)((at_lds.k ^ (32 * d)) + slot + 32 * f * tiles::kRowBytes);
       s[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[d], s[f], 0, 0, 0);
     }
   }
@@ -302,17 +332,13 @@ __device__ __forceinline__ void tile_step(const char* kt, const bf16x8 (&q)[8], 
         lo[e] = tiles::pack_bf16x2(y[0] - __uint_as_float(hi[e] << 16), y[1] - __uint_as_float(hi[e] & 0xffff0000u));
       }
       // V^T operands: dim 32 d + lane % 32 of keys 4 h .. +3 and 8 + 4 h .. +3 of the 16.
-      const int g = lane >> 4, i16 = lane & 15;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         uint32_t v[4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int at = 32 * f + 16 * t + 8 * x + 4 * h + (i16 >> 2);
-          const int chunk = (4 * d + 2 * (g & 1) + ((i16 & 3) >> 1)) ^ tiles::swz(at);
-          const char* from_lds = vt + at * tiles::kRowBytes + 16 * chunk + 8 * (i16 & 1);
           const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(uintptr_t)tiles::lds_addr(from_lds));
+              (LdsFour)(uintptr_t)((at_lds.v ^ (64 * d + 32 * x)) + slot + (32 * f + 16 * t + 8 * x) * tiles::kRowBytes));
           const uint2 two = __builtin_bit_cast(uint2, four);
           v[2 * x] = two.x;
           v[2 * x + 1] = two.y;
@@ -403,6 +429,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
   }
   const float c = fabsf(p.c);
   const int start = entry.y, latest = __builtin_amdgcn_readfirstlane(tiles::wave_max(start));
+  const LaneLds at_lds = lane_lds(lds, lane);
   RowState w;
   // Once, and with all tiles as masked ones if a sum is not finite then: an infinite value
   // times the second part of a weight may have made NaN of what is infinite.
@@ -420,11 +447,11 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
       if (j + 1 < steps)
         copy_tile(kb, vb, stride, key + kTileKeys, x.end - 1, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
       if (!busy) continue;
-      const char* kt = ring + (j & 1) * kSlotBytes;
+      const uint32_t slot = (j & 1) * kSlotBytes;
       if (careful || key < latest || key + kTileKeys > k1)
-        tile_step<true>(kt, q, c, key, start, k1, w, lane);
+        tile_step<true>(ring + slot, slot, at_lds, q, c, key, start, k1, w, lane);
       else
-        tile_step<false>(kt, q, c, key, start, k1, w, lane);
+        tile_step<false>(ring + slot, slot, at_lds, q, c, key, start, k1, w, lane);
     }
     if (careful) break;
     float sum = 0.f;   // not finite if one of them is not
@@ -448,13 +475,219 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
           make_float4(w.acc[d][4 * j], w.acc[d][4 * j + 1], w.acc[d][4 * j + 2], w.acc[d][4 * j + 3]);
 }
 
+// One partial (maximum, sum, unnormalised output) per wave and head.
+struct PieceLds {
+  float m[kOwnWaves][kMaxG], l[kOwnWaves][kMaxG];
+  float acc[kOwnWaves][kMaxG][kD];
+};
+
+// The partials of keys [k0, k1) with one key per wave at a time on the vector ALUs: where
+// the products met values that are not finite.  A weight is one fp32 number here, so that
+// an infinite value stays infinite, and nothing but the piece's rows is read.
+__device__ __forceinline__ void careful_piece(const uint16_t* q, const uint16_t* k, const uint16_t* v, int64_t stride,
+                                              int k0, int k1, int group, float c, int wave, int lane,
+                                              PieceLds& lds) {
+  for (int h = 0; h < group; ++h) {
+    const uint32_t qx = *reinterpret_cast<const uint32_t*>(q + h * kD + 2 * lane);
+    float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int key = k0 + wave; key < k1; key += kOwnWaves) {
+      const uint32_t kx = *reinterpret_cast<const uint32_t*>(k + key * stride + 2 * lane);
+      const uint32_t vx = *reinterpret_cast<const uint32_t*>(v + key * stride + 2 * lane);
+      const float s = c * wave_all(__builtin_fmaf(bf(qx >> 16), bf(kx >> 16), bf(qx & 0xffffu) * bf(kx & 0xffffu)), Add());
+      if (s > m) {
+        const float a = __builtin_amdgcn_exp2f(m - s);
+        l *= a;
+        a0 *= a;
+        a1 *= a;
+        m = s;
+      }
+      const float pr = __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.f : m));
+      l += pr;
+      a0 += pr * bf(vx & 0xffffu);
+      a1 += pr * bf(vx >> 16);
+    }
+    *reinterpret_cast<float2*>(&lds.acc[wave][h][2 * lane]) = make_float2(a0, a1);
+    if (lane == 0) {
+      lds.m[wave][h] = m;
+      lds.l[wave][h] = l;
+    }
+  }
+}
+
+// One share of the line: its pairs one after the other, a piece of each.  A wave takes 32
+// keys at once, steps w, w + 4, ... of a piece; rows outside it are read as its nearest
+// row and masked.
+// * S^T [16 keys x 16 columns] = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) = (lane % 16,
+//   lane / 16) holds key c of the tile, dims 32 j + 8 g .. +7; column c is head c % 8.
+// * O^T [16 dims x 16 columns] += V^T P^T, 32 keys at once: lane (c, g) holds dims 8 c .. +7
+//   of keys 4 g .. +3 of both key tiles; tile n takes dim 8 c + n of each, so that S^T's
+//   accumulator layout is P^T's operand layout, and V is transposed inside a lane.
+//   Columns 0-7 take a weight's first bf16 number, columns 8-15 what it leaves.
+// A piece's partial lies in slot wg + (pair's rank): both only grow along the line, one of
+// them at every step from piece to piece, so that no two pieces share a slot and a pair's
+// slots are consecutive.
+__device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, const SplitStart& st, const SeqEntry* s_ent,
+                                           PieceLds& lds) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  int r = uniform(st.r), kvh = uniform(st.kvh);
+  uint32_t key = uniform(st.key);
+  uint32_t left = uniform(st.take);
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int c = lane & 15, g = lane >> 4, G = p.group, head = c & 7;
+  const bool second = c >= 8;
+  const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
+  for (;;) {
+    const SeqEntry e = s_ent[r];
+    const int b = uniform(e.b);
+    const uint32_t n = uniform(e.n), len = uniform(e.len);
+    const uint32_t took = min(left, len - key);
+    left -= took;
+    if (key < n) {   // else this share starts in the pair's padding
+      const int64_t slot = static_cast<int64_t>(wg) + static_cast<int64_t>(r) * p.hkv + kvh;
+      const int k0 = uniform(e.lo) + static_cast<int>(key), k1 = k0 + static_cast<int>(min(took, n - key));
+      const uint16_t* qb = p.q + (static_cast<int64_t>(b) * p.hq + kvh * G) * kD;
+      const int64_t base = static_cast<int64_t>(b) * p.cache_len * stride + kvh * kD;
+      const uint16_t *kb = p.k + base + 8 * g, *vb = p.v + base + 8 * c;
+      bf16x8 q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4 u = *reinterpret_cast<const u32x4*>(qb + min(head, G - 1) * kD + 32 * j + 8 * g);
+        if (head >= G) u = u32x4{0, 0, 0, 0};
+        q[j] = __builtin_bit_cast(bf16x8, u);
+      }
+      const int steps = (k1 - k0 + kOwnStep - 1) / kOwnStep;
+      u32x4 kr[2][4], vr[8];
+      auto load = [&](int i) {
+        const int at = k0 + kOwnStep * i;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint16_t* row = kb + min(at + 16 * t + c, k1 - 1) * stride;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kr[t][j] = *reinterpret_cast<const u32x4*>(row + 32 * j);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          vr[t] = *reinterpret_cast<const u32x4*>(vb + min(at + 16 * (t >> 2) + 4 * g + (t & 3), k1 - 1) * stride);
+      };
+      load(wave);
+      float m = -INFINITY, l = 0.f;   // column c's maximum, and this lane's share of its sum
+      f32x4 acc[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = wave; i < steps; i += kOwnWaves) {
+        const int at = k0 + kOwnStep * i;
+        f32x4 s[2];
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[t][j]), q[j], s[t], 0, 0, 0);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[t][x] = at + 16 * t + 4 * g + x < k1 ? s[t][x] * p.c : -INFINITY;
+            top = fmaxf(top, s[t][x]);
+          }
+        }
+        if (__builtin_amdgcn_ballot_w64(top - m > 8.0f)) {   // rare: move the maxima, rescale
+          top = with_lane32(with_lane16(top, Max()), Max());
+          const float mn = top - m > 8.0f ? top : m;
+          const float a = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= a;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) acc[t] *= a;
+        }
+        const float from = m == -INFINITY ? 0.f : m;   // only scores of -inf so far: they weigh nothing
+        u32x4 pk;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {
+            float y[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              y[u] = __builtin_amdgcn_exp2f(s[t][x + u] - from);   // 0 behind the piece
+              l += y[u];
+            }
+            const uint32_t hi = tiles::pack_bf16x2(y[0], y[1]);
+            const uint32_t lo = tiles::pack_bf16x2(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
+            pk[2 * t + x / 2] = second ? lo : hi;
+          }
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          u32x4 a0, a1;   // dims 2 d and 2 d + 1 of this lane's eight
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            a0[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], 0x05040100u);
+            a1[t] = __builtin_amdgcn_perm(vr[2 * t + 1][d], vr[2 * t][d], 0x07060302u);
+          }
+          acc[2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), pb, acc[2 * d], 0, 0, 0);
+          acc[2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), pb, acc[2 * d + 1], 0, 0, 0);
+        }
+        load(i + kOwnWaves);   // past the end: the last row, never used
+      }
+      // This wave's partial: column c's sum over its four lanes, O^T with its second
+      // columns.  acc[t][x]: dim 8 (4 g + x) + t of column c.
+      l = with_lane32(with_lane16(l, Add()), Add());
+      float sum = 0.f;   // not 0 if one of the outputs is not finite
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          acc[t][x] += __shfl_xor(acc[t][x], 8);
+          sum = __builtin_fmaf(acc[t][x], 0.f, sum);
+        }
+      if (c < G) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int t = 0; t < 8; t += 4)
+            *reinterpret_cast<f32x4*>(&lds.acc[wave][c][8 * (4 * g + x) + t]) =
+                f32x4{acc[t][x], acc[t + 1][x], acc[t + 2][x], acc[t + 3][x]};
+        if (g == 0) {
+          lds.m[wave][c] = m;
+          lds.l[wave][c] = l;
+        }
+      }
+      if (__syncthreads_or(sum != 0.f)) {
+        careful_piece(qb, p.k + base, p.v + base, stride, k0, k1, G, p.c, wave, lane, lds);
+        __syncthreads();
+      }
+      // Combine the waves: one partial per head.  Where no maximum is finite the sums are 0
+      // or NaN, and stay.
+      float* po = p.part_o + slot * G * kD;
+      float* pml = p.part_ml + slot * G * 2;
+      auto combine = [&](int h, auto of) {
+        float mm = -INFINITY, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kOwnWaves; ++w) mm = fmaxf(mm, lds.m[w][h]);
+#pragma unroll
+        for (int w = 0; w < kOwnWaves; ++w) x += (mm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(lds.m[w][h] - mm)) * of(w);
+        return make_float2(mm, x);
+      };
+      for (int i = tid; i < G * kD; i += 256) po[i] = combine(i / kD, [&](int w) { return lds.acc[w][i / kD][i & (kD - 1)]; }).y;
+      if (tid < G) *reinterpret_cast<float2*>(pml + 2 * tid) = combine(tid, [&](int w) { return lds.l[w][tid]; });
+    }
+    // The rest of the share continues at the start of the next pair.
+    if (left == 0u) return;
+    key = 0;
+    if (++kvh == p.hkv) {
+      kvh = 0;
+      ++r;
+    }
+    __syncthreads();   // the next piece's partials lie in the same LDS
+  }
+}
+
 // The plan's words, a line share's entries and partials, or a ring of two tiles of K and V.
 constexpr int kEntOffset = 2 * kMaxGroups * static_cast<int>(sizeof(int));
 constexpr int kPieceOffset = kEntOffset + kInlineSeqs * static_cast<int>(sizeof(SeqEntry));
 constexpr int kLdsBytes = 2 * kSlotBytes;
-static_assert(kPieceOffset + sizeof(PieceLds<kMaxG>) <= kLdsBytes, "a share's words fit the ring");
+static_assert(kPieceOffset + sizeof(PieceLds) <= kLdsBytes, "a share's words fit the ring");
 
-template <int G>
 __global__ __launch_bounds__(256, 2) void shared_split_kernel(const SharedParams p) {
   __shared__ __align__(1024) char s_mem[kLdsBytes];
   __shared__ int2 s_rows[kTileRows];
@@ -469,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void shared_split_kernel(const SharedParams
   if (plan_shared(p, routes, per, counts, counts + kMaxGroups, ent, piece, st, wg))
     prefix_piece(p, routes, per, piece, s_rows, s_mem);
   else if (st.take > 0)
-    decode_pieces<G, true>(p, wg, st, ent, *reinterpret_cast<PieceLds<G>*>(s_mem + kPieceOffset));
+    own_pieces(p, wg, st, ent, *reinterpret_cast<PieceLds*>(s_mem + kPieceOffset));
 }
 
 // One workgroup of 256 threads per output row: merge_row over the row's shares of the line
@@ -665,16 +898,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.least = static_cast<uint32_t>(L.least);
   const hipStream_t st = as_stream(stream);
   const dim3 grid(static_cast<uint32_t>(L.pieces + L.least));
-  switch (p.group) {
-    case 1: hipLaunchKernelGGL(shared_split_kernel<1>, grid, dim3(256), 0, st, p); break;
-    case 2: hipLaunchKernelGGL(shared_split_kernel<2>, grid, dim3(256), 0, st, p); break;
-    case 3: hipLaunchKernelGGL(shared_split_kernel<3>, grid, dim3(256), 0, st, p); break;
-    case 4: hipLaunchKernelGGL(shared_split_kernel<4>, grid, dim3(256), 0, st, p); break;
-    case 5: hipLaunchKernelGGL(shared_split_kernel<5>, grid, dim3(256), 0, st, p); break;
-    case 6: hipLaunchKernelGGL(shared_split_kernel<6>, grid, dim3(256), 0, st, p); break;
-    case 7: hipLaunchKernelGGL(shared_split_kernel<7>, grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL(shared_split_kernel<8>, grid, dim3(256), 0, st, p); break;
-  }
+  hipLaunchKernelGGL(shared_split_kernel, grid, dim3(256), 0, st, p);
   hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(batch * heads_q)), dim3(256), 0, st, p);
   return launch_status(name);
 }
