@@ -53,6 +53,8 @@ constexpr int kMaxG = 8;
 constexpr int kOwnStep = 32;         // keys that a wave takes at once of a sequence's own
 constexpr uint32_t kPairPad = 192;   // a pair's start, in keys
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
 struct SharedParams : DecodeCommon {
   static constexpr uint32_t kMinShare = 128;
   static constexpr uint32_t kLongShare = UINT32_MAX;
@@ -76,6 +78,10 @@ struct SharedParams : DecodeCommon {
 };
 
 __device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const bf16x2 x = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  return __builtin_bit_cast(uint32_t, x);
+}
 __device__ __forceinline__ int uniform(uint32_t x) {
   return static_cast<int>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
 }
@@ -234,16 +240,17 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes&
 // copies rows 16 w .. 16 w + 15 of both, four rows per instruction; rows behind `last` are
 // read as that one.
 constexpr int kSlotBytes = 2 * tiles::kTileBytes;
-__device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, int64_t stride, int key, int last,
+__device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, uint32_t row_bytes, int key, int last,
                                           uint32_t lds, int wave, int lane) {
-  const int first = key + 16 * wave + (lane >> 4);
-  const int chunk = (lane & 15) ^ ((lane >> 4) << 2);   // of row 4 i + lane / 16: ^ i
+  asm volatile("" : "+v"(lane));   // offsets are made anew each time: kept, they spill, and a reload waits for the copies
+  const int64_t at = static_cast<int64_t>(key) * (row_bytes / 2);   // the tile's rows span less than 2^31 bytes
+  const int chunk = (lane & 15) ^ ((lane >> 4) << 2);               // of row 4 i + lane / 16: ^ i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t at = min(first + 4 * i, last) * stride + 8 * (chunk ^ i);
+    const uint32_t off = static_cast<uint32_t>(min(16 * wave + 4 * i + (lane >> 4), last - key)) * row_bytes + 16u * (chunk ^ i);
     const uint32_t to = lds + 1024u * static_cast<uint32_t>(4 * wave + i);
-    tiles::dma16_gather(kb + at, to);
-    tiles::dma16_gather(vb + at, to + tiles::kTileBytes);
+    tiles::dma16_from(kb + at, off, to);
+    tiles::dma16_from(vb + at, off, to + tiles::kTileBytes);
   }
 }
 
@@ -270,39 +277,66 @@ __device__ __forceinline__ LaneLds lane_lds(uint32_t ring, int lane) {
                  ring + tiles::kTileBytes + tiles::kRowBytes * (4 * h + (i >> 2)) +
                      16 * ((2 * half + ((i & 3) >> 1)) ^ (((i >> 2) << 2) | h)) + 8 * (i & 1)};
 }
+// The places in slot `slot` of the ring, made anew for each tile: kept, the XORed ones take
+// registers that the loop does not have.
+__device__ __forceinline__ LaneLds in_slot(LaneLds at, uint32_t slot) {
+  at.k += slot;
+  at.v += slot;
+  asm volatile("" : "+v"(at.k), "+v"(at.v));
+  return at;
+}
 typedef __attribute__((address_space(3))) const bf16x8* LdsChunk;
 typedef __attribute__((address_space(3))) s16x4* LdsFour;
 
-template <bool kMasked>
-__device__ __forceinline__ void tile_step(const char* kt, uint32_t slot, const LaneLds& at_lds, const bf16x8 (&q)[8], float c,
-                                          int key, int start, int end, RowState& w, int lane) {
-  const char* vt = kt + tiles::kTileBytes;
-  const int h = lane >> 5;
-  f32x16 s[2];
+// Scheduling groups (__builtin_amdgcn_sched_group_barrier).
+constexpr int kValu = 0x2, kMfma = 0x8, kLdsRead = 0x100, kTrans = 0x400;
+
+// A group of 16 keys of V^T, all 128 dims.
+struct VGroup {
+  uint32_t x[4][4];   // [32 dims][operand]
+};
+__device__ __forceinline__ void read_v(const LaneLds& at, int group, int d, VGroup& v) {
 #pragma unroll
-  for (int f = 0; f < 2; ++f) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[f][i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const bf16x8 a = *(LdsChunk)(uintptr_t)((at_lds.k ^ (32 * d)) + slot + 32 * f * tiles::kRowBytes);
-      s[f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[d], s[f], 0, 0, 0);
-    }
+  for (int x = 0; x < 2; ++x) {
+    const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (LdsFour)(uintptr_t)((at.v ^ (64 * d + 32 * x)) + (16 * group + 8 * x) * tiles::kRowBytes));
+    const uint2 two = __builtin_bit_cast(uint2, four);
+    v.x[d][2 * x] = two.x;
+    v.x[d][2 * x + 1] = two.y;
   }
-  auto live = [&](int f, int i) {
-    const int at = key + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
-    return !kMasked || (at >= start && at < end);
-  };
-  float top = -INFINITY;
+}
+
+// 8 weights of a group of 16 keys, as the two operands of their products.
+struct PGroup {
+  bf16x8 hi, lo;
+};
+__device__ __forceinline__ PGroup split_p(const float (&y)[8]) {
+  u32x4 hi, lo;
 #pragma unroll
-  for (int f = 0; f < 2; ++f)
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = pack2(y[2 * e], y[2 * e + 1]);   // the differences are exact
+    lo[e] = pack2(y[2 * e] - __uint_as_float(hi[e] << 16), y[2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
+  }
+  return PGroup{__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, lo)};
+}
+
+// 32 keys f of a tile: S^T = K Q^T.
+__device__ __forceinline__ f32x16 scores(const LaneLds& at, int f, const bf16x8 (&q)[8]) {
+  f32x16 s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (kMasked && !live(f, i)) s[f][i] = -INFINITY;
-      top = fmaxf(top, s[f][i]);
-    }
+  for (int d = 0; d < 8; ++d) {
+    const bf16x8 a = *(LdsChunk)(uintptr_t)((at.k ^ (32 * d)) + 32 * f * tiles::kRowBytes);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[d], s, 0, 0, 0);
+  }
+  return s;
+}
+
+// Moves the rows' maxima where a score exceeds one by more than 8 in the exp2 domain (rare);
+// top: this lane's largest raw score.  Returns what weights are taken from: the maximum, 0
+// where there were only scores of -inf so far, which then weigh nothing.
+__device__ __forceinline__ float move_maxima(float top, float c, RowState& w) {
   top *= c;
-  if (__builtin_amdgcn_ballot_w64(top - w.m > 8.0f)) {   // rare: move the maxima, rescale
+  if (__builtin_amdgcn_ballot_w64(top - w.m > 8.0f)) {
     top = tiles::xor32_max(top);
     const float mn = top - w.m > 8.0f ? top : w.m;
     const float a = mn == w.m ? 1.0f : __builtin_amdgcn_exp2f(w.m - mn);
@@ -311,77 +345,129 @@ __device__ __forceinline__ void tile_step(const char* kt, uint32_t slot, const L
 #pragma unroll
     for (int d = 0; d < 4; ++d) w.acc[d] *= a;
   }
-  const float from = w.m == -INFINITY ? 0.f : w.m;   // only scores of -inf so far: they weigh nothing
+  return w.m == -INFINITY ? 0.f : w.m;
+}
+
+// 64 keys that every row attends.  The weights of the next 16 keys are made, and their V
+// read, under the products of the last ones.
+__device__ __forceinline__ void whole_tile(const LaneLds& at, const bf16x8 (&q)[8], float c, RowState& w) {
+  f32x16 s[2] = {scores(at, 0, q), scores(at, 1, q)};
+  VGroup v;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) read_v(at, 0, d, v);
+  __builtin_amdgcn_sched_group_barrier(kLdsRead, 4, 0);
+#pragma unroll
+  for (int i = 0; i < 12; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, 2, 0);
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+  const float from = move_maxima(top, c, w);
+  auto weights = [&](int g) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], c, -from));
+      w.l += y[i];
+    }
+    return split_p(y);
+  };
+  PGroup p = weights(0);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    PGroup next = p;
+    if (g < 3) next = weights(g + 1);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const bf16x8 a = __builtin_bit_cast(bf16x8, v.x[d]);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.hi, w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.lo, w.acc[d], 0, 0, 0);
+      if (g < 3) read_v(at, g + 1, d, v);
+    }
+    p = next;
+  }
+#pragma unroll
+  for (int i = 0; i < 24; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kValu, 7, 0);
+    __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
+  }
+}
+
+// 64 keys of which each row attends those in [start, end) (key: the first one's number).
+__device__ __forceinline__ void masked_tile(const char* vt, const LaneLds& at_lds, const bf16x8 (&q)[8], float c,
+                                            int key, int start, int end, RowState& w, int lane) {
+  const int h = lane >> 5;
+  f32x16 s[2] = {scores(at_lds, 0, q), scores(at_lds, 1, q)};
+  auto live = [&](int f, int i) {
+    const int at = key + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
+    return at >= start && at < end;
+  };
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (!live(i >> 4, i & 15)) s[i >> 4][i & 15] = -INFINITY;
+    top = fmaxf(top, s[i >> 4][i & 15]);
+  }
+  const float from = move_maxima(top, c, w);
   bool odd = false;
 #pragma unroll
-  for (int f = 0; f < 2; ++f) {
+  for (int g = 0; g < 4; ++g) {
+    float y[8];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      u32x4 hi, lo;
+    for (int i = 0; i < 8; ++i) {
+      const int x = 8 * (g & 1) + i;
+      y[i] = !live(g >> 1, x) ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][x], c, -from));
+      w.l += y[i];
+      s[g >> 1][x] = y[i];
+    }
+    const PGroup p = split_p(y);
+    VGroup v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float y[2];
+    for (int d = 0; d < 4; ++d) {
+      read_v(at_lds, g, d, v);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int x = 8 * t + 2 * e + i;
-          y[i] = !live(f, x) ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][x], c, -from));
-          w.l += y[i];
-          s[f][x] = y[i];
-        }
-        hi[e] = tiles::pack_bf16x2(y[0], y[1]);
-        lo[e] = tiles::pack_bf16x2(y[0] - __uint_as_float(hi[e] << 16), y[1] - __uint_as_float(hi[e] & 0xffff0000u));
+      for (int x = 0; x < 4; ++x) {
+        uint32_t& u = v.x[d][x];
+        odd = odd || odd_pair(u);
+        if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+        if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
       }
-      // V^T operands: dim 32 d + lane % 32 of keys 4 h .. +3 and 8 + 4 h .. +3 of the 16.
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        uint32_t v[4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (LdsFour)(uintptr_t)((at_lds.v ^ (64 * d + 32 * x)) + slot + (32 * f + 16 * t + 8 * x) * tiles::kRowBytes));
-          const uint2 two = __builtin_bit_cast(uint2, four);
-          v[2 * x] = two.x;
-          v[2 * x + 1] = two.y;
-        }
-        if constexpr (kMasked) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            odd = odd || odd_pair(v[x]);
-            if ((v[x] & 0x7f80u) == 0x7f80u) v[x] &= 0xffff0000u;
-            if ((v[x] & 0x7f800000u) == 0x7f800000u) v[x] &= 0xffffu;
-          }
-        }
-        const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
-        w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, hi), w.acc[d], 0, 0, 0);
-        w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, lo), w.acc[d], 0, 0, 0);
-      }
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), p.hi, w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), p.lo, w.acc[d], 0, 0, 0);
     }
   }
-  if constexpr (kMasked) {
-    if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
-    // Values that are not finite, key by key: what they add to the rows that attend them.
-    for (int at = 0; at < kTileKeys; ++at) {
-      const char* row = vt + at * tiles::kRowBytes;
-      const uint32_t mine = *reinterpret_cast<const uint32_t*>(row + 16 * ((lane >> 2) ^ tiles::swz(at)) + 4 * (lane & 3));
-      if (__builtin_amdgcn_ballot_w64(odd_pair(mine)) == 0) continue;
-      float pr = 0.f;   // the weight, in the lane whose keys it is among
+  if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
+  // Values that are not finite, key by key: what they add to the rows that attend them.
+  for (int at = 0; at < kTileKeys; ++at) {
+    const char* row = vt + at * tiles::kRowBytes;
+    const uint32_t mine = *reinterpret_cast<const uint32_t*>(row + 16 * ((lane >> 2) ^ tiles::swz(at)) + 4 * (lane & 3));
+    if (__builtin_amdgcn_ballot_w64(odd_pair(mine)) == 0) continue;
+    float pr = 0.f;   // the weight, in the lane whose keys it is among
 #pragma unroll
-      for (int f = 0; f < 2; ++f)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (at >> 5 == f && ((at >> 3) & 3) == i >> 2 && (at & 3) == (i & 3)) pr = s[f][i];
-      const float other = __shfl_xor(pr, 32);
-      if (((at >> 2) & 1) != h) pr = other;
-      if (key + at < start || key + at >= end) continue;
+      for (int i = 0; i < 16; ++i)
+        if (at >> 5 == f && ((at >> 3) & 3) == i >> 2 && (at & 3) == (i & 3)) pr = s[f][i];
+    const float other = __shfl_xor(pr, 32);
+    if (((at >> 2) & 1) != h) pr = other;
+    if (key + at < start || key + at >= end) continue;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+    for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
-          const uint32_t bits = *reinterpret_cast<const uint16_t*>(row + 16 * ((dim >> 3) ^ tiles::swz(at)) + 2 * (dim & 7));
-          if ((bits & 0x7f80u) == 0x7f80u) w.acc[d][i] += pr * bf(bits);
-        }
-    }
+      for (int i = 0; i < 16; ++i) {
+        const int dim = 32 * d + 8 * (i >> 2) + 4 * h + (i & 3);
+        const uint32_t bits = *reinterpret_cast<const uint16_t*>(row + 16 * ((dim >> 3) ^ tiles::swz(at)) + 2 * (dim & 7));
+        if ((bits & 0x7f80u) == 0x7f80u) w.acc[d][i] += pr * bf(bits);
+      }
   }
 }
 
@@ -405,14 +491,15 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     if (x.kvh == 0 && x.part == 0)
       p.place[b] = make_int4(x.base + x.tile * p.hkv * x.parts, x.parts, at * p.group, 0);
   }
-  const int k0 = x.first + x.part * x.length, k1 = min(k0 + x.length, x.end);
+  const int k0 = uniform(x.first + x.part * x.length), k1 = min(k0 + uniform(x.length), uniform(x.end));
   const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
-  const int64_t stride = static_cast<int64_t>(p.hkv) * kD;
-  const int64_t base = (static_cast<int64_t>(x.group >> 1) * p.prefix_len * p.hkv + x.kvh) * kD;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * tiles::kRowBytes;
+  const int64_t base = (static_cast<int64_t>(uniform(x.group) >> 1) * p.prefix_len * p.hkv + uniform(x.kvh)) * kD;
+  const int last = uniform(x.end) - 1;
   const uint16_t *kb = p.prefix_k + base, *vb = p.prefix_v + base;
   const uint32_t lds = tiles::lds_addr(ring);
   __syncthreads();   // the rows; the ring was the plan's
-  copy_tile(kb, vb, stride, k0, x.end - 1, lds, wave, lane);
+  copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
   // This lane's row.
   const int rows = seqs * p.group, row = 32 * wave + (lane & 31), h = lane >> 5;
   const bool mine = row < rows, busy = 32 * wave < rows;   // busy: uniform
@@ -440,19 +527,28 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.acc[d][i] = 0.f;
-    for (int j = 0; j < steps; ++j) {
-      const int key = k0 + kTileKeys * j;
-      // Tile j has arrived, and every wave is done with the one before.
+    // Masked tiles (every row's start lies before those behind them), whole ones, the ragged end.
+    const int head = careful ? steps : min(max((latest - k0 + kTileKeys - 1) / kTileKeys, 0), steps);
+    const int tail = max(k1 - k0 == steps * kTileKeys ? steps : steps - 1, head);
+    int j = 0;
+    auto arrive = [&]() {   // tile j is there, and every wave is done with the one before
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (j + 1 < steps)
-        copy_tile(kb, vb, stride, key + kTileKeys, x.end - 1, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
-      if (!busy) continue;
-      const uint32_t slot = (j & 1) * kSlotBytes;
-      if (careful || key < latest || key + kTileKeys > k1)
-        tile_step<true>(ring + slot, slot, at_lds, q, c, key, start, k1, w, lane);
-      else
-        tile_step<false>(ring + slot, slot, at_lds, q, c, key, start, k1, w, lane);
+        copy_tile(kb, vb, row_bytes, k0 + kTileKeys * (j + 1), last, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
+      return static_cast<uint32_t>(j & 1) * kSlotBytes;
+    };
+    auto masked = [&]() {
+      const uint32_t slot = arrive();
+      if (busy)
+        masked_tile(ring + slot + tiles::kTileBytes, in_slot(at_lds, slot), q, c, k0 + kTileKeys * j, start, k1, w, lane);
+    };
+    for (; j < head; ++j) masked();
+    if (busy) {
+      for (; j < tail; ++j) whole_tile(in_slot(at_lds, arrive()), q, c, w);
+    } else {
+      for (; j < tail; ++j) arrive();
     }
+    for (; j < steps; ++j) masked();
     if (careful) break;
     float sum = 0.f;   // not finite if one of them is not
 #pragma unroll
@@ -460,7 +556,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(w.acc[d][i], 0.f, sum);
     if (!__syncthreads_or(mine && sum != 0.f)) break;
-    copy_tile(kb, vb, stride, k0, x.end - 1, lds, wave, lane);
+    copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
   }
   if (!mine) return;
   w.l = w.l + __shfl_xor(w.l, 32);
@@ -611,8 +707,8 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
               y[u] = __builtin_amdgcn_exp2f(s[t][x + u] - from);   // 0 behind the piece
               l += y[u];
             }
-            const uint32_t hi = tiles::pack_bf16x2(y[0], y[1]);
-            const uint32_t lo = tiles::pack_bf16x2(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
+            const uint32_t hi = pack2(y[0], y[1]);
+            const uint32_t lo = pack2(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
             pk[2 * t + x / 2] = second ? lo : hi;
           }
         const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
