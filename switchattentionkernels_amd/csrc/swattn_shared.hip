@@ -46,7 +46,7 @@ constexpr int kTileKeys = tiles::kBN;
 constexpr int kMaxGroups = 2 * SWATTN_SHARED_MAX_PREFIXES;   // (prefix, route)
 constexpr uint32_t kMinPiece = 128;  // keys of a prefix piece, at least
 // What a key of a prefix tile costs, in 16ths of a key of the line.
-constexpr uint32_t kTileCost = 10;
+constexpr uint32_t kTileCost = 24;
 
 constexpr int kOwnWaves = 4;         // waves per workgroup
 constexpr int kMaxG = 8;
@@ -308,16 +308,24 @@ __device__ __forceinline__ void read_v(const LaneLds& at, int group, int d, VGro
 
 // 8 weights of a group of 16 keys, as the two operands of their products.
 struct PGroup {
-  bf16x8 hi, lo;
+  u32x4 hi, lo;
 };
 __device__ __forceinline__ PGroup split_p(const float (&y)[8]) {
-  u32x4 hi, lo;
+  // y minus its first part, exact, by a product with (-1, 0) or (0, -1).  (From registers:
+  // the compiler writes the first as the inline constant -1.0, which is another pair.)
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first), "+s"(second));
+  PGroup p;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    hi[e] = pack2(y[2 * e], y[2 * e + 1]);   // the differences are exact
-    lo[e] = pack2(y[2 * e] - __uint_as_float(hi[e] << 16), y[2 * e + 1] - __uint_as_float(hi[e] & 0xffff0000u));
+    const uint32_t pair = pack2(y[2 * e], y[2 * e + 1]);
+    const bf16x2 h = __builtin_bit_cast(bf16x2, pair);
+    p.hi[e] = pair;
+    const float y0 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), y[2 * e], false);
+    const float y1 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), y[2 * e + 1], false);
+    p.lo[e] = pack2(y0, y1);
   }
-  return PGroup{__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, lo)};
+  return p;
 }
 
 // 32 keys f of a tile: S^T = K Q^T.
@@ -348,9 +356,20 @@ __device__ __forceinline__ float move_maxima(float top, float c, RowState& w) {
   return w.m == -INFINITY ? 0.f : w.m;
 }
 
-// 64 keys that every row attends.  The weights of the next 16 keys are made, and their V
-// read, under the products of the last ones.
-__device__ __forceinline__ void whole_tile(const LaneLds& at, const bf16x8 (&q)[8], float c, RowState& w) {
+// Scores of keys that a row does not attend become -inf: it attends `count` of them from
+// number `first` of the tile on (counted from this lane's first key, 4 h).
+__device__ __forceinline__ void mask(f32x16 (&s)[2], int first, uint32_t count) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int at = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+    if (static_cast<uint32_t>(at - first) >= count) s[i >> 4][i & 15] = -INFINITY;
+  }
+}
+
+// 64 keys; kMask: of which rows do not attend all.  The weights of the next 16 keys are
+// made, and their V read, under the products of the last ones.
+template <bool kMask>
+__device__ __forceinline__ void tile_step(const LaneLds& at, const bf16x8 (&q)[8], float c, int first, uint32_t count, RowState& w) {
   f32x16 s[2] = {scores(at, 0, q), scores(at, 1, q)};
   VGroup v;
 #pragma unroll
@@ -366,6 +385,7 @@ __device__ __forceinline__ void whole_tile(const LaneLds& at, const bf16x8 (&q)[
     __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
     __builtin_amdgcn_sched_group_barrier(kLdsRead, 2, 0);
   }
+  if (kMask) mask(s, first, count);
   float top = s[0][0];
 #pragma unroll
   for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
@@ -382,41 +402,42 @@ __device__ __forceinline__ void whole_tile(const LaneLds& at, const bf16x8 (&q)[
   PGroup p = weights(0);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
+    asm volatile("" : "+v"(p.hi), "+v"(p.lo));
+    __builtin_amdgcn_sched_barrier(0);
     PGroup next = p;
     if (g < 3) next = weights(g + 1);
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       const bf16x8 a = __builtin_bit_cast(bf16x8, v.x[d]);
-      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.hi, w.acc[d], 0, 0, 0);
-      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.lo, w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.hi), w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.lo), w.acc[d], 0, 0, 0);
       if (g < 3) read_v(at, g + 1, d, v);
     }
     p = next;
-  }
+    if (g < 3) {
 #pragma unroll
-  for (int i = 0; i < 24; ++i) {
-    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 7, 0);
-    __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
+      }
+    }
   }
 }
 
-// 64 keys of which each row attends those in [start, end) (key: the first one's number).
-__device__ __forceinline__ void masked_tile(const char* vt, const LaneLds& at_lds, const bf16x8 (&q)[8], float c,
-                                            int key, int start, int end, RowState& w, int lane) {
+// The same where values are not finite, which a weight of 0 does not keep out, and of which
+// an infinite one times a weight's second part can make NaN: the products go without them,
+// and they are added key by key to the rows that attend them.  vt: the tile of V.
+__device__ __forceinline__ void careful_step(const char* vt, const LaneLds& at_lds, const bf16x8 (&q)[8], float c, int first,
+                                             uint32_t count, RowState& w, int lane) {
   const int h = lane >> 5;
   f32x16 s[2] = {scores(at_lds, 0, q), scores(at_lds, 1, q)};
-  auto live = [&](int f, int i) {
-    const int at = key + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
-    return at >= start && at < end;
-  };
-  float top = -INFINITY;
+  mask(s, first, count);
+  float top = s[0][0];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (!live(i >> 4, i & 15)) s[i >> 4][i & 15] = -INFINITY;
-    top = fmaxf(top, s[i >> 4][i & 15]);
-  }
+  for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
   const float from = move_maxima(top, c, w);
   bool odd = false;
 #pragma unroll
@@ -425,7 +446,7 @@ __device__ __forceinline__ void masked_tile(const char* vt, const LaneLds& at_ld
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int x = 8 * (g & 1) + i;
-      y[i] = !live(g >> 1, x) ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][x], c, -from));
+      y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][x], c, -from));
       w.l += y[i];
       s[g >> 1][x] = y[i];
     }
@@ -441,8 +462,8 @@ __device__ __forceinline__ void masked_tile(const char* vt, const LaneLds& at_ld
         if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
         if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
       }
-      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), p.hi, w.acc[d], 0, 0, 0);
-      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), p.lo, w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), __builtin_bit_cast(bf16x8, p.hi), w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), __builtin_bit_cast(bf16x8, p.lo), w.acc[d], 0, 0, 0);
     }
   }
   if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
@@ -459,7 +480,7 @@ __device__ __forceinline__ void masked_tile(const char* vt, const LaneLds& at_ld
         if (at >> 5 == f && ((at >> 3) & 3) == i >> 2 && (at & 3) == (i & 3)) pr = s[f][i];
     const float other = __shfl_xor(pr, 32);
     if (((at >> 2) & 1) != h) pr = other;
-    if (key + at < start || key + at >= end) continue;
+    if (static_cast<uint32_t>(at - 4 * h - first) >= count) continue;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -514,12 +535,11 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     if (!mine) u = u32x4{0, 0, 0, 0};
     q[d] = __builtin_bit_cast(bf16x8, u);
   }
-  const float c = fabsf(p.c);
+  const float c = fmaxf(fabsf(p.c), 0x1p-126f);   // not 0, which would make NaN of masked scores
   const int start = entry.y, latest = __builtin_amdgcn_readfirstlane(tiles::wave_max(start));
   const LaneLds at_lds = lane_lds(lds, lane);
   RowState w;
-  // Once, and with all tiles as masked ones if a sum is not finite then: an infinite value
-  // times the second part of a weight may have made NaN of what is infinite.
+  // Once, and carefully if a sum is not finite then.
   for (int careful = 0; careful < 2; ++careful) {
     w.m = -INFINITY;
     w.l = 0.f;
@@ -527,8 +547,8 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.acc[d][i] = 0.f;
-    // Masked tiles (every row's start lies before those behind them), whole ones, the ragged end.
-    const int head = careful ? steps : min(max((latest - k0 + kTileKeys - 1) / kTileKeys, 0), steps);
+    // Tiles that some row attends in part (they start later), whole ones, the ragged end.
+    const int head = min(max((latest - k0 + kTileKeys - 1) / kTileKeys, 0), steps);
     const int tail = max(k1 - k0 == steps * kTileKeys ? steps : steps - 1, head);
     int j = 0;
     auto arrive = [&]() {   // tile j is there, and every wave is done with the one before
@@ -537,19 +557,30 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
         copy_tile(kb, vb, row_bytes, k0 + kTileKeys * (j + 1), last, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
       return static_cast<uint32_t>(j & 1) * kSlotBytes;
     };
-    auto masked = [&]() {
-      const uint32_t slot = arrive();
-      if (busy)
-        masked_tile(ring + slot + tiles::kTileBytes, in_slot(at_lds, slot), q, c, k0 + kTileKeys * j, start, k1, w, lane);
+    // What this row attends of tile j.
+    auto from = [&]() { return max(start - (k0 + kTileKeys * j), 0) - 4 * h; };
+    auto count = [&]() {
+      const int key = k0 + kTileKeys * j;
+      return static_cast<uint32_t>(max(min(k1 - key, kTileKeys) - max(start - key, 0), 0));
     };
+    auto masked = [&]() {
+      const LaneLds at = in_slot(at_lds, arrive());
+      if (busy) tile_step<true>(at, q, c, from(), count(), w);
+    };
+    if (careful) {
+      for (; j < steps; ++j) {
+        const uint32_t slot = arrive();
+        if (busy) careful_step(ring + slot + tiles::kTileBytes, in_slot(at_lds, slot), q, c, from(), count(), w, lane);
+      }
+      break;
+    }
     for (; j < head; ++j) masked();
     if (busy) {
-      for (; j < tail; ++j) whole_tile(in_slot(at_lds, arrive()), q, c, w);
+      for (; j < tail; ++j) tile_step<false>(in_slot(at_lds, arrive()), q, c, 0, 0, w);
     } else {
       for (; j < tail; ++j) arrive();
     }
     for (; j < steps; ++j) masked();
-    if (careful) break;
     float sum = 0.f;   // not finite if one of them is not
 #pragma unroll
     for (int d = 0; d < 4; ++d)
