@@ -236,24 +236,21 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes&
   return false;
 }
 
-// The ring: kSlots half tiles (32 keys) of K, then as many of V, rows of 256 bytes whose 16-byte
-// chunks are swizzled by tiles::swz.
-constexpr int kHalfKeys = 32, kSlots = 4;
-constexpr int kHalfBytes = kHalfKeys * tiles::kRowBytes;
-constexpr int kVRing = kSlots * kHalfBytes, kLdsBytes = 2 * kVRing;
-
-// 32 keys of K or V into a slot: wave w copies rows 8 w .. 8 w + 7, four per instruction.  Rows
-// behind `last` are read as that one.
-__device__ __forceinline__ void copy_half(const uint16_t* rows, uint32_t row_bytes, int key, int last, uint32_t lds, int wave,
-                                          int lane) {
+// 64 keys of K and V as LDS tiles [64][128], 16-byte chunks swizzled by tiles::swz: wave w
+// copies rows 16 w .. 16 w + 15 of both, four rows per instruction; rows behind `last` are
+// read as that one.
+constexpr int kSlotBytes = 2 * tiles::kTileBytes;
+__device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, uint32_t row_bytes, int key, int last,
+                                          uint32_t lds, int wave, int lane) {
   asm volatile("" : "+v"(lane));   // offsets are made anew each time: kept, they spill, and a reload waits for the copies
-  key = min(key, last);
-  const uint16_t* from = rows + static_cast<int64_t>(key) * (row_bytes / 2);   // the half spans less than 2^31 bytes
+  const int64_t at = static_cast<int64_t>(key) * (row_bytes / 2);   // the tile's rows span less than 2^31 bytes
+  const int chunk = (lane & 15) ^ ((lane >> 4) << 2);               // of row 4 i + lane / 16: ^ i
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = 8 * wave + 4 * i + (lane >> 4), chunk = (lane & 15) ^ (((lane >> 4) << 2) | ((2 * wave + i) & 3));
-    tiles::dma16_from(from, static_cast<uint32_t>(min(row, last - key)) * row_bytes + 16u * chunk,
-                      lds + 1024u * static_cast<uint32_t>(2 * wave + i));
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t off = static_cast<uint32_t>(min(16 * wave + 4 * i + (lane >> 4), last - key)) * row_bytes + 16u * (chunk ^ i);
+    const uint32_t to = lds + 1024u * static_cast<uint32_t>(4 * wave + i);
+    tiles::dma16_from(kb + at, off, to);
+    tiles::dma16_from(vb + at, off, to + tiles::kTileBytes);
   }
 }
 
@@ -265,27 +262,27 @@ __device__ __forceinline__ bool odd_pair(uint32_t x) {   // whether one of two b
 // each 32 and dims 32 d + 8 j + 4 h + i.
 struct RowState {
   float m, l;        // maximum (the same in both lanes of a row); this lane's share of the sum
-  float from;        // what weights are taken from: the maximum, 0 while that is -inf
   f32x16 acc[4];
 };
 
-// Where a lane's operands lie in slot 0 of K and of V, from LDS address 0: a chunk's number
-// enters by XOR, the rest of a row's place is added.
+// Where a lane's operands lie in a tile of K and one of V, from LDS address 0: a chunk's
+// number enters by XOR, the rest of a row's place is added.
 struct LaneLds {
-  uint32_t k;   // key r of K, dims 8 h .. +7; ^ 32 d: those of dims 16 d
-  uint32_t v;   // V^T operand: ^ (64 d + 32 x): dims 32 d, + 256 (16 t + 8 x): keys of group t, half x
+  uint32_t k;   // key r of K, dims 8 h .. +7; ^ 32 d: those of dims 16 d, + 8192 f: key 32 f + r
+  uint32_t v;   // V^T operand: ^ (64 d + 32 x): dims 32 d, + 256 (32 f + 16 t + 8 x): keys of group t, half x
 };
 __device__ __forceinline__ LaneLds lane_lds(uint32_t ring, int lane) {
   const int r = lane & 31, h = lane >> 5, half = (lane >> 4) & 1, i = lane & 15;
   return LaneLds{ring + tiles::kRowBytes * r + 16 * (h ^ tiles::swz(r)),
-                 ring + kVRing + tiles::kRowBytes * (4 * h + (i >> 2)) +
+                 ring + tiles::kTileBytes + tiles::kRowBytes * (4 * h + (i >> 2)) +
                      16 * ((2 * half + ((i & 3) >> 1)) ^ (((i >> 2) << 2) | h)) + 8 * (i & 1)};
 }
-// A place in a slot, made anew for each half: kept, the XORed ones take registers that the
-// loop does not have.
-__device__ __forceinline__ uint32_t in_slot(uint32_t at, uint32_t slot) {
-  at += slot * kHalfBytes;
-  asm volatile("" : "+v"(at));
+// The places in slot `slot` of the ring, made anew for each tile: kept, the XORed ones take
+// registers that the loop does not have.
+__device__ __forceinline__ LaneLds in_slot(LaneLds at, uint32_t slot) {
+  at.k += slot;
+  at.v += slot;
+  asm volatile("" : "+v"(at.k), "+v"(at.v));
   return at;
 }
 typedef __attribute__((address_space(3))) const bf16x8* LdsChunk;
@@ -298,52 +295,14 @@ constexpr int kValu = 0x2, kMfma = 0x8, kLdsRead = 0x100, kTrans = 0x400;
 struct VGroup {
   uint32_t x[4][4];   // [32 dims][operand]
 };
-__device__ __forceinline__ void read_v(uint32_t at, int t, int d, VGroup& v) {
+__device__ __forceinline__ void read_v(const LaneLds& at, int group, int d, VGroup& v) {
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (LdsFour)(uintptr_t)((at ^ (64 * d + 32 * x)) + (16 * t + 8 * x) * tiles::kRowBytes));
+        (LdsFour)(uintptr_t)((at.v ^ (64 * d + 32 * x)) + (16 * group + 8 * x) * tiles::kRowBytes));
     const uint2 two = __builtin_bit_cast(uint2, four);
     v.x[d][2 * x] = two.x;
     v.x[d][2 * x + 1] = two.y;
-  }
-}
-
-// S^T = K Q^T of 32 keys, raw.
-__device__ __forceinline__ f32x16 scores(uint32_t at, const bf16x8 (&q)[8]) {
-  f32x16 s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int d = 0; d < 8; ++d)
-    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(LdsChunk)(uintptr_t)(at ^ (32 * d)), q[d], s, 0, 0, 0);
-  return s;
-}
-__device__ __forceinline__ float largest(const f32x16& s) {
-  float top = s[0];
-#pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-  return top;
-}
-// Scores of keys that a row does not attend become -inf: it attends `count` of them from
-// number `first` of the 32 on (counted from this lane's first key, 4 h).
-__device__ __forceinline__ void mask(f32x16& s, int first, uint32_t count) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (static_cast<uint32_t>(8 * (i >> 2) + (i & 3) - first) >= count) s[i] = -INFINITY;
-}
-
-// Moves the rows' maxima where a score exceeds one by more than 8 in the exp2 domain (rare);
-// top: this lane's largest raw score.  Scores of -inf weigh nothing while there are only those.
-__device__ __forceinline__ void move_maxima(float top, float c, RowState& w) {
-  top *= c;
-  if (__builtin_amdgcn_ballot_w64(top - w.m > 8.0f)) {
-    top = tiles::xor32_max(top);
-    const float mn = top - w.m > 8.0f ? top : w.m;
-    const float a = mn == w.m ? 1.0f : __builtin_amdgcn_exp2f(w.m - mn);
-    w.m = mn;
-    w.from = mn == -INFINITY ? 0.f : mn;
-    w.l *= a;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) w.acc[d] *= a;
   }
 }
 
@@ -368,114 +327,134 @@ __device__ __forceinline__ PGroup split_p(const float (&y)[8]) {
   }
   return p;
 }
-__device__ __forceinline__ void weights(const f32x16& s, int t, float c, RowState& w, float (&y)[8]) {
+
+// 32 keys f of a tile: S^T = K Q^T.
+__device__ __forceinline__ f32x16 scores(const LaneLds& at, int f, const bf16x8 (&q)[8]) {
+  f32x16 s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + i], c, -w.from));
-    w.l += y[i];
+  for (int d = 0; d < 8; ++d) {
+    const bf16x8 a = *(LdsChunk)(uintptr_t)((at.k ^ (32 * d)) + 32 * f * tiles::kRowBytes);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[d], s, 0, 0, 0);
   }
-}
-__device__ __forceinline__ void products(const uint32_t (&v)[4], const PGroup& p, f32x16& acc) {
-  const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.hi), acc, 0, 0, 0);
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.lo), acc, 0, 0, 0);
+  return s;
 }
 
-// Operands that a step finds in registers, read under the step before: K of the next keys,
-// dims 0 .. 63, and V of its first 16 keys.
-struct Ahead {
-  bf16x8 k[4];
+// Moves the rows' maxima where a score exceeds one by more than 8 in the exp2 domain (rare);
+// top: this lane's largest raw score.  Returns what weights are taken from: the maximum, 0
+// where there were only scores of -inf so far, which then weigh nothing.
+__device__ __forceinline__ float move_maxima(float top, float c, RowState& w) {
+  top *= c;
+  if (__builtin_amdgcn_ballot_w64(top - w.m > 8.0f)) {
+    top = tiles::xor32_max(top);
+    const float mn = top - w.m > 8.0f ? top : w.m;
+    const float a = mn == w.m ? 1.0f : __builtin_amdgcn_exp2f(w.m - mn);
+    w.m = mn;
+    w.l *= a;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) w.acc[d] *= a;
+  }
+  return w.m == -INFINITY ? 0.f : w.m;
+}
+
+// Scores of keys that a row does not attend become -inf: it attends `count` of them from
+// number `first` of the tile on (counted from this lane's first key, 4 h).
+__device__ __forceinline__ void mask(f32x16 (&s)[2], int first, uint32_t count) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int at = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+    if (static_cast<uint32_t>(at - first) >= count) s[i >> 4][i & 15] = -INFINITY;
+  }
+}
+
+// 64 keys; kMask: of which rows do not attend all.  The weights of the next 16 keys are
+// made, and their V read, under the products of the last ones.
+template <bool kMask>
+__device__ __forceinline__ void tile_step(const LaneLds& at, const bf16x8 (&q)[8], float c, int first, uint32_t count, RowState& w) {
+  f32x16 s[2] = {scores(at, 0, q), scores(at, 1, q)};
   VGroup v;
-};
-__device__ __forceinline__ void read_ahead(uint32_t at_k, uint32_t at_v, Ahead& a) {
 #pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    a.k[d] = *(LdsChunk)(uintptr_t)(at_k ^ (32 * d));
-    read_v(at_v, 0, d, a.v);
-  }
-}
-
-// 32 keys whose scores s are there, masked, the maxima moved for them; the next 32 keys' raw
-// scores come out, and the largest of them.  Every MFMA (32 cycles) has about four vector
-// instructions and an exponential to cover:
-//   S of the next keys (8 MFMAs)    | weights of the first 16 keys
-//   O^T += V^T P^T of the first 16  | weights of the last 16
-//   the same of the last 16         | the next scores' largest, the next step's first operands
-// at_k, at_v: K of the next keys, V of these; ahead_k, ahead_v: a half further on.
-__device__ __forceinline__ float half_step(uint32_t at_k, uint32_t at_v, uint32_t ahead_k, uint32_t ahead_v, Ahead& a,
-                                           const bf16x8 (&q)[8], float c, const f32x16& s, f32x16& next, RowState& w) {
-  PGroup p[2];
-  float y[8];
-  next = f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < 4; ++d) read_v(at, 0, d, v);
+  __builtin_amdgcn_sched_group_barrier(kLdsRead, 4, 0);
 #pragma unroll
-  for (int d = 0; d < 4; ++d) next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.k[d], q[d], next, 0, 0, 0);
-#pragma unroll
-  for (int d = 4; d < 8; ++d)
-    next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(LdsChunk)(uintptr_t)(at_k ^ (32 * d)), q[d], next, 0, 0, 0);
-  weights(s, 0, c, w, y);
-  p[0] = split_p(y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 12; ++i) {
     __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
-    if (i < 4) __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
-  }
-  asm volatile("" : "+v"(p[0].hi), "+v"(p[0].lo));   // made here, not next to their products
-  __builtin_amdgcn_sched_barrier(0);
-  weights(s, 1, c, w, y);
-  p[1] = split_p(y);
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    products(a.v.x[d], p[0], w.acc[d]);
-    read_v(at_v, 1, d, a.v);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
     __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
   }
-  asm volatile("" : "+v"(p[1].hi), "+v"(p[1].lo));
-  __builtin_amdgcn_sched_barrier(0);
-  VGroup last = a.v;
 #pragma unroll
-  for (int d = 0; d < 4; ++d) products(last.x[d], p[1], w.acc[d]);
-  read_ahead(ahead_k, ahead_v, a);
-  const float top = largest(next);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
     __builtin_amdgcn_sched_group_barrier(kLdsRead, 2, 0);
   }
-  return top;
+  if (kMask) mask(s, first, count);
+  float top = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+  const float from = move_maxima(top, c, w);
+  auto weights = [&](int g) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], c, -from));
+      w.l += y[i];
+    }
+    return split_p(y);
+  };
+  PGroup p = weights(0);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    asm volatile("" : "+v"(p.hi), "+v"(p.lo));
+    __builtin_amdgcn_sched_barrier(0);
+    PGroup next = p;
+    if (g < 3) next = weights(g + 1);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const bf16x8 a = __builtin_bit_cast(bf16x8, v.x[d]);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.hi), w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, p.lo), w.acc[d], 0, 0, 0);
+      if (g < 3) read_v(at, g + 1, d, v);
+    }
+    p = next;
+    if (g < 3) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(kTrans, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kValu, 3, 0);
+      }
+    }
+  }
 }
 
-// 32 keys where values are not finite, which a weight of 0 does not keep out, and of which an
-// infinite one times a weight's second part can make NaN: the products go without them, and
-// they are added key by key to the rows that attend them.  K and V in slot 0; vt: that V.
+// The same where values are not finite, which a weight of 0 does not keep out, and of which
+// an infinite one times a weight's second part can make NaN: the products go without them,
+// and they are added key by key to the rows that attend them.  vt: the tile of V.
 __device__ __forceinline__ void careful_step(const char* vt, const LaneLds& at_lds, const bf16x8 (&q)[8], float c, int first,
                                              uint32_t count, RowState& w, int lane) {
   const int h = lane >> 5;
-  f32x16 s = scores(at_lds.k, q);
+  f32x16 s[2] = {scores(at_lds, 0, q), scores(at_lds, 1, q)};
   mask(s, first, count);
-  move_maxima(largest(s), c, w);
+  float top = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+  const float from = move_maxima(top, c, w);
   bool odd = false;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int g = 0; g < 4; ++g) {
     float y[8];
-    weights(s, t, c, w, y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[8 * t + i] = y[i];
+    for (int i = 0; i < 8; ++i) {
+      const int x = 8 * (g & 1) + i;
+      y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][x], c, -from));
+      w.l += y[i];
+      s[g >> 1][x] = y[i];
+    }
     const PGroup p = split_p(y);
     VGroup v;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      read_v(at_lds.v, t, d, v);
+      read_v(at_lds, g, d, v);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         uint32_t& u = v.x[d][x];
@@ -483,18 +462,22 @@ __device__ __forceinline__ void careful_step(const char* vt, const LaneLds& at_l
         if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
         if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
       }
-      products(v.x[d], p, w.acc[d]);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), __builtin_bit_cast(bf16x8, p.hi), w.acc[d], 0, 0, 0);
+      w.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v.x[d]), __builtin_bit_cast(bf16x8, p.lo), w.acc[d], 0, 0, 0);
     }
   }
   if (__builtin_amdgcn_ballot_w64(odd) == 0) return;
-  for (int at = 0; at < kHalfKeys; ++at) {
+  // Values that are not finite, key by key: what they add to the rows that attend them.
+  for (int at = 0; at < kTileKeys; ++at) {
     const char* row = vt + at * tiles::kRowBytes;
     const uint32_t mine = *reinterpret_cast<const uint32_t*>(row + 16 * ((lane >> 2) ^ tiles::swz(at)) + 4 * (lane & 3));
     if (__builtin_amdgcn_ballot_w64(odd_pair(mine)) == 0) continue;
     float pr = 0.f;   // the weight, in the lane whose keys it is among
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (at >> 3 == i >> 2 && (at & 3) == (i & 3)) pr = s[i];
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (at >> 5 == f && ((at >> 3) & 3) == i >> 2 && (at & 3) == (i & 3)) pr = s[f][i];
     const float other = __shfl_xor(pr, 32);
     if (((at >> 2) & 1) != h) pr = other;
     if (static_cast<uint32_t>(at - 4 * h - first) >= count) continue;
@@ -530,24 +513,14 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
       p.place[b] = make_int4(x.base + x.tile * p.hkv * x.parts, x.parts, at * p.group, 0);
   }
   const int k0 = uniform(x.first + x.part * x.length), k1 = min(k0 + uniform(x.length), uniform(x.end));
+  const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
   const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * tiles::kRowBytes;
   const int64_t base = (static_cast<int64_t>(uniform(x.group) >> 1) * p.prefix_len * p.hkv + uniform(x.kvh)) * kD;
   const int last = uniform(x.end) - 1;
   const uint16_t *kb = p.prefix_k + base, *vb = p.prefix_v + base;
   const uint32_t lds = tiles::lds_addr(ring);
   __syncthreads();   // the rows; the ring was the plan's
-  // Of half n: K goes to slot n % 4 four steps ahead of its own, V three.
-  const int halves = 2 * ((k1 - k0 + kTileKeys - 1) / kTileKeys);   // (a last one without keys takes an empty step)
-  auto copy_k = [&](int n, int slot) { copy_half(kb, row_bytes, k0 + kHalfKeys * n, last, lds + slot * kHalfBytes, wave, lane); };
-  auto copy_v = [&](int n, int slot) {
-    copy_half(vb, row_bytes, k0 + kHalfKeys * n, last, lds + kVRing + slot * kHalfBytes, wave, lane);
-  };
-  copy_k(0, 0);
-#pragma unroll
-  for (int n = 0; n < 3; ++n) {
-    copy_v(n, n);
-    copy_k(n + 1, n + 1);
-  }
+  copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
   // This lane's row.
   const int rows = seqs * p.group, row = 32 * wave + (lane & 31), h = lane >> 5;
   const bool mine = row < rows, busy = 32 * wave < rows;   // busy: uniform
@@ -566,77 +539,55 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
   const int start = entry.y, latest = __builtin_amdgcn_readfirstlane(tiles::wave_max(start));
   const LaneLds at_lds = lane_lds(lds, lane);
   RowState w;
-  // What this row attends of half n.
-  auto from = [&](int n) { return max(start - (k0 + kHalfKeys * n), 0) - 4 * h; };
-  auto count = [&](int n) {
-    const int key = k0 + kHalfKeys * n;
-    return static_cast<uint32_t>(max(min(k1 - key, kHalfKeys) - max(start - key, 0), 0));
-  };
-  auto clear = [&]() {
+  // Once, and carefully if a sum is not finite then.
+  for (int careful = 0; careful < 2; ++careful) {
     w.m = -INFINITY;
-    w.l = w.from = 0.f;
+    w.l = 0.f;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) w.acc[d][i] = 0.f;
-  };
-  // Before half n's step: its scores masked where some row does not attend all keys, the
-  // maxima moved.
-  auto ready = [&](int n, f32x16& s, float top) {
-    const int key = k0 + kHalfKeys * n;
-    if (key < latest || key + kHalfKeys > k1) {
-      mask(s, from(n), count(n));
-      top = largest(s);
-    }
-    move_maxima(top, c, w);
-  };
-  // Step n: K up to half n + 2 and V up to half n + 1 are there (copied in step n - 2; those of
-  // step n - 1 may be under way), and every wave is done with step n - 1, which frees K's slot
-  // of half n and V's of half n - 1.
-  auto arrive = [&](int n) {
-    if (n + 2 < halves)
-      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    else
+    // Tiles that some row attends in part (they start later), whole ones, the ragged end.
+    const int head = min(max((latest - k0 + kTileKeys - 1) / kTileKeys, 0), steps);
+    const int tail = max(k1 - k0 == steps * kTileKeys ? steps : steps - 1, head);
+    int j = 0;
+    auto arrive = [&]() {   // tile j is there, and every wave is done with the one before
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (n + 3 < halves) {
-      copy_v(n + 3, (n + 3) & 3);
-      copy_k(n + 4, n & 3);
-    }
-  };
-  clear();
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  if (busy) {
-    f32x16 s = scores(at_lds.k, q), next;
-    ready(0, s, largest(s));
-    Ahead ahead;
-    read_ahead(in_slot(at_lds.k, 1), in_slot(at_lds.v, 0), ahead);
-    auto step = [&](int n, const f32x16& s, f32x16& next) {
-      arrive(n);
-      const float top = half_step(in_slot(at_lds.k, (n + 1) & 3), in_slot(at_lds.v, n & 3), in_slot(at_lds.k, (n + 2) & 3),
-                                  in_slot(at_lds.v, (n + 1) & 3), ahead, q, c, s, next, w);
-      if (n + 1 < halves) ready(n + 1, next, top);   // (else there is no such half)
+      if (j + 1 < steps)
+        copy_tile(kb, vb, row_bytes, k0 + kTileKeys * (j + 1), last, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
+      return static_cast<uint32_t>(j & 1) * kSlotBytes;
     };
-    for (int n = 0; n < halves; n += 2) {
-      step(n, s, next);
-      step(n + 1, next, s);
+    // What this row attends of tile j.
+    auto from = [&]() { return max(start - (k0 + kTileKeys * j), 0) - 4 * h; };
+    auto count = [&]() {
+      const int key = k0 + kTileKeys * j;
+      return static_cast<uint32_t>(max(min(k1 - key, kTileKeys) - max(start - key, 0), 0));
+    };
+    auto masked = [&]() {
+      const LaneLds at = in_slot(at_lds, arrive());
+      if (busy) tile_step<true>(at, q, c, from(), count(), w);
+    };
+    if (careful) {
+      for (; j < steps; ++j) {
+        const uint32_t slot = arrive();
+        if (busy) careful_step(ring + slot + tiles::kTileBytes, in_slot(at_lds, slot), q, c, from(), count(), w, lane);
+      }
+      break;
     }
-  } else {
-    for (int n = 0; n < halves; ++n) arrive(n);
-  }
-  float sum = 0.f;   // not finite if one of them is not
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(w.acc[d][i], 0.f, sum);
-  if (__syncthreads_or(mine && sum != 0.f)) {
-    clear();
-    for (int n = 0; n < halves; ++n) {
-      copy_k(n, 0);
-      copy_v(n, 0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (busy) careful_step(ring + kVRing, at_lds, q, c, from(n), count(n), w, lane);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (; j < head; ++j) masked();
+    if (busy) {
+      for (; j < tail; ++j) tile_step<false>(in_slot(at_lds, arrive()), q, c, 0, 0, w);
+    } else {
+      for (; j < tail; ++j) arrive();
     }
+    for (; j < steps; ++j) masked();
+    float sum = 0.f;   // not finite if one of them is not
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(w.acc[d][i], 0.f, sum);
+    if (!__syncthreads_or(mine && sum != 0.f)) break;
+    copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
   }
   if (!mine) return;
   w.l = w.l + __shfl_xor(w.l, 32);
@@ -861,6 +812,7 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
 // The plan's words, a line share's entries and partials, or a ring of two tiles of K and V.
 constexpr int kEntOffset = 2 * kMaxGroups * static_cast<int>(sizeof(int));
 constexpr int kPieceOffset = kEntOffset + kInlineSeqs * static_cast<int>(sizeof(SeqEntry));
+constexpr int kLdsBytes = 2 * kSlotBytes;
 static_assert(kPieceOffset + sizeof(PieceLds) <= kLdsBytes, "a share's words fit the ring");
 
 __global__ __launch_bounds__(256, 2) void shared_split_kernel(const SharedParams p) {
