@@ -29,7 +29,6 @@ from .decode import (  # noqa: F401
     switch_gqa_decode_shared_forward,
 )
 from .rotary import (  # noqa: F401
-    SwitchQKRotaryFunction,
     switch_qk_rotary,
     switch_qk_rotary_append,
     switch_qk_rotary_backward,
@@ -69,6 +68,5 @@ __all__ = [
     "switch_qk_rotary_backward",
     "switch_qk_rotary",
     "switch_qk_rotary_append",
-    "SwitchQKRotaryFunction",
     "switch_gqa_decode_shared_forward",
 ]

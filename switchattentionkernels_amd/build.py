@@ -130,11 +130,13 @@ def build_native(verbose: bool = False) -> str:
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared",
            "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-D__HIP_PLATFORM_AMD__",   # what HIP's own headers ask for
            "-I", os.path.join(ROOT, "include"), "-I", CSRC]
-    for p in include_paths() + [sysconfig.get_paths()["include"]]:
+    rocm = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include")
+    for p in include_paths() + [sysconfig.get_paths()["include"], rocm]:
         cmd += ["-isystem", p]
     cmd += [os.path.join(CSRC, "native.cpp"), "-o", tmp, "-L", tl, "-ltorch", "-ltorch_cpu",
-            "-lc10", "-ltorch_python", "-L", HERE, "-lswattn", "-Wl,-rpath," + tl,
+            "-lc10", "-lc10_hip", "-ltorch_python", "-L", HERE, "-lswattn", "-Wl,-rpath," + tl,
             "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)

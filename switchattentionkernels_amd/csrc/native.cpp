@@ -9,6 +9,8 @@
 // which the GPU is idle; these take about 8.
 
 #include <ATen/core/CachingHostAllocator.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <limits>
@@ -44,6 +46,13 @@ Tensor bytes(const Tensor& like, size_t n) {
 Tensor like(const Tensor& t, const optional<Tensor>& made) {
   return made.has_value() ? *made : at::empty(t.sizes(), t.options());
 }
+
+// Makes a device current, with torch's current stream there.
+struct OnDevice {
+  c10::DeviceGuard guard;
+  void* stream;
+  explicit OnDevice(at::Device device) : guard(device), stream(c10::hip::getCurrentHIPStream(device.index()).stream()) {}
+};
 
 const int32_t* i32(const Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 const int32_t* i32(const optional<Tensor>& t) { return t.has_value() ? i32(*t) : nullptr; }
@@ -467,9 +476,16 @@ bool vector_ok(const Tensor& t, at::Device device) {
   return t.layout() == at::kStrided && t.dim() == 1 && t.is_contiguous() && t.device() == device;
 }
 
+// How a rotation goes, beside its tensors.
+struct RotaryHow {
+  std::vector<int32_t> sections;
+  bool interleaved;
+  double eps;
+};
+
 bool rotary_ok(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
-               const std::vector<int32_t>& sections, const optional<Tensor>& q_weight,
-               const optional<Tensor>& k_weight, double eps) {
+               const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, const RotaryHow& how) {
+  const std::vector<int32_t>& sections = how.sections;
   const at::Device dev = q.device();
   if (!rows_ok(q, dev) || !rows_ok(k, dev) || q.size(0) != k.size(0) || q.size(1) != k.size(1)) return false;
   if (!((inv_freq.scalar_type() == at::kFloat || inv_freq.scalar_type() == at::kDouble) && vector_ok(inv_freq, dev) &&
@@ -483,14 +499,16 @@ bool rotary_ok(const Tensor& q, const Tensor& k, const Tensor& positions, const 
   if (sections.empty() || sections.size() > SWATTN_ROTARY_MAX_AXES || sum != inv_freq.numel()) return false;
   const int64_t want[3] = {static_cast<int64_t>(sections.size()), q.size(0), q.size(1)};
   if (!(positions.scalar_type() == at::kInt && positions.layout() == at::kStrided &&
-        positions.sizes() == at::IntArrayRef(want, 3) && positions.is_contiguous() && positions.device() == dev))
+        (positions.sizes() == at::IntArrayRef(want, 3) ||
+         (sections.size() == 1 && positions.sizes() == at::IntArrayRef(want + 1, 2))) &&
+        positions.is_contiguous() && positions.device() == dev))
     return false;
   for (const optional<Tensor>* w : {&q_weight, &k_weight})
     if (w->has_value() && !(((*w)->scalar_type() == at::kFloat || (*w)->scalar_type() == at::kBFloat16) &&
                             vector_ok(**w, dev) && (*w)->numel() == 128))
       return false;
   if (q_weight.has_value() && k_weight.has_value() && q_weight->scalar_type() != k_weight->scalar_type()) return false;
-  return eps >= 0.0 && eps < std::numeric_limits<double>::infinity();
+  return how.eps >= 0.0 && how.eps < std::numeric_limits<double>::infinity();
 }
 
 bool rotary_append_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc, const Tensor& vc,
@@ -504,7 +522,8 @@ bool rotary_append_ok(const Tensor& q, const Tensor& k, const Tensor& v, const T
          lens_ok(lens, q) && (!counts.has_value() || lens_ok(*counts, q));
 }
 
-// apart() for tensors of any strides, by the span from their first to their last element.
+// apart() for tensors of any strides, by the span from their first to their last element;
+// undefined ones lie nowhere.
 bool rotary_apart(const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
   const auto span = [](const Tensor& t) {
     const char* first = static_cast<const char*>(t.const_data_ptr());
@@ -523,7 +542,7 @@ bool rotary_apart(const std::vector<Tensor>& written, const std::vector<Tensor>&
     for (size_t j = 0; j < i; ++j)
       if (overlap(written[i], written[j])) return false;
     for (const Tensor& t : read)
-      if (overlap(written[i], t)) return false;
+      if (t.defined() && overlap(written[i], t)) return false;
   }
   return true;
 }
@@ -533,32 +552,30 @@ int32_t weight_bf16(const optional<Tensor>& q, const optional<Tensor>& k) {
   return (q.has_value() && q->scalar_type() == at::kBFloat16) || (k.has_value() && k->scalar_type() == at::kBFloat16);
 }
 
-std::tuple<Tensor, Tensor> rotary_forward(const Tensor& q, const Tensor& k, const Tensor& positions,
-                                          const Tensor& inv_freq, const std::vector<int32_t>& sections,
-                                          bool interleaved, const optional<Tensor>& q_weight,
-                                          const optional<Tensor>& k_weight, double eps, int64_t stream,
-                                          const optional<Tensor>& q_made, const optional<Tensor>& k_made) {
+std::tuple<Tensor, Tensor> launch_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& inv_freq,
+                                         const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
+                                         const RotaryHow& how, const optional<Tensor>& q_made,
+                                         const optional<Tensor>& k_made) {
+  const OnDevice here(q.device());
   const Tensor q_out = like(q, q_made), k_out = like(k, k_made);
   if (q.size(1) == 0) return {q_out, k_out};
   const RowStrides qs(q), ks(k);
-  int status = 0;
-  {
-    pybind11::gil_scoped_release release;
-    status = swattn_rotary_fwd(q.const_data_ptr(), qs.s, k.const_data_ptr(), ks.s, i32(positions), inv_freq.const_data_ptr(),
-                               inv_freq.scalar_type() == at::kDouble, sections.data(), static_cast<int32_t>(sections.size()),
-                               interleaved, weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
-                               static_cast<float>(eps), q_out.data_ptr(), k_out.data_ptr(), static_cast<int32_t>(q.size(0)),
-                               q.size(1), static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128,
-                               as_stream(stream));
-  }
-  check(status, "swattn_rotary_fwd");
+  check(swattn_rotary_fwd(q.const_data_ptr(), qs.s, k.const_data_ptr(), ks.s, i32(positions), inv_freq.const_data_ptr(),
+                          inv_freq.scalar_type() == at::kDouble, how.sections.data(),
+                          static_cast<int32_t>(how.sections.size()), how.interleaved, weight_ptr(q_weight),
+                          weight_ptr(k_weight), weight_bf16(q_weight, k_weight), static_cast<float>(how.eps),
+                          q_out.data_ptr(), k_out.data_ptr(), static_cast<int32_t>(q.size(0)), q.size(1),
+                          static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128, here.stream),
+        "swattn_rotary_fwd");
   return {q_out, k_out};
 }
 
-std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>> rotary_backward(
-    const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k, const Tensor& positions,
-    const Tensor& inv_freq, const std::vector<int32_t>& sections, bool interleaved, const optional<Tensor>& q_weight,
-    const optional<Tensor>& k_weight, double eps, bool weight_grads, int64_t stream) {
+using RotaryGrads = std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>>;
+
+RotaryGrads launch_rotary_backward(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k,
+                                   const Tensor& positions, const Tensor& inv_freq, const optional<Tensor>& q_weight,
+                                   const optional<Tensor>& k_weight, const RotaryHow& how, bool weight_grads) {
+  const OnDevice here(q.device());
   const Tensor dq = at::empty(grad_q.sizes(), grad_q.options()), dk = at::empty(grad_k.sizes(), grad_k.options());
   optional<Tensor> dwq, dwk;
   const bool none = q.size(1) == 0;
@@ -574,48 +591,170 @@ std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>> rotary_backward(
   Tensor ws;
   if (sums) ws = bytes(q, ws_bytes);
   const RowStrides qs(q), ks(k);
-  int status = 0;
-  {
-    pybind11::gil_scoped_release release;
-    status = swattn_rotary_bwd(grad_q.const_data_ptr(), grad_k.const_data_ptr(), q.const_data_ptr(), qs.s,
-                               k.const_data_ptr(), ks.s, i32(positions), inv_freq.const_data_ptr(),
-                               inv_freq.scalar_type() == at::kDouble, sections.data(), static_cast<int32_t>(sections.size()),
-                               interleaved, weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
-                               static_cast<float>(eps), dq.data_ptr(), dk.data_ptr(),
-                               dwq.has_value() ? dwq->data_ptr() : nullptr, dwk.has_value() ? dwk->data_ptr() : nullptr,
-                               batch, q.size(1), hq, hkv, 128, sums ? ws.data_ptr() : nullptr, ws_bytes, as_stream(stream));
-  }
-  check(status, "swattn_rotary_bwd");
+  check(swattn_rotary_bwd(grad_q.const_data_ptr(), grad_k.const_data_ptr(), q.const_data_ptr(), qs.s, k.const_data_ptr(),
+                          ks.s, i32(positions), inv_freq.const_data_ptr(), inv_freq.scalar_type() == at::kDouble,
+                          how.sections.data(), static_cast<int32_t>(how.sections.size()), how.interleaved,
+                          weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
+                          static_cast<float>(how.eps), dq.data_ptr(), dk.data_ptr(),
+                          dwq.has_value() ? dwq->data_ptr() : nullptr, dwk.has_value() ? dwk->data_ptr() : nullptr, batch,
+                          q.size(1), hq, hkv, 128, sums ? ws.data_ptr() : nullptr, ws_bytes, here.stream),
+        "swattn_rotary_bwd");
   return {dq, dk, dwq, dwk};
 }
 
+// The bound calls give nothing where an argument needs a look (a copy, an error) by the
+// Python layer, which then calls again.  They hold no GIL.
+optional<RotaryHow> rotary_how(const Tensor& inv_freq, const optional<std::vector<int32_t>>& sections, bool interleaved,
+                               double eps) {
+  if (!sections.has_value() && inv_freq.dim() != 1) return std::nullopt;
+  return RotaryHow{sections.has_value() ? *sections : std::vector<int32_t>{static_cast<int32_t>(inv_freq.numel())},
+                   interleaved, eps};
+}
+
+optional<std::tuple<Tensor, Tensor>> rotary_forward(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                                    const Tensor& inv_freq, const optional<std::vector<int32_t>>& sections,
+                                                    bool interleaved, const optional<Tensor>& q_weight,
+                                                    const optional<Tensor>& k_weight, double eps,
+                                                    const optional<Tensor>& q_made, const optional<Tensor>& k_made) {
+  const auto how = rotary_how(inv_freq, sections, interleaved, eps);
+  if (!how.has_value() || !rotary_ok(q, k, positions, inv_freq, q_weight, k_weight, *how)) return std::nullopt;
+  return launch_rotary(q, k, positions, inv_freq, q_weight, k_weight, *how, q_made, k_made);
+}
+
+bool grad_ok(const Tensor& grad, const Tensor& x) {
+  return grad.scalar_type() == at::kBFloat16 && grad.device() == x.device() && grad.layout() == at::kStrided &&
+         grad.sizes() == x.sizes() && grad.is_contiguous() &&
+         (grad.numel() == 0 || reinterpret_cast<uintptr_t>(grad.const_data_ptr()) % 16 == 0);
+}
+
+optional<RotaryGrads> rotary_backward(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k,
+                                      const Tensor& positions, const Tensor& inv_freq,
+                                      const optional<std::vector<int32_t>>& sections, bool interleaved,
+                                      const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
+                                      bool weight_grads) {
+  const auto how = rotary_how(inv_freq, sections, interleaved, eps);
+  if (!how.has_value() || !rotary_ok(q, k, positions, inv_freq, q_weight, k_weight, *how) || !grad_ok(grad_q, q) ||
+      !grad_ok(grad_k, k))
+    return std::nullopt;
+  return launch_rotary_backward(grad_q, grad_k, q, k, positions, inv_freq, q_weight, k_weight, *how, weight_grads);
+}
+
+// The rotation as a node of autograd's graph.  In C++, since the backward runs on
+// autograd's own thread: B1 S1024 Hq8/Hkv2, forward and gradients, took 127 us of host
+// time with the node in Python.
+namespace ag = torch::autograd;
+
+// What a leaf already has of a graph on another stream would tie a captured backward to
+// that stream's uncaptured work, which ends the process.
+void refuse_captured_leaves(const Tensor& q, const Tensor& k, const optional<Tensor>& q_weight,
+                            const optional<Tensor>& k_weight) {
+  for (const Tensor& t : {q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())}) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto old = ag::impl::try_get_grad_accumulator(t);
+    if (old == nullptr) continue;
+    const auto stream = c10::hip::getCurrentHIPStream(q.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto was = old->stream();
+    TORCH_CHECK(was.has_value() && was->id() == stream.id(),
+                "switch_qk_rotary cannot be captured while an eager graph of the same leaves lives: drop its outputs first");
+  }
+}
+
+struct RotaryNode : ag::Function<RotaryNode> {
+  static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& positions,
+                                   const Tensor& inv_freq, const optional<Tensor>& q_weight,
+                                   const optional<Tensor>& k_weight, const RotaryHow& how,
+                                   const std::pair<optional<Tensor>, optional<Tensor>>& made) {
+    auto [q_out, k_out] = launch_rotary(q, k, positions, inv_freq, q_weight, k_weight, how, made.first, made.second);
+    ctx->save_for_backward({q, k, positions, inv_freq, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())});
+    ctx->saved_data["sections"] = std::vector<int64_t>(how.sections.begin(), how.sections.end());
+    ctx->saved_data["interleaved"] = how.interleaved;
+    ctx->saved_data["eps"] = how.eps;
+    ctx->saved_data["weight_grads"] =
+        (q_weight.has_value() && q_weight->requires_grad()) || (k_weight.has_value() && k_weight->requires_grad());
+    return {std::move(q_out), std::move(k_out)};
+  }
+
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    const bool twice = at::GradMode::is_enabled();
+    ag::variable_list out(8);   // one for each argument of forward
+    {
+      at::AutoGradMode off(false);
+      const ag::variable_list saved = ctx->get_saved_variables();
+      const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
+      const RotaryHow how{{sections.begin(), sections.end()}, ctx->saved_data["interleaved"].toBool(),
+                          ctx->saved_data["eps"].toDouble()};
+      const auto rows = [](const Tensor& grad, const Tensor& x) {
+        const Tensor g = grad.to(at::kBFloat16).contiguous();
+        return grad_ok(g, x) ? g : g.clone();   // (not at a multiple of 16 bytes)
+      };
+      const auto weight = [&](int i) { return saved[i].defined() ? optional<Tensor>(saved[i]) : std::nullopt; };
+      auto [dq, dk, dwq, dwk] =
+          launch_rotary_backward(rows(grads[0], saved[0]), rows(grads[1], saved[1]), saved[0], saved[1], saved[2], saved[3],
+                                 weight(4), weight(5), how, ctx->saved_data["weight_grads"].toBool());
+      out[0] = std::move(dq);
+      out[1] = std::move(dk);
+      if (dwq.has_value()) out[4] = std::move(*dwq);
+      if (dwk.has_value()) out[5] = std::move(*dwk);
+    }
+    if (twice) {   // gradients of gradients raise
+      ag::variable_list once;
+      for (const Tensor& t : out)
+        if (t.defined()) once.push_back(t.detach().requires_grad_());
+      const auto error = std::make_shared<ag::DelayedError>(
+          "trying to differentiate twice a function that is once_differentiable", static_cast<int64_t>(once.size()));
+      once = (*error)(std::move(once));
+      size_t n = 0;
+      for (Tensor& t : out)
+        if (t.defined()) t = once[n++];
+    }
+    return out;
+  }
+};
+
+optional<std::tuple<Tensor, Tensor>> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                                     const Tensor& inv_freq,
+                                                     const optional<std::vector<int32_t>>& sections, bool interleaved,
+                                                     const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
+                                                     double eps, const optional<Tensor>& q_made,
+                                                     const optional<Tensor>& k_made) {
+  const auto how = rotary_how(inv_freq, sections, interleaved, eps);
+  if (!how.has_value() || !rotary_ok(q, k, positions, inv_freq, q_weight, k_weight, *how)) return std::nullopt;
+  if (at::GradMode::is_enabled()) refuse_captured_leaves(q, k, q_weight, k_weight);
+  ag::variable_list out =
+      RotaryNode::apply(q, k, positions, inv_freq, q_weight, k_weight, *how, std::make_pair(q_made, k_made));
+  return std::make_tuple(std::move(out[0]), std::move(out[1]));
+}
+
 // (rotated q, the new lengths).
-std::tuple<Tensor, Tensor> rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc,
-                                         const Tensor& vc, const Tensor& lens, const optional<Tensor>& counts,
-                                         const Tensor& positions, const Tensor& inv_freq,
-                                         const std::vector<int32_t>& sections, bool interleaved,
-                                         const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
-                                         int64_t stream, const optional<Tensor>& q_made) {
+optional<std::tuple<Tensor, Tensor>> rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kc,
+                                                   const Tensor& vc, const Tensor& lens, const optional<Tensor>& counts,
+                                                   const Tensor& positions, const Tensor& inv_freq,
+                                                   const optional<std::vector<int32_t>>& sections, bool interleaved,
+                                                   const optional<Tensor>& q_weight, const optional<Tensor>& k_weight,
+                                                   double eps, const optional<Tensor>& q_made) {
+  const auto how = rotary_how(inv_freq, sections, interleaved, eps);
+  if (!how.has_value() || !rotary_ok(q, k, positions, inv_freq, q_weight, k_weight, *how) ||
+      !rotary_append_ok(q, k, v, kc, vc, lens, counts) ||
+      !rotary_apart({kc, vc}, {q, k, v, lens, positions, inv_freq, counts.value_or(Tensor()), q_weight.value_or(Tensor()),
+                               k_weight.value_or(Tensor())}))
+    return std::nullopt;
+  const OnDevice here(q.device());
   const Tensor q_out = like(q, q_made), lens_out = at::empty({q.size(0)}, lens.options());
   const RowStrides qs(q), ks(k), vs(v);
   const bool none = q.size(1) == 0;   // only the lengths are written
-  int status = 0;
-  {
-    pybind11::gil_scoped_release release;
-    status = swattn_rotary_append(none ? kc.const_data_ptr() : q.const_data_ptr(), qs.s,
-                                  none ? kc.const_data_ptr() : k.const_data_ptr(), ks.s,
-                                  none ? kc.const_data_ptr() : v.const_data_ptr(), vs.s,
-                                  none ? i32(lens) : i32(positions), inv_freq.const_data_ptr(),
-                                  inv_freq.scalar_type() == at::kDouble, sections.data(),
-                                  static_cast<int32_t>(sections.size()), interleaved, weight_ptr(q_weight),
-                                  weight_ptr(k_weight), weight_bf16(q_weight, k_weight), static_cast<float>(eps),
-                                  none ? kc.data_ptr() : q_out.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(lens),
-                                  i32(counts), lens_out.data_ptr<int32_t>(), static_cast<int32_t>(q.size(0)), q.size(1),
-                                  kc.size(1), static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128,
-                                  as_stream(stream));
-  }
-  check(status, "swattn_rotary_append");
-  return {q_out, lens_out};
+  check(swattn_rotary_append(none ? kc.const_data_ptr() : q.const_data_ptr(), qs.s,
+                             none ? kc.const_data_ptr() : k.const_data_ptr(), ks.s,
+                             none ? kc.const_data_ptr() : v.const_data_ptr(), vs.s, none ? i32(lens) : i32(positions),
+                             inv_freq.const_data_ptr(), inv_freq.scalar_type() == at::kDouble, how->sections.data(),
+                             static_cast<int32_t>(how->sections.size()), interleaved, weight_ptr(q_weight),
+                             weight_ptr(k_weight), weight_bf16(q_weight, k_weight), static_cast<float>(eps),
+                             none ? kc.data_ptr() : q_out.data_ptr(), kc.data_ptr(), vc.data_ptr(), i32(lens), i32(counts),
+                             lens_out.data_ptr<int32_t>(), static_cast<int32_t>(q.size(0)), q.size(1), kc.size(1),
+                             static_cast<int32_t>(q.size(2)), static_cast<int32_t>(k.size(2)), 128, here.stream),
+        "swattn_rotary_append");
+  return std::make_tuple(q_out, lens_out);
 }
 
 // Decode behind shared prefixes.
@@ -634,28 +773,25 @@ bool shared_ok(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor
          full.dim() == 1 && full.size(0) == q.size(0) && full.is_contiguous() && full.device() == dev;
 }
 
-std::tuple<Tensor, Tensor> shared_decode(const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& prefix_lens,
-                                         const Tensor& prefix_ids, const Tensor& k, const Tensor& v, const Tensor& lens,
-                                         const Tensor& full, int64_t window, double scale_log2, int64_t stream,
-                                         const optional<Tensor>& out_made) {
+optional<std::tuple<Tensor, Tensor>> shared_decode(const Tensor& q, const Tensor& kp, const Tensor& vp,
+                                                   const Tensor& prefix_lens, const Tensor& prefix_ids, const Tensor& k,
+                                                   const Tensor& v, const Tensor& lens, const Tensor& full, int64_t window,
+                                                   double scale_log2, const optional<Tensor>& out_made) {
+  if (!shared_ok(q, kp, vp, prefix_lens, prefix_ids, k, v, lens, full)) return std::nullopt;
+  const OnDevice here(q.device());
   const int32_t batch = static_cast<int32_t>(q.size(0)), hq = static_cast<int32_t>(q.size(2));
   const int32_t hkv = static_cast<int32_t>(k.size(2)), prefixes = static_cast<int32_t>(kp.size(0));
   const Tensor out = like(q, out_made);
   const Tensor lse = at::empty({q.size(0), 1, q.size(2)}, q.options().dtype(at::kFloat));
   const size_t ws_bytes = swattn_shared_decode_workspace_bytes(batch, k.size(1), prefixes, kp.size(1), hq, hkv);
   const Tensor ws = bytes(q, ws_bytes > 0 ? ws_bytes : 1);
-  int status = 0;
-  {
-    pybind11::gil_scoped_release release;
-    status = swattn_shared_decode_fwd(q.const_data_ptr(), kp.const_data_ptr(), vp.const_data_ptr(), i32(prefix_lens),
-                                      i32(prefix_ids), k.const_data_ptr(), v.const_data_ptr(), i32(lens),
-                                      static_cast<const uint8_t*>(full.const_data_ptr()), out.data_ptr(),
-                                      lse.data_ptr<float>(), batch, k.size(1), prefixes, kp.size(1), hq, hkv, 128,
-                                      static_cast<int32_t>(window), static_cast<float>(scale_log2), ws.data_ptr(),
-                                      ws_bytes, as_stream(stream));
-  }
-  check(status, "swattn_shared_decode_fwd");
-  return {out, lse};
+  check(swattn_shared_decode_fwd(q.const_data_ptr(), kp.const_data_ptr(), vp.const_data_ptr(), i32(prefix_lens),
+                                 i32(prefix_ids), k.const_data_ptr(), v.const_data_ptr(), i32(lens),
+                                 static_cast<const uint8_t*>(full.const_data_ptr()), out.data_ptr(), lse.data_ptr<float>(),
+                                 batch, k.size(1), prefixes, kp.size(1), hq, hkv, 128, static_cast<int32_t>(window),
+                                 static_cast<float>(scale_log2), ws.data_ptr(), ws_bytes, here.stream),
+        "swattn_shared_decode_fwd");
+  return std::make_tuple(out, lse);
 }
 
 }  // namespace
@@ -679,12 +815,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefill_key_weights", &prefill_key_weights);
   m.def("cache_evict", &cache_evict);
   m.def("cache_evict_new", &cache_evict_new);
-  m.def("rotary_ok", &rotary_ok);
-  m.def("rotary_append_ok", &rotary_append_ok);
+  const auto no_gil = py::call_guard<py::gil_scoped_release>();
   m.def("rotary_apart", &rotary_apart);
-  m.def("rotary_forward", &rotary_forward);
-  m.def("rotary_backward", &rotary_backward);
-  m.def("rotary_append", &rotary_append);
-  m.def("shared_ok", &shared_ok);
-  m.def("shared_decode", &shared_decode);
+  m.def("rotary_forward", &rotary_forward, no_gil);
+  m.def("rotary_backward", &rotary_backward, no_gil);
+  m.def("rotary_autograd", &rotary_autograd, no_gil);
+  m.def("rotary_append", &rotary_append, no_gil);
+  m.def("shared_decode", &shared_decode, no_gil);
 }

@@ -208,19 +208,20 @@ def switch_gqa_decode_shared_forward(
     squeeze = isinstance(q, torch.Tensor) and q.ndim == 3
     if squeeze:
         q = q.unsqueeze(1)
-    if not _all_tensors(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens,
-                        full_mask) or not _lib.native().shared_ok(
-            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask):
-        prefix_lens, prefix_ids, cache_lens, full_mask = _check_shared(
-            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask)
     if window_size <= 0:
         raise ValueError("window_size must be positive")
     scale = (128 ** -0.5 if sm_scale is None else float(sm_scale)) * LOG2E
-    dev = q.device
-    with _lib.on_device(dev):
-        out, lse = _lib.native().shared_decode(
-            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask,
-            min(int(window_size), 2 ** 31 - 1), scale, _lib.stream_handle(dev), _lib.like(q))
+    call, how = _lib.native().shared_decode, (min(int(window_size), 2 ** 31 - 1), scale)
+    try:
+        out = call(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask,
+                   *how, _lib.like(q))
+    except TypeError:   # not tensors
+        out = None
+    if out is None:
+        prefix_lens, prefix_ids, cache_lens, full_mask = _check_shared(
+            q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask)
+        out = call(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask,
+                   *how, _lib.like(q))
     if squeeze:
-        return out[:, 0], lse[:, 0]
-    return out, lse
+        return out[0][:, 0], out[1][:, 0]
+    return out

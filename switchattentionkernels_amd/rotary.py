@@ -6,7 +6,7 @@ slices, contiguous as the attention wants them:
 
 * ``switch_qk_rotary_forward`` normalises (optionally) and rotates;
 * ``switch_qk_rotary_backward`` gives the gradients, ``switch_qk_rotary`` is the
-  forward as a ``torch.autograd.Function``;
+  forward as a node of autograd's graph;
 * ``switch_qk_rotary_append`` rotates new tokens of a serving batch, with the keys and
   values going into bf16 caches (those of ``switch_gqa_decode_forward``).
 
@@ -25,10 +25,9 @@ from __future__ import annotations
 from typing import Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .cache import _all_tensors, check_lens
+from .cache import check_lens
 
 MAX_AXES = 4   # SWATTN_ROTARY_MAX_AXES
 
@@ -82,21 +81,25 @@ def _validate(q, k, positions, inv_freq, sections, q_weight, k_weight, eps) -> N
 
 
 def _arguments(q, k, positions, inv_freq, sections, q_weight, k_weight, eps):
-    """(positions [axes,B,S], inv_freq, sections, q_weight, k_weight), contiguous and
-    checked; in Python only where a condition fails or a copy is needed."""
+    """The same arguments, checked, positions ``[axes,B,S]`` and all but q and k contiguous."""
     if isinstance(positions, torch.Tensor) and positions.ndim == 2:
         positions = positions.unsqueeze(0)
     if sections is None:
         sections = [inv_freq.numel()] if isinstance(inv_freq, torch.Tensor) else [0]
     else:
         sections = [int(n) for n in sections]
-    eps = float(eps)
-    if not _all_tensors(q, k, positions, inv_freq) or not _lib.native().rotary_ok(
-            q, k, positions, inv_freq, sections, q_weight, k_weight, eps):
-        _validate(q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
-        positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-        q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    return positions, inv_freq, sections, q_weight, k_weight, eps
+    _validate(q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+    return (q, k, positions.contiguous(), inv_freq.contiguous(), sections,
+            *(None if w is None else w.contiguous() for w in (q_weight, k_weight)), eps)
+
+
+def _quick(call, *args):
+    """What the native call gives: None where its arguments need a look, which also holds
+    for those that it cannot take at all."""
+    try:
+        return call(*args)
+    except TypeError:
+        return None
 
 
 def switch_qk_rotary_forward(
@@ -119,13 +122,19 @@ def switch_qk_rotary_forward(
     ``q_weight`` / ``k_weight``: fp32 or bf16 ``[128]``, of one type; where one is given,
     its rows are normalised first (each head by itself).
     """
-    positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
-        q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
-    with _lib.on_device(q.device):
-        return _lib.native().rotary_forward(q, k, positions, inv_freq, sections, bool(interleaved),
-                                            q_weight, k_weight, eps, _lib.stream_handle(q.device),
-                                            _lib.like_contiguous(q),
-                                            _lib.like_contiguous(k))
+    return _rotate(_lib.native().rotary_forward, q, k, positions, inv_freq, sections, interleaved,
+                   q_weight, k_weight, eps)
+
+
+def _rotate(call, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps):
+    interleaved, eps = bool(interleaved), float(eps)
+    made = (_lib.like_contiguous(q), _lib.like_contiguous(k))
+    out = _quick(call, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, *made)
+    if out is None:
+        q, k, positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
+            q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+        out = call(q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, *made)
+    return out
 
 
 def switch_qk_rotary_backward(
@@ -140,41 +149,19 @@ def switch_qk_rotary_backward(
     gradients in the weights' type, None where there is no weight (or without
     ``weight_grads``).  They are summed in fp32 in a fixed order.
     """
-    positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
-        q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
-    for name, g, x in (("grad_q", grad_q, q), ("grad_k", grad_k, k)):
-        if (not isinstance(g, torch.Tensor) or g.shape != x.shape or g.dtype != torch.bfloat16
-                or g.device != x.device or not g.is_contiguous() or g.numel() and g.data_ptr() % 16):
-            raise ValueError(f"{name} must be a contiguous BF16 tensor shaped like {name[-1].upper()}")
-    with _lib.on_device(q.device):
-        return _lib.native().rotary_backward(grad_q, grad_k, q, k, positions, inv_freq, sections,
-                                             bool(interleaved), q_weight, k_weight, eps,
-                                             bool(weight_grads), _lib.stream_handle(q.device))
-
-
-class SwitchQKRotaryFunction(torch.autograd.Function):
-    """``switch_qk_rotary_forward`` with a backward: ``apply(q, k, positions, inv_freq,
-    q_weight, k_weight, sections, interleaved, eps) -> (q, k)``."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, q_weight, k_weight, sections, interleaved, eps):
-        out = switch_qk_rotary_forward(q, k, positions, inv_freq, sections=sections,
-                                       interleaved=interleaved, q_weight=q_weight,
-                                       k_weight=k_weight, eps=eps)
-        ctx.save_for_backward(q, k, positions, inv_freq, q_weight, k_weight)
-        ctx.how = {"sections": sections, "interleaved": interleaved, "eps": eps}
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_q, grad_k):
-        q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = switch_qk_rotary_backward(
-            grad_q.to(torch.bfloat16).contiguous(), grad_k.to(torch.bfloat16).contiguous(), q, k,
-            positions, inv_freq, q_weight=q_weight, k_weight=k_weight,
-            weight_grads=need[4] or need[5], **ctx.how)
-        return dq, dk, None, None, dwq, dwk, None, None, None
+    interleaved, eps, call = bool(interleaved), float(eps), _lib.native().rotary_backward
+    out = _quick(call, grad_q, grad_k, q, k, positions, inv_freq, sections, interleaved, q_weight,
+                 k_weight, eps, bool(weight_grads))
+    if out is None:
+        q, k, positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
+            q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+        for name, g, x in (("grad_q", grad_q, q), ("grad_k", grad_k, k)):
+            if (not isinstance(g, torch.Tensor) or g.shape != x.shape or g.dtype != torch.bfloat16
+                    or g.device != x.device or not g.is_contiguous() or g.numel() and g.data_ptr() % 16):
+                raise ValueError(f"{name} must be a contiguous BF16 tensor shaped like {name[-1].upper()}")
+        out = call(grad_q, grad_k, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight,
+                   eps, bool(weight_grads))
+    return out
 
 
 def switch_qk_rotary(q, k, positions, inv_freq, *, sections: Optional[Sequence[int]] = None,
@@ -182,10 +169,12 @@ def switch_qk_rotary(q, k, positions, inv_freq, *, sections: Optional[Sequence[i
                      k_weight: Optional[torch.Tensor] = None,
                      eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """``switch_qk_rotary_forward`` with autograd support for q, k and the weights (once:
-    gradients of gradients raise)."""
-    return SwitchQKRotaryFunction.apply(q, k, positions, inv_freq, q_weight, k_weight,
-                                        None if sections is None else tuple(sections),
-                                        interleaved, eps)
+    gradients of gradients raise).
+
+    Under capture the leaves among them must not belong to an eager graph that still lives
+    (such a call raises: the captured backward would end the process)."""
+    return _rotate(_lib.native().rotary_autograd, q, k, positions, inv_freq, sections, interleaved,
+                   q_weight, k_weight, eps)
 
 
 def _validate_append(q, k, v, k_cache, v_cache, lens, counts) -> None:
@@ -227,20 +216,20 @@ def switch_qk_rotary_append(
     caches keep their contents, and the q rows of tokens that are not appended are
     rotated like the rest.  ``positions`` are the tokens' own, whatever the cache holds.
     """
-    positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
-        q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
-    lens, counts = cache_lens, row_counts
-    if not _all_tensors(v, k_cache, v_cache, lens) or not _lib.native().rotary_append_ok(
-            q, k, v, k_cache, v_cache, lens, counts):
-        _validate_append(q, k, v, k_cache, v_cache, lens, counts)
-        lens = lens.contiguous()
-        counts = None if counts is None else counts.contiguous()
-    read = [q, k, v, lens, positions, inv_freq]
-    read += [t for t in (counts, q_weight, k_weight) if t is not None]
-    if not _lib.native().rotary_apart((k_cache, v_cache), read):
-        raise ValueError("the caches must not share memory with each other or the other arguments")
-    with _lib.on_device(q.device):
-        return _lib.native().rotary_append(q, k, v, k_cache, v_cache, lens, counts, positions,
-                                           inv_freq, sections, bool(interleaved), q_weight,
-                                           k_weight, eps, _lib.stream_handle(q.device),
-                                           _lib.like_contiguous(q))
+    interleaved, eps, call = bool(interleaved), float(eps), _lib.native().rotary_append
+    made = _lib.like_contiguous(q)
+    out = _quick(call, q, k, v, k_cache, v_cache, cache_lens, row_counts, positions, inv_freq, sections,
+                 interleaved, q_weight, k_weight, eps, made)
+    if out is None:
+        q, k, positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
+            q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+        _validate_append(q, k, v, k_cache, v_cache, cache_lens, row_counts)
+        lens = cache_lens.contiguous()
+        counts = None if row_counts is None else row_counts.contiguous()
+        read = [q, k, v, lens, positions, inv_freq]
+        read += [t for t in (counts, q_weight, k_weight) if t is not None]
+        if not _lib.native().rotary_apart((k_cache, v_cache), read):
+            raise ValueError("the caches must not share memory with each other or the other arguments")
+        out = call(q, k, v, k_cache, v_cache, lens, counts, positions, inv_freq, sections, interleaved,
+                   q_weight, k_weight, eps, made)
+    return out

@@ -251,6 +251,86 @@ def test_autograd():
         torch.autograd.grad(q.float().square().sum(), x, create_graph=True)[0].sum().backward()
 
 
+def test_gradients_that_start_anywhere():
+    """Gradients that come as views: not contiguous, and not at a multiple of 16 bytes."""
+    c = _case(25, 2, 5, 4, 2)
+    leaves = [_up(c[x]).requires_grad_() for x in ("q", "k", "qw", "kw")]
+    outs = switch_qk_rotary(leaves[0], leaves[1], _up(c["pos"]), _up(c["freq"]), sections=c["sections"],
+                            q_weight=leaves[2], k_weight=leaves[3])
+    grads = [_rows(c["gen"], *x.shape) for x in outs]
+    odd = torch.empty(grads[0].numel() + 1, dtype=BF16, device=DEV)[1:].view(grads[0].shape)
+    odd.copy_(grads[0])
+    turned = _up(grads[1]).transpose(1, 2).contiguous().transpose(1, 2)
+    got = torch.autograd.grad(outs, leaves, (odd, turned))
+    _check_backward(c, False, 1e-6, got, grads)
+
+
+def test_one_gradient_only():
+    """What is not asked for is not given; an output that nothing uses has a gradient of 0."""
+    c = _case(26, 2, 5, 4, 2)
+    names = ("q", "k", "qw", "kw")
+    for want in names:
+        leaf = {x: _up(c[x]).requires_grad_(x == want) for x in names}
+        q, k = switch_qk_rotary(leaf["q"], leaf["k"], _up(c["pos"]), _up(c["freq"]), q_weight=leaf["qw"],
+                                k_weight=leaf["kw"])
+        out, other = (q, k) if want[0] == "q" else (k, q)
+        out.backward(torch.ones_like(out))
+        ones = [torch.ones_like(x) if x is out else torch.zeros_like(x) for x in (q, k)]
+        full = switch_qk_rotary_backward(*ones, leaf["q"], leaf["k"], _up(c["pos"]), _up(c["freq"]),
+                                         q_weight=leaf["qw"], k_weight=leaf["kw"])
+        assert torch.equal(leaf[want].grad, full[names.index(want)])
+        assert all(leaf[x].grad is None for x in names if x != want)
+
+
+def test_training_step_captured_and_replayed():
+    c = _case(27, 1, 40, 8, 2)
+    leaves = [_up(c[x]).requires_grad_() for x in ("q", "k", "qw", "kw")]
+    pos, freq = _up(c["pos"]), _up(c["freq"])
+    grads = [_up(_rows(c["gen"], *c[x].shape)) for x in "qk"]
+
+    def step():
+        outs = switch_qk_rotary(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3])
+        return outs + torch.autograd.grad(outs, leaves, grads)
+
+    def eager():
+        return [x.detach().clone() for x in step()]
+
+    eager()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [x.detach() for x in step()]
+    for i in range(4):
+        with torch.no_grad():
+            for x in leaves + grads:
+                x.copy_(x * (1.0 + 0.25 * i))
+        pos.add_(i + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, eager())), i
+
+
+def test_capture_is_refused_while_an_eager_graph_of_the_leaves_lives():
+    c = _case(28, 1, 9, 4, 2)
+    q, w = _up(c["q"]).requires_grad_(), _up(c["qw"]).requires_grad_()
+    k, pos, freq = _up(c["k"]), _up(c["pos"]), _up(c["freq"])
+    run = lambda: switch_qk_rotary(q, k, pos, freq, q_weight=w)  # noqa: E731
+    kept = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two = k + 1
+        with pytest.raises(RuntimeError, match="eager graph"):
+            run()
+        with torch.no_grad():                    # without a graph of its own it stays allowed
+            out = run()
+    two.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(two, k + 1) and all(torch.equal(a, b) for a, b in zip(out, kept))
+
+
 def test_changed_inputs_are_noticed_by_autograd():
     c = _case(24, 1, 4, 2, 1)
     x, pos = _up(c["q"]).requires_grad_(), _up(c["pos"])
