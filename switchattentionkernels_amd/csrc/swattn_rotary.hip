@@ -6,12 +6,23 @@
 //   backward, g = dy rotated by -t:  dw = sum g u,  dx = r (g w - u mean(g w u))
 //
 // HBM-bound: 512 bytes per head row forward, 768 backward (512 without a norm) against
-// about a dozen operations per value.  A wave takes a token and goes through its head
-// rows eight at a time, eight lanes per row; a lane holds two 16-byte chunks of its row
-// whose dims form whole pairs, so that the rotation needs no exchange between lanes and
-// the norm a sum over eight lanes.  The token's angles are the same for all its heads:
-// each lane computes one frequency's sine and cosine, and the lanes pick up the eight
-// that their dims need from LDS.
+// about a dozen operations per value.  A wave takes eight head rows of a token at once (a
+// pass), eight lanes per row; a lane holds two 16-byte chunks of its row whose dims form
+// whole pairs, so that the rotation needs no exchange between lanes and the norm a sum over
+// eight lanes.  The token's angles are the same for all its heads: each lane computes one
+// frequency's sine and cosine, and the lanes pick up the eight that their dims need from
+// LDS, as the norms' weights: kept in registers, both cost a third of the waves.
+// The grid is what the chip takes at once.  Waves go over whole tokens in rounds, side by
+// side, and share out the passes of the tokens that are left: with tokens alone a batch of
+// 5998 left a third of the waves idle, with one run of passes per wave B1 S16384 Hq32/Hkv8
+// took 72 us instead of 69.  Rows are read one pass ahead.
+//
+// Measured, as a large copy's 5.2 TB/s goes (a copy of 74 MB: 5.0): rotations of strided
+// rows B1 S16384 Hq32/Hkv8 62.5 us (5.4 TB/s), B2 S2999 Hq40/Hkv8 29.9 (4.9); backward of
+// S16384 with norms 93.5 us (5.4 TB/s), of B2 S4096 without 28.9; appends of B8 T517 Hq64/Hkv8
+// 33.2 (4.7), of 64 single tokens 6.6, bound by dependent latencies and the host's call.
+// One pass at a time without reading ahead, angles and weights in registers: 71, 42, 117, 42,
+// 50 and 7.5.
 //
 // Angles are exact where fp32 products are not (a position of 2^17 times a frequency of
 // 1 is off by up to 2^-8 in fp32): a frequency is held as a 64-bit fixed-point fraction
@@ -31,6 +42,12 @@ namespace {
 constexpr int kD = 128;
 constexpr int kWaves = 4;          // waves per workgroup
 constexpr int kRowsAtOnce = 8;     // head rows that a wave takes at once
+constexpr int kGroupsPerCu = 5;    // workgroups that a CU takes at once
+constexpr int kBackPerCu = 3;      // and of the backward
+// Calls that move more than kStreamBytes go past the 256 MB memory-side cache, whose lines
+// others may still have a use for: the forward in both directions, the backward with what
+// it writes, and with what it reads if that alone fills the cache.
+constexpr int64_t kStreamBytes = 96 << 20, kCacheBytes = 256 << 20;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -45,6 +62,43 @@ struct Angles {
   int f64, count, axes;
   int ends[SWATTN_ROTARY_MAX_AXES - 1];   // frequencies before each axis but the first
 };
+
+// How the waves share the tokens' passes over eight head rows: whole tokens in rounds,
+// neighbours to neighbours, then the passes of the tokens that are left in equal shares.
+struct Shares {
+  int waves, rounds;
+  int64_t each;   // passes of what is left, and one more for the first `more` waves
+  int more;
+};
+struct Part {     // passes [pass, end) of a token; end 0: none
+  int token, pass, end;
+};
+struct Walk {
+  uint32_t token;   // of the next round
+  int rounds, left_token, left_pass;
+  int64_t left;
+};
+__device__ __forceinline__ Walk walk_of(const Shares& s, int wave, int passes) {
+  const int64_t from = wave * s.each + min(wave, s.more);   // below waves * passes
+  const int token = from >> 32 == 0 ? static_cast<int>(static_cast<uint32_t>(from) / static_cast<uint32_t>(passes))
+                                    : static_cast<int>(from / passes);
+  return Walk{static_cast<uint32_t>(wave), s.rounds, s.waves * s.rounds + token,
+              static_cast<int>(from - static_cast<int64_t>(token) * passes), s.each + (wave < s.more ? 1 : 0)};
+}
+__device__ __forceinline__ Part advance(Walk& w, const Shares& s, int passes) {
+  if (w.rounds > 0) {
+    const int token = static_cast<int>(w.token);
+    --w.rounds;
+    w.token += s.waves;
+    return Part{token, 0, passes};
+  }
+  if (w.left == 0) return Part{0, 0, 0};
+  const Part x{w.left_token, w.left_pass, static_cast<int>(min(static_cast<int64_t>(passes), w.left_pass + w.left))};
+  w.left -= x.end - x.pass;
+  ++w.left_token;
+  w.left_pass = 0;
+  return x;
+}
 
 struct RotaryParams {
   Rows q, k, v;
@@ -61,7 +115,7 @@ struct RotaryParams {
   int32_t* lens_out;
   int64_t cache_len;
   int batch, seq, tokens, hq, hkv;
-  int per_token;      // waves that share a token's head rows
+  Shares shares;
 };
 
 // Turns per position as a 64-bit fraction: f / (2 pi), with 1 / (2 pi) and the product
@@ -110,9 +164,6 @@ template <bool kPairs>
 __device__ __forceinline__ Lane lane_setup(const Angles& g, int lane) {
   Lane o;
   const int i = min(lane, g.count - 1), l = lane & 7;
-  const double f = g.f64 ? static_cast<const double*>(g.freq)[i] : static_cast<double>(static_cast<const float*>(g.freq)[i]);
-  o.nan = !(__builtin_fabs(f) < 0x1p40);
-  o.turns = fixed_turns(o.nan ? 0.0 : f);
   o.axis = 0;
 #pragma unroll
   for (int x = 0; x < SWATTN_ROTARY_MAX_AXES - 1; ++x) o.axis += x + 1 < g.axes && i >= g.ends[x] ? 1 : 0;
@@ -122,42 +173,42 @@ __device__ __forceinline__ Lane lane_setup(const Angles& g, int lane) {
   o.b = beside ? o.a + 8 : o.a + g.count;
   return o;
 }
+__device__ __forceinline__ void lane_turns(const Angles& g, int lane, Lane& o) {
+  const int i = min(lane, g.count - 1);
+  const double f = g.f64 ? static_cast<const double*>(g.freq)[i] : static_cast<double>(static_cast<const float*>(g.freq)[i]);
+  o.nan = !(__builtin_fabs(f) < 0x1p40);
+  o.turns = fixed_turns(o.nan ? 0.0 : f);
+}
 
-// Cosines and sines of the eight frequencies that this lane's pairs have, through the
-// wave's own LDS words (a wave's LDS operations complete in order).
-struct Turn {
-  float c[8], s[8];
-};
-__device__ __forceinline__ void token_turn(const Angles& g, const Lane& o, int token, int tokens, int lane,
-                                           float (*lds)[64], Turn& t) {
-  const int pos = g.positions[static_cast<int64_t>(o.axis) * tokens + token];
+__device__ __forceinline__ int token_position(const Angles& g, const Lane& o, int64_t token, int tokens) {
+  return g.positions[static_cast<int64_t>(o.axis) * tokens + token];
+}
+
+// Cosines and sines of a token's frequencies, in the wave's own LDS words (a wave's LDS
+// operations complete in order).
+__device__ __forceinline__ void token_turn(const Lane& o, int pos, int lane, float (*lds)[64]) {
   const uint64_t at = o.turns * static_cast<uint64_t>(static_cast<int64_t>(pos));
   float s, c;
   sine_cosine(static_cast<uint32_t>((at + 0x80000000u) >> 32), s, c);
+  __builtin_amdgcn_wave_barrier();
   lds[0][lane] = o.nan ? NAN : c;
   lds[1][lane] = o.nan ? NAN : s;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  const int first = min(8 * (lane & 7), 56);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    t.c[e] = lds[0][first + e];
-    t.s[e] = lds[1][first + e];
-  }
   __builtin_amdgcn_wave_barrier();
 }
 
 // x: dims a .. a + 7, then b .. b + 7, rotated by +t or -t.
 template <bool kPairs, bool kBack>
-__device__ __forceinline__ void rotate(const Lane& o, const Turn& t, float (&x)[16]) {
+__device__ __forceinline__ void rotate(const Lane& o, const float (*lds)[64], int lane, float (&x)[16]) {
   if (!o.turned) return;
+  const int first = 8 * (lane & 7);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int i = kPairs ? 2 * e : e, j = kPairs ? 2 * e + 1 : e + 8;
-    const float s = kBack ? -t.s[e] : t.s[e];
+    const float c = lds[0][first + e], s = kBack ? -lds[1][first + e] : lds[1][first + e];
     const float a = x[i], b = x[j];
-    x[i] = a * t.c[e] - b * s;
-    x[j] = b * t.c[e] + a * s;
+    x[i] = a * c - b * s;
+    x[j] = b * c + a * s;
   }
 }
 
@@ -172,9 +223,22 @@ __device__ __forceinline__ float row_sum(float x) {
 struct Chunks {
   u32x4 a, b;
 };
+template <bool kStream>
 __device__ __forceinline__ void load_chunks(const uint16_t* row, const Lane& o, Chunks& c) {
-  c.a = *reinterpret_cast<const u32x4*>(row + o.a);
-  c.b = *reinterpret_cast<const u32x4*>(row + o.b);
+  const u32x4 *a = reinterpret_cast<const u32x4*>(row + o.a), *b = reinterpret_cast<const u32x4*>(row + o.b);
+  c.a = kStream ? __builtin_nontemporal_load(a) : *a;
+  c.b = kStream ? __builtin_nontemporal_load(b) : *b;
+}
+template <bool kStream>
+__device__ __forceinline__ void store_chunks(uint16_t* row, const Lane& o, const Chunks& c) {
+  u32x4 *a = reinterpret_cast<u32x4*>(row + o.a), *b = reinterpret_cast<u32x4*>(row + o.b);
+  if constexpr (kStream) {
+    __builtin_nontemporal_store(c.a, a);
+    __builtin_nontemporal_store(c.b, b);
+  } else {
+    *a = c.a;
+    *b = c.b;
+  }
 }
 __device__ __forceinline__ void unpack(const Chunks& c, float (&x)[16]) {
 #pragma unroll
@@ -190,33 +254,44 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
   return __builtin_bit_cast(uint32_t, v);
 }
+template <bool kStream>
 __device__ __forceinline__ void store_row(uint16_t* row, const Lane& o, const float (&x)[16]) {
-  *reinterpret_cast<u32x4*>(row + o.a) = u32x4{pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7])};
-  *reinterpret_cast<u32x4*>(row + o.b) = u32x4{pack(x[8], x[9]), pack(x[10], x[11]), pack(x[12], x[13]), pack(x[14], x[15])};
+  store_chunks<kStream>(row, o,
+                        Chunks{u32x4{pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7])},
+                               u32x4{pack(x[8], x[9]), pack(x[10], x[11]), pack(x[12], x[13]), pack(x[14], x[15])}});
 }
 
-// This lane's 16 weights of a tensor (1 where it has none).
-__device__ __forceinline__ void load_weights(const void* w, int bf16, const Lane& o, float (&x)[16]) {
+// A tensor's weights in LDS, by the workgroup's first or second 128 threads.
+__device__ __forceinline__ void stage_weights(const void* w, int bf16, int d, float* lds) {
+  if (w == nullptr) return;
+  lds[d] = bf16 ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(w)[d]) << 16) : static_cast<const float*>(w)[d];
+}
+__device__ __forceinline__ void load_weights(const float* lds, const Lane& o, float (&w)[16]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int d = i < 8 ? o.a + i : o.b + i - 8;
-    x[i] = w == nullptr ? 1.f
-           : bf16       ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(w)[d]) << 16)
-                        : static_cast<const float*>(w)[d];
+  for (int i = 0; i < 8; ++i) {
+    w[i] = lds[o.a + i];
+    w[8 + i] = lds[o.b + i];
   }
 }
 
-// 1 / sqrt(mean(x^2) + eps) of the row.
+// 1 / sqrt(mean(x^2) + eps) of the row: the hardware's, within one last place, which takes
+// no denormal number.
 __device__ __forceinline__ float row_scale(const float (&x)[16], float eps) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s = __builtin_fmaf(x[i], x[i], s);
-  return 1.0f / __builtin_sqrtf(__builtin_fmaf(row_sum(s), 1.0f / kD, eps));
+  const float m = __builtin_fmaf(row_sum(s), 1.0f / kD, eps);
+  const bool small = m < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(small ? m * 0x1p64f : m) * (small ? 0x1p32f : 1.0f);
 }
 
-template <bool kPairs, bool kAppend>
-__global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const RotaryParams p) {
+// A wave goes through its share of the passes: a token's q rows, then its k rows, then its
+// v rows, which are copied.  A pass's rows are read one pass ahead, a token's positions one
+// token ahead.
+template <bool kPairs, bool kAppend, bool kStream>
+__global__ __launch_bounds__(64 * kWaves, kGroupsPerCu) void rotary_kernel(const RotaryParams p) {
   __shared__ float s_turn[kWaves][2][64];
+  __shared__ float s_weight[2][kD];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if constexpr (kAppend) {
@@ -226,49 +301,75 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const RotaryParams 
       p.lens_out[b] = static_cast<int32_t>(min(len + count, p.cache_len));
     }
   }
-  const Lane o = lane_setup<kPairs>(p.angles, lane);
-  float wq[16], wk[16];
-  load_weights(p.q_weight, p.weight_bf16, o, wq);
-  load_weights(p.k_weight, p.weight_bf16, o, wk);
-  const int first = blockIdx.x * kWaves + wave, part = first % p.per_token;
-  const int step = gridDim.x * kWaves / p.per_token;
   const int q_passes = (p.hq + kRowsAtOnce - 1) / kRowsAtOnce, k_passes = (p.hkv + kRowsAtOnce - 1) / kRowsAtOnce;
   const int passes = q_passes + (kAppend ? 2 : 1) * k_passes;
-  for (int64_t token = first / p.per_token; token < p.tokens; token += step) {
-    const int b = static_cast<int>(token) / p.seq, s = static_cast<int>(token) - b * p.seq;
-    Turn t;
-    token_turn(p.angles, o, static_cast<int>(token), p.tokens, lane, s_turn[wave], t);
-    int64_t at = token;       // of the row that K (and V) go to, in k_out
+  Walk walk = walk_of(p.shares, blockIdx.x * kWaves + wave, passes);
+  Lane o = lane_setup<kPairs>(p.angles, lane);
+  auto tensor = [&](int pass) { return pass < q_passes ? 0 : pass < q_passes + k_passes ? 1 : 2; };
+  auto head = [&](int pass, int x) {
+    return (pass - (x == 0 ? 0 : x == 1 ? q_passes : q_passes + k_passes)) * kRowsAtOnce + (lane >> 3);
+  };
+  auto load = [&](int b, int s, int pass, Chunks& c) {
+    const int x = tensor(pass), h = head(pass, x);
+    const Rows& in = x == 0 ? p.q : x == 1 ? p.k : p.v;
+    if (h < (x == 0 ? p.hq : p.hkv)) load_chunks<kStream>(in.p + b * in.sb + s * in.ss + h * in.sh, o, c);
+  };
+  Part now = advance(walk, p.shares, passes);
+  int b = 0, s = 0, pos = 0;
+  Chunks next;
+  if (now.end > 0) {
+    b = now.token / p.seq;
+    s = now.token - b * p.seq;
+    load(b, s, now.pass, next);
+    pos = token_position(p.angles, o, now.token, p.tokens);
+  }
+  stage_weights(tid < kD ? p.q_weight : p.k_weight, p.weight_bf16, tid & (kD - 1), s_weight[tid / kD]);
+  lane_turns(p.angles, lane, o);
+  __syncthreads();
+  while (now.end > 0) {
+    token_turn(o, pos, lane, s_turn[wave]);
+    int64_t at = now.token;       // of the row that K (and V) go to, in k_out
     bool live = true;
     if constexpr (kAppend) {
       const int64_t len = min(max(static_cast<int64_t>(p.lens[b]), int64_t{0}), p.cache_len);
       live = len + s < p.cache_len && (p.counts == nullptr || s < p.counts[b]);
       at = b * p.cache_len + len + s;
     }
-    for (int pass = part; pass < passes; pass += p.per_token) {
-      const bool is_q = pass < q_passes;
-      const bool is_v = kAppend && pass >= q_passes + k_passes;
-      const int h = (pass - (is_q ? 0 : is_v ? q_passes + k_passes : q_passes)) * kRowsAtOnce + (lane >> 3);
-      if (h >= (is_q ? p.hq : p.hkv) || !(is_q || live)) continue;
-      const Rows& in = is_q ? p.q : is_v ? p.v : p.k;
-      Chunks c;
-      load_chunks(in.p + b * in.sb + s * in.ss + h * in.sh, o, c);
-      if (is_v) {
-        uint16_t* row = p.v_out + (at * p.hkv + h) * kD;
-        *reinterpret_cast<u32x4*>(row + o.a) = c.a;
-        *reinterpret_cast<u32x4*>(row + o.b) = c.b;
+    const Part then = advance(walk, p.shares, passes);
+    const int b1 = b, s1 = s;
+    if (then.end > 0) {
+      b = then.token / p.seq;
+      s = then.token - b * p.seq;
+      pos = token_position(p.angles, o, then.token, p.tokens);
+    }
+    for (int pass = now.pass; pass < now.end; ++pass) {
+      const Chunks c = next;
+      if (pass + 1 < now.end) {
+        if (live || pass + 1 < q_passes) load(b1, s1, pass + 1, next);
+      } else if (then.end > 0) {
+        load(b, s, then.pass, next);
+      }
+      const int which = tensor(pass), h = head(pass, which);
+      if (h >= (which == 0 ? p.hq : p.hkv) || !(which == 0 || live)) continue;
+      uint16_t* row = which == 0 ? p.q_out + (static_cast<int64_t>(now.token) * p.hq + h) * kD
+                                 : (which == 1 ? p.k_out : p.v_out) + (at * p.hkv + h) * kD;
+      if (which == 2) {
+        store_chunks<kStream>(row, o, c);
         continue;
       }
       float x[16];
       unpack(c, x);
-      if ((is_q ? p.q_weight : p.k_weight) != nullptr) {
+      if ((which == 0 ? p.q_weight : p.k_weight) != nullptr) {
+        float w[16];
+        load_weights(s_weight[which], o, w);
         const float r = row_scale(x, p.eps);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = x[i] * r * (is_q ? wq[i] : wk[i]);
+        for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
       }
-      rotate<kPairs, false>(o, t, x);
-      store_row(is_q ? p.q_out + (token * p.hq + h) * kD : p.k_out + (at * p.hkv + h) * kD, o, x);
+      rotate<kPairs, false>(o, s_turn[wave], lane, x);
+      store_row<kStream>(row, o, x);
     }
+    now = then;
   }
 }
 
@@ -280,45 +381,78 @@ struct BackwardParams {
   uint16_t* dx[2];
   float* part[2];               // [workgroups][128] sums of g u, or null
   int heads[2], groups[2];      // workgroups of each tensor
+  Shares shares[2];
   int weight_bf16;
   float eps;
   int seq, tokens;
 };
 
-// The first groups[0] workgroups take q's rows, the others k's.
-template <bool kPairs>
-__global__ __launch_bounds__(64 * kWaves) void rotary_backward_kernel(const BackwardParams p) {
+// The first groups[0] workgroups take q's rows, the others k's; a wave's loop is the
+// forward's.
+template <bool kPairs, bool kStreamIn, bool kStreamOut>
+__global__ __launch_bounds__(64 * kWaves, kBackPerCu) void rotary_backward_kernel(const BackwardParams p) {
   __shared__ float s_turn[kWaves][2][64];
+  __shared__ float s_weight[kD];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int which = static_cast<int>(blockIdx.x) < p.groups[0] ? 0 : 1;
   const int group = blockIdx.x - (which ? p.groups[0] : 0);
   const Rows in = p.x[which];
+  const uint16_t* grad = p.grad[which];
   const void* weight = p.weight[which];
   float* part = p.part[which];
   const int heads = p.heads[which], passes = (heads + kRowsAtOnce - 1) / kRowsAtOnce;
-  const Lane o = lane_setup<kPairs>(p.angles, lane);
-  float w[16], dw[16];
-  load_weights(weight, p.weight_bf16, o, w);
+  Lane o = lane_setup<kPairs>(p.angles, lane);
+  struct Both {
+    Chunks g, x;
+  };
+  auto load = [&](int token, int b, int s, int pass, Both& c) {
+    const int h = pass * kRowsAtOnce + (lane >> 3);
+    if (h >= heads) return;
+    load_chunks<kStreamIn>(grad + (static_cast<int64_t>(token) * heads + h) * kD, o, c.g);
+    if (weight != nullptr) load_chunks<kStreamIn>(in.p + b * in.sb + s * in.ss + h * in.sh, o, c.x);
+  };
+  float dw[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) dw[i] = 0.f;
-  for (int64_t token = group * kWaves + wave; token < p.tokens; token += p.groups[which] * kWaves) {
-    const int b = static_cast<int>(token) / p.seq, s = static_cast<int>(token) - b * p.seq;
-    Turn t;
-    token_turn(p.angles, o, static_cast<int>(token), p.tokens, lane, s_turn[wave], t);
-    for (int pass = 0; pass < passes; ++pass) {
+  const Shares& shares = p.shares[which];
+  Walk walk = walk_of(shares, group * kWaves + wave, passes);
+  Part now = advance(walk, shares, passes);
+  int b = 0, s = 0, pos = 0;
+  Both next;
+  if (now.end > 0) {
+    b = now.token / p.seq;
+    s = now.token - b * p.seq;
+    load(now.token, b, s, now.pass, next);
+    pos = token_position(p.angles, o, now.token, p.tokens);
+  }
+  if (tid < kD) stage_weights(weight, p.weight_bf16, tid, s_weight);
+  lane_turns(p.angles, lane, o);
+  __syncthreads();
+  while (now.end > 0) {
+    token_turn(o, pos, lane, s_turn[wave]);
+    const Part then = advance(walk, shares, passes);
+    const int b1 = b, s1 = s;
+    if (then.end > 0) {
+      b = then.token / p.seq;
+      s = then.token - b * p.seq;
+      pos = token_position(p.angles, o, then.token, p.tokens);
+    }
+    for (int pass = now.pass; pass < now.end; ++pass) {
+      const Both c = next;
+      if (pass + 1 < now.end)
+        load(now.token, b1, s1, pass + 1, next);
+      else if (then.end > 0)
+        load(then.token, b, s, then.pass, next);
       const int h = pass * kRowsAtOnce + (lane >> 3);
       if (h >= heads) continue;
-      const int64_t row = (token * heads + h) * kD;
-      Chunks cg, cx;
-      load_chunks(p.grad[which] + row, o, cg);
-      if (weight != nullptr) load_chunks(in.p + b * in.sb + s * in.ss + h * in.sh, o, cx);
       float g[16];
-      unpack(cg, g);
-      rotate<kPairs, true>(o, t, g);
+      unpack(c.g, g);
+      rotate<kPairs, true>(o, s_turn[wave], lane, g);
       if (weight != nullptr) {
-        float u[16];
-        unpack(cx, u);
+        float u[16], w[16];
+        unpack(c.x, u);
+        load_weights(s_weight, o, w);
         const float r = row_scale(u, p.eps);
         float dot = 0.f;
 #pragma unroll
@@ -332,8 +466,9 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_backward_kernel(const Back
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] = r * __builtin_fmaf(-u[i], dot, g[i]);
       }
-      store_row(p.dx[which] + row, o, g);
+      store_row<kStreamOut>(p.dx[which] + (static_cast<int64_t>(now.token) * heads + h) * kD, o, g);
     }
+    now = then;
   }
   if (part == nullptr) return;   // uniform
   // Sums over the wave's eight rows, then over the waves.
@@ -390,19 +525,24 @@ int cus() {
   return n;
 }
 
-constexpr int kGroupsPerCu = 8;    // workgroups of a rotation, at most
-constexpr int kBackPerCu = 4;      // and of its backward
 
 int64_t passes_of(int64_t heads) { return (heads + kRowsAtOnce - 1) / kRowsAtOnce; }
+
+Shares shares_of(int64_t tokens, int64_t passes, int64_t groups) {
+  const int64_t waves = groups * kWaves, rounds = tokens / waves, left = (tokens - rounds * waves) * passes;
+  return Shares{static_cast<int>(waves), static_cast<int>(rounds), left / waves, static_cast<int>(left % waves)};
+}
 
 // Workgroups of the backward for q and for k: as their rows, at least one each.
 void backward_groups(int64_t tokens, int64_t hq, int64_t hkv, int (&groups)[2]) {
   const int64_t pq = passes_of(hq), pk = passes_of(hkv), most = int64_t{kBackPerCu} * cus();
-  const int64_t need = (tokens + kWaves - 1) / kWaves;   // of one tensor
   const int64_t q = most * pq / (pq + pk), k = most - q;
-  auto within = [&](int64_t x) { return static_cast<int>(x < 1 ? 1 : x > need ? need : x); };
-  groups[0] = within(q);
-  groups[1] = within(k);
+  auto within = [&](int64_t x, int64_t passes) {
+    const int64_t need = (tokens * passes + kWaves - 1) / kWaves;
+    return static_cast<int>(x < 1 || need < 1 ? 1 : x > need ? need : x);
+  };
+  groups[0] = within(q, pq);
+  groups[1] = within(k, pk);
 }
 
 bool rows_ok(const void* p, const int64_t* strides, Rows& out) {
@@ -437,21 +577,25 @@ int check_angles(const std::string& n, const int32_t* positions, const void* inv
   return SWATTN_OK;
 }
 
-// Grid and waves per token: a wave per token where tokens fill the chip's waves, else
-// its head rows are shared out over up to four (64 tokens of 48 rows: see the launch).
+// A pass per wave, or equal shares of the waves that the chip takes at once.
 template <bool kAppend>
 int launch_rotary(const char* name, bool pairs, RotaryParams& p, void* stream) {
   if (p.tokens == 0 && !kAppend) return SWATTN_OK;
-  const int64_t most = int64_t{kGroupsPerCu} * cus();
   const int64_t passes = passes_of(p.hq) + (kAppend ? 2 : 1) * passes_of(p.hkv);
-  p.per_token = 1;
-  while (p.per_token < kWaves && p.per_token * 2 <= passes && int64_t{p.tokens} * p.per_token * 2 <= most) p.per_token *= 2;
-  const int64_t groups = (int64_t{p.tokens} * p.per_token + kWaves - 1) / kWaves;
-  const dim3 grid(static_cast<uint32_t>(groups < 1 ? 1 : groups < most ? groups : most));
-  if (pairs)
-    hipLaunchKernelGGL((rotary_kernel<true, kAppend>), grid, dim3(64 * kWaves), 0, as_stream(stream), p);
+  const int64_t most = int64_t{kGroupsPerCu} * cus(), need = (p.tokens * passes + kWaves - 1) / kWaves;
+  const int64_t groups = need < 1 ? 1 : need < most ? need : most;
+  p.shares = shares_of(p.tokens, passes, groups);
+  const dim3 grid(static_cast<uint32_t>(groups));
+  const bool stream_past = p.tokens * (p.hq + (kAppend ? 2 : 1) * int64_t{p.hkv}) * (4 * kD) >= kStreamBytes;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, as_stream(stream), p); };
+  if (pairs && stream_past)
+    launch(rotary_kernel<true, kAppend, true>);
+  else if (pairs)
+    launch(rotary_kernel<true, kAppend, false>);
+  else if (stream_past)
+    launch(rotary_kernel<false, kAppend, true>);
   else
-    hipLaunchKernelGGL((rotary_kernel<false, kAppend>), grid, dim3(64 * kWaves), 0, as_stream(stream), p);
+    launch(rotary_kernel<false, kAppend, false>);
   return launch_status(name);
 }
 
@@ -586,11 +730,25 @@ int swattn_rotary_bwd(const void* grad_q, const void* grad_k, const void* q, con
   p.eps = eps;
   p.seq = static_cast<int>(seq);
   p.tokens = static_cast<int>(tokens);
+  p.shares[0] = shares_of(tokens, passes_of(heads_q), p.groups[0]);
+  p.shares[1] = shares_of(tokens, passes_of(heads_kv), p.groups[1]);
   const dim3 grid(static_cast<uint32_t>(p.groups[0] + p.groups[1]));
-  if (interleaved)
-    hipLaunchKernelGGL(rotary_backward_kernel<true>, grid, dim3(64 * kWaves), 0, as_stream(stream), p);
+  const int64_t rows = tokens * (int64_t{heads_q} + heads_kv) * (2 * kD);   // bytes of one set of rows
+  const int64_t read = tokens * 2 * kD * (heads_q * (q_weight != nullptr ? 2 : 1) + heads_kv * int64_t{k_weight != nullptr ? 2 : 1});
+  const bool out = read + rows >= kStreamBytes, in = read >= kCacheBytes;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, as_stream(stream), p); };
+  if (interleaved && in)
+    launch(rotary_backward_kernel<true, true, true>);
+  else if (interleaved && out)
+    launch(rotary_backward_kernel<true, false, true>);
+  else if (interleaved)
+    launch(rotary_backward_kernel<true, false, false>);
+  else if (in)
+    launch(rotary_backward_kernel<false, true, true>);
+  else if (out)
+    launch(rotary_backward_kernel<false, false, true>);
   else
-    hipLaunchKernelGGL(rotary_backward_kernel<false>, grid, dim3(64 * kWaves), 0, as_stream(stream), p);
+    launch(rotary_backward_kernel<false, false, false>);
   if (sums) {
     const SumParams s{{p.part[0], p.part[1]}, {dq_weight, dk_weight}, {p.groups[0], p.groups[1]}, weight_bf16};
     hipLaunchKernelGGL(rotary_sum_kernel, dim3(kD / kSumDims, 2), dim3(256), 0, as_stream(stream), s);

@@ -98,6 +98,36 @@ def test_far_positions(dtype):
         _check_rows(c, name, x, False, 1e-6)
 
 
+@pytest.mark.parametrize("tokens,heads", [(5119, (1, 1)), (5120, (9, 1)), (5121, (1, 9)), (6000, (3, 2)), (10241, (17, 1))])
+def test_tokens_shared_out_over_the_waves(tokens, heads):
+    """Whole rounds of tokens, and what is left of them, to every token's last row; calls large
+    enough to go past the memory-side cache are tested by the sizes below."""
+    c = _case(12, 1, tokens, *heads, n=8)
+    got = switch_qk_rotary_forward(_up(c["q"]), _up(c["k"]), _up(c["pos"]), _up(c["freq"]), **_how(c, False, 1e-6))
+    for name, x in zip("qk", got):
+        _check_rows(c, name, x, False, 1e-6)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,weights", [(6001, F32), (6001, None), (17001, F32)])
+def test_large_calls_as_small_ones(tokens, weights, interleaved):
+    """Calls of 100 MB and more, streamed, against the same rows in small calls."""
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    q, k, gq, gk = (torch.randn(1, tokens, h, 128, generator=gen, device=DEV).to(BF16) for h in (32, 8, 32, 8))
+    c = _case(13, 1, tokens, 1, 1, weights=weights)
+    how, pos, freq = _how(c, interleaved, 1e-6), _up(c["pos"]), _up(c["freq"])
+    got = switch_qk_rotary_forward(q, k, pos, freq, **how)
+    grads = switch_qk_rotary_backward(gq, gk, q, k, pos, freq, **how)
+    kc, vc = (torch.zeros(1, tokens, 8, 128, dtype=BF16, device=DEV) for _ in range(2))
+    switch_qk_rotary_append(q, k, k, kc, vc, _int32([0]), pos, freq, **how)
+    assert torch.equal(kc, got[1]) and torch.equal(vc, k)
+    for i in range(0, tokens, 2500):
+        s = slice(i, i + 2500)
+        part = switch_qk_rotary_forward(q[:, s], k[:, s], pos[..., s].contiguous(), freq, **how)
+        dx = switch_qk_rotary_backward(gq[:, s], gk[:, s], q[:, s], k[:, s], pos[..., s].contiguous(), freq, **how)
+        assert all(torch.equal(a[:, s], b) for a, b in zip(got + grads[:2], part + dx[:2]))
+
+
 def test_one_weight_only():
     c = _case(6, 2, 5, 4, 2)
     for drop in ("qw", "kw"):
