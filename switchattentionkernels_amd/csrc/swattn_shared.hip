@@ -43,8 +43,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 128;       // query rows of a prefix tile, at most
 constexpr int kTileKeys = tiles::kBN;
-constexpr int kMaxGroups = 2 * SWATTN_SHARED_MAX_PREFIXES;   // (prefix, route)
-constexpr uint32_t kMinPiece = 128;  // keys of a prefix piece, at least
+constexpr uint32_t kMinPiece = 64;   // keys of a prefix piece, at least
 // What a key of a prefix tile costs, in 16ths of a key of the line.
 constexpr uint32_t kTileCost = 24;
 
@@ -72,6 +71,7 @@ struct SharedParams : DecodeCommon {
   int4* place;        // per sequence {first piece of KV head 0, pieces, first row, -}
   int prefixes, prefix_len;
   int tile_seqs;      // sequences of a tile, at most
+  uint32_t tile_inv;  // 2^20 / tile_seqs, rounded up
   int tile_rows;      // rows that a partial has room for
   uint32_t least;     // workgroups that take the line, at least
   float c;            // sm_scale * log2(e)
@@ -95,103 +95,130 @@ struct Piece {
   int base;                     // the group's first piece
 };
 
-struct Routes {   // of a thread's sequences
-  int group[kInlinePer], start[kInlinePer];   // group -1: attends no prefix row
-  int lo[kInlinePer], n[kInlinePer];          // own rows
+// A thread's sequences and prefixes: one of each, for up to 256 in a call, or four.  (The
+// plan is straight-line code that every launch fetches anew: B4, four 3.4 us, one 2.2.)
+template <int kPer>
+struct Routes {
+  int group[kPer], start[kPer];   // group -1: attends no prefix row
+  int lo[kPer], n[kPer];          // own rows
 };
 
-__device__ __forceinline__ int prefix_rows(const SharedParams& p, int prefix) {
-  return min(max(p.prefix_lens[prefix], 0), p.prefix_len);
-}
+// The plan's LDS words of the prefixes: rows, sequences that attend them (routed full in the
+// low 16 bits, local in the high ones), and the first key that a local one attends.
+template <int kPer>
+struct PrefixWords {
+  int rows[256 * kPer];
+  uint32_t seqs[256 * kPer];
+  int first[256 * kPer];
+};
+constexpr int kMostPer = SWATTN_SHARED_MAX_PREFIXES / 256;
+static_assert(kMostPer == kInlinePer && SWATTN_SHARED_MAX_SEQS == kInlineSeqs, "as many prefixes as sequences");
 
-__device__ __forceinline__ void routes_of(const SharedParams& p, int per, Routes& r) {
+// What a thread's sequences attend; lengths, routes and prefixes are loaded at once.
+template <int kPer>
+__device__ __forceinline__ void routes_of(const SharedParams& p, int per, PrefixWords<kPer>& s, Routes<kPer>& r) {
+  int id[kPer];
+  bool full[kPer];
 #pragma unroll
-  for (int j = 0; j < kInlinePer; ++j) {
+  for (int j = 0; j < kPer; ++j) {
     const int b = static_cast<int>(threadIdx.x) * per + j;
-    r.group[j] = -1;
-    r.start[j] = r.lo[j] = r.n[j] = 0;
+    id[j] = -1;
+    full[j] = false;
+    r.lo[j] = r.n[j] = 0;
     if (j >= per || b >= p.batch) continue;
     key_range(p, b, r.lo[j], r.n[j]);
-    const int id = p.prefix_ids[b];
-    if (id < 0 || id >= p.prefixes) continue;
-    const int rows = prefix_rows(p, id), len = r.lo[j] + r.n[j];
-    const bool full = p.full[b] != 0;
-    r.start[j] = full ? 0 : max(rows - max(p.window - len, 0), 0);
-    if (r.start[j] < rows) r.group[j] = 2 * id + (full ? 0 : 1);
+    id[j] = p.prefix_ids[b];
+    full[j] = p.full[b] != 0;
+  }
+  for (int i = threadIdx.x; i < p.prefixes; i += 256) {
+    s.rows[i] = min(max(p.prefix_lens[i], 0), p.prefix_len);
+    s.seqs[i] = 0;
+    s.first[i] = INT_MAX;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    r.group[j] = -1;
+    r.start[j] = 0;
+    if (id[j] < 0 || id[j] >= p.prefixes) continue;
+    const int rows = s.rows[id[j]], len = r.lo[j] + r.n[j];
+    r.start[j] = full[j] ? 0 : max(rows - max(p.window - len, 0), 0);
+    if (r.start[j] >= rows) continue;
+    r.group[j] = 2 * id[j] + (full[j] ? 0 : 1);
+    atomicAdd(&s.seqs[id[j]], full[j] ? 1u : 1u << 16);
+    if (!full[j]) atomicMin(&s.first[id[j]], r.start[j]);
   }
 }
 
 // The workgroup's part: a prefix piece (true), or a share of the line (false; st.take 0
-// past its end).  s_counts: LDS words for the groups' sequences, and the local groups'
-// first keys.
-__device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes& r, int per, int* s_counts, int* s_first,
+// past its end).
+template <int kPer>
+__device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<kPer>& r, int per, const PrefixWords<kPer>& s,
                                             SeqEntry* s_ent, Piece& piece, SplitStart& st, uint32_t& wg) {
   __shared__ Piece s_piece;
   __shared__ SplitStart s_start;
   const int tid = threadIdx.x;
-  const int groups = 2 * p.prefixes, gper = (groups + 255) >> 8;
-  for (int g = tid; g < groups; g += 256) {
-    s_counts[g] = 0;
-    s_first[g] = g & 1 ? INT_MAX : 0;
-  }
-  __syncthreads();
   uint32_t keys = 0, cnt = 0;
 #pragma unroll
-  for (int j = 0; j < kInlinePer; ++j) {
+  for (int j = 0; j < kPer; ++j) {
     keys += r.n[j];
     cnt += r.n[j] > 0 ? 1 : 0;
-    if (r.group[j] >= 0) {
-      atomicAdd(&s_counts[r.group[j]], 1);
-      if (r.group[j] & 1) atomicMin(&s_first[r.group[j]], r.start[j]);
-    }
   }
   uint32_t before, rank, all_keys, all_cnt;
   scan_keys<4, 0, uint32_t>(keys, cnt, before, rank, all_keys, all_cnt);   // (its barrier orders the atomics too)
   const uint32_t line = (all_keys + all_cnt * p.pad) * p.hkv;
-  // Positions of all prefix tiles; this thread's groups: tid * gper and on.
-  auto tiles_of = [&](int g) { return static_cast<uint32_t>((s_counts[g] + p.tile_seqs - 1) / p.tile_seqs); };
-  auto keys_of = [&](int g) { return static_cast<uint32_t>(prefix_rows(p, g >> 1) - s_first[g]); };
-  uint32_t positions = 0, tile_cnt = 0, unused0, unused1, all_positions, all_tiles;
-  for (int i = 0; i < gper; ++i) {
-    const int g = tid * gper + i;
-    if (g < groups && s_counts[g] > 0) {
-      positions += tiles_of(g) * keys_of(g);
-      tile_cnt += tiles_of(g);
-    }
+  // This thread's groups, (prefix, route), in order: sequences, tiles, keys.
+  const int pper = kPer == 1 ? 1 : (p.prefixes + 255) >> 8;
+  struct Group {
+    uint32_t seqs, tiles, first, keys;
+  };
+  Group g[2 * kPer];
+  uint32_t positions = 0, all_positions, unused0, unused1, unused2;
+#pragma unroll
+  for (int i = 0; i < 2 * kPer; ++i) {
+    const int x = tid * pper + i / 2;
+    g[i] = Group{0, 0, 0, 0};
+    if (i / 2 >= pper || x >= p.prefixes) continue;
+    g[i].seqs = i & 1 ? s.seqs[x] >> 16 : s.seqs[x] & 0xffffu;
+    if (g[i].seqs == 0) continue;
+    g[i].tiles = ((g[i].seqs + p.tile_seqs - 1) * p.tile_inv) >> 20;   // below 2^11 by 2^16: exact
+    g[i].first = i & 1 ? s.first[x] : 0;
+    g[i].keys = static_cast<uint32_t>(s.rows[x]) - g[i].first;
+    positions += g[i].tiles * g[i].keys;
   }
-  scan_keys<4, 1, uint32_t>(positions, tile_cnt, unused0, unused1, all_positions, all_tiles);
+  scan_keys<4, 1, uint32_t>(positions, 0, unused0, unused1, all_positions, unused2);
   // Equal shares of the whole cost, and the keys of a piece at that; a tile is spread
   // over at most 255 pieces.
   const uint64_t cost = line + (static_cast<uint64_t>(all_positions) * p.hkv * kTileCost + 15u) / 16u;
-  const uint32_t share = static_cast<uint32_t>((cost + p.target - 1) / p.target);
+  const uint32_t share = quotient(cost + p.target - 1, p.target);
   const uint32_t by_len = (static_cast<uint32_t>(p.prefix_len) + 254u) / 255u;
   const uint32_t length = (max(max((share * 16u + kTileCost - 1u) / kTileCost, by_len), kMinPiece) + kTileKeys - 1u) & ~(kTileKeys - 1u);
-  auto length_of = [&](uint32_t n) {   // equal pieces, whole tiles of keys
-    const uint32_t parts = (n + length - 1u) / length;
-    return ((n + parts - 1u) / parts + kTileKeys - 1u) & ~(kTileKeys - 1u);
-  };
-  uint32_t pieces = 0, base, all_pieces;
-  for (int i = 0; i < gper; ++i) {
-    const int g = tid * gper + i;
-    if (g < groups && s_counts[g] > 0) {
-      const uint32_t n = keys_of(g), l = length_of(n);
-      pieces += tiles_of(g) * p.hkv * ((n + l - 1u) / l);
-    }
+  uint32_t pieces = 0, base, all_pieces, parts[2 * kPer], len[2 * kPer];
+#pragma unroll
+  for (int i = 0; i < 2 * kPer; ++i) {
+    parts[i] = len[i] = 0;
+    if (g[i].seqs == 0) continue;
+    const uint32_t n = (g[i].keys + length - 1u) / length;   // equal pieces, whole tiles of keys
+    len[i] = ((g[i].keys + n - 1u) / n + kTileKeys - 1u) & ~(kTileKeys - 1u);
+    parts[i] = (g[i].keys + len[i] - 1u) / len[i];
+    pieces += g[i].tiles * p.hkv * parts[i];
   }
   scan_keys<4, 2, uint32_t>(pieces, 0, base, unused0, all_pieces, unused1);
   const uint32_t block = blockIdx.x;
   if (block < all_pieces) {   // uniform
-    for (int i = 0; i < gper; ++i) {
-      const int g = tid * gper + i;
-      if (g >= groups || s_counts[g] == 0) continue;
-      const uint32_t n = keys_of(g), l = length_of(n), parts = (n + l - 1u) / l, here = tiles_of(g) * p.hkv * parts;
-      if (block >= base && block - base < here) {
-        const uint32_t at = block - base, pair = at / parts, tile = pair / p.hkv;
-        s_piece = Piece{g, static_cast<int>(tile), static_cast<int>(pair - tile * p.hkv), static_cast<int>(at - pair * parts),
-                        static_cast<int>(parts), static_cast<int>(l), s_first[g], s_first[g] + static_cast<int>(n),
-                        s_counts[g], static_cast<int>(base)};
+    if (block - base < pieces) {
+#pragma unroll
+      for (int i = 0; i < 2 * kPer; ++i) {
+        const uint32_t here = g[i].tiles * p.hkv * parts[i];
+        if (block - base < here) {
+          const uint32_t at = block - base, pair = at / parts[i], tile = pair / p.hkv;
+          s_piece = Piece{2 * (tid * pper + i / 2) + (i & 1), static_cast<int>(tile), static_cast<int>(pair - tile * p.hkv),
+                          static_cast<int>(at - pair * parts[i]), static_cast<int>(parts[i]), static_cast<int>(len[i]),
+                          static_cast<int>(g[i].first), static_cast<int>(g[i].first + g[i].keys), static_cast<int>(g[i].seqs),
+                          static_cast<int>(base)};
+        }
+        base += here;
       }
-      base += here;
     }
     __syncthreads();
     piece = s_piece;
@@ -206,14 +233,14 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes&
   if (L.aligned) {
     uint32_t len = 0, none;
 #pragma unroll
-    for (int j = 0; j < kInlinePer; ++j) len += L.length(r.n[j], 0);
+    for (int j = 0; j < kPer; ++j) len += L.length(r.n[j], 0);
     scan_keys<4, 3, uint32_t>(len, 0, before, none, L.total, none);
     L.total *= p.hkv;
   }
   const uint64_t pos64 = static_cast<uint64_t>(wg) * L.share;
   const uint32_t pos = static_cast<uint32_t>(min(pos64, static_cast<uint64_t>(L.total)));
 #pragma unroll
-  for (int j = 0; j < kInlinePer; ++j) {
+  for (int j = 0; j < kPer; ++j) {
     const int b = tid * per + j;
     const uint32_t off = before * p.hkv, len = L.length(r.n[j], p.pad);
     if (wg == 0 && j < per && b < p.batch) {
@@ -242,15 +269,27 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes&
 constexpr int kSlotBytes = 2 * tiles::kTileBytes;
 __device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, uint32_t row_bytes, int key, int last,
                                           uint32_t lds, int wave, int lane) {
-  asm volatile("" : "+v"(lane));   // offsets are made anew each time: kept, they spill, and a reload waits for the copies
-  const int64_t at = static_cast<int64_t>(key) * (row_bytes / 2);   // the tile's rows span less than 2^31 bytes
-  const int chunk = (lane & 15) ^ ((lane >> 4) << 2);               // of row 4 i + lane / 16: ^ i
+  const int64_t at = static_cast<int64_t>(key + 16 * wave) * (row_bytes / 2);
+  const uint32_t chunk = 16u * ((lane & 15) ^ ((lane >> 4) << 2));   // of row 4 i + lane / 16: ^ 16 i
+  uint32_t row = (lane >> 4) * row_bytes;   // a tile's rows span less than 2^31 bytes
+  lds += 4096u * static_cast<uint32_t>(wave);
+  if (key + kTileKeys - 1 <= last) {   // uniform
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t off = static_cast<uint32_t>(min(16 * wave + 4 * i + (lane >> 4), last - key)) * row_bytes + 16u * (chunk ^ i);
-    const uint32_t to = lds + 1024u * static_cast<uint32_t>(4 * wave + i);
-    tiles::dma16_from(kb + at, off, to);
-    tiles::dma16_from(vb + at, off, to + tiles::kTileBytes);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t to = at + static_cast<int64_t>(4 * i) * (row_bytes / 2);
+      const uint32_t off = (chunk ^ (16u * i)) + row;
+      tiles::dma16_from(kb + to, off, lds + 1024u * i);
+      tiles::dma16_from(vb + to, off, lds + 1024u * i + tiles::kTileBytes);
+    }
+  } else {
+    const int rest = last - key - 16 * wave;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // Rows count from the wave's first, or back from it to the last one.
+      const int64_t off = static_cast<int64_t>(min(4 * i + (lane >> 4), rest)) * static_cast<int64_t>(row_bytes) + (chunk ^ (16u * i));
+      tiles::dma16_gather(reinterpret_cast<const char*>(kb + at) + off, lds + 1024u * i);
+      tiles::dma16_gather(reinterpret_cast<const char*>(vb + at) + off, lds + 1024u * i + tiles::kTileBytes);
+    }
   }
 }
 
@@ -493,18 +532,34 @@ __device__ __forceinline__ void careful_step(const char* vt, const LaneLds& at_l
 }
 
 // One workgroup: piece `part` of a tile's keys, for KV head kvh.
-__device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes& routes, int per, const Piece& x,
+template <int kPer>
+__device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes<kPer>& routes, int per, const Piece& x,
                                              int2* s_rows, char* ring) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int k0 = uniform(x.first + x.part * x.length), k1 = min(k0 + uniform(x.length), uniform(x.end));
+  const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * tiles::kRowBytes;
+  const int64_t base = (static_cast<int64_t>(uniform(x.group) >> 1) * p.prefix_len * p.hkv + uniform(x.kvh)) * kD;
+  const int last = uniform(x.end) - 1;
+  const uint16_t *kb = p.prefix_k + base, *vb = p.prefix_v + base;
+  const uint32_t lds = tiles::lds_addr(ring);
+  const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
+  auto copy = [&](int j) {
+    copy_tile(kb, vb, row_bytes, k0 + kTileKeys * j, last, lds + (j & 1) * kSlotBytes, wave, lane);
+  };
+  auto copy_first = [&]() {
+    copy(0);
+    if (steps > 1) copy(1);
+  };
+  copy_first();
   // The tile's sequences, in order.
   uint32_t cnt = 0, rank, unused0, unused1, unused2;
 #pragma unroll
-  for (int j = 0; j < kInlinePer; ++j) cnt += routes.group[j] == x.group ? 1 : 0;
+  for (int j = 0; j < kPer; ++j) cnt += routes.group[j] == x.group ? 1 : 0;
   scan_keys<4, 4, uint32_t>(0, cnt, unused0, rank, unused1, unused2);
   const int first_seq = x.tile * p.tile_seqs, seqs = min(x.seqs - first_seq, p.tile_seqs);
 #pragma unroll
-  for (int j = 0; j < kInlinePer; ++j) {
+  for (int j = 0; j < kPer; ++j) {
     if (routes.group[j] != x.group) continue;
     const int at = static_cast<int>(rank++) - first_seq, b = tid * per + j;
     if (at < 0 || at >= seqs) continue;
@@ -512,15 +567,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     if (x.kvh == 0 && x.part == 0)
       p.place[b] = make_int4(x.base + x.tile * p.hkv * x.parts, x.parts, at * p.group, 0);
   }
-  const int k0 = uniform(x.first + x.part * x.length), k1 = min(k0 + uniform(x.length), uniform(x.end));
-  const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
-  const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * tiles::kRowBytes;
-  const int64_t base = (static_cast<int64_t>(uniform(x.group) >> 1) * p.prefix_len * p.hkv + uniform(x.kvh)) * kD;
-  const int last = uniform(x.end) - 1;
-  const uint16_t *kb = p.prefix_k + base, *vb = p.prefix_v + base;
-  const uint32_t lds = tiles::lds_addr(ring);
-  __syncthreads();   // the rows; the ring was the plan's
-  copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
+  __syncthreads();   // the rows
   // This lane's row.
   const int rows = seqs * p.group, row = 32 * wave + (lane & 31), h = lane >> 5;
   const bool mine = row < rows, busy = 32 * wave < rows;   // busy: uniform
@@ -553,8 +600,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
     int j = 0;
     auto arrive = [&]() {   // tile j is there, and every wave is done with the one before
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (j + 1 < steps)
-        copy_tile(kb, vb, row_bytes, k0 + kTileKeys * (j + 1), last, lds + ((j + 1) & 1) * kSlotBytes, wave, lane);
+      if (j > 0 && j + 1 < steps) copy(j + 1);
       return static_cast<uint32_t>(j & 1) * kSlotBytes;
     };
     // What this row attends of tile j.
@@ -587,7 +633,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(w.acc[d][i], 0.f, sum);
     if (!__syncthreads_or(mine && sum != 0.f)) break;
-    copy_tile(kb, vb, row_bytes, k0, last, lds, wave, lane);
+    copy_first();
   }
   if (!mine) return;
   w.l = w.l + __shfl_xor(w.l, 32);
@@ -641,6 +687,12 @@ __device__ __forceinline__ void careful_piece(const uint16_t* q, const uint16_t*
   }
 }
 
+template <bool kStream>
+__device__ __forceinline__ u32x4 load16(const uint16_t* p) {
+  const u32x4* at = reinterpret_cast<const u32x4*>(p);
+  return kStream ? __builtin_nontemporal_load(at) : *at;
+}
+
 // One share of the line: its pairs one after the other, a piece of each.  A wave takes 32
 // keys at once, steps w, w + 4, ... of a piece; rows outside it are read as its nearest
 // row and masked.
@@ -653,6 +705,7 @@ __device__ __forceinline__ void careful_piece(const uint16_t* q, const uint16_t*
 // A piece's partial lies in slot wg + (pair's rank): both only grow along the line, one of
 // them at every step from piece to piece, so that no two pieces share a slot and a pair's
 // slots are consecutive.
+template <bool kStream>
 __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, const SplitStart& st, const SeqEntry* s_ent,
                                            PieceLds& lds) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -690,11 +743,11 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
         for (int t = 0; t < 2; ++t) {
           const uint16_t* row = kb + min(at + 16 * t + c, k1 - 1) * stride;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) kr[t][j] = *reinterpret_cast<const u32x4*>(row + 32 * j);
+          for (int j = 0; j < 4; ++j) kr[t][j] = load16<kStream>(row + 32 * j);
         }
 #pragma unroll
         for (int t = 0; t < 8; ++t)
-          vr[t] = *reinterpret_cast<const u32x4*>(vb + min(at + 16 * (t >> 2) + 4 * g + (t & 3), k1 - 1) * stride);
+          vr[t] = load16<kStream>(vb + min(at + 16 * (t >> 2) + 4 * g + (t & 3), k1 - 1) * stride);
       };
       load(wave);
       float m = -INFINITY, l = 0.f;   // column c's maximum, and this lane's share of its sum
@@ -809,27 +862,27 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
   }
 }
 
-// The plan's words, a line share's entries and partials, or a ring of two tiles of K and V.
-constexpr int kEntOffset = 2 * kMaxGroups * static_cast<int>(sizeof(int));
-constexpr int kPieceOffset = kEntOffset + kInlineSeqs * static_cast<int>(sizeof(SeqEntry));
+// A line share's entries and partials, or a ring of two tiles of K and V.
+constexpr int kPieceOffset = kInlineSeqs * static_cast<int>(sizeof(SeqEntry));
 constexpr int kLdsBytes = 2 * kSlotBytes;
 static_assert(kPieceOffset + sizeof(PieceLds) <= kLdsBytes, "a share's words fit the ring");
 
+template <int kPer, bool kStream>
 __global__ __launch_bounds__(256, 2) void shared_split_kernel(const SharedParams p) {
   __shared__ __align__(1024) char s_mem[kLdsBytes];
+  __shared__ PrefixWords<kPer> s_prefix;
   __shared__ int2 s_rows[kTileRows];
-  const int per = (p.batch + 255) >> 8;
-  Routes routes;
-  routes_of(p, per, routes);
+  const int per = kPer == 1 ? 1 : (p.batch + 255) >> 8;
+  Routes<kPer> routes;
+  routes_of(p, per, s_prefix, routes);
   Piece piece;
   SplitStart st;
   uint32_t wg = 0;
-  int* counts = reinterpret_cast<int*>(s_mem);
-  SeqEntry* ent = reinterpret_cast<SeqEntry*>(s_mem + kEntOffset);
-  if (plan_shared(p, routes, per, counts, counts + kMaxGroups, ent, piece, st, wg))
+  SeqEntry* ent = reinterpret_cast<SeqEntry*>(s_mem);
+  if (plan_shared(p, routes, per, s_prefix, ent, piece, st, wg))
     prefix_piece(p, routes, per, piece, s_rows, s_mem);
   else if (st.take > 0)
-    own_pieces(p, wg, st, ent, *reinterpret_cast<PieceLds*>(s_mem + kPieceOffset));
+    own_pieces<kStream>(p, wg, st, ent, *reinterpret_cast<PieceLds*>(s_mem + kPieceOffset));
 }
 
 // One workgroup of 256 threads per output row: merge_row over the row's shares of the line
@@ -907,6 +960,10 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
 
 constexpr int kTarget = 2;         // workgroups per CU
 constexpr int kLineLeast = 8;      // of the target, the part that the line gets at least
+// Own rows are read past the 256 MB memory-side cache where it cannot hold caches and
+// prefixes: B64 of 1024 rows behind 8192 54.4 -> 51.7 us.  Smaller ones may still be there
+// from the last call: B40 of 777 rows 30.5 us, streamed 32.6.
+constexpr int64_t kStreamBytes = int64_t{256} << 20;
 
 int shared_cus() {
   int dev = 0, n = 0;
@@ -1021,11 +1078,23 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.prefixes = prefixes;
   p.prefix_len = static_cast<int>(prefix_len);
   p.tile_seqs = static_cast<int>(L.tile_seqs);
+  p.tile_inv = static_cast<uint32_t>((1u << 20) / L.tile_seqs + 1);
   p.tile_rows = static_cast<int>(L.tile_rows);
   p.least = static_cast<uint32_t>(L.least);
   const hipStream_t st = as_stream(stream);
   const dim3 grid(static_cast<uint32_t>(L.pieces + L.least));
-  hipLaunchKernelGGL(shared_split_kernel, grid, dim3(256), 0, st, p);
+  const bool stream_past = (batch * cache_len + prefixes * prefix_len) * heads_kv * (4 * kD) >= kStreamBytes;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p); };
+  if (batch > 256 || prefixes > 256) {
+    if (stream_past)
+      launch(shared_split_kernel<kMostPer, true>);
+    else
+      launch(shared_split_kernel<kMostPer, false>);
+  } else if (stream_past) {
+    launch(shared_split_kernel<1, true>);
+  } else {
+    launch(shared_split_kernel<1, false>);
+  }
   hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(batch * heads_q)), dim3(256), 0, st, p);
   return launch_status(name);
 }
