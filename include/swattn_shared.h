@@ -40,7 +40,8 @@ extern "C" {
  *                       device; 256-byte aligned
  * heads_q / heads_kv at most 8; batch up to SWATTN_SHARED_MAX_SEQS, prefixes 1 to
  * SWATTN_SHARED_MAX_PREFIXES; batch * cache_len * heads_kv and the prefix positions (see
- * the workspace query, which returns 0 for shapes that are refused) below 2^31.
+ * the workspace query, which returns 0 for shapes that are refused) below 2^31, batch *
+ * heads_q below 2^24.  scale_log2 is finite.
  */
 size_t swattn_shared_decode_workspace_bytes(int32_t batch, int64_t cache_len, int32_t prefixes,
                                             int64_t prefix_len, int32_t heads_q,

@@ -996,6 +996,9 @@ bool shared_layout(int64_t batch, int64_t cache_len, int64_t prefixes, int64_t p
   L.least = (L.target + kLineLeast - 1) / kLineLeast;
   L.slots = L.target + L.least + batch * hkv;
   L.pieces = L.target + tiles * hkv;
+  // A launch takes fewer than 2^32 threads: the merge 256 per output row (pieces are fewer, a
+  // pair's start and its keys being positions of the line).
+  if (batch * hq >= int64_t{1} << 24) return false;
   auto al = [](int64_t x) { return (x + 255) & ~int64_t{255}; };
   int64_t o = al(L.slots * group * kD * 4);
   L.off_ml = o;       o = al(o + L.slots * group * 2 * 4);
@@ -1034,6 +1037,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   if (heads_q % heads_kv) return invalid(n + ": heads_q must be a multiple of heads_kv");
   if (heads_q / heads_kv > kMaxG) return invalid(n + ": heads_q / heads_kv must be at most 8");
   if (window <= 0) return invalid(n + ": window must be positive");
+  if (!isfinite(scale_log2)) return invalid(n + ": scale_log2 must be finite");
   SharedLayout L;
   if (!shared_layout(batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, L))
     return invalid(n + ": batch, prefixes, heads_kv or the lengths too large");

@@ -211,6 +211,8 @@ def switch_gqa_decode_shared_forward(
     if window_size <= 0:
         raise ValueError("window_size must be positive")
     scale = (128 ** -0.5 if sm_scale is None else float(sm_scale)) * LOG2E
+    if not abs(scale) < 2.0 ** 127:
+        raise ValueError("sm_scale must be finite")
     call, how = _lib.native().shared_decode, (min(int(window_size), 2 ** 31 - 1), scale)
     try:
         out = call(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cache, cache_lens, full_mask,

@@ -144,6 +144,16 @@ def test_largest_batch_and_number_of_prefixes():
     _check(c, 50)
 
 
+@pytest.mark.parametrize("batch,prefixes", [(256, 256), (257, 3), (5, 257), (300, 700)])
+def test_plans_of_one_and_of_four_per_thread(batch, prefixes):
+    gen = torch.Generator().manual_seed(batch)
+    ids = torch.randint(-1, prefixes, (batch,), generator=gen).tolist()
+    ids[0], ids[-1] = 0, prefixes - 1
+    c = _case(18, [(11 * i) % 70 for i in range(prefixes)], 70, ids, [(5 * i) % 12 for i in range(batch)], 11, 4, 2,
+              [i % 3 != 1 for i in range(batch)])
+    _check(c, 20)
+
+
 def test_long_prefix_in_many_pieces():
     c = _case(9, [20000], 20011, [0, 0, 0], [7, 300, 2], 300, 4, 1, [True, True, False])
     _check(c, 5000)
@@ -313,6 +323,8 @@ def test_refusals():
         (ValueError, "prefix_lens", dict(prefix_lens=ok["cache_lens"])),
         (ValueError, "full_mask", dict(full_mask=ok["cache_lens"])),
         (ValueError, "window_size", dict(window_size=0)),
+        (ValueError, "sm_scale", dict(sm_scale=math.nan)),
+        (ValueError, "sm_scale", dict(sm_scale=-math.inf)),
     ]
     for kind, words, change in bad:
         with pytest.raises(kind, match=words):

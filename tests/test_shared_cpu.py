@@ -2,6 +2,7 @@
 workspace relies on, and the oracle."""
 
 import ctypes
+import math
 import os
 import re
 
@@ -28,11 +29,11 @@ def test_library_exports_what_the_header_declares():
 
 
 def _call(**change):
-    a = dict(dict(q=P, kp=P, kc=P, full=P, out=P, batch=2, cap=10, prefixes=1, plen=20, hq=8, hkv=2, dim=128, window=4,
+    a = dict(dict(q=P, kp=P, kc=P, full=P, out=P, batch=2, cap=10, prefixes=1, plen=20, hq=8, hkv=2, dim=128, window=4, scale=0.1,
                   ws=P, ws_bytes=1 << 40), **change)
     return _lib.lib().swattn_shared_decode_fwd(
         a["q"], a["kp"], P, P, P, a["kc"], P, P, a["full"], a["out"], P, a["batch"], a["cap"], a["prefixes"], a["plen"],
-        a["hq"], a["hkv"], a["dim"], a["window"], ctypes.c_float(0.1), a["ws"], a["ws_bytes"], None)
+        a["hq"], a["hkv"], a["dim"], a["window"], ctypes.c_float(a["scale"]), a["ws"], a["ws_bytes"], None)
 
 
 def _refused(status, words, code=-1):
@@ -82,11 +83,21 @@ def test_workspace_holds_every_part():
     assert L.swattn_shared_decode_workspace_bytes(1025, 100, 1, 100, 8, 8) == 0
 
 
+def test_launches_of_2_32_threads_are_refused():
+    """256 threads per output row (prefix pieces are fewer: positions below 2^31 leave 2^24 / 1.5)."""
+    size = _lib.lib().swattn_shared_decode_workspace_bytes
+    rows = 2 ** 24
+    assert size(1024, 1, 1, 1, rows // 1024, rows // 1024 // 8) == 0
+    assert size(1023, 1, 1, 1, rows // 1024, rows // 1024 // 8) > 0
+    for scale in (math.nan, math.inf, -math.inf):
+        _refused(_call(scale=scale), "scale_log2")
+
+
 def test_planned_pieces_stay_within_the_workspace():
     """The device's arithmetic for random lengths: no more pieces than the workspace and the
     grid hold, none empty, every key in one of them, shares of the line within theirs."""
     rng = np.random.default_rng(0)
-    target, cost16, least = 512, 10, 64
+    target, cost16, least = 512, 24, 64
     for _ in range(3000):
         g, hkv = int(rng.integers(1, 9)), int(rng.integers(1, 17))
         seqs = 128 // g
@@ -106,7 +117,7 @@ def test_planned_pieces_stay_within_the_workspace():
         positions = sum(t * n for t, n in groups)
         cost = line + -(-positions * hkv * cost16 // 16)
         share = -(-cost // target)
-        length = -(-max(-(-share * 16 // cost16), -(-plen // 255), 128) // 64) * 64
+        length = -(-max(-(-share * 16 // cost16), -(-plen // 255), 64) // 64) * 64
         pieces = 0
         for t, n in groups:
             parts = -(-n // length)
