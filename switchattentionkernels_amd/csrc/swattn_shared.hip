@@ -14,15 +14,29 @@
 //   one per workgroup.  K and V are read once per tile, 64 keys at a time, into LDS
 //   (global -> LDS DMA, double-buffered) and both products run on the matrix cores, a
 //   wave per 32 rows: S^T = K Q^T, and O^T = V^T P^T with V transposed by the LDS
-//   reads.  S^T's accumulator layout is P^T's operand layout.  P enters its product as two
-//   bf16 numbers, its value and what that leaves (17 bits; the prefill rounds P to one).
+//   reads.  S^T's accumulator layout is P^T's operand layout.
 // The first workgroups take prefix pieces, the others shares of the line; how many of
 // each is settled on the device by every workgroup for itself, from the lengths.
 //
+// P enters its product as two bf16 numbers, its value and what that leaves: 17 bits, for a
+// third of the matrix instructions (the prefill rounds P to one).  Of 524288 outputs over up to
+// 33792 keys 893 then differ from the exact value's rounding, by one last place, and 627 of a
+// plain evaluation in fp32; with one number B64 behind 32768 rows would take 17 us less.
+//
 // Local rows attend the last rows of their prefix only, each from its own start on.
-// Masked weights are 0 there, and V elements that are not finite, which 0 would turn
-// into NaN, are taken out of a masked tile's product and added key by key to the rows
-// that attend them.
+// Masked scores are -inf, their weights 0.  A piece whose sums are not finite runs again
+// carefully: values that are not finite, which a weight of 0 would turn into NaN, are
+// taken out of the products and added key by key to the rows that attend them.
+//
+// Measured (Hkv 8), as a large copy's 5.2 TB/s and a large matrix product's 1210 TFLOP/s go:
+// B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 51 us against 39 for its bytes,
+// own rows being read until 36 us of a split kernel of 43 (plan 2.2, merge and gap 7); B64 Hq64
+// behind 32768 rows, all full: 133 us against 58 for its operations: the matrix cores are busy
+// 64 % of the cycles, at the 1.7 GHz that the board's power limit leaves.  Three documents, B40
+// Hq40: 30 us against 19; B4 Hq8/Hkv2 behind 1024 rows 13 us, latency: plan, one tile, merge.
+// Tried without gain: half tiles with operands read a step ahead (145 us instead of 134
+// behind 32768 rows: more barriers), waves that share a short tile's keys and dims (such pieces
+// wait for memory), unlike wave priorities.
 
 #include <limits.h>
 #include <math.h>
@@ -43,8 +57,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 128;       // query rows of a prefix tile, at most
 constexpr int kTileKeys = tiles::kBN;
-constexpr uint32_t kMinPiece = 64;   // keys of a prefix piece, at least
-// What a key of a prefix tile costs, in 16ths of a key of the line.
+constexpr uint32_t kMinPiece = 64;   // keys of a prefix piece, at least (128: B4 14.0 us instead of 13.0)
+// What a key of a prefix tile costs, in 16ths of a key of the line.  B64 behind 8192 and 32768
+// rows with 20: 49.7 and 136 us, 24: 51.0 and 132, 32: 55.7 and 155; 10: 72 and 174.
 constexpr uint32_t kTileCost = 24;
 
 constexpr int kOwnWaves = 4;         // waves per workgroup
@@ -96,7 +111,7 @@ struct Piece {
 };
 
 // A thread's sequences and prefixes: one of each, for up to 256 in a call, or four.  (The
-// plan is straight-line code that every launch fetches anew: B4, four 3.4 us, one 2.2.)
+// plan is straight-line code that every launch fetches anew: four 3.0 us, one 2.2.)
 template <int kPer>
 struct Routes {
   int group[kPer], start[kPer];   // group -1: attends no prefix row
@@ -211,9 +226,13 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
       for (int i = 0; i < 2 * kPer; ++i) {
         const uint32_t here = g[i].tiles * p.hkv * parts[i];
         if (block - base < here) {
-          const uint32_t at = block - base, pair = at / parts[i], tile = pair / p.hkv;
-          s_piece = Piece{2 * (tid * pper + i / 2) + (i & 1), static_cast<int>(tile), static_cast<int>(pair - tile * p.hkv),
-                          static_cast<int>(at - pair * parts[i]), static_cast<int>(parts[i]), static_cast<int>(len[i]),
+          // Pieces of the same keys, a tile's each, one after the other on one XCD (blocks go to the
+          // eight in turn), which then reads them once: B64 Hq64/Hkv8 behind 32768 rows 136 -> 133.5 us.
+          const uint32_t at = block - base, x = at & 7u;
+          const uint32_t id = x * (here >> 3) + min(x, here & 7u) + (at >> 3);
+          const uint32_t keys_of = id / g[i].tiles, tile = id - keys_of * g[i].tiles, kvh = keys_of / parts[i];
+          s_piece = Piece{2 * (tid * pper + i / 2) + (i & 1), static_cast<int>(tile), static_cast<int>(kvh),
+                          static_cast<int>(keys_of - kvh * parts[i]), static_cast<int>(parts[i]), static_cast<int>(len[i]),
                           static_cast<int>(g[i].first), static_cast<int>(g[i].first + g[i].keys), static_cast<int>(g[i].seqs),
                           static_cast<int>(base)};
         }
@@ -350,19 +369,11 @@ struct PGroup {
   u32x4 hi, lo;
 };
 __device__ __forceinline__ PGroup split_p(const float (&y)[8]) {
-  // y minus its first part, exact, by a product with (-1, 0) or (0, -1).  (From registers:
-  // the compiler writes the first as the inline constant -1.0, which is another pair.)
-  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
-  asm("" : "+s"(first), "+s"(second));
   PGroup p;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t pair = pack2(y[2 * e], y[2 * e + 1]);
-    const bf16x2 h = __builtin_bit_cast(bf16x2, pair);
-    p.hi[e] = pair;
-    const float y0 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), y[2 * e], false);
-    const float y1 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), y[2 * e + 1], false);
-    p.lo[e] = pack2(y0, y1);
+  for (int e = 0; e < 4; ++e) {   // the differences are exact
+    p.hi[e] = pack2(y[2 * e], y[2 * e + 1]);
+    p.lo[e] = pack2(y[2 * e] - __uint_as_float(p.hi[e] << 16), y[2 * e + 1] - __uint_as_float(p.hi[e] & 0xffff0000u));
   }
   return p;
 }
@@ -637,7 +648,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
   }
   if (!mine) return;
   w.l = w.l + __shfl_xor(w.l, 32);
-  const int64_t to = static_cast<int64_t>(blockIdx.x) * p.tile_rows + row;
+  const int64_t to = static_cast<int64_t>(x.base + (x.tile * p.hkv + x.kvh) * x.parts + x.part) * p.tile_rows + row;
   if (h == 0) *reinterpret_cast<float2*>(p.tile_ml + 2 * to) = make_float2(w.m, w.l);
   float* o = p.tile_o + to * kD + 4 * h;
 #pragma unroll
