@@ -32,7 +32,7 @@
 // B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 51 us against 39 for its bytes,
 // own rows being read until 36 us of a split kernel of 43 (plan 2.2, merge and gap 7); B64 Hq64
 // behind 32768 rows, all full: 133 us against 58 for its operations: the matrix cores are busy
-// 64 % of the cycles, at the 1.7 GHz that the board's power limit leaves.  Three documents, B40
+// 48 % of the cycles, the vector ALUs 50 %, at the 1.7 GHz that the board's power limit leaves.  Three documents, B40
 // Hq40: 30 us against 19; B4 Hq8/Hkv2 behind 1024 rows 13 us, latency: plan, one tile, merge.
 // Tried without gain: half tiles with operands read a step ahead (145 us instead of 134
 // behind 32768 rows: more barriers), waves that share a short tile's keys and dims (such pieces
