@@ -215,6 +215,8 @@ def switch_qk_rotary_append(
     cache any more are dropped and the new length is the capacity.  Other rows of the
     caches keep their contents, and the q rows of tokens that are not appended are
     rotated like the rest.  ``positions`` are the tokens' own, whatever the cache holds.
+    A captured call writes the same q and lengths at each replay; copy the lengths where the
+    next replay reads them.
     """
     interleaved, eps, call = bool(interleaved), float(eps), _lib.native().rotary_append
     made = _lib.like_contiguous(q)

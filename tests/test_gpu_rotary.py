@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from oracle import rotary as R
-from switchattentionkernels_amd import (switch_qk_rotary, switch_qk_rotary_append,
+from switchattentionkernels_amd import (build_switch_query_indices, switch_gqa_prefill, switch_gqa_prefill_backward,
+                                        switch_gqa_prefill_forward, switch_qk_rotary, switch_qk_rotary_append,
                                         switch_qk_rotary_backward, switch_qk_rotary_forward)
 
 pytestmark = pytest.mark.gpu
@@ -359,6 +360,42 @@ def test_capture_is_refused_while_an_eager_graph_of_the_leaves_lives():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(two, k + 1) and all(torch.equal(a, b) for a, b in zip(out, kept))
+
+
+def test_arguments_that_are_copied_keep_their_gradients():
+    """Weights that are strided views, positions of one axis without its dimension."""
+    c = _case(29, 2, 5, 4, 2)
+    wide = torch.stack([c["qw"], c["kw"]], dim=-1).to(DEV).requires_grad_()
+    q, k = (_up(c[x]).requires_grad_() for x in "qk")
+    pos = torch.stack([c["pos"][0]] * 2, dim=-1).to(DEV)[..., 0]
+    outs = switch_qk_rotary(q, k, pos, _up(c["freq"]), q_weight=wide[:, 0], k_weight=wide[:, 1])
+    grads = [_rows(c["gen"], *x.shape) for x in outs]
+    got = torch.autograd.grad(outs, (q, k, wide), [_up(g) for g in grads])
+    _check_backward(c, False, 1e-6, (*got[:2], got[2][:, 0], got[2][:, 1]), grads)
+
+
+def test_training_step_with_the_prefill():
+    """Projection slices, norm and rotation, routed attention, and back: as the calls by themselves."""
+    b, s, hq, hkv = 1, 300, 8, 2
+    c = _case(31, b, s, hq, hkv)
+    qkv = torch.cat([c["q"], c["k"], _rows(c["gen"], b, s, hkv, 128)], dim=2).to(DEV).requires_grad_()
+    w = [_up(c[x]).requires_grad_() for x in ("qw", "kw")]
+    pos, freq = torch.arange(s, dtype=torch.int32, device=DEV)[None], _up(c["freq"])
+    how = dict(q_weight=w[0], k_weight=w[1])
+    q, k, v = qkv[:, :, :hq], qkv[:, :, hq:hq + hkv], qkv[:, :, hq + hkv:].contiguous()
+    lists = build_switch_query_indices(torch.rand(s, generator=c["gen"]).to(DEV) < 0.4)
+    qr, kr = switch_qk_rotary(q, k, pos, freq, **how)
+    out, lse = switch_gqa_prefill(qr, kr, v, *lists, window_size=64)
+    dout = _up(_rows(c["gen"], *out.shape))
+    out.backward(dout)
+    with torch.no_grad():
+        q1, k1 = switch_qk_rotary_forward(q, k, pos, freq, **how)
+        o1, lse1 = switch_gqa_prefill_forward(q1, k1, v, *lists, window_size=64)
+        dq, dk, dv = switch_gqa_prefill_backward(q1, k1, v, o1, lse1, dout, *lists, window_size=64)
+        want = switch_qk_rotary_backward(dq, dk, q, k, pos, freq, **how)
+    assert torch.equal(out, o1) and torch.equal(lse, lse1)
+    assert torch.equal(qkv.grad, torch.cat([want[0], want[1], dv], dim=2))
+    assert torch.equal(w[0].grad, want[2]) and torch.equal(w[1].grad, want[3])
 
 
 def test_changed_inputs_are_noticed_by_autograd():
