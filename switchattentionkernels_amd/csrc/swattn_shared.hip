@@ -29,11 +29,11 @@
 // taken out of the products and added key by key to the rows that attend them.
 //
 // Measured (Hkv 8), as a large copy's 5.2 TB/s and a large matrix product's 1210 TFLOP/s go:
-// B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 51 us against 39 for its bytes,
+// B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 49 us against 39 for its bytes,
 // own rows being read until 36 us of a split kernel of 43 (plan 2.2, merge and gap 7); B64 Hq64
-// behind 32768 rows, all full: 133 us against 58 for its operations: the matrix cores are busy
+// behind 32768 rows, all full: 130 us against 58 for its operations: the matrix cores are busy
 // 48 % of the cycles, the vector ALUs 50 %, at the 1.7 GHz that the board's power limit leaves.  Three documents, B40
-// Hq40: 30 us against 19; B4 Hq8/Hkv2 behind 1024 rows 13 us, latency: plan, one tile, merge.
+// Hq40: 28 us against 19; B4 Hq8/Hkv2 behind 1024 rows 10.3 us, latency: plan, one tile, merge.
 // Tried without gain: half tiles with operands read a step ahead (145 us instead of 134
 // behind 32768 rows: more barriers), waves that share a short tile's keys and dims (such pieces
 // wait for memory), unlike wave priorities.
@@ -88,6 +88,7 @@ struct SharedParams : DecodeCommon {
   int tile_seqs;      // sequences of a tile, at most
   uint32_t tile_inv;  // 2^20 / tile_seqs, rounded up
   int tile_rows;      // rows that a partial has room for
+  uint32_t target_inv;   // 2^32 / target, rounded up
   uint32_t least;     // workgroups that take the line, at least
   float c;            // sm_scale * log2(e)
 };
@@ -205,7 +206,7 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
   // Equal shares of the whole cost, and the keys of a piece at that; a tile is spread
   // over at most 255 pieces.
   const uint64_t cost = line + (static_cast<uint64_t>(all_positions) * p.hkv * kTileCost + 15u) / 16u;
-  const uint32_t share = quotient(cost + p.target - 1, p.target);
+  const uint32_t share = static_cast<uint32_t>((cost * p.target_inv) >> 32) + 1u;
   const uint32_t by_len = (static_cast<uint32_t>(p.prefix_len) + 254u) / 255u;
   const uint32_t length = (max(max((share * 16u + kTileCost - 1u) / kTileCost, by_len), kMinPiece) + kTileKeys - 1u) & ~(kTileKeys - 1u);
   uint32_t pieces = 0, base, all_pieces, parts[2 * kPer], len[2 * kPer];
@@ -273,7 +274,7 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
     }
     before += len;
   }
-  if (wg == 0 && tid == 0) p.plan[0] = make_uint4(L.share, L.total, 0u, 0u);
+  if (wg == 0 && tid == 0) p.plan[0] = make_uint4(L.share, L.total, 0u, UINT32_MAX / L.share);
   st.take = 0;
   if (pos >= L.total) return false;   // uniform
   __syncthreads();
@@ -902,16 +903,20 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
   __shared__ float s_w[2 * kMaxSplitsDev];
   __shared__ float s_red[8];
   __shared__ float4 s_part[8][kD / 4];
-  const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = static_cast<int>(row / p.hq), hq = static_cast<int>(row - static_cast<int64_t>(b) * p.hq);
-  const int kvh = hq / p.group, h = hq - kvh * p.group;
+  const int h = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int64_t row = static_cast<int64_t>(b) * p.hq + kvh * p.group + h;
   const SeqPlace seq = seq_place(p.plan[1 + b]);
-  const uint32_t share = p.plan[0].x;
+  const uint4 line = p.plan[0];
   const int4 place = p.place[b];
-  const uint64_t off = seq.off + static_cast<uint64_t>(kvh) * seq.len;
-  const uint32_t wg0 = quotient(off, share);
-  const int own = seq.n > 0 ? static_cast<int>(quotient(off + seq.n - 1, share) - wg0) + 1 : 0;   // at most 256
+  // Of a position below 2^31, its share: by 2^32 / share, rounded down, one too low at most.
+  auto share_of = [&](uint32_t at) {
+    const uint32_t n = __umulhi(at, line.w);
+    return n + (at - n * line.x >= line.x ? 1u : 0u);
+  };
+  const uint32_t off = static_cast<uint32_t>(seq.off) + static_cast<uint32_t>(kvh) * seq.len;
+  const uint32_t wg0 = share_of(off);
+  const int own = seq.n > 0 ? static_cast<int>(share_of(off + seq.n - 1) - wg0) + 1 : 0;   // at most 256
   const int pieces = place.y, all = own + pieces;
   const int64_t slot0 = static_cast<int64_t>(wg0) + static_cast<int64_t>(seq.rank) * p.hkv + kvh;
   const int64_t row0 = (static_cast<int64_t>(place.x) + static_cast<int64_t>(kvh) * pieces) * p.tile_rows + place.z + h;
@@ -1082,6 +1087,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.group = heads_q / heads_kv;
   p.window = window;
   p.target = static_cast<uint32_t>(L.target);
+  p.target_inv = static_cast<uint32_t>(((int64_t{1} << 32) + L.target - 1) / L.target);
   p.pad = kPairPad;
   p.prefix_k = static_cast<const uint16_t*>(k_prefix);
   p.prefix_v = static_cast<const uint16_t*>(v_prefix);
@@ -1110,7 +1116,8 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   } else {
     launch(shared_split_kernel<1, false>);
   }
-  hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(batch * heads_q)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(p.group), static_cast<uint32_t>(heads_kv), static_cast<uint32_t>(batch)),
+                     dim3(256), 0, st, p);
   return launch_status(name);
 }
 

@@ -116,7 +116,8 @@ def test_planned_pieces_stay_within_the_workspace():
         bound = target + min(batch, 2 * prefixes + batch // seqs) * hkv
         positions = sum(t * n for t, n in groups)
         cost = line + -(-positions * hkv * cost16 // 16)
-        share = -(-cost // target)
+        share = (cost * -(-2 ** 32 // target) >> 32) + 1       # cost / target at least
+        assert share * target >= cost and share <= cost // target + 2
         length = -(-max(-(-share * 16 // cost16), -(-plen // 255), 64) // 64) * 64
         pieces = 0
         for t, n in groups:
