@@ -342,6 +342,30 @@ def test_training_step_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, eager())), i
 
 
+def test_two_layers_of_the_same_weights_captured():
+    """The second call meets what the first one's leaves hold on the capturing stream: allowed."""
+    c = _case(32, 2, 21, 4, 2)
+    leaves = [_up(c[x]).requires_grad_() for x in ("q", "k", "qw", "kw")]
+    pos, freq = _up(c["pos"]), _up(c["freq"])
+    grads = [_up(_rows(c["gen"], *c[x].shape)) for x in "qk"]
+
+    def step():
+        how = dict(q_weight=leaves[2], k_weight=leaves[3])
+        q, k = switch_qk_rotary(leaves[0], leaves[1], pos, freq, **how)
+        return torch.autograd.grad(switch_qk_rotary(q, k, pos, freq, **how), leaves, grads)
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
 def test_capture_is_refused_while_an_eager_graph_of_the_leaves_lives():
     c = _case(28, 1, 9, 4, 2)
     q, w = _up(c["q"]).requires_grad_(), _up(c["qw"]).requires_grad_()
