@@ -42,11 +42,13 @@ namespace {
 constexpr int kD = 128;
 constexpr int kWaves = 4;          // waves per workgroup
 constexpr int kRowsAtOnce = 8;     // head rows that a wave takes at once
-constexpr int kGroupsPerCu = 5;    // workgroups that a CU takes at once
-constexpr int kBackPerCu = 3;      // and of the backward
-// Calls that move more than kStreamBytes go past the 256 MB memory-side cache, whose lines
-// others may still have a use for: the forward in both directions, the backward with what
-// it writes, and with what it reads if that alone fills the cache.
+constexpr int kGroupsPerCu = 5;    // workgroups that a CU takes at once (4 and 6: within 2 %)
+constexpr int kBackPerCu = 3;      // and of the backward (4: S16384 108 us instead of 101, 5 spill: 187)
+// Calls that move more than kStreamBytes go past the 256 MB memory-side cache, the forward in
+// both directions (S16384 Hq32/Hkv8 69.5 -> 62.5 us, B2 S2999 Hq40/Hkv8 33.4 -> 29.9; B1 S2729
+// Hq32/Hkv8, 56 MB that a projection may have left there, 11.0, streamed 13.5), the backward with
+// what it writes (B1 S3077 Hq40/Hkv8 30.6 -> 27.1), and with what it reads if that alone fills the
+// cache (S16384 98 -> 93.5; S3077 27.1 -> 32).
 constexpr int64_t kStreamBytes = 96 << 20, kCacheBytes = 256 << 20;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -91,6 +91,7 @@ struct SharedParams : DecodeCommon {
   uint32_t target_inv;   // 2^32 / target, rounded up
   uint32_t least;     // workgroups that take the line, at least
   float c;            // sm_scale * log2(e)
+  int stream_prefix;
 };
 
 __device__ __forceinline__ float bf(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
@@ -288,19 +289,25 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
 // read as that one.
 constexpr int kSlotBytes = 2 * tiles::kTileBytes;
 __device__ __forceinline__ void copy_tile(const uint16_t* kb, const uint16_t* vb, uint32_t row_bytes, int key, int last,
-                                          uint32_t lds, int wave, int lane) {
+                                          uint32_t lds, int wave, int lane, bool stream) {
   const int64_t at = static_cast<int64_t>(key + 16 * wave) * (row_bytes / 2);
   const uint32_t chunk = 16u * ((lane & 15) ^ ((lane >> 4) << 2));   // of row 4 i + lane / 16: ^ 16 i
   uint32_t row = (lane >> 4) * row_bytes;   // a tile's rows span less than 2^31 bytes
   lds += 4096u * static_cast<uint32_t>(wave);
   if (key + kTileKeys - 1 <= last) {   // uniform
+    auto whole = [&](auto dma) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t to = at + static_cast<int64_t>(4 * i) * (row_bytes / 2);
-      const uint32_t off = (chunk ^ (16u * i)) + row;
-      tiles::dma16_from(kb + to, off, lds + 1024u * i);
-      tiles::dma16_from(vb + to, off, lds + 1024u * i + tiles::kTileBytes);
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int64_t to = at + static_cast<int64_t>(4 * i) * (row_bytes / 2);
+        const uint32_t off = (chunk ^ (16u * i)) + row;
+        dma(kb + to, off, lds + 1024u * i);
+        dma(vb + to, off, lds + 1024u * i + tiles::kTileBytes);
+      }
+    };
+    if (stream)   // uniform
+      whole([](const void* from, uint32_t off, uint32_t to) { tiles::dma16_stream_from(from, off, to); });
+    else
+      whole([](const void* from, uint32_t off, uint32_t to) { tiles::dma16_from(from, off, to); });
   } else {
     const int rest = last - key - 16 * wave;
 #pragma unroll
@@ -557,7 +564,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
   const uint32_t lds = tiles::lds_addr(ring);
   const int steps = (k1 - k0 + kTileKeys - 1) / kTileKeys;
   auto copy = [&](int j) {
-    copy_tile(kb, vb, row_bytes, k0 + kTileKeys * j, last, lds + (j & 1) * kSlotBytes, wave, lane);
+    copy_tile(kb, vb, row_bytes, k0 + kTileKeys * j, last, lds + (j & 1) * kSlotBytes, wave, lane, p.stream_prefix != 0);
   };
   auto copy_first = [&]() {
     copy(0);
@@ -980,6 +987,10 @@ constexpr int kLineLeast = 8;      // of the target, the part that the line gets
 // prefixes: B64 of 1024 rows behind 8192 54.4 -> 51.7 us.  Smaller ones may still be there
 // from the last call: B40 of 777 rows 30.5 us, streamed 32.6.
 constexpr int64_t kStreamBytes = int64_t{256} << 20;
+// Prefixes too, from a size on that other layers' rows push out before the next step, where one
+// tile takes all sequences: one of 30720 rows, 8 KV heads, B20 39.9 -> 34.8 us, B1 of 32768 35.4 ->
+// 32.8.  Tiles that share a prefix find it in the caches: B64 Hq64 behind 32768 136, streamed 141.
+constexpr int64_t kStreamPrefixBytes = int64_t{96} << 20;
 
 int shared_cus() {
   int dev = 0, n = 0;
@@ -1097,6 +1108,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.tile_ml = reinterpret_cast<float*>(ws + L.off_tile_ml);
   p.place = reinterpret_cast<int4*>(ws + L.off_place);
   p.prefixes = prefixes;
+  p.stream_prefix = batch <= L.tile_seqs && prefixes * prefix_len * heads_kv * (4 * kD) >= kStreamPrefixBytes;
   p.prefix_len = static_cast<int>(prefix_len);
   p.tile_seqs = static_cast<int>(L.tile_seqs);
   p.tile_inv = static_cast<uint32_t>((1u << 20) / L.tile_seqs + 1);

@@ -137,6 +137,13 @@ __device__ __forceinline__ void dma16_from(const void* base, uint32_t voff, uint
                : "v"(voff), "s"(base), "s"(lds_base)
                : "memory", "m0");
 }
+// And past the memory-side cache.
+__device__ __forceinline__ void dma16_stream_from(const void* base, uint32_t voff, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+               :
+               : "v"(voff), "s"(base), "s"(lds_base)
+               : "memory", "m0");
+}
 __device__ __forceinline__ uint32_t lds_addr(const char* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(p)));

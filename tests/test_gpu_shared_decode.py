@@ -252,6 +252,24 @@ def test_far_rows():
     _check(c, 100, got=got)
 
 
+@pytest.mark.parametrize("batch", [5, 70])
+def test_a_large_prefix(batch):
+    """Of more than 96 MB, with a ragged end: streamed where one tile takes all sequences."""
+    n, hkv = 24011, 8
+    gen = torch.Generator(device=DEV).manual_seed(batch)
+    rows = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(BF16)  # noqa: E731
+    q, kp, vp = rows(batch, 1, 16, 128), rows(1, n, hkv, 128), rows(1, n, hkv, 128)
+    kc, vc = rows(batch, 40, hkv, 128), rows(batch, 40, hkv, 128)
+    lens = _int32([(7 * i) % 41 for i in range(batch)])
+    full = torch.tensor([i % 2 == 0 for i in range(batch)], device=DEV)
+    plens, ids = _int32([n - 3]), _int32([0] * batch)
+    o, lse = switch_gqa_decode_shared_forward(q, kp, vp, plens, ids, kc, vc, lens, full, window_size=700)
+    picked = [0, 1, batch - 1]
+    c = dict(q=q[picked].cpu(), kp=kp.cpu(), vp=vp.cpu(), kc=kc[picked].cpu(), vc=vc[picked].cpu(), plens=[n - 3],
+             ids=[0] * 3, lens=lens[picked].tolist(), full=full[picked].tolist())
+    _check(c, 700, got=(o[picked], lse[picked]))
+
+
 def test_a_serving_loop():
     """Prompts behind a shared prefix, then steps: rotated queries and keys, appended, attended;
     each step against one cache that holds the prefix and the own rows together."""
