@@ -22,8 +22,10 @@
  *                 base 16-byte aligned.
  *   positions     int32 [axes, batch, seq], any sign
  *   inv_freq      fp32 (freq_f64 0) or fp64 (freq_f64 1) [rotary / 2], below 2^40 in
- *                 magnitude; angles are its values times the positions to 2^-31 turns
- *                 wherever the position lies.  Others, NaN among them, give NaN.
+ *                 magnitude; angles are its values times the positions, off by at most
+ *                 2^-65 turns per position (2^-34 turns at the ends of int32), and their
+ *                 sines and cosines by 8 roundings of fp32 of themselves beside that.
+ *                 Others, NaN among them, give NaN.
  *   sections      host int32 [axes]: how many of the frequencies, in order, belong to
  *                 each axis; positive, their sum is the number of frequencies.  axes 1 to 4
  *   q_weight, k_weight  fp32 (weight_bf16 0) or bf16 (1) [128], or NULL: not normalised

@@ -42,7 +42,7 @@ def turn(x, cos, sin, interleaved):
 def forward(x, weight, eps, cos, sin, interleaved):
     """(rotated rows, their bound).  The norm: 16 products of squares in a lane's chain, 3
     sums over lanes, mean and eps (22 roundings, half of them in the root), root, quotient
-    and two products: 16 U.  The angle: 2^-31 turns, its conversion and scaling, the series
+    and two products: 16 U.  The angle: 2^-34 turns at most, its conversion and scaling, the series
     and its end: 5 U of sine and cosine.  Two products and a sum: 3 U."""
     if weight is not None:
         x = x / np.sqrt((x * x).mean(axis=-1, keepdims=True) + eps) * weight

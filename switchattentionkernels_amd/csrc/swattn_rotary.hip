@@ -26,8 +26,8 @@
 //
 // Angles are exact where fp32 products are not (a position of 2^17 times a frequency of
 // 1 is off by up to 2^-8 in fp32): a frequency is held as a 64-bit fixed-point fraction
-// of turns per position, the product with the position is taken mod 2^64, which drops
-// whole turns, and its upper 32 bits are the angle.
+// of turns per position, and the product with the position is taken mod 2^64, which drops
+// whole turns: an angle is off by 2^-65 turns per position.
 
 #include <math.h>
 
@@ -132,11 +132,17 @@ __device__ __forceinline__ uint64_t fixed_turns(double f) {
   return (static_cast<uint64_t>(static_cast<int64_t>(whole)) << 32) + static_cast<uint64_t>(rest);
 }
 
-// Sine and cosine of an angle in 2^-32 turns: the nearest quarter turn, and the Taylor
-// series of what is left, at most pi / 4 (the next terms are below 2^-29).
-__device__ __forceinline__ void sine_cosine(uint32_t turns, float& s, float& c) {
-  const uint32_t quarter = (turns + 0x20000000u) >> 30;
-  const float x = static_cast<float>(static_cast<int32_t>(turns - (quarter << 30))) * 1.46291807926716e-9f;   // 2 pi / 2^32
+// Sine and cosine of an angle in 2^-64 turns: the nearest quarter turn, and the Taylor
+// series of what is left, at most pi / 4 (the next terms are below 2^-29).  What is left
+// enters with fp32's bits however small it is: its upper 32 bits, rounded, and what that
+// leaves.  (The upper 32 bits alone, steps of 1.5e-9 radians, were 1 % of the sine of a
+// frequency of 1e-8 at position 1.)
+__device__ __forceinline__ void sine_cosine(uint64_t turns, float& s, float& c) {
+  const uint32_t quarter = static_cast<uint32_t>((turns + 0x2000000000000000u) >> 62);
+  const uint64_t rest = turns - (static_cast<uint64_t>(quarter) << 62);
+  const int32_t high = static_cast<int32_t>((rest + 0x80000000u) >> 32), low = static_cast<int32_t>(rest);
+  constexpr float kStep = 1.46291807926716e-9f;   // 2 pi / 2^32
+  const float x = __builtin_fmaf(static_cast<float>(low), kStep * 0x1p-32f, static_cast<float>(high) * kStep);
   const float z = x * x;
   float a = __builtin_fmaf(z, 2.75573192e-6f, -1.98412698e-4f);   // 1 / 9!, 1 / 7!, ..
   a = __builtin_fmaf(z, a, 8.33333333e-3f);
@@ -191,7 +197,7 @@ __device__ __forceinline__ int token_position(const Angles& g, const Lane& o, in
 __device__ __forceinline__ void token_turn(const Lane& o, int pos, int lane, float (*lds)[64]) {
   const uint64_t at = o.turns * static_cast<uint64_t>(static_cast<int64_t>(pos));
   float s, c;
-  sine_cosine(static_cast<uint32_t>((at + 0x80000000u) >> 32), s, c);
+  sine_cosine(at, s, c);
   __builtin_amdgcn_wave_barrier();
   lds[0][lane] = o.nan ? NAN : c;
   lds[1][lane] = o.nan ? NAN : s;
