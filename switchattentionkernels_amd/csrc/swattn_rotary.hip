@@ -282,15 +282,29 @@ __device__ __forceinline__ void load_weights(const float* lds, const Lane& o, fl
   }
 }
 
-// 1 / sqrt(mean(x^2) + eps) of the row: the hardware's, within one last place, which takes
-// no denormal number.
-__device__ __forceinline__ float row_scale(const float (&x)[16], float eps) {
+// x becomes x / sqrt(mean(x^2) + eps); returns what it was multiplied by.  The root is the
+// hardware's, within one last place, which takes no denormal number.  A row whose mean
+// square leaves [2^-96, 2^120) (finite rows of bf16 may have 2^-266 to 2^256) is scaled by a power of
+// two first, so that its squares and their sum stay fp32 numbers.
+__device__ __forceinline__ float normalise(float (&x)[16], float eps) {
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s = __builtin_fmaf(x[i], x[i], s);
   const float m = __builtin_fmaf(row_sum(s), 1.0f / kD, eps);
-  const bool small = m < 0x1p-96f;
-  return __builtin_amdgcn_rsqf(small ? m * 0x1p64f : m) * (small ? 0x1p32f : 1.0f);
+  float r = __builtin_amdgcn_rsqf(m), by = 1.0f;
+  if (!(m >= 0x1p-96f && m < 0x1p120f)) {   // the same in a row's lanes; rare
+    by = m < 1.0f ? 0x1p100f : 0x1p-68f;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] *= by;
+      s = __builtin_fmaf(x[i], x[i], s);
+    }
+    r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum(s), 1.0f / kD, eps * by * by));
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] *= r;
+  return r * by;
 }
 
 // A wave goes through its share of the passes: a token's q rows, then its k rows, then its
@@ -370,9 +384,9 @@ __global__ __launch_bounds__(64 * kWaves, kGroupsPerCu) void rotary_kernel(const
       if ((which == 0 ? p.q_weight : p.k_weight) != nullptr) {
         float w[16];
         load_weights(s_weight[which], o, w);
-        const float r = row_scale(x, p.eps);
+        normalise(x, p.eps);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = x[i] * r * w[i];
+        for (int i = 0; i < 16; ++i) x[i] *= w[i];
       }
       rotate<kPairs, false>(o, s_turn[wave], lane, x);
       store_row<kStream>(row, o, x);
@@ -461,11 +475,10 @@ __global__ __launch_bounds__(64 * kWaves, kBackPerCu) void rotary_backward_kerne
         float u[16], w[16];
         unpack(c.x, u);
         load_weights(s_weight, o, w);
-        const float r = row_scale(u, p.eps);
+        const float r = normalise(u, p.eps);
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          u[i] *= r;
           dw[i] = __builtin_fmaf(g[i], u[i], dw[i]);
           g[i] *= w[i];
           dot = __builtin_fmaf(g[i], u[i], dot);
