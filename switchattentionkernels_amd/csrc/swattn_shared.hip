@@ -18,11 +18,13 @@
 // The first workgroups take prefix pieces, the others shares of the line; how many of
 // each is settled on the device by every workgroup for itself, from the lengths.
 //
-// P enters its product as two bf16 numbers, its value and what that leaves: 17 bits, for a
-// third of the matrix instructions (the prefill rounds P to one).  Of 524288 outputs over up to
-// 33792 keys 893 then differ from the exact value's rounding, by one last place, and 627 of a
-// plain evaluation in fp32; with one number B64 behind 32768 rows would take 17 us less.
-//
+// P enters its product as bf16 numbers: of a sequence's own rows three, 24 bits, as HBM is the limit
+// there (B64 of 1024 rows behind 8192: 49.0 us with two, 49.5 with three); of a prefix two, its value and
+// what that leaves, 17 bits (the prefill rounds P to one), as each is a third of a tile's matrix
+// instructions: B64 Hq64 behind 32768 rows 131 us, with three 154, with one 17 less.  Of 524288
+// outputs there 889 differ from the exact value's rounding, by one last place, with three 269,
+// and 627 of a plain evaluation in fp32; behind 8192 rows 328 of 262144, 90 and 113.
+
 // Local rows attend the last rows of their prefix only, each from its own start on.
 // Masked scores are -inf, their weights 0.  A piece whose sums are not finite runs again
 // carefully: values that are not finite, which a weight of 0 would turn into NaN, are
@@ -720,7 +722,8 @@ __device__ __forceinline__ u32x4 load16(const uint16_t* p) {
 // * O^T [16 dims x 16 columns] += V^T P^T, 32 keys at once: lane (c, g) holds dims 8 c .. +7
 //   of keys 4 g .. +3 of both key tiles; tile n takes dim 8 c + n of each, so that S^T's
 //   accumulator layout is P^T's operand layout, and V is transposed inside a lane.
-//   Columns 0-7 take a weight's first bf16 number, columns 8-15 what it leaves.
+//   A weight enters as three bf16 numbers, 24 bits: columns 0-7 take the first in one product
+//   and the third in a second, columns 8-15 the one between.
 // A piece's partial lies in slot wg + (pair's rank): both only grow along the line, one of
 // them at every step from piece to piece, so that no two pieces share a slot and a pair's
 // slots are consecutive.
@@ -799,7 +802,7 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
           for (int t = 0; t < 8; ++t) acc[t] *= a;
         }
         const float from = m == -INFINITY ? 0.f : m;   // only scores of -inf so far: they weigh nothing
-        u32x4 pk;
+        u32x4 pk, pk2;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -810,11 +813,16 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
               y[u] = __builtin_amdgcn_exp2f(s[t][x + u] - from);   // 0 behind the piece
               l += y[u];
             }
-            const uint32_t hi = pack2(y[0], y[1]);
-            const uint32_t lo = pack2(y[0] - __uint_as_float(hi << 16), y[1] - __uint_as_float(hi & 0xffff0000u));
-            pk[2 * t + x / 2] = second ? lo : hi;
+            const uint32_t high = pack2(y[0], y[1]);   // the differences are exact
+            y[0] -= __uint_as_float(high << 16);
+            y[1] -= __uint_as_float(high & 0xffff0000u);
+            const uint32_t mid = pack2(y[0], y[1]);
+            y[0] -= __uint_as_float(mid << 16);
+            y[1] -= __uint_as_float(mid & 0xffff0000u);
+            pk[2 * t + x / 2] = second ? mid : high;
+            pk2[2 * t + x / 2] = second ? 0u : pack2(y[0], y[1]);
           }
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, pk);
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, pk), pb2 = __builtin_bit_cast(bf16x8, pk2);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           u32x4 a0, a1;   // dims 2 d and 2 d + 1 of this lane's eight
@@ -825,6 +833,8 @@ __device__ __forceinline__ void own_pieces(const SharedParams& p, uint32_t wg, c
           }
           acc[2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), pb, acc[2 * d], 0, 0, 0);
           acc[2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), pb, acc[2 * d + 1], 0, 0, 0);
+          acc[2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a0), pb2, acc[2 * d], 0, 0, 0);
+          acc[2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a1), pb2, acc[2 * d + 1], 0, 0, 0);
         }
         load(i + kOwnWaves);   // past the end: the last row, never used
       }
