@@ -56,7 +56,8 @@ int swattn_rotary_fwd(const void* q, const int64_t* q_strides, const void* k,
 
 /*
  * Gradients of swattn_rotary_fwd's outputs: grad_q, grad_k as its outputs, q and k as its
- * inputs (looked at only where the tensor has a weight); dq and dk like the outputs.
+ * inputs (looked at only where the tensor has a weight, else NULL will do); dq and dk like
+ * the outputs.
  *   dq_weight, dk_weight  [128] of the weights' type, or NULL: not wanted (always NULL
  *                         where there is no weight).  Summed in fp32 in a fixed order.
  *   workspace   >= swattn_rotary_bwd_workspace_bytes(), asked on the current device;

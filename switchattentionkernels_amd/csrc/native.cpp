@@ -466,7 +466,8 @@ bool rows_ok(const Tensor& t, at::Device device) {
 }
 
 struct RowStrides {
-  int64_t s[3];
+  int64_t s[3] = {0, 0, 0};
+  RowStrides() = default;
   explicit RowStrides(const Tensor& t) {
     for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
   }
@@ -572,32 +573,39 @@ std::tuple<Tensor, Tensor> launch_rotary(const Tensor& q, const Tensor& k, const
 
 using RotaryGrads = std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>>;
 
+// q and k are looked at (and may be undefined otherwise) where they have a weight.
 RotaryGrads launch_rotary_backward(const Tensor& grad_q, const Tensor& grad_k, const Tensor& q, const Tensor& k,
                                    const Tensor& positions, const Tensor& inv_freq, const optional<Tensor>& q_weight,
                                    const optional<Tensor>& k_weight, const RotaryHow& how, bool weight_grads) {
-  const OnDevice here(q.device());
+  const OnDevice here(grad_q.device());
   const Tensor dq = at::empty(grad_q.sizes(), grad_q.options()), dk = at::empty(grad_k.sizes(), grad_k.options());
   optional<Tensor> dwq, dwk;
-  const bool none = q.size(1) == 0;
+  const bool none = grad_q.size(1) == 0;
   if (weight_grads && q_weight.has_value())
     dwq = none ? at::zeros(q_weight->sizes(), q_weight->options()) : at::empty(q_weight->sizes(), q_weight->options());
   if (weight_grads && k_weight.has_value())
     dwk = none ? at::zeros(k_weight->sizes(), k_weight->options()) : at::empty(k_weight->sizes(), k_weight->options());
   if (none) return {dq, dk, dwq, dwk};
-  const int32_t batch = static_cast<int32_t>(q.size(0)), hq = static_cast<int32_t>(q.size(2));
-  const int32_t hkv = static_cast<int32_t>(k.size(2));
+  const int64_t seq = grad_q.size(1);
+  const int32_t batch = static_cast<int32_t>(grad_q.size(0)), hq = static_cast<int32_t>(grad_q.size(2));
+  const int32_t hkv = static_cast<int32_t>(grad_k.size(2));
   const bool sums = dwq.has_value() || dwk.has_value();
-  const size_t ws_bytes = sums ? swattn_rotary_bwd_workspace_bytes(batch, q.size(1), hq, hkv) : 0;
+  const size_t ws_bytes = sums ? swattn_rotary_bwd_workspace_bytes(batch, seq, hq, hkv) : 0;
   Tensor ws;
-  if (sums) ws = bytes(q, ws_bytes);
-  const RowStrides qs(q), ks(k);
-  check(swattn_rotary_bwd(grad_q.const_data_ptr(), grad_k.const_data_ptr(), q.const_data_ptr(), qs.s, k.const_data_ptr(),
-                          ks.s, i32(positions), inv_freq.const_data_ptr(), inv_freq.scalar_type() == at::kDouble,
-                          how.sections.data(), static_cast<int32_t>(how.sections.size()), how.interleaved,
-                          weight_ptr(q_weight), weight_ptr(k_weight), weight_bf16(q_weight, k_weight),
-                          static_cast<float>(how.eps), dq.data_ptr(), dk.data_ptr(),
+  if (sums) ws = bytes(grad_q, ws_bytes);
+  const auto rows = [](const Tensor& t, const optional<Tensor>& weight) {
+    return weight.has_value() ? std::make_pair(t.const_data_ptr(), RowStrides(t))
+                              : std::make_pair(static_cast<const void*>(nullptr), RowStrides());
+  };
+  const auto [qp, qs] = rows(q, q_weight);
+  const auto [kp, ks] = rows(k, k_weight);
+  check(swattn_rotary_bwd(grad_q.const_data_ptr(), grad_k.const_data_ptr(), qp, qs.s, kp, ks.s, i32(positions),
+                          inv_freq.const_data_ptr(), inv_freq.scalar_type() == at::kDouble, how.sections.data(),
+                          static_cast<int32_t>(how.sections.size()), how.interleaved, weight_ptr(q_weight),
+                          weight_ptr(k_weight), weight_bf16(q_weight, k_weight), static_cast<float>(how.eps), dq.data_ptr(),
+                          dk.data_ptr(),
                           dwq.has_value() ? dwq->data_ptr() : nullptr, dwk.has_value() ? dwk->data_ptr() : nullptr, batch,
-                          q.size(1), hq, hkv, 128, sums ? ws.data_ptr() : nullptr, ws_bytes, here.stream),
+                          seq, hq, hkv, 128, sums ? ws.data_ptr() : nullptr, ws_bytes, here.stream),
         "swattn_rotary_bwd");
   return {dq, dk, dwq, dwk};
 }
@@ -667,7 +675,9 @@ struct RotaryNode : ag::Function<RotaryNode> {
                                    const optional<Tensor>& k_weight, const RotaryHow& how,
                                    const std::pair<optional<Tensor>, optional<Tensor>>& made) {
     auto [q_out, k_out] = launch_rotary(q, k, positions, inv_freq, q_weight, k_weight, how, made.first, made.second);
-    ctx->save_for_backward({q, k, positions, inv_freq, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())});
+    // Rows without a norm are not read again: nothing of theirs is kept alive, and they may change.
+    ctx->save_for_backward({q_weight.has_value() ? q : Tensor(), k_weight.has_value() ? k : Tensor(), positions, inv_freq,
+                            q_weight.value_or(Tensor()), k_weight.value_or(Tensor())});
     ctx->saved_data["sections"] = std::vector<int64_t>(how.sections.begin(), how.sections.end());
     ctx->saved_data["interleaved"] = how.interleaved;
     ctx->saved_data["eps"] = how.eps;
@@ -685,13 +695,13 @@ struct RotaryNode : ag::Function<RotaryNode> {
       const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
       const RotaryHow how{{sections.begin(), sections.end()}, ctx->saved_data["interleaved"].toBool(),
                           ctx->saved_data["eps"].toDouble()};
-      const auto rows = [](const Tensor& grad, const Tensor& x) {
+      const auto rows = [](const Tensor& grad) {
         const Tensor g = grad.to(at::kBFloat16).contiguous();
-        return grad_ok(g, x) ? g : g.clone();   // (not at a multiple of 16 bytes)
+        return grad_ok(g, g) ? g : g.clone();   // (not at a multiple of 16 bytes)
       };
       const auto weight = [&](int i) { return saved[i].defined() ? optional<Tensor>(saved[i]) : std::nullopt; };
       auto [dq, dk, dwq, dwk] =
-          launch_rotary_backward(rows(grads[0], saved[0]), rows(grads[1], saved[1]), saved[0], saved[1], saved[2], saved[3],
+          launch_rotary_backward(rows(grads[0]), rows(grads[1]), saved[0], saved[1], saved[2], saved[3],
                                  weight(4), weight(5), how, ctx->saved_data["weight_grads"].toBool());
       out[0] = std::move(dq);
       out[1] = std::move(dk);

@@ -718,7 +718,7 @@ int swattn_rotary_bwd(const void* grad_q, const void* grad_k, const void* q, con
   BackwardParams p{};
   if (st == SWATTN_OK) st = check_angles(n, positions, inv_freq, freq_f64, sections, axes, p.angles);
   if (st != SWATTN_OK) return st;
-  if (!rows_ok(q, q_strides, p.x[0]) || !rows_ok(k, k_strides, p.x[1]))
+  if ((q_weight != nullptr && !rows_ok(q, q_strides, p.x[0])) || (k_weight != nullptr && !rows_ok(k, k_strides, p.x[1])))
     return invalid(n + ": q and k must be 16-byte aligned, their strides multiples of 8 and not negative");
   if (grad_q == nullptr || grad_k == nullptr || dq == nullptr || dk == nullptr || !aligned16(grad_q) ||
       !aligned16(grad_k) || !aligned16(dq) || !aligned16(dk))

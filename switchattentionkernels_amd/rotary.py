@@ -169,7 +169,8 @@ def switch_qk_rotary(q, k, positions, inv_freq, *, sections: Optional[Sequence[i
                      k_weight: Optional[torch.Tensor] = None,
                      eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """``switch_qk_rotary_forward`` with autograd support for q, k and the weights (once:
-    gradients of gradients raise).
+    gradients of gradients raise).  The graph keeps the rows of a tensor that has a weight;
+    without one they may be freed or changed before the backward.
 
     Under capture the leaves among them must not belong to an eager graph that still lives
     (such a call raises: the captured backward would end the process)."""
