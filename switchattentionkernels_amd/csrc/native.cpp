@@ -653,11 +653,13 @@ optional<RotaryGrads> rotary_backward(const Tensor& grad_q, const Tensor& grad_k
 namespace ag = torch::autograd;
 
 // What a leaf already has of a graph on another stream would tie a captured backward to
-// that stream's uncaptured work, which ends the process.
+// that stream's uncaptured work, which ends the process.  A view of a leaf leads there too.
 void refuse_captured_leaves(const Tensor& q, const Tensor& k, const optional<Tensor>& q_weight,
                             const optional<Tensor>& k_weight) {
-  for (const Tensor& t : {q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())}) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+  for (const Tensor& x : {q, k, q_weight.value_or(Tensor()), k_weight.value_or(Tensor())}) {
+    if (!x.defined() || !x.requires_grad()) continue;
+    const Tensor t = !x.is_leaf() && x.is_view() ? Tensor(at::TensorBase(x._base())) : x;
+    if (!t.requires_grad() || !t.is_leaf()) continue;
     const auto old = ag::impl::try_get_grad_accumulator(t);
     if (old == nullptr) continue;
     const auto stream = c10::hip::getCurrentHIPStream(q.device().index());
@@ -735,6 +737,11 @@ optional<std::tuple<Tensor, Tensor>> rotary_autograd(const Tensor& q, const Tens
   ag::variable_list out =
       RotaryNode::apply(q, k, positions, inv_freq, q_weight, k_weight, *how, std::make_pair(q_made, k_made));
   return std::make_tuple(std::move(out[0]), std::move(out[1]));
+}
+
+// The same check before arguments are copied, which hides their leaves.
+void rotary_leaves(const Tensor& q, const Tensor& k, const optional<Tensor>& q_weight, const optional<Tensor>& k_weight) {
+  if (at::GradMode::is_enabled()) refuse_captured_leaves(q, k, q_weight, k_weight);
 }
 
 // (rotated q, the new lengths).
@@ -830,6 +837,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary_forward", &rotary_forward, no_gil);
   m.def("rotary_backward", &rotary_backward, no_gil);
   m.def("rotary_autograd", &rotary_autograd, no_gil);
+  m.def("rotary_leaves", &rotary_leaves, no_gil);
   m.def("rotary_append", &rotary_append, no_gil);
   m.def("shared_decode", &shared_decode, no_gil);
 }

@@ -80,8 +80,9 @@ def _validate(q, k, positions, inv_freq, sections, q_weight, k_weight, eps) -> N
         raise ValueError("eps must be finite and not negative")
 
 
-def _arguments(q, k, positions, inv_freq, sections, q_weight, k_weight, eps):
-    """The same arguments, checked, positions ``[axes,B,S]`` and all but q and k contiguous."""
+def _arguments(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, look=None):
+    """The same arguments, checked (``look``: at q, k and the weights as they came, too),
+    positions ``[axes,B,S]`` and all but q and k contiguous."""
     if isinstance(positions, torch.Tensor) and positions.ndim == 2:
         positions = positions.unsqueeze(0)
     if sections is None:
@@ -89,6 +90,8 @@ def _arguments(q, k, positions, inv_freq, sections, q_weight, k_weight, eps):
     else:
         sections = [int(n) for n in sections]
     _validate(q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+    if look is not None:
+        look(q, k, q_weight, k_weight)
     return (q, k, positions.contiguous(), inv_freq.contiguous(), sections,
             *(None if w is None else w.contiguous() for w in (q_weight, k_weight)), eps)
 
@@ -126,13 +129,13 @@ def switch_qk_rotary_forward(
                    q_weight, k_weight, eps)
 
 
-def _rotate(call, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps):
+def _rotate(call, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, look=None):
     interleaved, eps = bool(interleaved), float(eps)
     made = (_lib.like_contiguous(q), _lib.like_contiguous(k))
     out = _quick(call, q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, *made)
     if out is None:
         q, k, positions, inv_freq, sections, q_weight, k_weight, eps = _arguments(
-            q, k, positions, inv_freq, sections, q_weight, k_weight, eps)
+            q, k, positions, inv_freq, sections, q_weight, k_weight, eps, look)
         out = call(q, k, positions, inv_freq, sections, interleaved, q_weight, k_weight, eps, *made)
     return out
 
@@ -172,10 +175,12 @@ def switch_qk_rotary(q, k, positions, inv_freq, *, sections: Optional[Sequence[i
     gradients of gradients raise).  The graph keeps the rows of a tensor that has a weight;
     without one they may be freed or changed before the backward.
 
-    Under capture the leaves among them must not belong to an eager graph that still lives
-    (such a call raises: the captured backward would end the process)."""
-    return _rotate(_lib.native().rotary_autograd, q, k, positions, inv_freq, sections, interleaved,
-                   q_weight, k_weight, eps)
+    Under capture the leaves among them, and those that they are views of, must not belong to
+    an eager graph that still lives (such a call raises: the captured backward would end the
+    process).  Leaves further back are the caller's to look after."""
+    native = _lib.native()
+    return _rotate(native.rotary_autograd, q, k, positions, inv_freq, sections, interleaved, q_weight,
+                   k_weight, eps, native.rotary_leaves)
 
 
 def _validate_append(q, k, v, k_cache, v_cache, lens, counts) -> None:
