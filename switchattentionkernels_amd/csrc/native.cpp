@@ -468,8 +468,8 @@ bool rows_ok(const Tensor& t, at::Device device) {
 struct RowStrides {
   int64_t s[3] = {0, 0, 0};
   RowStrides() = default;
-  explicit RowStrides(const Tensor& t) {
-    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  explicit RowStrides(const Tensor& t) {   // of no rows any will do
+    for (int i = 0; i < 3; ++i) s[i] = t.numel() > 0 && t.size(i) > 1 ? t.stride(i) : 0;
   }
 };
 
