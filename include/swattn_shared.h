@@ -23,7 +23,8 @@ extern "C" {
  * b are the first prefix_lens[i] rows of prefix i = prefix_ids[b], then the first
  * cache_lens[b] rows of its own cache.  With n of them together the new token sits at
  * position n - 1 and attends all n where full[b], else the last `window` of them.  A
- * prefix's rows are read once for all sequences that attend them.
+ * prefix's rows are read once for every 128 query rows of a KV head that attend them (of
+ * G = heads_q / heads_kv for each sequence), full and local routes apart.
  *
  *   q                   bf16 [batch, heads_q, 128]
  *   k_prefix, v_prefix  bf16 [prefixes, prefix_len, heads_kv, 128]
@@ -39,9 +40,10 @@ extern "C" {
  *   workspace           >= swattn_shared_decode_workspace_bytes(), asked on the current
  *                       device; 256-byte aligned
  * heads_q / heads_kv at most 8; batch up to SWATTN_SHARED_MAX_SEQS, prefixes 1 to
- * SWATTN_SHARED_MAX_PREFIXES; batch * cache_len * heads_kv and the prefix positions (see
- * the workspace query, which returns 0 for shapes that are refused) below 2^31, batch *
- * heads_q below 2^24.  scale_log2 is finite.
+ * SWATTN_SHARED_MAX_PREFIXES; below 2^31 both batch * heads_kv * (cache_len + 192) and
+ * tiles * heads_kv * (prefix_len + 64), with tiles = min(batch, 2 * prefixes + batch /
+ * (128 / G)), divisions rounded down; batch * heads_q below 2^24.  The workspace query
+ * returns 0 for shapes that are refused.  scale_log2 is finite.
  */
 size_t swattn_shared_decode_workspace_bytes(int32_t batch, int64_t cache_len, int32_t prefixes,
                                             int64_t prefix_len, int32_t heads_q,

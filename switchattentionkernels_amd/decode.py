@@ -191,7 +191,7 @@ def switch_gqa_decode_shared_forward(
         sm_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Routed decode step of sequences that continue shared prefixes:
     ``switch_gqa_decode_forward`` where the rows of a system prompt or a document are kept
-    once, and read once for all sequences that attend them.
+    once, and read once for every 128 query rows of a KV head that attend them.
 
     ``q``: bf16 ``[B, 1, Hq, 128]`` (or ``[B, Hq, 128]``); ``k_prefix`` / ``v_prefix``: bf16
     ``[P, Lp, Hkv, 128]``, of which prefix i holds the first ``prefix_lens[i]`` rows (int32
@@ -200,7 +200,8 @@ def switch_gqa_decode_shared_forward(
     Hkv, 128]``, each sequence's own rows behind its prefix, ``cache_lens[b]`` of them, the
     new token's among them (int32 ``[B]``, clamped to ``[0, L]``); ``full_mask``: bool
     ``[B]``.  With ``n`` rows of prefix and cache together a sequence attends all of them
-    when routed full, else the last ``window_size``.  Up to 1024 sequences and 1024 prefixes.
+    when routed full, else the last ``window_size``.  Up to 1024 sequences and 1024 prefixes,
+    of fewer than 2^31 rows of all KV heads (``include/swattn_shared.h`` has the bounds).
 
     Returns ``(O [B, 1, Hq, 128] bf16, LSE [B, 1, Hq] fp32)``; a sequence without any row
     gives O = NaN and LSE = -inf.
