@@ -100,6 +100,8 @@ INTERNAL_SIGNATURES = {
                                                           _vp, _vp, _vp, _i32, _i64, _i64, _i32,
                                                           _i32, _i32, _i32, ctypes.c_float, _vp,
                                                           ctypes.c_size_t, _vp, _vp, _vp]),
+    "swattn_shared_plan": (ctypes.c_int, [_vp] * 4 + [_i32, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp,
+                                                      _i64, _vp]),
     "swattn_check_bounds": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
 }
 

@@ -69,12 +69,12 @@ template <typename Pos>
 struct Line {
   uint32_t share, aligned;
   Pos total;   // positions of the line
-  __device__ __forceinline__ uint32_t length(uint32_t n, uint32_t pad) const {
+  __host__ __device__ __forceinline__ uint32_t length(uint32_t n, uint32_t pad) const {
     return n == 0 ? 0u : aligned ? (n + share - 1u) / share * share : n + pad;
   }
 };
 template <typename Pos, class P>
-__device__ __forceinline__ Line<Pos> plan_line(const P& p, Pos keys, uint32_t pairs) {
+__host__ __device__ __forceinline__ Line<Pos> plan_line(const P& p, Pos keys, uint32_t pairs) {
   const uint32_t target = p.target;
   const uint32_t by_len = (static_cast<uint32_t>(p.cache_len) + kMaxSplitsDev - 2u) / (kMaxSplitsDev - 1u);
   const uint32_t least = max(by_len, P::kMinShare);

@@ -86,6 +86,24 @@ int swattn_prefill_key_weights_checked(const void* q, const void* k, const float
                                        size_t workspace_bytes, void* stream, int32_t* host,
                                        int32_t* flags);
 
+/*
+ * What the workgroups of swattn_shared_decode_fwd work out on the device, from lengths,
+ * prefix numbers and routes in host memory and by the same functions (shared_plan.h,
+ * plan_line of decode_line.h): for tests of the bounds that its workspace and grid rely on.
+ *   totals  int64 [8]: prefix pieces, pieces that the workspace holds; shares of the line,
+ *           slots that their partials reach to, slots that the workspace holds; workgroups
+ *           of the grid; positions of a share and of the line
+ *   pieces  int32 [max_pieces][8], by workgroup: prefix, local route (0 or 1), tile, KV
+ *           head, first key, key behind the last, number of its partial, pieces of the tile
+ *   own     int64 [batch][heads_kv][4]: position of the first key on the line, keys, slot
+ *           of the first partial, partials
+ */
+int swattn_shared_plan(const int32_t* prefix_lens, const int32_t* prefix_ids,
+                       const int32_t* cache_lens, const uint8_t* full, int32_t batch,
+                       int64_t cache_len, int32_t prefixes, int64_t prefix_len, int32_t heads_q,
+                       int32_t heads_kv, int32_t window, int64_t* totals, int32_t* pieces,
+                       int64_t max_pieces, int64_t* own);
+
 #ifdef __cplusplus
 }  // extern "C"
 #endif

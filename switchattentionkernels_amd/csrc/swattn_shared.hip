@@ -24,7 +24,7 @@
 // instructions: B64 Hq64 behind 32768 rows 131 us, with three 154, with one 17 less.  Of 524288
 // outputs there 889 differ from the exact value's rounding, by one last place, with three 269,
 // and 627 of a plain evaluation in fp32; behind 8192 rows 328 of 262144, 90 and 113.
-
+//
 // Local rows attend the last rows of their prefix only, each from its own start on.
 // Masked scores are -inf, their weights 0.  A piece whose sums are not finite runs again
 // carefully: values that are not finite, which a weight of 0 would turn into NaN, are
@@ -46,6 +46,8 @@
 #include <string>
 
 #include "decode_line.h"
+#include "shared_plan.h"
+#include "swattn_internal.h"
 #include "swattn_shared.h"
 #include "tiles.h"
 
@@ -57,17 +59,11 @@ using tiles::f32x16;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTileRows = 128;       // query rows of a prefix tile, at most
-constexpr int kTileKeys = tiles::kBN;
-constexpr uint32_t kMinPiece = 64;   // keys of a prefix piece, at least (128: B4 14.0 us instead of 13.0)
-// What a key of a prefix tile costs, in 16ths of a key of the line.  B64 behind 8192 and 32768
-// rows with 20: 49.7 and 136 us, 24: 51.0 and 132, 32: 55.7 and 155; 10: 72 and 174.
-constexpr uint32_t kTileCost = 24;
+static_assert(kTileKeys == tiles::kBN, "a step takes a tile of K");
 
 constexpr int kOwnWaves = 4;         // waves per workgroup
 constexpr int kMaxG = 8;
 constexpr int kOwnStep = 32;         // keys that a wave takes at once of a sequence's own
-constexpr uint32_t kPairPad = 192;   // a pair's start, in keys
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
@@ -161,7 +157,7 @@ __device__ __forceinline__ void routes_of(const SharedParams& p, int per, Prefix
     r.start[j] = 0;
     if (id[j] < 0 || id[j] >= p.prefixes) continue;
     const int rows = s.rows[id[j]], len = r.lo[j] + r.n[j];
-    r.start[j] = full[j] ? 0 : max(rows - max(p.window - len, 0), 0);
+    r.start[j] = prefix_start(full[j], rows, len, p.window);
     if (r.start[j] >= rows) continue;
     r.group[j] = 2 * id[j] + (full[j] ? 0 : 1);
     atomicAdd(&s.seqs[id[j]], full[j] ? 1u : 1u << 16);
@@ -200,26 +196,21 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
     if (i / 2 >= pper || x >= p.prefixes) continue;
     g[i].seqs = i & 1 ? s.seqs[x] >> 16 : s.seqs[x] & 0xffffu;
     if (g[i].seqs == 0) continue;
-    g[i].tiles = ((g[i].seqs + p.tile_seqs - 1) * p.tile_inv) >> 20;   // below 2^11 by 2^16: exact
+    g[i].tiles = tiles_of(g[i].seqs, p.tile_seqs, p.tile_inv);
     g[i].first = i & 1 ? s.first[x] : 0;
     g[i].keys = static_cast<uint32_t>(s.rows[x]) - g[i].first;
     positions += g[i].tiles * g[i].keys;
   }
   scan_keys<4, 1, uint32_t>(positions, 0, unused0, unused1, all_positions, unused2);
-  // Equal shares of the whole cost, and the keys of a piece at that; a tile is spread
-  // over at most 255 pieces.
-  const uint64_t cost = line + (static_cast<uint64_t>(all_positions) * p.hkv * kTileCost + 15u) / 16u;
-  const uint32_t share = static_cast<uint32_t>((cost * p.target_inv) >> 32) + 1u;
-  const uint32_t by_len = (static_cast<uint32_t>(p.prefix_len) + 254u) / 255u;
-  const uint32_t length = (max(max((share * 16u + kTileCost - 1u) / kTileCost, by_len), kMinPiece) + kTileKeys - 1u) & ~(kTileKeys - 1u);
+  const uint32_t length = piece_length(line, all_positions, p.hkv, p.target_inv, p.prefix_len);
   uint32_t pieces = 0, base, all_pieces, parts[2 * kPer], len[2 * kPer];
 #pragma unroll
   for (int i = 0; i < 2 * kPer; ++i) {
     parts[i] = len[i] = 0;
     if (g[i].seqs == 0) continue;
-    const uint32_t n = (g[i].keys + length - 1u) / length;   // equal pieces, whole tiles of keys
-    len[i] = ((g[i].keys + n - 1u) / n + kTileKeys - 1u) & ~(kTileKeys - 1u);
-    parts[i] = (g[i].keys + len[i] - 1u) / len[i];
+    const Cut cut = cut_keys(g[i].keys, length);
+    len[i] = cut.length;
+    parts[i] = cut.parts;
     pieces += g[i].tiles * p.hkv * parts[i];
   }
   scan_keys<4, 2, uint32_t>(pieces, 0, base, unused0, all_pieces, unused1);
@@ -230,13 +221,9 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
       for (int i = 0; i < 2 * kPer; ++i) {
         const uint32_t here = g[i].tiles * p.hkv * parts[i];
         if (block - base < here) {
-          // Pieces of the same keys, a tile's each, one after the other on one XCD (blocks go to the
-          // eight in turn), which then reads them once: B64 Hq64/Hkv8 behind 32768 rows 136 -> 133.5 us.
-          const uint32_t at = block - base, x = at & 7u;
-          const uint32_t id = x * (here >> 3) + min(x, here & 7u) + (at >> 3);
-          const uint32_t keys_of = id / g[i].tiles, tile = id - keys_of * g[i].tiles, kvh = keys_of / parts[i];
-          s_piece = Piece{2 * (tid * pper + i / 2) + (i & 1), static_cast<int>(tile), static_cast<int>(kvh),
-                          static_cast<int>(keys_of - kvh * parts[i]), static_cast<int>(parts[i]), static_cast<int>(len[i]),
+          const PieceOf x = piece_of(block - base, here, g[i].tiles, parts[i]);
+          s_piece = Piece{2 * (tid * pper + i / 2) + (i & 1), static_cast<int>(x.tile), static_cast<int>(x.kvh),
+                          static_cast<int>(x.part), static_cast<int>(parts[i]), static_cast<int>(len[i]),
                           static_cast<int>(g[i].first), static_cast<int>(g[i].first + g[i].keys), static_cast<int>(g[i].seqs),
                           static_cast<int>(base)};
         }
@@ -250,7 +237,7 @@ __device__ __forceinline__ bool plan_shared(const SharedParams& p, const Routes<
   // The line, as plan_inline lays it out for the workgroups that the pieces leave.
   wg = block - all_pieces;
   SharedParams q = p;
-  q.target = max(p.target > all_pieces ? p.target - all_pieces : 0u, p.least);
+  q.target = line_target(p.target, all_pieces, p.least);
   Line<uint32_t> L = plan_line<uint32_t>(q, all_keys * p.hkv, all_cnt * p.hkv);
   before += rank * p.pad;
   if (L.aligned) {
@@ -558,7 +545,7 @@ __device__ __forceinline__ void prefix_piece(const SharedParams& p, const Routes
                                              int2* s_rows, char* ring) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int k0 = uniform(x.first + x.part * x.length), k1 = min(k0 + uniform(x.length), uniform(x.end));
+  const int k0 = uniform(x.first + x.part * x.length), k1 = k0 + min(uniform(x.length), uniform(x.end) - k0);
   const uint32_t row_bytes = static_cast<uint32_t>(p.hkv) * tiles::kRowBytes;
   const int64_t base = (static_cast<int64_t>(uniform(x.group) >> 1) * p.prefix_len * p.hkv + uniform(x.kvh)) * kD;
   const int last = uniform(x.end) - 1;
@@ -926,14 +913,9 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(const SharedParams p)
   const SeqPlace seq = seq_place(p.plan[1 + b]);
   const uint4 line = p.plan[0];
   const int4 place = p.place[b];
-  // Of a position below 2^31, its share: by 2^32 / share, rounded down, one too low at most.
-  auto share_of = [&](uint32_t at) {
-    const uint32_t n = __umulhi(at, line.w);
-    return n + (at - n * line.x >= line.x ? 1u : 0u);
-  };
   const uint32_t off = static_cast<uint32_t>(seq.off) + static_cast<uint32_t>(kvh) * seq.len;
-  const uint32_t wg0 = share_of(off);
-  const int own = seq.n > 0 ? static_cast<int>(share_of(off + seq.n - 1) - wg0) + 1 : 0;   // at most 256
+  const uint32_t wg0 = share_of(off, line.x, line.w);
+  const int own = seq.n > 0 ? static_cast<int>(share_of(off + seq.n - 1, line.x, line.w) - wg0) + 1 : 0;   // at most 256
   const int pieces = place.y, all = own + pieces;
   const int64_t slot0 = static_cast<int64_t>(wg0) + static_cast<int64_t>(seq.rank) * p.hkv + kvh;
   const int64_t row0 = (static_cast<int64_t>(place.x) + static_cast<int64_t>(kvh) * pieces) * p.tile_rows + place.z + h;
@@ -1047,6 +1029,26 @@ bool shared_layout(int64_t batch, int64_t cache_len, int64_t prefixes, int64_t p
   return true;
 }
 
+// What the plan goes by of a call's sizes.
+void plan_sizes(SharedParams& p, const SharedLayout& L, int32_t batch, int64_t cache_len, int32_t prefixes, int64_t prefix_len,
+                int32_t heads_q, int32_t heads_kv, int32_t window) {
+  p.cache_len = static_cast<int>(cache_len);
+  p.batch = batch;
+  p.hq = heads_q;
+  p.hkv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.window = window;
+  p.target = static_cast<uint32_t>(L.target);
+  p.target_inv = static_cast<uint32_t>(((int64_t{1} << 32) + L.target - 1) / L.target);
+  p.pad = kPairPad;
+  p.prefixes = prefixes;
+  p.prefix_len = static_cast<int>(prefix_len);
+  p.tile_seqs = static_cast<int>(L.tile_seqs);
+  p.tile_inv = static_cast<uint32_t>((1u << 20) / L.tile_seqs + 1);
+  p.tile_rows = static_cast<int>(L.tile_rows);
+  p.least = static_cast<uint32_t>(L.least);
+}
+
 }  // namespace
 }  // namespace swattn
 
@@ -1101,15 +1103,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.plan = reinterpret_cast<uint4*>(ws + L.off_plan);
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
-  p.cache_len = static_cast<int>(cache_len);
-  p.batch = batch;
-  p.hq = heads_q;
-  p.hkv = heads_kv;
-  p.group = heads_q / heads_kv;
-  p.window = window;
-  p.target = static_cast<uint32_t>(L.target);
-  p.target_inv = static_cast<uint32_t>(((int64_t{1} << 32) + L.target - 1) / L.target);
-  p.pad = kPairPad;
+  plan_sizes(p, L, batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, window);
   p.prefix_k = static_cast<const uint16_t*>(k_prefix);
   p.prefix_v = static_cast<const uint16_t*>(v_prefix);
   p.prefix_lens = prefix_lens;
@@ -1117,13 +1111,7 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   p.tile_o = reinterpret_cast<float*>(ws + L.off_tile_o);
   p.tile_ml = reinterpret_cast<float*>(ws + L.off_tile_ml);
   p.place = reinterpret_cast<int4*>(ws + L.off_place);
-  p.prefixes = prefixes;
   p.stream_prefix = batch <= L.tile_seqs && prefixes * prefix_len * heads_kv * (4 * kD) >= kStreamPrefixBytes;
-  p.prefix_len = static_cast<int>(prefix_len);
-  p.tile_seqs = static_cast<int>(L.tile_seqs);
-  p.tile_inv = static_cast<uint32_t>((1u << 20) / L.tile_seqs + 1);
-  p.tile_rows = static_cast<int>(L.tile_rows);
-  p.least = static_cast<uint32_t>(L.least);
   const hipStream_t st = as_stream(stream);
   const dim3 grid(static_cast<uint32_t>(L.pieces + L.least));
   const bool stream_past = (batch * cache_len + prefixes * prefix_len) * heads_kv * (4 * kD) >= kStreamBytes;
@@ -1141,6 +1129,80 @@ int swattn_shared_decode_fwd(const void* q, const void* k_prefix, const void* v_
   hipLaunchKernelGGL(shared_merge_kernel, dim3(static_cast<uint32_t>(p.group), static_cast<uint32_t>(heads_kv), static_cast<uint32_t>(batch)),
                      dim3(256), 0, st, p);
   return launch_status(name);
+}
+
+int swattn_shared_plan(const int32_t* prefix_lens, const int32_t* prefix_ids, const int32_t* cache_lens, const uint8_t* full,
+                       int32_t batch, int64_t cache_len, int32_t prefixes, int64_t prefix_len, int32_t heads_q,
+                       int32_t heads_kv, int32_t window, int64_t* totals, int32_t* pieces, int64_t max_pieces, int64_t* own) {
+  SharedLayout L;
+  if (window <= 0 || !shared_layout(batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, L))
+    return invalid("swattn_shared_plan: shapes that the decode refuses");
+  SharedParams p{};
+  plan_sizes(p, L, batch, cache_len, prefixes, prefix_len, heads_q, heads_kv, window);
+  auto clamped = [](int32_t x, int most) { return x < 0 ? 0 : x > most ? most : x; };
+  struct Group {
+    uint32_t seqs, first;
+  };
+  Group groups[2 * SWATTN_SHARED_MAX_PREFIXES];
+  uint32_t keys[SWATTN_SHARED_MAX_SEQS];
+  for (int i = 0; i < 2 * prefixes; ++i) groups[i] = Group{0u, UINT32_MAX};
+  uint32_t all_keys = 0, all_cnt = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int len = clamped(cache_lens[b], p.cache_len), id = prefix_ids[b];
+    keys[b] = full[b] ? len : len < window ? len : window;
+    all_keys += keys[b];
+    all_cnt += keys[b] > 0 ? 1 : 0;
+    if (id < 0 || id >= prefixes) continue;
+    const int rows = clamped(prefix_lens[id], p.prefix_len), start = prefix_start(full[b] != 0, rows, len, window);
+    if (start >= rows) continue;
+    Group& g = groups[2 * id + (full[b] ? 0 : 1)];
+    ++g.seqs;
+    if (static_cast<uint32_t>(start) < g.first) g.first = start;
+  }
+  auto keys_of = [&](int i) { return static_cast<uint32_t>(clamped(prefix_lens[i / 2], p.prefix_len)) - groups[i].first; };
+  uint32_t positions = 0;
+  for (int i = 0; i < 2 * prefixes; ++i)
+    if (groups[i].seqs > 0) positions += tiles_of(groups[i].seqs, p.tile_seqs, p.tile_inv) * keys_of(i);
+  const uint32_t line = (all_keys + all_cnt * p.pad) * p.hkv;
+  const uint32_t length = piece_length(line, positions, p.hkv, p.target_inv, p.prefix_len);
+  uint32_t base = 0;
+  for (int i = 0; i < 2 * prefixes; ++i) {
+    if (groups[i].seqs == 0) continue;
+    const uint32_t tiles = tiles_of(groups[i].seqs, p.tile_seqs, p.tile_inv), n = keys_of(i);
+    const Cut cut = cut_keys(n, length);
+    const uint32_t here = tiles * p.hkv * cut.parts;
+    for (uint32_t at = 0; at < here && base + at < max_pieces; ++at) {
+      const PieceOf x = piece_of(at, here, tiles, cut.parts);
+      const uint32_t from = x.part * cut.length, to = from + cut.length < n ? from + cut.length : n;
+      const uint32_t row[8] = {static_cast<uint32_t>(i / 2), static_cast<uint32_t>(i & 1), x.tile, x.kvh, groups[i].first + from,
+                               groups[i].first + to, base + (x.tile * p.hkv + x.kvh) * cut.parts + x.part, cut.parts};
+      for (int j = 0; j < 8; ++j) pieces[8 * (static_cast<int64_t>(base) + at) + j] = static_cast<int32_t>(row[j]);
+    }
+    base += here;
+  }
+  p.target = line_target(p.target, base, p.least);
+  Line<uint32_t> S = plan_line<uint32_t>(p, all_keys * p.hkv, all_cnt * p.hkv);
+  uint32_t total = 0, rank = 0;
+  int64_t slots = 0;
+  const uint32_t inv = UINT32_MAX / S.share;
+  for (int b = 0; b < batch; ++b) {
+    const uint32_t len = S.length(keys[b], p.pad);
+    for (int kvh = 0; kvh < p.hkv; ++kvh) {
+      int64_t* to = own + 4 * (static_cast<int64_t>(b) * p.hkv + kvh);
+      const uint32_t wg0 = share_of(total, S.share, inv);
+      to[0] = total;
+      to[1] = keys[b];
+      to[2] = static_cast<int64_t>(wg0) + static_cast<int64_t>(rank) * p.hkv + kvh;
+      to[3] = keys[b] > 0 ? share_of(total + keys[b] - 1, S.share, inv) - wg0 + 1 : 0;
+      if (to[3] > 0 && to[2] + to[3] > slots) slots = to[2] + to[3];
+      total += len;
+    }
+    rank += keys[b] > 0 ? 1 : 0;
+  }
+  const int64_t out[8] = {base, L.pieces, (static_cast<int64_t>(total) + S.share - 1) / S.share, slots, L.slots, L.pieces + L.least,
+                          S.share, total};
+  for (int i = 0; i < 8; ++i) totals[i] = out[i];
+  return SWATTN_OK;
 }
 
 }  // extern "C"
