@@ -152,6 +152,10 @@ def _check_shared(q, k_prefix, v_prefix, prefix_lens, prefix_ids, k_cache, v_cac
     rows = (q, k_prefix, v_prefix, k_cache, v_cache)
     if not _all_tensors(*rows) or any(t.dtype != torch.bfloat16 for t in rows):
         raise TypeError("Switch Attention decode requires BF16 Q, prefixes and KV cache")
+    for name, t in (("prefix_lens", prefix_lens), ("prefix_ids", prefix_ids), ("cache_lens", cache_lens),
+                    ("full_mask", full_mask)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
     dev = q.device
     if not q.is_cuda or any(t.device != dev for t in rows):
         raise ValueError("Q, prefixes and KV cache must be on one supported accelerator device")

@@ -198,6 +198,9 @@ def _validate_append(q, k, v, k_cache, v_cache, lens, counts) -> None:
     if (k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] == 0
             or k_cache.shape[0] != k.shape[0] or k_cache.shape[2:] != k.shape[2:]):
         raise ValueError("the caches must be [B,L,Hkv,128] of one shape, with K's batch size and heads")
+    for name, t in (("cache_lens", lens), ("row_counts", counts)):
+        if not isinstance(t, torch.Tensor) and not (t is None and name == "row_counts"):
+            raise TypeError(f"{name} must be a tensor")
     check_lens(lens, q.shape[0], dev, "cache_lens")
     if counts is not None:
         check_lens(counts, q.shape[0], dev, "row_counts")
