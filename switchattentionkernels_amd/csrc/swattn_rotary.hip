@@ -18,9 +18,9 @@
 // took 72 us instead of 69.  Rows are read one pass ahead.
 //
 // Measured, as a large copy's 5.2 TB/s goes (a copy of 74 MB: 5.0): rotations of strided
-// rows B1 S16384 Hq32/Hkv8 62.5 us (5.4 TB/s), B2 S2999 Hq40/Hkv8 29.9 (4.9); backward of
-// S16384 with norms 93.5 us (5.4 TB/s), of B2 S4096 without 28.9; appends of B8 T517 Hq64/Hkv8
-// 33.2 (4.7), of 64 single tokens 6.6, bound by dependent latencies and the host's call.
+// rows B1 S16384 Hq32/Hkv8 62.7 us (5.4 TB/s), B2 S2999 Hq40/Hkv8 30.0 (4.9); backward of
+// S16384 with norms 92 us (5.4 TB/s), of B2 S4096 without 28.9; appends of B8 T517 Hq64/Hkv8
+// 33.5 (4.7), of 64 single tokens 6.6, bound by dependent latencies and the host's call.
 // One pass at a time without reading ahead, angles and weights in registers: 71, 42, 117, 42,
 // 50 and 7.5.
 //

@@ -31,11 +31,12 @@
 // taken out of the products and added key by key to the rows that attend them.
 //
 // Measured (Hkv 8), as a large copy's 5.2 TB/s and a large matrix product's 1210 TFLOP/s go:
-// B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 49 us against 39 for its bytes,
-// own rows being read until 36 us of a split kernel of 43 (plan 2.2, merge and gap 7); B64 Hq64
-// behind 32768 rows, all full: 130 us against 58 for its operations: the matrix cores are busy
-// 48 % of the cycles, the vector ALUs 50 %, at the 1.7 GHz that the board's power limit leaves.  Three documents, B40
-// Hq40: 28 us against 19; B4 Hq8/Hkv2 behind 1024 rows 10.3 us, latency: plan, one tile, merge.
+// B64 Hq32 behind 8192 rows, own caches of 1024, a quarter full: 49.5 us against 39 for its bytes,
+// own rows being read until 36 us of a split kernel of 45 (plan 2.2, merge and gap 7); B64 Hq64
+// behind 32768 rows, all full: 131 to 134 us against 58 for its operations: the matrix cores are busy
+// 48 % of the cycles and the vector ALUs 50 %, at 1.7 GHz, the two waves of a SIMD taking turns
+// (a wave waits 28 % of its cycles for tiles and barriers, 34 % to issue).  Three documents, B40
+// Hq40: 28.4 us against 19; B4 Hq8/Hkv2 behind 1024 rows 10.4 us, latency: plan, one tile, merge.
 // Tried without gain: half tiles with operands read a step ahead (145 us instead of 134
 // behind 32768 rows: more barriers), waves that share a short tile's keys and dims (such pieces
 // wait for memory), unlike wave priorities.
